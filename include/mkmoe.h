@@ -260,6 +260,119 @@ int mkmoe_workspace_region(const mkmoe_shape* shape, int32_t region, size_t* off
 
 const char* mkmoe_status_string(int status);
 
+/* ---------------------------------------------------------------- latent attention
+ * The attention that precedes the MoE block in a DeepSeek-V3 decode layer, one TP rank's heads.
+ * A token's keys and values are one shared row: MKMOE_LATENT_DIM latent values c, RMS-normed,
+ * and MKMOE_LATENT_ROPE rotated values k_pe, in a paged cache. In the absorbed form
+ *   s = scale (q_lat . c + q_pe . k_pe),  o = sum over visible tokens of softmax(s) c
+ * with q_lat = W_UK^T q_nope and the head's output W_UV o. No counterpart in the reference's
+ * scope here (its attention is another, sparse one: deepseek_v41/gfx950/attention).
+ *
+ * Every call runs on the caller's stream, allocates nothing, does not synchronise with the host
+ * and can be captured in a graph; arguments are checked before anything is launched. Values read
+ * on the device (slots, positions, lengths, pages, query starts) are checked there: one outside
+ * its bounds is never used as an address, and is recorded in the workspace's error words.
+ * A workspace serves one stream at a time. */
+#define MKMOE_LATENT_DIM 512
+#define MKMOE_LATENT_ROPE 64
+#define MKMOE_LATENT_NOPE 128      /* a head's query values without rotation */
+#define MKMOE_LATENT_V 128         /* a head's output values */
+#define MKMOE_LATENT_MX_ROW 656    /* bytes of an MXFP8 cache row */
+#define MKMOE_LATENT_MAX_HEADS 128
+#define MKMOE_LATENT_MAX_SEQS 512
+
+/* cache formats. BF16: 576 bf16 a row (latent, then rope). MXFP8: 512 e4m3 codes, 16 E8M0 scales
+ * (one per 32 latent values; a value is code 2^(scale - 127), below 2^-126 taken as 0), 64 bf16
+ * rope values. */
+#define MKMOE_LATENT_BF16 1
+#define MKMOE_LATENT_MXFP8 2
+
+/* rope: pairs (2 i, 2 i + 1), or (i, i + 32) */
+#define MKMOE_ROPE_INTERLEAVED 0
+#define MKMOE_ROPE_HALF 1
+
+/* error words at the head of a latent workspace (the caller clears them by zeroing them) */
+#define MKMOE_LATENT_ERRW_CODE 0  /* 0, or the first error's code (MKMOE_LATENT_ERR_*) */
+#define MKMOE_LATENT_ERRW_WHERE 1 /* its token (slot, position) or sequence (length, page) */
+#define MKMOE_LATENT_ERRW_COUNT 2 /* how many were seen */
+#define MKMOE_LATENT_ERRW_WORDS 4
+#define MKMOE_LATENT_ERR_SLOT 1     /* slot >= pages page_size: the row is not written / read as 0 */
+#define MKMOE_LATENT_ERR_POSITION 2 /* position outside cos_sin: the token's rows are not written */
+#define MKMOE_LATENT_ERR_LENGTH 3   /* length or query starts outside their bounds: clamped */
+#define MKMOE_LATENT_ERR_PAGE 4     /* page outside the cache: its tokens read as rows of zeros */
+
+typedef struct mkmoe_latent_cache {
+  void* data;        /* [pages][page_size] rows, 16-byte aligned */
+  int64_t pages;     /* pages page_size < 2^31 */
+  int32_t page_size; /* tokens a page: a power of two, 1 .. 1024 */
+  int32_t fmt;       /* MKMOE_LATENT_BF16 / _MXFP8 */
+} mkmoe_latent_cache;
+
+/* strides in elements, multiples of 8 (0: broadcast); the last axis is contiguous */
+typedef struct mkmoe_latent_append_io {
+  mkmoe_latent_cache cache;
+  int32_t tokens;       /* any number, 0 included */
+  int32_t heads;        /* of q_pe; 0: no query */
+  int32_t rope;         /* MKMOE_ROPE_* */
+  int32_t index_bytes;  /* of positions and slots: 4 or 8 */
+  int64_t cos_sin_rows;
+  int64_t kv_stride;    /* >= 576 */
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  const void* kv;        /* [tokens][576] bf16: latent, rope part before the rotation */
+  const void* norm_w;    /* [512] bf16; NULL: the latent is stored as it is */
+  const float* cos_sin;  /* [cos_sin_rows][64]: 32 cosines, 32 sines */
+  const void* positions; /* [tokens] */
+  const void* slots;     /* [tokens] cache rows, distinct; negative: a padded token, not written */
+  const void* q_pe;      /* [tokens][heads][64] bf16 */
+  void* q_out;           /* the same, rotated; may be q_pe itself */
+  float norm_eps;
+  int32_t reserved;
+} mkmoe_latent_append_io;
+
+typedef struct mkmoe_latent_attend_io {
+  mkmoe_latent_cache cache;
+  int32_t seqs;       /* 1 .. MKMOE_LATENT_MAX_SEQS */
+  int32_t tokens;     /* query tokens; without q_starts a multiple of seqs */
+  int32_t heads;      /* 1 .. MKMOE_LATENT_MAX_HEADS */
+  int32_t max_pages;  /* table entries a sequence: its length is at most max_pages page_size */
+  int64_t table_stride;
+  int64_t ql_token_stride, ql_head_stride, qp_token_stride, qp_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  const void* q_lat;       /* [tokens][heads][512] bf16 */
+  const void* q_pe;        /* [tokens][heads][64] bf16, rotated */
+  const int32_t* table;    /* [seqs][max_pages] pages */
+  const int32_t* lens;     /* [seqs] cached tokens, the queries' own among them; 0: none */
+  const int32_t* q_starts; /* [seqs + 1] first query token of each sequence, or NULL: equal counts */
+  void* out;               /* [tokens][heads][512] bf16; 0 for a query that sees nothing */
+  float* lse;              /* [tokens][heads] log of the sum of exp(s), or NULL; -inf there */
+  float scale;
+  int32_t reserved;
+} mkmoe_latent_attend_io;
+
+/* y = W_UK^T x ([tokens][heads][128] -> 512, expand 0) or W_UV x (512 -> 128, expand 1), each head
+ * by its own weights; fp32 sums */
+typedef struct mkmoe_latent_project_io {
+  int32_t tokens, heads, expand, reserved;
+  int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+  const void* x;
+  const void* w; /* [heads][256][512] bf16 (kv_b): W_UK rows 0 .. 127, W_UV rows 128 .. 255 */
+  void* y;
+} mkmoe_latent_project_io;
+
+/* Workspace bytes of every latent call (256-byte aligned; zeroed once by the caller). */
+int mkmoe_latent_workspace_bytes(size_t* bytes);
+/* Norm, rotate and store the step's rows; rotate the query's rope part. One launch. */
+int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_bytes, void* stream);
+/* The values that cache rows stand for: out [tokens][576] bf16; a negative slot's row is 0. */
+int mkmoe_latent_rows(const mkmoe_latent_cache* cache, const void* slots, int32_t index_bytes, int32_t tokens, void* out,
+                      void* ws, size_t ws_bytes, void* stream);
+/* The absorbed attention: query token i of a sequence's n sees its first len - n + 1 + i tokens.
+ * Rows of out behind the last sequence's queries stay as they were. Two launches. */
+int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_bytes, void* stream);
+int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream);
+/* Copy n error words to host memory (synchronises stream). */
+int mkmoe_latent_read_errors(const void* ws, int32_t* words, int32_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

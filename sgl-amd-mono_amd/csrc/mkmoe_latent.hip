@@ -1,0 +1,1009 @@
+// Latent attention of a decode step on gfx950 (MI355X): HIP kernels and the C ABI of the latent
+// section of include/mkmoe.h.
+//
+// A token's keys and values are one shared row: 512 latent values c (RMS-normed) and 64 rotated
+// rope values k_pe, in a paged cache, as bf16 (1152 bytes) or MXFP8 (512 e4m3 codes, 16 E8M0
+// scales, 64 bf16 rope values: 656 bytes). In the absorbed form every head's query is 512 + 64
+// values against that row, and the row's latent part is the value too:
+//   s = scale (q_lat . c + q_pe . k_pe),  o = sum softmax(s) c.
+//
+//   k_latent_append   norm, rotate and write a step's rows; rotate the query's rope part
+//   k_latent_rows     the values that cache rows stand for
+//   k_latent_attend   the absorbed attention, its work cut into equal shares over the card
+//   k_latent_merge    joins the shares of a sequence that was cut
+//   k_latent_absorb / k_latent_expand   the two products of every head with its weights
+
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/mkmoe.h"
+#include "mkmoe_numerics.h"
+
+namespace mkmoe_latent {
+
+using mkmoe::bf2f;
+using mkmoe::f2u;
+using mkmoe::u2f;
+
+constexpr int kL = MKMOE_LATENT_DIM;    // 512
+constexpr int kR = MKMOE_LATENT_ROPE;   // 64
+constexpr int kRow = kL + kR;           // values a cache row
+constexpr int kMxScales = kL / 32;
+constexpr int kMxRow = MKMOE_LATENT_MX_ROW;
+constexpr int kNope = MKMOE_LATENT_NOPE, kV = MKMOE_LATENT_V;
+static_assert(kMxRow == kL + kMxScales + 2 * kR && kMxRow % 16 == 0, "MXFP8 rows in whole 16-byte pieces");
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+#define MKMOE_LDS __attribute__((address_space(3)))
+
+__device__ __forceinline__ float bf_lo(uint32_t w) { return u2f(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return u2f(w & 0xffff0000u); }
+// two fp32 as bf16 (nearest even, NaN kept), a in the low half
+__device__ __forceinline__ uint32_t pack_bf(float a, float b) {
+  const bf16x2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// 8 e4m3 codes (bytes of w0 then w1) times s, a power of two, as bf16: exact
+__device__ __forceinline__ u32x4 fp8x8(uint32_t w0, uint32_t w1, float s) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
+  return u32x4{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+               __builtin_bit_cast(uint32_t, d)};
+}
+__device__ __forceinline__ float e8m0(uint32_t e) { return u2f(e << 23); }
+
+// the first error of a call since the last clear: a page, slot, position, length or query range
+// outside its bounds, and the token or sequence that had it
+__device__ void record(int32_t* err, int code, int where) {
+  if (atomicCAS(err + MKMOE_LATENT_ERRW_CODE, 0, code) == 0) err[MKMOE_LATENT_ERRW_WHERE] = where;
+  atomicAdd(err + MKMOE_LATENT_ERRW_COUNT, 1);
+}
+
+// ---------------------------------------------------------------- append
+struct AppendParams {
+  const uint16_t* kv;
+  const uint16_t* norm_w;
+  const float* cos_sin;
+  const void* positions;
+  const void* slots;
+  const uint16_t* q;
+  uint16_t* q_out;
+  uint8_t* cache;
+  int32_t* err;
+  int64_t kv_stride, q_ts, q_hs, o_ts, o_hs;
+  int64_t rows, table_rows;
+  int tokens, heads, half, wide, kv_blocks;
+  float eps;
+};
+
+__device__ __forceinline__ int64_t index_at(const void* p, int i, int wide) {
+  return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+// the lane's 8 values (16 bytes at value 8 j of a 64-value row, j = lane % 8) rotated by the
+// row's angles: pairs (2 i, 2 i + 1), or (i, i + 32) with the partner's values 4 lanes away
+__device__ __forceinline__ u32x4 rotate8(u32x4 v, const float* cs, int j, int half) {
+  float x[8];
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf_lo(w[i]);
+    x[2 * i + 1] = bf_hi(w[i]);
+  }
+  uint32_t o[4];
+  if (!half) {
+    const f32x4 c = *(const f32x4*)(cs + 4 * j), s = *(const f32x4*)(cs + kR / 2 + 4 * j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = pack_bf(x[2 * i] * c[i] - x[2 * i + 1] * s[i], x[2 * i + 1] * c[i] + x[2 * i] * s[i]);
+  } else {
+    const int jj = j & 3;
+    const f32x4 c0 = *(const f32x4*)(cs + 8 * jj), c1 = *(const f32x4*)(cs + 8 * jj + 4);
+    const f32x4 s0 = *(const f32x4*)(cs + kR / 2 + 8 * jj), s1 = *(const f32x4*)(cs + kR / 2 + 8 * jj + 4);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float other = __shfl_xor(x[i], 4, 64);
+      const float c = i < 4 ? c0[i & 3] : c1[i & 3], s = i < 4 ? s0[i & 3] : s1[i & 3];
+      y[i] = j < 4 ? x[i] * c - other * s : x[i] * c + other * s;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = pack_bf(y[2 * i], y[2 * i + 1]);
+  }
+  return u32x4{o[0], o[1], o[2], o[3]};
+}
+
+// A wave a token of the first kv_blocks workgroups: lane l holds latent values 8 l .. 8 l + 7,
+// lanes 0 .. 7 the rope values too. The other workgroups rotate the query, 8 lanes a head's 64
+// values. Bytes: each value is read and written once; a decode step's few rows are one trip to
+// memory and back.
+template <bool MX>
+__global__ __launch_bounds__(256) void k_latent_append(AppendParams p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x < p.kv_blocks) {
+    const int t = blockIdx.x * 4 + wave;
+    if (t >= p.tokens) return;
+    const int64_t slot = index_at(p.slots, t, p.wide), pos = index_at(p.positions, t, p.wide);
+    if (slot < 0) return;  // a padded row
+    if (slot >= p.rows || pos < 0 || pos >= p.table_rows) {
+      if (lane == 0) record(p.err, slot >= p.rows ? MKMOE_LATENT_ERR_SLOT : MKMOE_LATENT_ERR_POSITION, t);
+      return;
+    }
+    const uint16_t* src = p.kv + (int64_t)t * p.kv_stride;
+    uint8_t* dst = p.cache + slot * (MX ? kMxRow : 2 * kRow);
+    const u32x4 v = *(const u32x4*)(src + 8 * lane);
+    u32x4 pe = {0, 0, 0, 0};
+    if (lane < 8) pe = *(const u32x4*)(src + kL + 8 * lane);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[2 * i] = bf_lo(w[i]);
+      y[2 * i + 1] = bf_hi(w[i]);
+    }
+    if (p.norm_w) {
+      const u32x4 nv = *(const u32x4*)(p.norm_w + 8 * lane);
+      const uint32_t nw[4] = {nv.x, nv.y, nv.z, nv.w};
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) ss += __shfl_xor(ss, d, 64);
+      const float rstd = 1.0f / sqrtf(ss / (float)kL + p.eps);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[2 * i] = y[2 * i] * rstd * bf_lo(nw[i]);
+        y[2 * i + 1] = y[2 * i + 1] * rstd * bf_hi(nw[i]);
+      }
+    }
+    if constexpr (MX) {
+      // 32 values are 4 lanes; the scale is the least power of two that keeps them within 448
+      // (the "vllm" MXFP8 rule), so no code saturates; codes straight from the fp32 values
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(y[i]));
+      top = fmaxf(top, __shfl_xor(top, 1, 64));
+      top = fmaxf(top, __shfl_xor(top, 2, 64));
+      const int e = mkmoe::vllm_code(top);
+      const float inv = mkmoe::mx_inv(e);
+      int w0 = 0, w1 = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // (NaN passes both comparisons)
+        const float q = y[i] * inv;
+        y[i] = q > 448.0f ? 448.0f : (q < -448.0f ? -448.0f : q);
+      }
+      w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w0, false);
+      w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w0, true);
+      w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], w1, false);
+      w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], w1, true);
+      *(u32x2*)(dst + 8 * lane) = u32x2{(uint32_t)w0, (uint32_t)w1};
+      if ((lane & 3) == 0) dst[kL + (lane >> 2)] = (uint8_t)e;
+    } else {
+      *(u32x4*)(dst + 16 * lane) = u32x4{pack_bf(y[0], y[1]), pack_bf(y[2], y[3]), pack_bf(y[4], y[5]), pack_bf(y[6], y[7])};
+    }
+    if (lane < 8) {
+      const u32x4 o = rotate8(pe, p.cos_sin + pos * kR, lane, p.half);
+      *(u32x4*)(dst + (MX ? kL + kMxScales : 2 * kL) + 16 * lane) = o;
+    }
+    return;
+  }
+  const int64_t r = ((int64_t)(blockIdx.x - p.kv_blocks) * 4 + wave) * 8 + (lane >> 3);
+  if (r >= (int64_t)p.tokens * p.heads) return;
+  const int t = (int)(r / p.heads), h = (int)(r - (int64_t)t * p.heads), j = lane & 7;
+  const int64_t pos = index_at(p.positions, t, p.wide);
+  if (pos < 0 || pos >= p.table_rows) {
+    if (j == 0 && h == 0) record(p.err, MKMOE_LATENT_ERR_POSITION, t);
+    return;
+  }
+  const u32x4 v = *(const u32x4*)(p.q + t * p.q_ts + h * p.q_hs + 8 * j);
+  *(u32x4*)(p.q_out + t * p.o_ts + h * p.o_hs + 8 * j) = rotate8(v, p.cos_sin + pos * kR, j, p.half);
+}
+
+// ---------------------------------------------------------------- rows as values
+struct RowsParams {
+  const uint8_t* cache;
+  const void* slots;
+  uint16_t* out;
+  int32_t* err;
+  int64_t rows;
+  int tokens, wide;
+};
+
+// a wave a row: lane l writes the latent values 8 l .. 8 l + 7, lanes 0 .. 7 the rope values
+template <bool MX>
+__global__ __launch_bounds__(256) void k_latent_rows(RowsParams p) {
+  const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= p.tokens) return;
+  const int64_t slot = index_at(p.slots, t, p.wide);
+  u32x4 c = {0, 0, 0, 0}, pe = {0, 0, 0, 0};
+  if (slot >= p.rows) {
+    if (lane == 0) record(p.err, MKMOE_LATENT_ERR_SLOT, t);
+  } else if (slot >= 0) {
+    const uint8_t* src = p.cache + slot * (MX ? kMxRow : 2 * kRow);
+    if constexpr (MX) {
+      const u32x2 q = *(const u32x2*)(src + 8 * lane);
+      c = fp8x8(q.x, q.y, e8m0(src[kL + (lane >> 2)]));
+    } else {
+      c = *(const u32x4*)(src + 16 * lane);
+    }
+    if (lane < 8) pe = *(const u32x4*)(src + (MX ? kL + kMxScales : 2 * kL) + 16 * lane);
+  }
+  uint16_t* dst = p.out + (int64_t)t * kRow;
+  *(u32x4*)(dst + 8 * lane) = c;
+  if (lane < 8) *(u32x4*)(dst + kL + 8 * lane) = pe;
+}
+
+// ---------------------------------------------------------------- attend
+constexpr int kN = 64;          // cached tokens a tile
+constexpr int kShares = 256;    // equal shares of the work, a workgroup each: one a CU
+constexpr int kThreads = 512;   // 8 waves
+constexpr int kMaxSeqs = MKMOE_LATENT_MAX_SEQS;
+constexpr int kRowsMax = 64;    // query rows a tile holds at most
+constexpr int kChunks = kRow * 2 / 16;   // 16-byte pieces of a row in LDS: 72
+constexpr int kPStride = kN + 8;         // bf16 of a row of P: 144 bytes, rows on other banks
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_inff();
+
+struct AttendParams {
+  const uint16_t* ql;
+  const uint16_t* qp;
+  const uint8_t* cache;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* starts;  // NULL: n query tokens a sequence
+  uint16_t* out;
+  float* lse;
+  int32_t* err;
+  int32_t* plan;   // [0] tiles a share, [1 ..] each sequence's first tile of the work
+  float* part_o;   // [2 kShares][M][512]
+  float* part_ml;  // [2 kShares][M][2]
+  int64_t ql_ts, ql_hs, qp_ts, qp_hs, o_ts, o_hs;
+  int64_t table_stride;
+  int64_t pages;
+  int seqs, tokens, heads, n, max_len, page_shift;
+  float scale2;  // scale log2(e)
+};
+
+// a sequence's query tokens and length, clamped to their bounds
+struct Seq {
+  int t0, n, len;
+  bool bad;
+};
+__device__ __forceinline__ Seq seq_of(const AttendParams& p, int b) {
+  Seq s;
+  const int len = p.lens[b];
+  s.len = min(max(len, 0), p.max_len);
+  s.bad = s.len != len;
+  if (p.starts) {
+    const int a = p.starts[b], e = p.starts[b + 1];
+    s.t0 = min(max(a, 0), p.tokens);
+    const int t1 = min(max(e, s.t0), p.tokens);
+    s.n = t1 - s.t0;
+    s.bad = s.bad || a != s.t0 || e != t1;
+  } else {
+    s.t0 = b * p.n;
+    s.n = p.n;
+  }
+  return s;
+}
+// tiles of a sequence: query row tiles times tiles of its cached tokens (an empty sequence has
+// one, which writes its rows)
+template <int M>
+__device__ __forceinline__ int row_tiles(const AttendParams& p, const Seq& s) {
+  return (int)(((int64_t)s.n * p.heads + M - 1) / M);
+}
+__device__ __forceinline__ int kv_tiles(const Seq& s) { return max(1, (s.len + kN - 1) / kN); }
+
+// 16-byte pieces of LDS row r are stored at piece c ^ swz(r): a wave's reads down 8 rows (the
+// keys) and its transposing reads of 4 rows by 32 bytes (the values) both meet every bank once
+__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+
+__device__ const u32x4 g_zero16 = {0, 0, 0, 0};
+
+// 16 bytes a lane from global memory straight into LDS: lane l's bytes land at lds + 16 l. One
+// asm statement, so that the compiler does not wait for it before other reads of LDS; the
+// caller waits (wait_vm0) before the bytes are read
+__device__ __forceinline__ void lds_dma16(const void* g, void* lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)(uint8_t*)lds);
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(m0) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_vm0() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
+  asm volatile("" ::: "memory");
+}
+
+template <int M>
+struct __align__(16) AttendSmem {
+  uint8_t tile[2][kN * kRow * 2];  // two tiles of cached rows, bf16, swizzled pieces
+  uint16_t p[M * kPStride];        // softmax numerators of the tile [row][token]
+  float mx[M * 4];                 // [row][token group]: tile maxima; at the end the sums
+  int rowid[2][kN];                // cache rows of a tile's tokens, -1: none
+  int start[kMaxSeqs + 1];         // first tile of each sequence in the work
+  int scan[8];
+  int first;
+  uint8_t bad[kN];                 // tokens of the tile with a non-finite latent value
+};
+
+// The absorbed attention. The work is a list of tiles: sequence by sequence, query row tile by
+// row tile (M rows: consecutive (token, head) pairs), kN cached tokens each. Every workgroup
+// computes the list's prefix sums itself and takes one equal contiguous share, so ragged
+// lengths load every CU alike. A row tile inside one share is finished there; one that was cut
+// leaves its running maximum, sum and fp32 outputs in the workspace for k_latent_merge.
+//
+// A tile: 64 rows of 576 bf16 in LDS, read once from memory for all M query rows and used twice.
+//   S^T = K Q^T   wave (tg, rg): tokens 16 tg .., rows (M / 2) rg ..: A = K (16-byte reads of
+//                 LDS), B = Q^T, which stays in registers
+//   maxima        over a lane's 4 tokens, the 4 lanes of a column, then the 4 token groups by LDS
+//   P             bf16, [row][token] in LDS (values at most 1; the sums stay fp32)
+//   O^T += V^T P^T   wave w: latent values 64 w .. 64 w + 63 of every row: A = V^T by transposing
+//                 LDS reads of the same tile, B = P^T
+// The next tile's loads are in flight throughout.
+template <int M, bool MX>
+__global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
+  constexpr int MB = M / 16;      // row blocks
+  constexpr int RB = MB / 2;      // row blocks of a wave's scores
+  constexpr int KS = kRow / 32;   // MFMA steps of a score: 18
+  __shared__ AttendSmem<M> sm;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tg = wave & 3, rg = wave >> 2, col = lane & 15, g = lane >> 4;
+
+  // ---- the work list
+  int mine = 0;
+  if (tid < p.seqs) {
+    const Seq s = seq_of(p, tid);
+    mine = row_tiles<M>(p, s) * kv_tiles(s);
+    if (s.bad && blockIdx.x == 0) record(p.err, MKMOE_LATENT_ERR_LENGTH, tid);
+  }
+  int inc = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(inc, d, 64);
+    if (lane >= d) inc += v;
+  }
+  if (lane == 63) sm.scan[wave] = inc;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int v = sm.scan[i];
+    if (i < wave) before += v;
+    total += v;
+  }
+  const int share = (total + kShares - 1) / kShares;
+  const int w0 = min((int64_t)blockIdx.x * share, (int64_t)total), w1 = min((int64_t)w0 + share, (int64_t)total);
+  const int from = before + inc - mine;
+  if (tid < p.seqs) {
+    sm.start[tid] = from;
+    if (w0 >= from && w0 < from + mine) sm.first = tid;
+    if (blockIdx.x == 0) p.plan[1 + tid] = from;
+  }
+  if (tid == 0 && blockIdx.x == 0) p.plan[0] = share;
+  if (w0 >= w1) return;
+  __syncthreads();
+
+  // ---- constant places in LDS
+  // keys: this lane's row of the wave's 16, pieces 4 ks + g
+  const int ktok = 16 * tg + col;
+  const uint32_t k_even = ktok * (2 * kRow) + ((g ^ swz(ktok)) << 4);
+  const uint32_t k_odd = ktok * (2 * kRow) + (((4 + g) ^ swz(ktok)) << 4);
+  // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16
+  const int vtok = 8 * g + (col >> 2);
+
+  int b = sm.first;
+  for (int w = w0; w < w1;) {
+    while (b + 1 < p.seqs && sm.start[b + 1] <= w) ++b;
+    const Seq s = seq_of(p, b);
+    const int kt = kv_tiles(s);
+    const int rt = (w - sm.start[b]) / kt, tile0 = (w - sm.start[b]) % kt;
+    const int tile1 = min(kt, tile0 + (w1 - w));
+    const int unit0 = w - tile0;
+    const int r0 = rt * M, nrows = min(M, s.n * p.heads - r0);
+    w += tile1 - tile0;
+
+    // each row's visible tokens: query token i of n sees len - n + 1 + i
+    const int base = s.len - s.n + 1;
+    const int lim_lo = max(0, base + r0 / p.heads), lim_hi = max(0, base + (r0 + nrows - 1) / p.heads);
+    const int tend = min(tile1, (lim_hi + kN - 1) / kN);
+    const int32_t* table = p.table + (int64_t)b * p.table_stride;
+
+    // ---- queries into registers
+    bf16x8 q[RB][KS];
+    int lim[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int r = (rg * RB + rb) * 16 + col;
+      const bool real = r < nrows;
+      const int i = real ? (r0 + r) / p.heads : 0, h = real ? (r0 + r) - i * p.heads : 0;
+      lim[rb] = real ? max(0, base + i) : 0;
+      const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)h * p.ql_hs + 8 * g;
+      const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)h * p.qp_hs + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint16_t* src = ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32);
+        q[rb][ks] = real ? *(const bf16x8*)src : bf16x8{};
+      }
+    }
+
+    float m[MB], l[RB];
+    f32x4 o[4][MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      m[i] = -kInf;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c][i] = f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < RB; ++i) l[i] = 0.0f;
+
+    // cache rows of tile t's tokens (threads 0 .. 63 of the workgroup): the page's table entry is
+    // requested early, and looked at when the row is needed; -1 where no token is visible
+    auto page_of = [&](int t) -> int {
+      const int tok = t * kN + tid;
+      return tok < lim_hi ? table[tok >> p.page_shift] : -1;
+    };
+    auto row_of = [&](int t, int pg) -> int {
+      const int tok = t * kN + tid;
+      if (tok >= lim_hi) return -1;
+      if (pg < 0 || (int64_t)pg >= p.pages) {
+        record(p.err, MKMOE_LATENT_ERR_PAGE, b);
+        return -1;
+      }
+      return (int)(((int64_t)pg << p.page_shift) + (tok & ((1 << p.page_shift) - 1)));
+    };
+    // bf16: 9 direct loads a thread move a tile
+    auto issue = [&](int buf) {
+      if constexpr (!MX) {
+#pragma unroll
+        for (int i = 0; i < 9; ++i) {
+          const int at = i * kThreads + tid, r = at / kChunks, c = at - r * kChunks;
+          const int row = sm.rowid[buf][r];
+          const uint8_t* src = row < 0 ? (const uint8_t*)&g_zero16
+                                       : p.cache + (int64_t)row * (2 * kRow) + ((c ^ swz(r)) << 4);
+          lds_dma16(src, sm.tile[buf] + (i * kThreads + wave * 64) * 16);
+        }
+      }
+    };
+    // MXFP8: 8 threads a row; codes 16 (8 i + j) .., i < 4, the row's scales, rope piece j
+    u32x4 mq[4], ms, mr;
+    bool mnone = true;
+    const int mrow = tid >> 3, mj = tid & 7;
+    auto fetch = [&](int buf) {
+      if constexpr (MX) {
+        const int row = sm.rowid[buf][mrow];
+        mnone = row < 0;  // (row 0 is read in its place, and not used)
+        const uint8_t* src = p.cache + (int64_t)max(row, 0) * kMxRow;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mq[i] = *(const u32x4*)(src + 16 * (8 * i + mj));
+        ms = *(const u32x4*)(src + kL);
+        mr = *(const u32x4*)(src + kL + kMxScales + 16 * mj);
+      }
+    };
+    auto unpack = [&](int buf) {
+      if constexpr (MX) {
+        uint8_t* row = sm.tile[buf] + mrow * (2 * kRow);
+        const int x = swz(mrow);
+        const uint32_t sw[4] = {ms.x, ms.y, ms.z, ms.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float sc = e8m0((sw[i] >> (8 * (mj >> 1))) & 0xffu);
+          const int c = 2 * (8 * i + mj);
+          const u32x4 zero = {0, 0, 0, 0};
+          *(u32x4*)(row + ((c ^ x) << 4)) = mnone ? zero : fp8x8(mq[i].x, mq[i].y, sc);
+          *(u32x4*)(row + (((c + 1) ^ x) << 4)) = mnone ? zero : fp8x8(mq[i].z, mq[i].w, sc);
+        }
+        *(u32x4*)(row + (((64 + mj) ^ x) << 4)) = mnone ? u32x4{0, 0, 0, 0} : mr;
+      }
+    };
+
+    // ---- the first tile
+    __syncthreads();  // the last row tile's reads of LDS are over
+    if (tid < kN) {
+      const int a = page_of(tile0), c = page_of(tile0 + 1);
+      sm.rowid[0][tid] = row_of(tile0, a);
+      sm.rowid[1][tid] = row_of(tile0 + 1, c);
+    }
+    __syncthreads();
+    if (tile0 < tend) {
+      issue(0);
+      fetch(0);
+      unpack(0);
+    }
+
+    for (int t = tile0; t < tend; ++t) {
+      const int buf = (t - tile0) & 1;
+      wait_vm0();
+      __syncthreads();
+      const bool more = t + 1 < tend;
+      const int next_page = tid < kN ? page_of(t + 2) : -1;
+      if (more) {
+        issue(buf ^ 1);
+        fetch(buf ^ 1);
+      }
+      const uint8_t* tile = sm.tile[buf];
+
+      // tokens that only some of the rows see: their non-finite values must not reach the
+      // others through 0 * V. They are cleared, and the rows that see them become NaN below
+      const bool edge = lim_lo < lim_hi && (t + 1) * kN > lim_lo;
+      if (edge) {
+        for (int i = 0; i < kN / 8; ++i) {
+          const int r = wave * (kN / 8) + i;
+          u32x4* at = (u32x4*)(sm.tile[buf] + r * (2 * kRow) + ((lane ^ swz(r)) << 4));
+          u32x4 v = *at;
+          bool any = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if ((v[k] & 0x7f80u) == 0x7f80u) any = true, v[k] &= 0xffff0000u;
+            if ((v[k] & 0x7f800000u) == 0x7f800000u) any = true, v[k] &= 0x0000ffffu;
+          }
+          if (t * kN + r < lim_lo) any = false;
+          if (any) *at = v;
+          const bool some = __any(any);
+          if (lane == 0) sm.bad[r] = some;
+        }
+        __syncthreads();
+      }
+
+      // ---- scores
+      f32x4 sc[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) sc[rb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const bf16x8 a = *(const bf16x8*)(tile + (ks & 1 ? k_odd : k_even) + (ks >> 1) * 128);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) sc[rb] = mfma(a, q[rb][ks], sc[rb]);
+      }
+      const int tok0 = t * kN + 16 * tg + 4 * g;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float top = -kInf;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float v = sc[rb][k] * p.scale2;
+          if (edge && sm.bad[16 * tg + 4 * g + k]) v = __builtin_nanf("");
+          v = tok0 + k < lim[rb] ? v : -kInf;
+          sc[rb][k] = v;
+          top = fmaxf(top, v);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (g == 0) sm.mx[((rg * RB + rb) * 16 + col) * 4 + tg] = top;
+      }
+      __syncthreads();
+
+      // ---- running maxima of every row; numerators of this wave's rows
+      float alpha[MB], mu[MB];
+      bool same = true;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const f32x4 v = *(const f32x4*)(sm.mx + (16 * i + col) * 4);
+        const float mn = fmaxf(m[i], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+        mu[i] = mn == -kInf ? 0.0f : mn;
+        alpha[i] = __builtin_amdgcn_exp2f(m[i] - mu[i]);
+        same = same && mn == m[i];
+        m[i] = mn;
+      }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float mr_ = mu[rb], al = alpha[rb];
+        if (rg == 1) mr_ = mu[RB + rb], al = alpha[RB + rb];
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[rb][k] - mr_);
+        l[rb] = l[rb] * al + ((e[0] + e[1]) + (e[2] + e[3]));
+        *(u32x2*)(sm.p + ((rg * RB + rb) * 16 + col) * kPStride + 16 * tg + 4 * g) =
+            u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
+      }
+      if (!__all(same)) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c][i] *= alpha[i];
+      }
+      __syncthreads();
+
+      // ---- outputs
+#pragma unroll
+      for (int ks = 0; ks < kN / 32; ++ks) {
+        bf16x8 pb[MB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) pb[i] = *(const bf16x8*)(sm.p + (16 * i + col) * kPStride + 32 * ks + 8 * g);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int piece = 8 * wave + 2 * c + ((lane & 3) >> 1);
+          i16x4 lo, hi;
+          {
+            const int r = 32 * ks + vtok;
+            lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (MKMOE_LDS i16x4*)(tile + r * (2 * kRow) + ((piece ^ swz(r)) << 4) + 8 * (lane & 1)));
+            hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (MKMOE_LDS i16x4*)(tile + (r + 4) * (2 * kRow) + ((piece ^ swz(r + 4)) << 4) + 8 * (lane & 1)));
+          }
+          struct { i16x4 a, b; } both = {lo, hi};
+          const bf16x8 a = __builtin_bit_cast(bf16x8, both);
+#pragma unroll
+          for (int i = 0; i < MB; ++i) o[c][i] = mfma(a, pb[i], o[c][i]);
+        }
+      }
+      if (more) unpack(buf ^ 1);
+      if (tid < kN) sm.rowid[buf][tid] = row_of(t + 2, next_page);
+    }
+
+    // ---- the row sums, then the rows out
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      l[rb] += __shfl_xor(l[rb], 16, 64);
+      l[rb] += __shfl_xor(l[rb], 32, 64);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      if (g == 0) sm.mx[((rg * RB + rb) * 16 + col) * 4 + tg] = l[rb];
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == kt;
+    const int slot = 2 * blockIdx.x + (unit0 > w0 ? 1 : 0);
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const int r = 16 * i + col;
+      if (r >= nrows) continue;
+      const f32x4 v = *(const f32x4*)(sm.mx + r * 4);
+      const float sum = (v.x + v.y) + (v.z + v.w);
+      if (whole) {
+        const int qi = (r0 + r) / p.heads, h = (r0 + r) - qi * p.heads;
+        const bool none = base + qi <= 0;
+        const float inv = none ? 0.0f : 1.0f / sum;
+        uint16_t* dst = p.out + (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 64 * wave + 4 * g;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4 x = o[c][i] * inv;
+          *(u32x2*)(dst + 16 * c) = u32x2{pack_bf(x[0], x[1]), pack_bf(x[2], x[3])};
+        }
+        if (p.lse && wave == 0 && g == 0)
+          p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = none ? -kInf : (m[i] + log2f(sum)) * (1.0f / kLog2e);
+      } else {
+        float* dst = p.part_o + ((int64_t)slot * M + r) * kL + 64 * wave + 4 * g;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) *(f32x4*)(dst + 16 * c) = o[c][i];
+        if (wave == 0 && g == 0) {
+          p.part_ml[((int64_t)slot * M + r) * 2] = m[i];
+          p.part_ml[((int64_t)slot * M + r) * 2 + 1] = sum;
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- merge
+// 128 threads a query row: the parts of the row's tile, in order, scaled to their common maximum
+template <int M>
+__global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
+  __shared__ int s_b[2];
+  const int half = threadIdx.x >> 7, th = threadIdx.x & 127;
+  const int64_t row = (int64_t)blockIdx.x * 2 + half;
+  const bool in = row < (int64_t)p.tokens * p.heads;
+  const int t = in ? (int)(row / p.heads) : 0;
+  int b;
+  if (p.starts) {
+    if (th == 0) s_b[half] = -1;
+    __syncthreads();
+    for (int i = th; i < p.seqs; i += 128) {
+      const Seq s = seq_of(p, i);
+      if (t >= s.t0 && t < s.t0 + s.n) s_b[half] = i;
+    }
+    __syncthreads();
+    b = s_b[half];
+  } else {
+    b = t / p.n;
+  }
+  if (!in || b < 0) return;  // (a row behind the last sequence stays as it was)
+  const Seq s = seq_of(p, b);
+  const int kt = kv_tiles(s), h = (int)(row - (int64_t)t * p.heads);
+  const int r = (t - s.t0) * p.heads + h, rt = r / M, rr = r % M;
+  const int share = p.plan[0], u0 = p.plan[1 + b] + rt * kt, u1 = u0 + kt - 1;
+  const int g0 = u0 / share, g1 = u1 / share;
+  if (g0 == g1) return;  // finished where it was computed
+  auto slot_of = [&](int gi) { return (int64_t)(2 * gi + (u0 > gi * share ? 1 : 0)) * M + rr; };
+  float top = -kInf;
+  for (int gi = g0; gi <= g1; ++gi) top = fmaxf(top, p.part_ml[slot_of(gi) * 2]);
+  const float mu = top == -kInf ? 0.0f : top;
+  float sum = 0.0f;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int gi = g0; gi <= g1; ++gi) {
+    const int64_t at = slot_of(gi);
+    const float wgt = __builtin_amdgcn_exp2f(p.part_ml[at * 2] - mu);
+    sum += wgt * p.part_ml[at * 2 + 1];
+    acc += wgt * *(const f32x4*)(p.part_o + at * kL + 4 * th);
+  }
+  const bool none = s.len - s.n + 1 + (t - s.t0) <= 0;
+  const float inv = none ? 0.0f : 1.0f / sum;
+  acc *= inv;
+  *(u32x2*)(p.out + (int64_t)t * p.o_ts + (int64_t)h * p.o_hs + 4 * th) = u32x2{pack_bf(acc[0], acc[1]), pack_bf(acc[2], acc[3])};
+  if (p.lse && th == 0) p.lse[row] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
+}
+
+// ---------------------------------------------------------------- the heads' products
+struct ProjectParams {
+  const uint16_t* x;
+  const uint16_t* w;  // [heads][256][512]: rows 0 .. 127 W_UK, 128 .. 255 W_UV
+  uint16_t* y;
+  int64_t x_ts, x_hs, y_ts, y_hs;
+  int tokens;
+};
+
+// y[t, h, l] = sum_d x[t, h, d] W_UK[h, d, l]: a workgroup a head, 64 columns and 64 tokens; the
+// 128 x 64 weight block in LDS, its transposing reads the A operand, 16 tokens a wave
+__global__ __launch_bounds__(256) void k_latent_absorb(ProjectParams p) {
+  constexpr int S = 144;  // bytes an LDS row of 64 values: 16 past the banks' period
+  __shared__ __align__(16) uint8_t wl[kNope * S];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  const int c0 = blockIdx.x * 64, h = blockIdx.y, t = blockIdx.z * 64 + 16 * wave + col;
+  const uint16_t* w = p.w + (int64_t)h * (kNope + kV) * kL + c0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = i * 256 + tid, d = at >> 3, c = at & 7;
+    *(u32x4*)(wl + d * S + 16 * c) = *(const u32x4*)(w + (int64_t)d * kL + 8 * c);
+  }
+  const bool real = t < p.tokens;
+  const uint16_t* x = p.x + (int64_t)(real ? t : 0) * p.x_ts + (int64_t)h * p.x_hs + 8 * g;
+  bf16x8 xb[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) xb[ks] = real ? *(const bf16x8*)(x + 32 * ks) : bf16x8{};
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const uint8_t* at = wl + (32 * ks + 8 * g + (col >> 2)) * S + 32 * c + 8 * (lane & 3);
+      struct { i16x4 a, b; } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)at),
+                                     __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(at + 4 * S))};
+      acc = mfma(__builtin_bit_cast(bf16x8, both), xb[ks], acc);
+    }
+    if (real)
+      *(u32x2*)(p.y + (int64_t)t * p.y_ts + (int64_t)h * p.y_hs + c0 + 16 * c + 4 * g) =
+          u32x2{pack_bf(acc[0], acc[1]), pack_bf(acc[2], acc[3])};
+  }
+}
+
+// y[t, h, j] = sum_l x[t, h, l] W_UV[h, j, l]: a workgroup a head, 16 columns and 64 tokens, 16
+// tokens a wave; both operands are contiguous along l and come straight from memory
+__global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int j0 = blockIdx.x * 16, h = blockIdx.y, t = blockIdx.z * 64 + 16 * wave + col;
+  if (blockIdx.z * 64 + 16 * wave >= p.tokens) return;
+  const bool real = t < p.tokens;
+  const uint16_t* w = p.w + ((int64_t)h * (kNope + kV) + kNope + j0 + col) * kL + 8 * g;
+  const uint16_t* x = p.x + (int64_t)(real ? t : 0) * p.x_ts + (int64_t)h * p.x_hs + 8 * g;
+  f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int ks = 0; ks < kL / 32; ++ks) {
+    const bf16x8 b = real ? *(const bf16x8*)(x + 32 * ks) : bf16x8{};
+    acc = mfma(*(const bf16x8*)(w + 32 * ks), b, acc);
+  }
+  if (real)
+    *(u32x2*)(p.y + (int64_t)t * p.y_ts + (int64_t)h * p.y_hs + j0 + 4 * g) =
+        u32x2{pack_bf(acc[0], acc[1]), pack_bf(acc[2], acc[3])};
+}
+
+// ---------------------------------------------------------------- host
+constexpr size_t kCtlBytes = 256;
+constexpr size_t kPlanBytes = (1 + kMaxSeqs + 63) / 64 * 64 * 4;
+constexpr size_t kMlBytes = (size_t)2 * kShares * kRowsMax * 2 * 4;
+constexpr size_t kPartBytes = (size_t)2 * kShares * kRowsMax * kL * 4;
+constexpr size_t kWsBytes = kCtlBytes + kPlanBytes + kMlBytes + kPartBytes;
+constexpr int64_t kMaxRows = (int64_t)1 << 24;  // query rows (tokens x heads) and tokens a call
+
+inline bool aligned(const void* q, size_t a) { return ((uintptr_t)q % a) == 0; }
+inline bool strides8(int64_t a, int64_t b) { return a >= 0 && b >= 0 && a % 8 == 0 && b % 8 == 0; }
+
+inline int check_ws(const void* ws, size_t bytes) {
+  if (!ws) return MKMOE_ERR_NULL;
+  if (!aligned(ws, 256)) return MKMOE_ERR_ALIGN;
+  return bytes < kWsBytes ? MKMOE_ERR_WORKSPACE : MKMOE_OK;
+}
+inline int check_cache(const mkmoe_latent_cache& c) {
+  if (!c.data) return MKMOE_ERR_NULL;
+  if (!aligned(c.data, 16)) return MKMOE_ERR_ALIGN;
+  if (c.fmt != MKMOE_LATENT_BF16 && c.fmt != MKMOE_LATENT_MXFP8) return MKMOE_ERR_ARG;
+  if (c.page_size < 1 || c.page_size > 1024 || (c.page_size & (c.page_size - 1)) != 0) return MKMOE_ERR_ARG;
+  if (c.pages < 1 || c.pages > (int64_t)0x7fffffff / c.page_size) return MKMOE_ERR_ARG;
+  return MKMOE_OK;
+}
+inline int launched() { return hipGetLastError() == hipSuccess ? MKMOE_OK : MKMOE_ERR_LAUNCH; }
+
+template <int M, bool MX>
+int attend(const AttendParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((k_latent_attend<M, MX>), dim3(kShares), dim3(kThreads), 0, st, p);
+  if (int rc = launched()) return rc;
+  const int64_t rows = (int64_t)p.tokens * p.heads;
+  hipLaunchKernelGGL(k_latent_merge<M>, dim3((unsigned)((rows + 1) / 2)), dim3(256), 0, st, p);
+  return launched();
+}
+
+}  // namespace mkmoe_latent
+
+extern "C" {
+
+int mkmoe_latent_workspace_bytes(size_t* bytes) {
+  if (!bytes) return MKMOE_ERR_NULL;
+  *bytes = mkmoe_latent::kWsBytes;
+  return MKMOE_OK;
+}
+
+int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_bytes, void* stream) {
+  using namespace mkmoe_latent;
+  if (!io) return MKMOE_ERR_NULL;
+  if (int rc = check_ws(ws, ws_bytes)) return rc;
+  if (int rc = check_cache(io->cache)) return rc;
+  if (!io->kv || !io->cos_sin || !io->positions || !io->slots) return MKMOE_ERR_NULL;
+  if (io->tokens < 0 || io->tokens > kMaxRows) return MKMOE_ERR_ROWS;
+  if (io->heads < 0 || io->heads > MKMOE_LATENT_MAX_HEADS || (io->rope & ~1) != 0 ||
+      (io->index_bytes != 4 && io->index_bytes != 8) || io->cos_sin_rows < 1 || !(io->norm_eps >= 0.0f) ||
+      !isfinite(io->norm_eps) || io->kv_stride < kRow)
+    return MKMOE_ERR_ARG;
+  if (io->heads > 0 && (!io->q_pe || !io->q_out)) return MKMOE_ERR_NULL;
+  if (!aligned(io->kv, 16) || !aligned(io->norm_w, 16) || !aligned(io->cos_sin, 16) || io->kv_stride % 8 ||
+      !aligned(io->positions, io->index_bytes) || !aligned(io->slots, io->index_bytes))
+    return MKMOE_ERR_ALIGN;
+  if (io->heads > 0 && (!aligned(io->q_pe, 16) || !aligned(io->q_out, 16) ||
+                        !strides8(io->q_token_stride, io->q_head_stride) ||
+                        !strides8(io->out_token_stride, io->out_head_stride)))
+    return MKMOE_ERR_ALIGN;
+  if (io->tokens == 0) return MKMOE_OK;
+  AppendParams p;
+  p.kv = (const uint16_t*)io->kv;
+  p.norm_w = (const uint16_t*)io->norm_w;
+  p.cos_sin = (const float*)io->cos_sin;
+  p.positions = io->positions;
+  p.slots = io->slots;
+  p.q = (const uint16_t*)io->q_pe;
+  p.q_out = (uint16_t*)io->q_out;
+  p.cache = (uint8_t*)io->cache.data;
+  p.err = (int32_t*)ws;
+  p.kv_stride = io->kv_stride;
+  p.q_ts = io->q_token_stride;
+  p.q_hs = io->q_head_stride;
+  p.o_ts = io->out_token_stride;
+  p.o_hs = io->out_head_stride;
+  p.rows = io->cache.pages * io->cache.page_size;
+  p.table_rows = io->cos_sin_rows;
+  p.tokens = io->tokens;
+  p.heads = io->heads;
+  p.half = io->rope == MKMOE_ROPE_HALF;
+  p.wide = io->index_bytes == 8;
+  p.kv_blocks = (io->tokens + 3) / 4;
+  p.eps = io->norm_eps;
+  const unsigned blocks = (unsigned)(p.kv_blocks + ((int64_t)io->tokens * io->heads + 31) / 32);
+  hipStream_t st = (hipStream_t)stream;
+  if (io->cache.fmt == MKMOE_LATENT_MXFP8)
+    hipLaunchKernelGGL(k_latent_append<true>, dim3(blocks), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL(k_latent_append<false>, dim3(blocks), dim3(256), 0, st, p);
+  return launched();
+}
+
+int mkmoe_latent_rows(const mkmoe_latent_cache* cache, const void* slots, int32_t index_bytes, int32_t tokens, void* out,
+                      void* ws, size_t ws_bytes, void* stream) {
+  using namespace mkmoe_latent;
+  if (!cache || !slots || !out) return MKMOE_ERR_NULL;
+  if (int rc = check_ws(ws, ws_bytes)) return rc;
+  if (int rc = check_cache(*cache)) return rc;
+  if (tokens < 0 || tokens > kMaxRows) return MKMOE_ERR_ROWS;
+  if (index_bytes != 4 && index_bytes != 8) return MKMOE_ERR_ARG;
+  if (!aligned(slots, index_bytes) || !aligned(out, 16)) return MKMOE_ERR_ALIGN;
+  if (tokens == 0) return MKMOE_OK;
+  RowsParams p{(const uint8_t*)cache->data, slots, (uint16_t*)out, (int32_t*)ws, cache->pages * cache->page_size, tokens,
+               index_bytes == 8};
+  const dim3 grid((tokens + 3) / 4);
+  if (cache->fmt == MKMOE_LATENT_MXFP8)
+    hipLaunchKernelGGL(k_latent_rows<true>, grid, dim3(256), 0, (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL(k_latent_rows<false>, grid, dim3(256), 0, (hipStream_t)stream, p);
+  return launched();
+}
+
+int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_bytes, void* stream) {
+  using namespace mkmoe_latent;
+  if (!io) return MKMOE_ERR_NULL;
+  if (int rc = check_ws(ws, ws_bytes)) return rc;
+  if (int rc = check_cache(io->cache)) return rc;
+  if (!io->q_lat || !io->q_pe || !io->table || !io->lens || !io->out) return MKMOE_ERR_NULL;
+  if (io->seqs < 1 || io->seqs > kMaxSeqs || io->tokens < 0) return MKMOE_ERR_ROWS;
+  if (io->heads < 1 || io->heads > MKMOE_LATENT_MAX_HEADS) return MKMOE_ERR_ARG;
+  if ((int64_t)io->tokens * io->heads > kMaxRows) return MKMOE_ERR_ROWS;
+  if (!io->q_starts && io->tokens % io->seqs != 0) return MKMOE_ERR_ROWS;
+  if (!isfinite(io->scale) || io->max_pages < 1 || io->table_stride < io->max_pages) return MKMOE_ERR_ARG;
+  const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
+  if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
+  // the work list's tiles are counted in 32 bits
+  const int64_t tiles = ((int64_t)io->tokens * io->heads / 32 + io->seqs) * ((max_len + kN - 1) / kN);
+  if (tiles > 0x3fffffff) return MKMOE_ERR_ARG;
+  const void* wide[] = {io->q_lat, io->q_pe, io->out};
+  for (const void* q : wide)
+    if (!aligned(q, 16)) return MKMOE_ERR_ALIGN;
+  const void* narrow[] = {io->table, io->lens, io->q_starts, io->lse};
+  for (const void* q : narrow)
+    if (!aligned(q, 4)) return MKMOE_ERR_ALIGN;
+  if (!strides8(io->ql_token_stride, io->ql_head_stride) || !strides8(io->qp_token_stride, io->qp_head_stride) ||
+      !strides8(io->out_token_stride, io->out_head_stride))
+    return MKMOE_ERR_ALIGN;
+  if (io->tokens == 0) return MKMOE_OK;
+  AttendParams p;
+  p.ql = (const uint16_t*)io->q_lat;
+  p.qp = (const uint16_t*)io->q_pe;
+  p.cache = (const uint8_t*)io->cache.data;
+  p.table = io->table;
+  p.lens = io->lens;
+  p.starts = io->q_starts;
+  p.out = (uint16_t*)io->out;
+  p.lse = io->lse;
+  uint8_t* at = (uint8_t*)ws;
+  p.err = (int32_t*)at;
+  p.plan = (int32_t*)(at += kCtlBytes);
+  p.part_ml = (float*)(at += kPlanBytes);
+  p.part_o = (float*)(at += kMlBytes);
+  p.ql_ts = io->ql_token_stride;
+  p.ql_hs = io->ql_head_stride;
+  p.qp_ts = io->qp_token_stride;
+  p.qp_hs = io->qp_head_stride;
+  p.o_ts = io->out_token_stride;
+  p.o_hs = io->out_head_stride;
+  p.table_stride = io->table_stride;
+  p.pages = io->cache.pages;
+  p.seqs = io->seqs;
+  p.tokens = io->tokens;
+  p.heads = io->heads;
+  p.n = io->q_starts ? 0 : io->tokens / io->seqs;
+  p.max_len = (int)max_len;
+  p.page_shift = __builtin_ctz((unsigned)io->cache.page_size);
+  p.scale2 = io->scale * kLog2e;
+  hipStream_t st = (hipStream_t)stream;
+  const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8;
+  // 32 query rows a tile where a sequence has no more of them on average, else 64
+  const bool small = (int64_t)io->tokens * io->heads <= (int64_t)32 * io->seqs;
+  if (small) return mx ? attend<32, true>(p, st) : attend<32, false>(p, st);
+  return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
+}
+
+int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream) {
+  using namespace mkmoe_latent;
+  if (!io || !io->x || !io->w || !io->y) return MKMOE_ERR_NULL;
+  if (io->tokens < 0 || io->tokens > (1 << 20)) return MKMOE_ERR_ROWS;
+  if (io->heads < 1 || io->heads > MKMOE_LATENT_MAX_HEADS || (io->expand & ~1) != 0) return MKMOE_ERR_ARG;
+  if (!aligned(io->x, 16) || !aligned(io->w, 16) || !aligned(io->y, 16) ||
+      !strides8(io->x_token_stride, io->x_head_stride) || !strides8(io->y_token_stride, io->y_head_stride))
+    return MKMOE_ERR_ALIGN;
+  if (io->tokens == 0) return MKMOE_OK;
+  ProjectParams p{(const uint16_t*)io->x, (const uint16_t*)io->w, (uint16_t*)io->y, io->x_token_stride,
+                  io->x_head_stride, io->y_token_stride, io->y_head_stride, io->tokens};
+  const unsigned tb = (io->tokens + 63) / 64;
+  if (io->expand)
+    hipLaunchKernelGGL(k_latent_expand, dim3(kV / 16, io->heads, tb), dim3(256), 0, (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL(k_latent_absorb, dim3(kL / 64, io->heads, tb), dim3(256), 0, (hipStream_t)stream, p);
+  return launched();
+}
+
+int mkmoe_latent_read_errors(const void* ws, int32_t* words, int32_t n, void* stream) {
+  if (!ws || !words) return MKMOE_ERR_NULL;
+  if (n < 1 || n > MKMOE_LATENT_ERRW_WORDS) return MKMOE_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  if (hipMemcpyAsync(words, ws, (size_t)n * 4, hipMemcpyDeviceToHost, st) != hipSuccess) return MKMOE_ERR_HIP;
+  return hipStreamSynchronize(st) == hipSuccess ? MKMOE_OK : MKMOE_ERR_HIP;
+}
+
+}  // extern "C"

@@ -53,6 +53,18 @@ REGIONS = {
 }
 STAGES = {1: "norm", 2: "router + quantize", 3: "route", 4: "gate_up (routed + shared)", 5: "down (shared + routed) + combine", 6: "quantize the intermediates"}
 
+# latent attention (the section of include/mkmoe.h)
+LATENT_DIM, LATENT_ROPE, LATENT_NOPE, LATENT_V, LATENT_MX_ROW = 512, 64, 128, 128, 656
+LATENT_MAX_HEADS, LATENT_MAX_SEQS = 128, 512
+LATENT_BF16, LATENT_MXFP8 = 1, 2
+LATENT_ERRW_WORDS = 4
+LATENT_ERRORS = {
+    1: "a slot outside the cache, at token",
+    2: "a position outside cos_sin, at token",
+    3: "a length or query start outside its bounds, at sequence",
+    4: "a page outside the cache, at sequence",
+}
+
 # every symbol include/mkmoe.h and include/mkmoe_seam.h declare
 EXPORTS = (
     "mkmoe_abi_version",
@@ -69,6 +81,12 @@ EXPORTS = (
     "mkmoe_seam_workspace_bytes",
     "mkmoe_seam_forward",
     "mkmoe_seam_gate",
+    "mkmoe_latent_workspace_bytes",
+    "mkmoe_latent_append",
+    "mkmoe_latent_rows",
+    "mkmoe_latent_attend",
+    "mkmoe_latent_project",
+    "mkmoe_latent_read_errors",
 )
 # every symbol include/mkmoe_testing.h declares (libmkmoe_testing.so)
 TESTING_EXPORTS = (
@@ -144,6 +162,62 @@ class SeamIO(ctypes.Structure):
     ]  # fmt: skip
 
 
+class LatentCache(ctypes.Structure):
+    """mkmoe_latent_cache of include/mkmoe.h."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("fmt", ctypes.c_int32),
+    ]
+
+
+class LatentAppendIO(ctypes.Structure):
+    """mkmoe_latent_append_io of include/mkmoe.h."""
+
+    _fields_ = (
+        [("cache", LatentCache)]
+        + [(n, ctypes.c_int32) for n in ("tokens", "heads", "rope", "index_bytes")]
+        + [
+            (n, ctypes.c_int64)
+            for n in (
+                "cos_sin_rows", "kv_stride", "q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride",
+            )
+        ]
+        + [(n, ctypes.c_void_p) for n in ("kv", "norm_w", "cos_sin", "positions", "slots", "q_pe", "q_out")]
+        + [("norm_eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+    )  # fmt: skip
+
+
+class LatentAttendIO(ctypes.Structure):
+    """mkmoe_latent_attend_io of include/mkmoe.h."""
+
+    _fields_ = (
+        [("cache", LatentCache)]
+        + [(n, ctypes.c_int32) for n in ("seqs", "tokens", "heads", "max_pages")]
+        + [
+            (n, ctypes.c_int64)
+            for n in (
+                "table_stride", "ql_token_stride", "ql_head_stride", "qp_token_stride", "qp_head_stride",
+                "out_token_stride", "out_head_stride",
+            )
+        ]
+        + [(n, ctypes.c_void_p) for n in ("q_lat", "q_pe", "table", "lens", "q_starts", "out", "lse")]
+        + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+    )  # fmt: skip
+
+
+class LatentProjectIO(ctypes.Structure):
+    """mkmoe_latent_project_io of include/mkmoe.h."""
+
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("tokens", "heads", "expand", "reserved")]
+        + [(n, ctypes.c_int64) for n in ("x_token_stride", "x_head_stride", "y_token_stride", "y_head_stride")]
+        + [(n, ctypes.c_void_p) for n in ("x", "w", "y")]
+    )
+
+
 SEAM_HC = 4
 SEAM_MIX = 24
 SEAM_HIDDEN = 5120
@@ -190,6 +264,12 @@ def lib() -> ctypes.CDLL:
         L.mkmoe_seam_workspace_bytes.argtypes = [i32, i32, ctypes.POINTER(sz)]
         L.mkmoe_seam_forward.argtypes = [ctypes.POINTER(SeamIO), vp, sz, vp]
         L.mkmoe_seam_gate.argtypes = [ctypes.POINTER(SeamIO), vp, sz, vp]
+        L.mkmoe_latent_workspace_bytes.argtypes = [ctypes.POINTER(sz)]
+        L.mkmoe_latent_append.argtypes = [ctypes.POINTER(LatentAppendIO), vp, sz, vp]
+        L.mkmoe_latent_rows.argtypes = [ctypes.POINTER(LatentCache), vp, i32, i32, vp, vp, sz, vp]
+        L.mkmoe_latent_attend.argtypes = [ctypes.POINTER(LatentAttendIO), vp, sz, vp]
+        L.mkmoe_latent_project.argtypes = [ctypes.POINTER(LatentProjectIO), vp]
+        L.mkmoe_latent_read_errors.argtypes = [vp, ctypes.POINTER(i32), i32, vp]
         if L.mkmoe_abi_version() != ABI_VERSION:
             raise RuntimeError(
                 f"{LIB_PATH} has ABI {L.mkmoe_abi_version()}, this binding wants {ABI_VERSION}: rebuild it"

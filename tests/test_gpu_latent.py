@@ -1,0 +1,525 @@
+"""Latent attention's kernels (``sgl_amd_mono.moe.latent``) against a plain 64-bit form
+(``latent_ref``), each value within the bound that the kernels' roundings allow."""
+
+import pytest
+import torch
+
+import latent_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+SCALE = 192**-0.5
+NAN, INF = float("nan"), float("inf")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda").to(BF)
+
+
+def _runner(heads, **kw):
+    from sgl_amd_mono.moe.latent import LatentRunner
+
+    return LatentRunner(heads, scale=SCALE, **kw)
+
+
+def _cos_sin(n):
+    a = torch.arange(n, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    return torch.cat([a.cos(), a.sin()], 1).float().cuda()
+
+
+def _tables(g, seqs, max_len, page, spare=3):
+    per = -(-max_len // page)
+    pages = seqs * per + spare
+    perm = torch.randperm(pages, generator=g, device="cuda").int()
+    return perm[: seqs * per].view(seqs, per).contiguous(), pages
+
+
+# ---------------------------------------------------------------- append and rows
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("rope", ["interleaved", "half"])
+@pytest.mark.parametrize("tokens,heads,page,index", [(1, 1, 1, torch.int64), (3, 5, 64, torch.int32), (77, 32, 16, torch.int64), (1021, 16, 2, torch.int64)])
+def test_append(fmt, rope, tokens, heads, page, index):
+    print(f"\nappend {fmt} {rope} tokens={tokens} heads={heads} page={page}", flush=True)
+    from sgl_amd_mono.moe.latent import cache_like
+
+    g = _gen(tokens + heads)
+    run = _runner(heads, rope=rope)
+    pages = -(-2 * tokens // page) + 1
+    cache = ref.random_cache(pages, page, fmt, g, "cuda")
+    before = cache.clone()
+    kv = _randn(g, tokens, 640)[:, 32:608]  # rows of a wider projection
+    kv[:, :512] *= 3.0
+    w = (1 + 0.1 * torch.randn(512, generator=g, device="cuda")).to(BF)
+    q = _randn(g, tokens, heads, 192)
+    cs = _cos_sin(4096)
+    pos = torch.randint(4096, (tokens,), generator=g, device="cuda").to(index)
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:tokens].to(index)
+    out = torch.empty(heads, tokens, 64, dtype=BF, device="cuda").transpose(0, 1)
+    run.append(cache, kv, w, cs, pos, slots, q_pe=q[..., 128:], q_out=out)
+    got = run.rows(cache, slots)
+    torch.cuda.synchronize()
+    run.raise_on_device_error()
+    flat, keep = cache.view(pages * page, -1), torch.ones(pages * page, dtype=torch.bool, device="cuda")
+    keep[slots.long()] = False
+    assert torch.equal(flat[keep], before.view(pages * page, -1)[keep])  # no other row was touched
+    stored = flat[slots.long()]
+    c = ref.norm(kv[:, :512], w, 1e-6)
+    cpos = cs[pos.long()]
+    pe, size = ref.rotate(kv[:, 512:].double(), cpos, rope == "half")
+    vals = ref.row_values(stored)
+    # fp32: 512 squares, their mean, the root, the division and two products
+    near = c.abs() * 540 * ref.U32
+    if fmt == "bf16":
+        ref.assert_within(vals[:, :512], c, c.abs() * ref.U16 + 2 * near, "latent")
+    else:
+        sc = torch.exp2(stored[:, 512:528].double() - 127)
+        top = c.view(tokens, 16, 32).abs().amax(-1) / 448
+        assert bool((top <= sc * (1 + 1e-4)).all()) and bool((top > sc / 2 * (1 - 1e-4)).all())
+        step = torch.maximum(c.abs() * 2.0**-4, (sc * 2.0**-10).repeat_interleave(32, 1))
+        ref.assert_within(vals[:, :512], c, step * (1 + 1e-4) + 2 * near, "latent")
+    ref.assert_within(vals[:, 512:], pe, pe.abs() * ref.U16 + 3 * ref.U32 * size, "rope part")
+    qr, qsize = ref.rotate(q[..., 128:].double(), cpos[:, None], rope == "half")
+    ref.assert_within(out, qr, qr.abs() * ref.U16 + 3 * ref.U32 * qsize, "query")
+    assert torch.equal(got.double(), vals)  # bf16 holds every row's values exactly
+    # the same rows again into an empty cache, the query in place, no norm
+    c2 = cache_like(pages, page, fmt)
+    q2 = q[..., 128:].contiguous()
+    assert run.append(c2, kv, None, cs, pos, slots, q_pe=q2, q_out=q2) is q2
+    assert torch.equal(q2, out)
+    raw = ref.row_values(c2.view(pages * page, -1)[slots.long()])[:, :512]
+    if fmt == "bf16":
+        assert torch.equal(raw, kv[:, :512].double())
+    else:
+        assert float(((raw - kv[:, :512].double()).abs() / kv[:, :512].double().abs().clamp_min(0.05)).max()) <= 2.0**-4
+
+
+def test_append_skips_padding_and_records_bad_indices():
+    from sgl_amd_mono.moe.latent import cache_like
+
+    g = _gen(5)
+    for fmt in ("bf16", "mxfp8"):
+        run = _runner(4)
+        cache = cache_like(4, 8, fmt)
+        kv, cs = _randn(g, 5, 576), _cos_sin(16)
+        q = _randn(g, 5, 4, 64)
+        pos = torch.tensor([1, 2, 3, 4, 5], device="cuda")
+        slots = torch.tensor([3, -1, 31, -7, 0], device="cuda")
+        run.append(cache, kv, None, cs, pos, slots)
+        run.raise_on_device_error()
+        assert (cache.view(32, -1) != 0).any(1).nonzero().flatten().tolist() == [0, 3, 31]
+        # a slot behind the cache, a position behind the table
+        before = cache.clone()
+        out = torch.full((5, 4, 64), 7.0, dtype=BF, device="cuda")
+        run.append(cache, kv, None, cs, torch.tensor([1, 16, 3, -1, 5], device="cuda"),
+                   torch.tensor([32, 4, 1 << 40, 5, -1], device="cuda"), q_pe=q, q_out=out)  # fmt: skip
+        assert torch.equal(cache, before)
+        assert bool((out[1] == 7).all()) and bool((out[3] == 7).all()) and not bool((out[0] == 7).all())
+        with pytest.raises(RuntimeError, match="outside"):
+            run.raise_on_device_error()
+        run.clear_errors()
+        run.raise_on_device_error()
+        rows = run.rows(cache, torch.tensor([3, -1, 32], device="cuda"))
+        assert bool((rows[1:] == 0).all()) and bool((rows[0] != 0).any())
+        with pytest.raises(RuntimeError, match="a slot outside the cache, at token 2"):
+            run.raise_on_device_error()
+
+
+def test_append_extremes():
+    """Zero rows, the largest values, NaN and infinity in a row."""
+    from sgl_amd_mono.moe.latent import cache_like
+
+    run = _runner(1)
+    kv = torch.zeros(6, 576, dtype=BF, device="cuda")
+    kv[1, :512] = 1e-30
+    kv[2, :512] = 3e38  # its squares pass fp32: the norm's root is infinite, the row 0
+    kv[3, 5] = NAN
+    kv[4, 5] = INF
+    kv[5, 0] = 1.0  # one value among zeros
+    w = torch.ones(512, dtype=BF, device="cuda")
+    pos, slots = torch.zeros(6, dtype=torch.int64, device="cuda"), torch.arange(6, device="cuda")
+    for fmt in ("bf16", "mxfp8"):
+        cache = cache_like(6, 1, fmt)
+        run.append(cache, kv, w, _cos_sin(1), pos, slots)
+        got = run.rows(cache, slots).double().cpu()
+        assert bool((got[0] == 0).all()) and bool((got[2, :512] == 0).all())
+        assert float((got[1, :512] - 1e-27).abs().max()) <= 1e-27 * 2.0**-3
+        assert bool(got[3, :512].isnan().all())
+        assert bool(got[4, 5].isnan())
+        assert abs(float(got[5, 0]) - 512**0.5) <= 512**0.5 * 2.0**-4 and bool((got[5, 1:] == 0).all())
+
+
+# ---------------------------------------------------------------- attend
+def _attend_case(fmt, heads, page, lens, n=1, starts=None, seed=0, stride=0):
+    g = _gen(seed)
+    seqs, t = len(lens), (len(lens) * n if starts is None else starts[-1])
+    table, pages = _tables(g, seqs, max(max(lens), 1), page)
+    cache = ref.random_cache(pages, page, fmt, g, "cuda")
+    if stride:  # the head axis outermost, rows padded
+        q_lat = _randn(g, heads, t, 512 + stride)[..., :512].transpose(0, 1)
+        q_pe = _randn(g, t, heads, 128 + 64)[..., 128:]
+    else:
+        q_lat, q_pe = _randn(g, t, heads, 512), _randn(g, t, heads, 64)
+    return cache, q_lat, q_pe, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def _check_attend(run, fmt, heads, page, lens, n=1, starts=None, seed=0, stride=0):
+    cache, q_lat, q_pe, table, dl = _attend_case(fmt, heads, page, lens, n, starts, seed, stride)
+    t = q_lat.shape[0]
+    ds = None if starts is None else torch.tensor(starts, dtype=torch.int32, device="cuda")
+    lse = torch.empty(t, heads, device="cuda")
+    out = run.attend(cache, q_lat, q_pe, table, dl, q_starts=ds, lse=lse)
+    torch.cuda.synchronize()
+    run.raise_on_device_error()
+    r, rl, bound, lbound = ref.attend(cache, q_lat, q_pe, table, lens, SCALE, starts)
+    ref.assert_within(out, r, bound, "out")
+    ref.assert_within(lse, rl, lbound, "lse")
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads", [1, 16, 20, 32, 64, 128])
+def test_attend_heads(fmt, heads):
+    print(f"\nattend {fmt} heads={heads}", flush=True)
+    _check_attend(_runner(heads), fmt, heads, 16, [1, 63, 64, 65, 300, 0, 17], seed=heads, stride=8 * (heads % 3))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("page", [1, 2, 16, 64, 128, 1024])
+def test_attend_pages(fmt, page):
+    print(f"\nattend {fmt} page={page}", flush=True)
+    _check_attend(_runner(8), fmt, 8, page, [1500, 1, 129, 1024, 1023, 2], seed=page)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads,lens,n", [(16, [5, 64, 190, 0, 2], 2), (32, [66, 3, 400], 4), (64, [129, 1000], 5), (1, [200, 70], 65), (128, [4, 260], 3)])
+def test_attend_several_queries(fmt, heads, lens, n):
+    """A sequence's last n tokens, causal among them; sequences shorter than n leave rows empty."""
+    print(f"\nattend {fmt} heads={heads} n={n}", flush=True)
+    _check_attend(_runner(heads), fmt, heads, 16, lens, n, seed=n)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads", [8, 64])
+def test_attend_ragged_queries(fmt, heads):
+    """q_starts: sequences with no, one and many query tokens; rows behind the last stay."""
+    print(f"\nattend ragged {fmt} heads={heads}", flush=True)
+    run = _runner(heads)
+    starts, lens = [0, 3, 3, 4, 24, 24], [70, 50, 129, 40, 9]
+    _check_attend(run, fmt, heads, 16, lens, starts=starts, seed=3)
+    cache, q_lat, q_pe, table, dl = _attend_case(fmt, heads, 16, lens, starts=starts, seed=3)
+    wide = torch.full((30, heads, 512), 7.0, dtype=BF, device="cuda")
+    lse = torch.full((30, heads), 7.0, device="cuda")
+    pad = lambda q: torch.cat([q, torch.full((6, *q.shape[1:]), NAN, dtype=BF, device="cuda")])  # noqa: E731
+    ds = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    run.attend(cache, pad(q_lat), pad(q_pe), table, dl, q_starts=ds, out=wide, lse=lse)
+    exact = run.attend(cache, q_lat, q_pe, table, dl, q_starts=ds)
+    assert torch.equal(wide[:24], exact) and bool((wide[24:] == 7).all()) and bool((lse[24:] == 7).all())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads,lens", [(32, [20011]), (16, [9000, 1, 17000, 0, 300]), (64, [16385, 64])])
+def test_attend_long(fmt, heads, lens):
+    """Sequences cut into shares over the whole card, and joined."""
+    print(f"\nattend long {fmt} heads={heads} {lens}", flush=True)
+    _check_attend(_runner(heads), fmt, heads, 64, lens, seed=1)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_attend_many_sequences(fmt):
+    print(f"\nattend many {fmt}", flush=True)
+    lens = [(i * 37) % 131 for i in range(512)]
+    _check_attend(_runner(4), fmt, 4, 8, lens, seed=2)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_attend_scores_far_apart(fmt):
+    """Scores whose differences pass what exp holds, rising and falling along the sequence: the
+    running maximum moves at almost every tile, and the last tokens alone count (or the first)."""
+    run, g = _runner(2), _gen(9)
+    lens = [700]
+    cache, q_lat, q_pe, table, dl = _attend_case(fmt, 2, 1, lens, seed=4)
+    rows = table[0, :700].long()
+    ramp = torch.linspace(0, 30, 700, device="cuda")[:, None].expand(700, 64).to(BF)
+    flat = cache.view(-1, cache.shape[-1])
+    if fmt == "bf16":
+        flat[rows, 512:] = ramp
+    else:
+        flat[rows, 528:] = ramp.contiguous().view(torch.uint8)
+    q_pe[:, 0] = 30.0
+    q_pe[:, 1] = -30.0
+    out = run.attend(cache, q_lat, q_pe, table, dl)
+    r, _, bound, _ = ref.attend(cache, q_lat, q_pe, table, lens, SCALE)
+    ref.assert_within(out, r, bound, "out")
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads", [8, 32])
+def test_attend_garbage_out_of_sight(fmt, heads):
+    """NaN in every row behind a sequence's end, in the rest of its last page and in pages of no
+    sequence; page entries behind the length point anywhere."""
+    run = _runner(heads)
+    lens = [70, 1, 64, 333]
+    cache, q_lat, q_pe, table, dl = _attend_case(fmt, heads, 16, lens, seed=6)
+    want = run.attend(cache, q_lat, q_pe, table, dl).clone()
+    flat = cache.view(-1, cache.shape[-1])
+    used = torch.zeros(flat.shape[0], dtype=torch.bool, device="cuda")
+    for b, n in enumerate(lens):
+        at = torch.arange(n, device="cuda")
+        used[table[b].long()[at // 16] * 16 + at % 16] = True
+    flat[~used] = NAN if fmt == "bf16" else 0xFF
+    t2 = table.clone()
+    for b, n in enumerate(lens):
+        t2[b, -(-n // 16) :] = [-1, 1 << 30, -(1 << 31), 12345][b]
+    assert torch.equal(run.attend(cache, q_lat, q_pe, t2, dl), want)
+    run.raise_on_device_error()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads,n", [(8, 4), (32, 3), (64, 2)])
+def test_attend_non_finite_tokens_reach_only_their_queries(fmt, heads, n):
+    """A later query token's own row holds NaN or infinity: the earlier queries do not see it, and
+    their rows stay as they were; those that see it are not finite."""
+    run = _runner(heads)
+    lens = [70, 64 + n, 200]
+    cache, q_lat, q_pe, table, dl = _attend_case(fmt, heads, 16, lens, n, seed=8)
+    want = run.attend(cache, q_lat, q_pe, table, dl).clone()
+    flat = cache.view(-1, cache.shape[-1])
+    for b, length in enumerate(lens):  # the last token of each
+        at = int(table[b, (length - 1) // 16]) * 16 + (length - 1) % 16
+        if fmt == "bf16":
+            flat[at, 100 + b] = [NAN, INF, -INF][b]
+        else:
+            flat[at, 100 + b] = 0x7F
+    out = run.attend(cache, q_lat, q_pe, table, dl)
+    last = torch.arange(n - 1, 3 * n, n, device="cuda")
+    first = torch.ones(3 * n, dtype=torch.bool, device="cuda")
+    first[last] = False
+    assert torch.equal(out[first], want[first])
+    assert not bool(out[last].isfinite().all(-1).any())
+
+
+def test_attend_non_finite_query_stays_in_its_row():
+    run = _runner(16)
+    cache, q_lat, q_pe, table, dl = _attend_case("bf16", 16, 16, [100, 30], seed=11)
+    want = run.attend(cache, q_lat, q_pe, table, dl).clone()
+    q_lat[0, 3, 7], q_pe[1, 5, 2] = NAN, INF
+    out = run.attend(cache, q_lat, q_pe, table, dl)
+    hit = torch.zeros(2, 16, dtype=torch.bool, device="cuda")
+    hit[0, 3] = hit[1, 5] = True
+    assert torch.equal(out[~hit], want[~hit]) and not bool(out[hit].isfinite().any())
+
+
+def test_attend_records_bad_pages_lengths_and_starts():
+    """Pages outside the cache count as rows of zeros, lengths and starts are clamped; all recorded."""
+    run = _runner(8)
+    cache, q_lat, q_pe, table, dl = _attend_case("bf16", 8, 16, [40, 100], seed=12)
+    bad = table.clone()
+    bad[1, 2] = cache.shape[0]
+    run.attend(cache, q_lat, q_pe, bad, dl)
+    with pytest.raises(RuntimeError, match="a page outside the cache, at sequence 1"):
+        run.raise_on_device_error()
+    run.clear_errors()
+    full = table.shape[1] * 16
+    got = run.attend(cache, q_lat, q_pe, table, torch.tensor([full + 1, -5], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got, run.attend(cache, q_lat, q_pe, table, torch.tensor([full, 0], dtype=torch.int32, device="cuda")))
+    assert bool((got[1] == 0).all())
+    with pytest.raises(RuntimeError, match="a length or query start"):
+        run.raise_on_device_error()
+    run.clear_errors()
+    for starts in ([0, 3, 1], [-4, 1, 2], [0, 1, 1 << 30]):
+        run.attend(cache, q_lat, q_pe, table, dl, q_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+        with pytest.raises(RuntimeError, match="a length or query start"):
+            run.raise_on_device_error()
+        run.clear_errors()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_attend_offsets_past_32_bits(fmt):
+    """A cache of more than 2^32 bytes, its last pages in use."""
+    print(f"\nattend far {fmt}", flush=True)
+    run, g = _runner(16), _gen(13)
+    row = 1152 if fmt == "bf16" else 656
+    pages = (1 << 32) // (row * 64) + 20
+    small = ref.random_cache(12, 64, fmt, g, "cuda")
+    cache = torch.empty(pages, *small.shape[1:], dtype=small.dtype, device="cuda")
+    cache[-12:] = small
+    table = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)
+    q_lat, q_pe = _randn(g, 2, 16, 512), _randn(g, 2, 16, 64)
+    dl = torch.tensor([380, 200], dtype=torch.int32, device="cuda")
+    want = run.attend(small, q_lat, q_pe, table, dl)
+    assert torch.equal(run.attend(cache, q_lat, q_pe, table + (pages - 12), dl), want)
+    slots = torch.arange(5, device="cuda") + (pages * 64 - 5)
+    kv, cs, pos = _randn(g, 5, 576), _cos_sin(8), torch.arange(5, device="cuda")
+    run.append(cache, kv, None, cs, pos, slots)
+    run.append(small, kv, None, cs, pos, torch.arange(5, device="cuda") + (12 * 64 - 5))
+    assert torch.equal(cache[-12:], small)
+    assert torch.equal(run.rows(cache, slots), run.rows(small, slots - (pages - 12) * 64))
+
+
+def test_attend_same_bits_every_time():
+    run = _runner(32)
+    cache, q_lat, q_pe, table, dl = _attend_case("mxfp8", 32, 64, [5000, 64, 9000, 1], seed=14)
+    want = run.attend(cache, q_lat, q_pe, table, dl).clone()
+    for _ in range(5):
+        assert torch.equal(run.attend(cache, q_lat, q_pe, table, dl), want)
+
+
+# ---------------------------------------------------------------- the heads' products
+@pytest.mark.parametrize("tokens,heads", [(1, 1), (5, 16), (48, 32), (67, 3), (130, 64)])
+def test_absorb_and_expand(tokens, heads):
+    print(f"\nproject tokens={tokens} heads={heads}", flush=True)
+    from sgl_amd_mono.moe.latent import LatentWeights
+
+    g, run = _gen(tokens), _runner(heads)
+    w = LatentWeights(norm=_randn(g, 512), kv_b=_randn(g, heads * 256, 512))
+    wk = w.kv_b.double().view(heads, 256, 512)
+    q = _randn(g, tokens, heads, 192)[..., :128]
+    x, a = q.double().transpose(0, 1), q.double().abs().transpose(0, 1)
+    want = (x @ wk[:, :128]).transpose(0, 1)
+    size = (a @ wk[:, :128].abs()).transpose(0, 1)
+    ref.assert_within(run.absorb(w, q), want, want.abs() * ref.U16 + 130 * ref.U32 * size, "absorb")
+    o = _randn(g, heads, tokens, 512).transpose(0, 1)
+    out = torch.empty(heads, tokens, 128, dtype=BF, device="cuda").transpose(0, 1)
+    x, a = o.double().transpose(0, 1), o.double().abs().transpose(0, 1)
+    want = (x @ wk[:, 128:].transpose(1, 2)).transpose(0, 1)
+    size = (a @ wk[:, 128:].abs().transpose(1, 2)).transpose(0, 1)
+    assert run.expand(w, o, out=out) is out
+    ref.assert_within(out, want, want.abs() * ref.U16 + 514 * ref.U32 * size, "expand")
+
+
+# ---------------------------------------------------------------- together
+def _layer(fmt, heads, lens, n, page=16, seed=0):
+    from sgl_amd_mono.moe.latent import LatentWeights
+
+    g = _gen(seed)
+    seqs, t = len(lens), len(lens) * n
+    table, pages = _tables(g, seqs, max(lens), page)
+    at = torch.tensor([max(0, m - n + i) for m in lens for i in range(n)], device="cuda")
+    seq = torch.arange(seqs, device="cuda").repeat_interleave(n)
+    slots = table[seq, at // page].long() * page + at % page
+    slots[torch.tensor([m - n + i < 0 for m in lens for i in range(n)], device="cuda")] = -1
+    return dict(
+        w=LatentWeights(norm=(1 + 0.1 * torch.randn(512, generator=g, device="cuda")).to(BF),
+                        kv_b=(torch.randn(heads * 256, 512, generator=g, device="cuda") * 512**-0.5).to(BF)),
+        cache=ref.random_cache(pages, page, fmt, g, "cuda"), q=_randn(g, t, heads, 192), kv=_randn(g, t, 576),
+        cos_sin=_cos_sin(max(lens)), positions=at, slots=slots, table=table,
+        lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+    )  # fmt: skip
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads,lens,n", [(32, [1, 70, 400, 64], 1), (16, [90, 33], 4), (64, [5, 0, 130], 1), (128, [2000], 2)])
+def test_attention_is_its_parts(fmt, heads, lens, n):
+    """One call against append, absorb, attend and expand, bit for bit, and against 64 bits.
+
+    Five bf16 roundings lie on the way (absorbed query, rotated query, numerators, attended
+    latents, output), each off by at most 2^-8 of its value and 2^-8 / sqrt(3) in the mean square;
+    those of the query reach the output through scores of spread about 1. Their root mean square
+    is below sqrt(5 / 3) 2^-8 = 1.3 2^-8 of the output's; twice that is asked for."""
+    print(f"\nattention {fmt} heads={heads} lens={lens} n={n}", flush=True)
+    d = _layer(fmt, heads, lens, n, seed=heads)
+    run = _runner(heads)
+    c2 = d["cache"].clone()
+    out = run.attention(**d)
+    torch.cuda.synchronize()
+    run.raise_on_device_error()
+    w, q = d["w"], d["q"]
+    q_pe = run.append(c2, d["kv"], w.norm, d["cos_sin"], d["positions"], d["slots"], q_pe=q[..., 128:])
+    o = run.attend(c2, run.absorb(w, q[..., :128]), q_pe, d["table"], d["lens"])
+    assert torch.equal(c2, d["cache"])
+    assert torch.equal(run.expand(w, o), out)
+    wk = w.kv_b.double().view(heads, 256, 512)
+    ql = (q[..., :128].double().transpose(0, 1) @ wk[:, :128]).transpose(0, 1)
+    qr, _ = ref.rotate(q[..., 128:].double(), d["cos_sin"][d["positions"]][:, None], False)
+    want, *_ = ref.attend(d["cache"], ql, qr, d["table"], lens, SCALE)
+    want = (want.transpose(0, 1) @ wk[:, 128:].transpose(1, 2)).transpose(0, 1)
+    err = float((out.double() - want).norm() / want.norm())
+    assert err <= 2 * 1.3 * ref.U16, err
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_attention_in_a_graph(fmt):
+    """A captured step replayed with new lengths, rows and queries in its buffers, eager work on
+    the same runner in between; another stream."""
+    d, run = _layer(fmt, 32, [300, 70, 1, 4000], 1, seed=21), _runner(32)
+    first, base = d["lens"].clone(), d["cache"].clone()
+    out = torch.empty(4, 32, 128, dtype=BF, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        run.attention(**d, out=out)
+        with torch.cuda.graph(g, stream=s):
+            run.attention(**d, out=out)
+    torch.cuda.current_stream().wait_stream(s)
+    q0 = d["q"].clone()
+    for rep, lens in enumerate([[300, 70, 1, 4000], [10, 70, 1, 64], [300, 1, 0, 2500], [300, 70, 1, 4000]]):
+        d["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        d["q"].copy_(q0 * (1 + rep % 3))
+        d["cache"].copy_(base)
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        got, after = out.clone(), d["cache"].clone()
+        d["cache"].copy_(base)
+        want = run.attention(**d)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(after, d["cache"]), rep
+    d["lens"].copy_(first)
+    run.raise_on_device_error()
+
+
+def test_two_runners_on_two_streams():
+    a, b = _layer("bf16", 32, [5000, 80], 1, seed=31), _layer("mxfp8", 32, [300, 7000], 1, seed=32)
+    ra, rb = _runner(32), _runner(32)
+    wa, wb = ra.attention(**a).clone(), rb.attention(**b).clone()
+    torch.cuda.synchronize()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(4):
+        with torch.cuda.stream(sa):
+            got.append((ra.attention(**a), wa))
+        with torch.cuda.stream(sb):
+            got.append((rb.attention(**b), wb))
+    torch.cuda.synchronize()
+    for x, y in got:
+        assert torch.equal(x, y)
+
+
+def test_decode_steps_then_the_moe_block():
+    """Three decode steps of a layer's attention, each reading the rows that the last one stored,
+    then the MoE block on rows of its output, as a decode layer runs them."""
+    from oracle import gen
+    from sgl_amd_mono.moe.presets import PRESETS, workload_dict
+    from sgl_amd_mono.moe.runner import MoeRunner, MoeWeights
+
+    heads, seqs, page = 8, 3, 4
+    d, run = _layer("bf16", heads, [9, 5, 12], 1, page=page, seed=41), _runner(heads)
+    g = _gen(42)
+    lens = torch.tensor([6, 2, 9], dtype=torch.int32, device="cuda")
+    for step in range(3):
+        lens = lens + 1
+        at = (lens - 1).long()
+        slots = d["table"][torch.arange(seqs, device="cuda"), at // page].long() * page + at % page
+        q, kv = _randn(g, seqs, heads, 192), _randn(g, seqs, 576)
+        out = run.attention(d["w"], d["cache"], q, kv, d["cos_sin"], at, slots, d["table"], lens)
+    run.raise_on_device_error()
+    wk = d["w"].kv_b.double().view(heads, 256, 512)
+    ql = (q[..., :128].double().transpose(0, 1) @ wk[:, :128]).transpose(0, 1)
+    qr, _ = ref.rotate(q[..., 128:].double(), d["cos_sin"][at][:, None], False)
+    want, *_ = ref.attend(d["cache"], ql, qr, d["table"], lens.tolist(), SCALE)
+    want = (want.transpose(0, 1) @ wk[:, 128:].transpose(1, 2)).transpose(0, 1)
+    assert float((out.double() - want).norm() / want.norm()) <= 2 * 1.3 * ref.U16
+    p = workload_dict("cfg1_plumbing_fp8")
+    dense, ex = gen.make_dense(p, 0), gen.LazyExperts(p, 0)
+    st = {k: torch.stack([torch.as_tensor(ex.get(e)[i]) for e in range(p["experts"])]).cuda()
+          for i, k in enumerate(("w13", "w13_s", "w2", "w2_s"))}  # fmt: skip
+    mw = MoeWeights(**{k: v.cuda() for k, v in dense.items() if k != "norm"}, **st)
+    moe = MoeRunner(PRESETS["plumbing_fp8"])
+    x = out.reshape(seqs, heads * 128)
+    assert bool(moe.moe(mw, x).isfinite().all())
+    moe.raise_on_device_error()
