@@ -247,13 +247,16 @@ __global__ __launch_bounds__(256) void k_latent_rows(RowsParams p) {
 }
 
 // ---------------------------------------------------------------- attend
-constexpr int kN = 64;          // cached tokens a tile
+constexpr int kN = 32;          // cached tokens a tile
 constexpr int kShares = 256;    // equal shares of the work, a workgroup each: one a CU
 constexpr int kThreads = 512;   // 8 waves
 constexpr int kMaxSeqs = MKMOE_LATENT_MAX_SEQS;
-constexpr int kRowsMax = 64;    // query rows a tile holds at most
-constexpr int kChunks = kRow * 2 / 16;   // 16-byte pieces of a row in LDS: 72
-constexpr int kPStride = kN + 8;         // bf16 of a row of P: 144 bytes, rows on other banks
+constexpr int kRowsMax = 128;   // query rows a row tile holds at most
+constexpr int kPStride = kN + 16;  // bf16 of a row of P: 96 bytes, whose 16-byte reads meet every bank once
+constexpr int kTileBytes = kN * kRow * 2;  // a tile's rows in LDS, bf16
+constexpr int kRing = 4;        // bf16 cache: tiles in LDS, one in use and three on their way
+constexpr int kMxRing = 3;      // MXFP8: raw tiles on their way
+constexpr int kEnts = 8;        // tiles whose page entries are in LDS
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
 
@@ -272,8 +275,7 @@ struct AttendParams {
   float* part_ml;  // [2 kShares][M][2]
   int64_t ql_ts, ql_hs, qp_ts, qp_hs, o_ts, o_hs;
   int64_t table_stride;
-  int64_t pages;
-  int seqs, tokens, heads, n, max_len, page_shift;
+  int pages, seqs, tokens, heads, n, max_len, page_shift;
   float scale2;  // scale log2(e)
 };
 
@@ -307,35 +309,70 @@ __device__ __forceinline__ int row_tiles(const AttendParams& p, const Seq& s) {
 }
 __device__ __forceinline__ int kv_tiles(const Seq& s) { return max(1, (s.len + kN - 1) / kN); }
 
-// 16-byte pieces of LDS row r are stored at piece c ^ swz(r): a wave's reads down 8 rows (the
-// keys) and its transposing reads of 4 rows by 32 bytes (the values) both meet every bank once
-__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+// 16-byte pieces of LDS row r are stored at piece c ^ swz(r). The LDS has 64 banks (16 pieces);
+// rows are 72 pieces, so odd rows start half way round. A 16-byte read serves lanes 0 .. 3,
+// 12 .. 15, 20 .. 27 at once (and so on), which for the keys are 16 rows at pieces c and c ^ 1; a
+// transposing read serves 32 lanes, rows r .. r + 3 and r + 8 .. r + 11 by 32 bytes. With these
+// bits both meet every bank once (measured: no conflicts; with bits 0 .. 2 of r one of them has)
+__device__ __forceinline__ int swz(int r) { return ((r & 2) << 1) | ((r & 8) >> 2); }
 
-__device__ const u32x4 g_zero16 = {0, 0, 0, 0};
+// the row of tokens that are not there
+__device__ const u32x4 g_zero_row[kRow * 2 / 16] = {};
 
-// 16 bytes a lane from global memory straight into LDS: lane l's bytes land at lds + 16 l. One
-// asm statement, so that the compiler does not wait for it before other reads of LDS; the
-// caller waits (wait_vm0) before the bytes are read
-__device__ __forceinline__ void lds_dma16(const void* g, void* lds) {
-  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)(uint8_t*)lds);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(m0) : "memory", "m0");
+// Bytes from global memory straight into LDS: lane l's land at lds + 16 l (4 l). One asm
+// statement, so that the compiler does not wait for it before other reads of LDS; the caller
+// waits (wait_loads) before the bytes are read
+__device__ __forceinline__ uint32_t lds_at(const void* lds) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)(uint8_t*)const_cast<void*>(lds));
 }
-__device__ __forceinline__ void wait_vm0() {
+__device__ __forceinline__ void lds_dma16(const void* g, const void* lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_at(lds)) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_dma4(const void* g, const void* lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_at(lds)) : "memory", "m0");
+}
+// waits until at most N of the wave's loads are on their way (they complete in order)
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// the same for all of them, as the compiler's own wait: it would otherwise place a wait for the
+// queries' registers in the tile loop, which counts the tiles' loads too
+__device__ __forceinline__ void wait_queries() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0, expcnt 7 (none), lgkmcnt 15 (none)
   asm volatile("" ::: "memory");
 }
+// every wave's LDS accesses before it are done, and loads stay on their way across it
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
-template <int M>
-struct __align__(16) AttendSmem {
-  uint8_t tile[2][kN * kRow * 2];  // two tiles of cached rows, bf16, swizzled pieces
-  uint16_t p[M * kPStride];        // softmax numerators of the tile [row][token]
-  float mx[M * 4];                 // [row][token group]: tile maxima; at the end the sums
-  int rowid[2][kN];                // cache rows of a tile's tokens, -1: none
-  int start[kMaxSeqs + 1];         // first tile of each sequence in the work
+// v, which the compiler then forms anew where it is used: lane constants that it kept in
+// registers across the tile loop cost more there than the few instructions that make them
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// LDS at a byte offset
+template <class T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+  return *(MKMOE_LDS const T*)(uintptr_t)at;
+}
+
+template <int M, bool MX>
+struct __align__(128) AttendSmem {
+  uint8_t tile[MX ? 2 : kRing][kTileBytes];  // cached rows, bf16, swizzled pieces
+  uint8_t raw[MX ? kMxRing : 1][MX ? kN * kMxRow : 16];
+  uint16_t p[M * kPStride];    // softmax numerators of the tile [row][token]
+  float mx[M < 128 ? M * 2 : 4];  // [row][token group]: tile maxima
+  float al[M];                 // the tile's rescaling of each row; at the end the maxima
+  const uint8_t* addr[kN];     // the rows of the tile that is requested next
+  int ent[kEnts][kN];          // page entries of a tile's tokens
+  int start[kMaxSeqs];         // first tile of each sequence in the work
   int scan[8];
   int first;
-  uint8_t bad[kN];                 // tokens of the tile with a non-finite latent value
+  uint8_t bad[kN];             // tokens of the tile with a non-finite latent value
 };
 
 // The absorbed attention. The work is a list of tiles: sequence by sequence, query row tile by
@@ -344,22 +381,30 @@ struct __align__(16) AttendSmem {
 // lengths load every CU alike. A row tile inside one share is finished there; one that was cut
 // leaves its running maximum, sum and fp32 outputs in the workspace for k_latent_merge.
 //
-// A tile: 64 rows of 576 bf16 in LDS, read once from memory for all M query rows and used twice.
-//   S^T = K Q^T   wave (tg, rg): tokens 16 tg .., rows (M / 2) rg ..: A = K (16-byte reads of
-//                 LDS), B = Q^T, which stays in registers
-//   maxima        over a lane's 4 tokens, the 4 lanes of a column, then the 4 token groups by LDS
-//   P             bf16, [row][token] in LDS (values at most 1; the sums stay fp32)
+// A tile: 32 rows of 576 bf16 in LDS, read once from memory for all M query rows and used twice.
+//   S^T = K Q^T   wave (rg, tg): rows 16 rg .., 16 TB tokens from 16 TB tg: A = K (16-byte reads
+//                 of LDS), B = Q^T, which stays in registers
+//   P             exp2 of the scores less the rows' running maxima (joined over the token groups
+//                 in LDS), bf16, [row][token] in LDS; the sums stay fp32
 //   O^T += V^T P^T   wave w: latent values 64 w .. 64 w + 63 of every row: A = V^T by transposing
 //                 LDS reads of the same tile, B = P^T
-// The next tile's loads are in flight throughout.
+// bf16 rows go straight from memory to LDS, three tiles ahead; MXFP8 rows go there as they are,
+// and a pass of the workgroup turns the next tile's into bf16 (exact) beside the softmax.
 template <int M, bool MX>
 __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
-  constexpr int MB = M / 16;      // row blocks
-  constexpr int RB = MB / 2;      // row blocks of a wave's scores
-  constexpr int KS = kRow / 32;   // MFMA steps of a score: 18
-  __shared__ AttendSmem<M> sm;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tg = wave & 3, rg = wave >> 2, col = lane & 15, g = lane >> 4;
+  constexpr int MB = M / 16;             // row blocks
+  constexpr int TG = M < 128 ? 2 : 1;    // token groups
+  constexpr int TB = kN / 16 / TG;       // blocks of 16 tokens a wave scores
+  constexpr int KS = kRow / 32;          // MFMA steps of a score: 18
+  constexpr int G = M == 32 ? 18 : M == 64 ? 6 : 2;     // of them whose keys are read at once
+  constexpr int kPieces = MX ? kMxRow / 16 : kRow * 2 / 16;  // 16-byte pieces of a row on its way: 41 or 72
+  constexpr int kLoads = (kN * kPieces + 63) / 64;           // wave loads of a tile: 21 or 36
+  constexpr int kAhead = MX ? kMxRing : kRing - 1;           // tiles on their way
+  __shared__ AttendSmem<M, MX> sm;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int rg = wave % MB, tg = wave / MB;
+  const bool scores = wave < MB * TG;  // (M = 32: four waves score)
 
   // ---- the work list
   int mine = 0;
@@ -384,7 +429,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     total += v;
   }
   const int share = (total + kShares - 1) / kShares;
-  const int w0 = min((int64_t)blockIdx.x * share, (int64_t)total), w1 = min((int64_t)w0 + share, (int64_t)total);
+  const int w0 = (int)min((int64_t)blockIdx.x * share, (int64_t)total), w1 = (int)min((int64_t)w0 + share, (int64_t)total);
   const int from = before + inc - mine;
   if (tid < p.seqs) {
     sm.start[tid] = from;
@@ -395,20 +440,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   if (w0 >= w1) return;
   __syncthreads();
 
-  // ---- constant places in LDS
-  // keys: this lane's row of the wave's 16, pieces 4 ks + g
-  const int ktok = 16 * tg + col;
-  const uint32_t k_even = ktok * (2 * kRow) + ((g ^ swz(ktok)) << 4);
-  const uint32_t k_odd = ktok * (2 * kRow) + (((4 + g) ^ swz(ktok)) << 4);
-  // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16
-  const int vtok = 8 * g + (col >> 2);
+  const uint32_t tiles = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)sm.tile[0];
+  const uint32_t p_at = (uint32_t)(uintptr_t)(MKMOE_LDS uint16_t*)sm.p;
 
-  int b = sm.first;
+  int b = __builtin_amdgcn_readfirstlane(sm.first);
   for (int w = w0; w < w1;) {
-    while (b + 1 < p.seqs && sm.start[b + 1] <= w) ++b;
+    while (b + 1 < p.seqs && __builtin_amdgcn_readfirstlane(sm.start[b + 1]) <= w) ++b;
     const Seq s = seq_of(p, b);
-    const int kt = kv_tiles(s);
-    const int rt = (w - sm.start[b]) / kt, tile0 = (w - sm.start[b]) % kt;
+    const int kt = kv_tiles(s), at = w - __builtin_amdgcn_readfirstlane(sm.start[b]);
+    const int rt = at / kt, tile0 = at - rt * kt;
     const int tile1 = min(kt, tile0 + (w1 - w));
     const int unit0 = w - tile0;
     const int r0 = rt * M, nrows = min(M, s.n * p.heads - r0);
@@ -420,120 +460,117 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     const int tend = min(tile1, (lim_hi + kN - 1) / kN);
     const int32_t* table = p.table + (int64_t)b * p.table_stride;
 
-    // ---- queries into registers
-    bf16x8 q[RB][KS];
-    int lim[RB];
+    // ---- a tile's rows on their way. Its page entries come first, to the last wave (whose other
+    // loads are the fewest), which turns them into the rows' addresses a tile before the loads
+    auto entries = [&](int t) {
+      const int tok = min(t * kN + lane, lim_hi - 1);
+      if (wave == 7 && lane < kN) lds_dma4(table + (tok >> p.page_shift), sm.ent[t % kEnts]);
+    };
+    bool lost = false;  // a page outside the cache
+    auto resolve = [&](int t) {
+      if (t < tend && wave == 7 && lane < kN) {
+        const int tok = t * kN + lane, pg = sm.ent[t % kEnts][lane];
+        const bool real = tok < lim_hi, in = (uint32_t)pg < (uint32_t)p.pages;
+        lost = lost || (real && !in);
+        const uint32_t row = ((uint32_t)pg << p.page_shift) + (tok & ((1 << p.page_shift) - 1));
+        sm.addr[lane] = real && in ? p.cache + (uint64_t)row * (kPieces * 16) : (const uint8_t*)g_zero_row;
+      }
+    };
+    // load i of wave w is number 8 i + w of the tile
+    const int mine_n = (kLoads - wave + 7) / 8;  // loads of this wave a tile
+    auto issue = [&](int t) {
+      constexpr int A = (kLoads + 7) / 8;
+      uint8_t* dst = (MX ? sm.raw[(t - tile0) % kMxRing] : sm.tile[(t - tile0) % kRing]) + wave * 1024;
+      const int ln = (M < 128 ? lane : anew(lane)) + wave * 64;
+      const uint8_t* src[A];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int r = (rg * RB + rb) * 16 + col;
-      const bool real = r < nrows;
-      const int i = real ? (r0 + r) / p.heads : 0, h = real ? (r0 + r) - i * p.heads : 0;
-      lim[rb] = real ? max(0, base + i) : 0;
+      for (int i = 0; i < A; ++i) {
+        const uint32_t at = i * 512 + ln, r = at / kPieces, c = at - r * kPieces;
+        src[i] = sm.addr[min(r, (uint32_t)kN - 1)] + ((MX ? c : c ^ swz(r)) << 4);
+      }
+#pragma unroll
+      for (int i = 0; i < A; ++i)
+        if ((i < A - 1 || 8 * i + wave < kLoads) && (kN * kPieces % 64 == 0 || i * 512 + ln < kN * kPieces))
+          lds_dma16(src[i], dst + i * 8192);
+    };
+    // the raw rows of tile t as bf16: 16 threads a row, each the codes 16 j .. and 256 + 16 j ..
+    auto unpack = [&](int t) {
+      if constexpr (MX) {
+        const uint8_t* src = sm.raw[(t - tile0) % kMxRing] + (tid >> 4) * kMxRow;
+        uint8_t* dst = sm.tile[(t - tile0) & 1] + (tid >> 4) * (2 * kRow);
+        const int x = swz(tid >> 4), j = tid & 15;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = 16 * i + j;
+          const u32x4 q = *(const u32x4*)(src + 16 * c);
+          const float sc = e8m0(src[kL + (c >> 1)]);
+          *(u32x4*)(dst + (((2 * c) ^ x) << 4)) = fp8x8(q.x, q.y, sc);
+          *(u32x4*)(dst + (((2 * c + 1) ^ x) << 4)) = fp8x8(q.z, q.w, sc);
+        }
+        if (j < 8) *(u32x4*)(dst + (((64 + j) ^ x) << 4)) = *(const u32x4*)(src + kL + kMxScales + 16 * j);
+      }
+    };
+    // waits until the tile after which `newer` more were requested has landed
+    auto landed = [&](int newer) {
+      const bool more = mine_n == (kLoads + 7) / 8;
+      constexpr int A = (kLoads + 7) / 8, B = A - 1;
+      if (newer <= 0) wait_loads<0>();
+      else if (newer == 1) { if (more) wait_loads<A>(); else wait_loads<B>(); }
+      else { if (more) wait_loads<2 * A>(); else wait_loads<2 * B>(); }
+    };
+
+    // ---- the first tiles, and the queries into registers
+    __syncthreads();  // the last row tile's reads of LDS are over
+    for (int i = tid; i < 5 * kN; i += kThreads) {
+      const int t = tile0 + i / kN, tok = t * kN + i % kN;
+      sm.ent[t % kEnts][i % kN] = tok < lim_hi ? table[tok >> p.page_shift] : 0;
+    }
+    // (a row past the tile's rows takes the first one's query: it sees no token and is not stored)
+    bf16x8 q[KS];
+    int lim = 0;
+    {
+      const int r = rg * 16 + col;
+      const bool real = scores && r < nrows;
+      const int i = (r0 + (real ? r : 0)) / p.heads, h = r0 + (real ? r : 0) - i * p.heads;
+      if (real) lim = max(0, base + i);
       const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)h * p.ql_hs + 8 * g;
       const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)h * p.qp_hs + 8 * g;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const uint16_t* src = ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32);
-        q[rb][ks] = real ? *(const bf16x8*)src : bf16x8{};
-      }
+      for (int ks = 0; ks < KS; ++ks)
+        q[ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
+    }
+    wait_queries();
+    __syncthreads();
+    for (int i = 0; i < kAhead && tile0 + i < tend; ++i) {
+      resolve(tile0 + i);
+      barrier();
+      issue(tile0 + i);
+      barrier();
     }
 
-    float m[MB], l[RB];
+    float m = -kInf, l = 0.0f;
     f32x4 o[4][MB];
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      m[i] = -kInf;
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[c][i] = f32x4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int i = 0; i < RB; ++i) l[i] = 0.0f;
+      for (int i = 0; i < MB; ++i) o[c][i] = f32x4{0, 0, 0, 0};
 
-    // cache rows of tile t's tokens (threads 0 .. 63 of the workgroup): the page's table entry is
-    // requested early, and looked at when the row is needed; -1 where no token is visible
-    auto page_of = [&](int t) -> int {
-      const int tok = t * kN + tid;
-      return tok < lim_hi ? table[tok >> p.page_shift] : -1;
-    };
-    auto row_of = [&](int t, int pg) -> int {
-      const int tok = t * kN + tid;
-      if (tok >= lim_hi) return -1;
-      if (pg < 0 || (int64_t)pg >= p.pages) {
-        record(p.err, MKMOE_LATENT_ERR_PAGE, b);
-        return -1;
-      }
-      return (int)(((int64_t)pg << p.page_shift) + (tok & ((1 << p.page_shift) - 1)));
-    };
-    // bf16: 9 direct loads a thread move a tile
-    auto issue = [&](int buf) {
-      if constexpr (!MX) {
-#pragma unroll
-        for (int i = 0; i < 9; ++i) {
-          const int at = i * kThreads + tid, r = at / kChunks, c = at - r * kChunks;
-          const int row = sm.rowid[buf][r];
-          const uint8_t* src = row < 0 ? (const uint8_t*)&g_zero16
-                                       : p.cache + (int64_t)row * (2 * kRow) + ((c ^ swz(r)) << 4);
-          lds_dma16(src, sm.tile[buf] + (i * kThreads + wave * 64) * 16);
-        }
-      }
-    };
-    // MXFP8: 8 threads a row; codes 16 (8 i + j) .., i < 4, the row's scales, rope piece j
-    u32x4 mq[4], ms, mr;
-    bool mnone = true;
-    const int mrow = tid >> 3, mj = tid & 7;
-    auto fetch = [&](int buf) {
-      if constexpr (MX) {
-        const int row = sm.rowid[buf][mrow];
-        mnone = row < 0;  // (row 0 is read in its place, and not used)
-        const uint8_t* src = p.cache + (int64_t)max(row, 0) * kMxRow;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mq[i] = *(const u32x4*)(src + 16 * (8 * i + mj));
-        ms = *(const u32x4*)(src + kL);
-        mr = *(const u32x4*)(src + kL + kMxScales + 16 * mj);
-      }
-    };
-    auto unpack = [&](int buf) {
-      if constexpr (MX) {
-        uint8_t* row = sm.tile[buf] + mrow * (2 * kRow);
-        const int x = swz(mrow);
-        const uint32_t sw[4] = {ms.x, ms.y, ms.z, ms.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float sc = e8m0((sw[i] >> (8 * (mj >> 1))) & 0xffu);
-          const int c = 2 * (8 * i + mj);
-          const u32x4 zero = {0, 0, 0, 0};
-          *(u32x4*)(row + ((c ^ x) << 4)) = mnone ? zero : fp8x8(mq[i].x, mq[i].y, sc);
-          *(u32x4*)(row + (((c + 1) ^ x) << 4)) = mnone ? zero : fp8x8(mq[i].z, mq[i].w, sc);
-        }
-        *(u32x4*)(row + (((64 + mj) ^ x) << 4)) = mnone ? u32x4{0, 0, 0, 0} : mr;
-      }
-    };
-
-    // ---- the first tile
-    __syncthreads();  // the last row tile's reads of LDS are over
-    if (tid < kN) {
-      const int a = page_of(tile0), c = page_of(tile0 + 1);
-      sm.rowid[0][tid] = row_of(tile0, a);
-      sm.rowid[1][tid] = row_of(tile0 + 1, c);
-    }
-    __syncthreads();
     if (tile0 < tend) {
-      issue(0);
-      fetch(0);
-      unpack(0);
+      landed(min(kAhead - 1, tend - 1 - tile0));
+      barrier();
+      if constexpr (MX) {
+        unpack(tile0);
+        resolve(tile0 + kAhead);
+        barrier();
+        if (tile0 + kAhead < tend) {
+          entries(tile0 + kAhead + 2);
+          issue(tile0 + kAhead);
+        }
+      }
     }
 
     for (int t = tile0; t < tend; ++t) {
-      const int buf = (t - tile0) & 1;
-      wait_vm0();
-      __syncthreads();
-      const bool more = t + 1 < tend;
-      const int next_page = tid < kN ? page_of(t + 2) : -1;
-      if (more) {
-        issue(buf ^ 1);
-        fetch(buf ^ 1);
-      }
-      const uint8_t* tile = sm.tile[buf];
+      const uint32_t tile = tiles + (MX ? (t - tile0) & 1 : (t - tile0) % kRing) * kTileBytes;
 
       // tokens that only some of the rows see: their non-finite values must not reach the
       // others through 0 * V. They are cleared, and the rows that see them become NaN below
@@ -541,7 +578,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       if (edge) {
         for (int i = 0; i < kN / 8; ++i) {
           const int r = wave * (kN / 8) + i;
-          u32x4* at = (u32x4*)(sm.tile[buf] + r * (2 * kRow) + ((lane ^ swz(r)) << 4));
+          u32x4* at = (u32x4*)(sm.tile[0] + (tile - tiles) + r * (2 * kRow) + (lane << 4));
           u32x4 v = *at;
           bool any = false;
 #pragma unroll
@@ -554,105 +591,152 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           const bool some = __any(any);
           if (lane == 0) sm.bad[r] = some;
         }
-        __syncthreads();
+        barrier();
       }
 
       // ---- scores
-      f32x4 sc[RB];
+      f32x4 sc[TB];
+      float top = -kInf;
+      if (scores) {
+        f32x4 odd = {0, 0, 0, 0};  // (a second chain of sums where one block leaves the MFMA waiting)
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) sc[rb] = f32x4{0, 0, 0, 0};
+        for (int tb = 0; tb < TB; ++tb) sc[tb] = f32x4{0, 0, 0, 0};
+        // keys: this lane's row of the wave's 16, pieces 4 ks + g
+        const int ktok = 16 * TB * tg + anew(col);
+        const uint32_t k_even = tile + ktok * (2 * kRow) + ((g ^ swz(ktok)) << 4), k_odd = k_even ^ 64;
+        // (keys read a few steps ahead, and no further: the registers are the queries')
+        bf16x8 a[G < KS ? 2 : 1][G][TB];
+        auto keys = [&](int ks0, bf16x8(&to)[G][TB]) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8 a = *(const bf16x8*)(tile + (ks & 1 ? k_odd : k_even) + (ks >> 1) * 128);
+          for (int i = 0; i < G; ++i)
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) sc[rb] = mfma(a, q[rb][ks], sc[rb]);
-      }
-      const int tok0 = t * kN + 16 * tg + 4 * g;
+            for (int tb = 0; tb < TB; ++tb)
+              to[i][tb] = lds_read<bf16x8>(((ks0 + i) & 1 ? k_odd : k_even) + ((ks0 + i) >> 1) * 128 +
+                                           tb * 16 * (2 * kRow));
+        };
+        keys(0, a[0]);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float top = -kInf;
+        for (int k0 = 0; k0 < KS; k0 += G) {
+          if (k0 + G < KS) keys(k0 + G, a[(k0 / G + 1) % 2]);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float v = sc[rb][k] * p.scale2;
-          if (edge && sm.bad[16 * tg + 4 * g + k]) v = __builtin_nanf("");
-          v = tok0 + k < lim[rb] ? v : -kInf;
-          sc[rb][k] = v;
-          top = fmaxf(top, v);
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb) {
+              f32x4& to = TB == 1 && ((k0 + i) & 1) ? odd : sc[tb];
+              to = mfma(a[(k0 / G) & 1][i][tb], q[k0 + i], to);
+            }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (TB == 1) sc[0] += odd;
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb) {
+          const int r = 16 * TB * tg + 16 * tb + 4 * g;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float v = sc[tb][k] * p.scale2;
+            if (edge && sm.bad[r + k]) v = __builtin_nanf("");
+            v = t * kN + r + k < lim ? v : -kInf;
+            sc[tb][k] = v;
+            top = fmaxf(top, v);
+          }
         }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        if (g == 0) sm.mx[((rg * RB + rb) * 16 + col) * 4 + tg] = top;
+        if (TG == 2 && g == 0) sm.mx[(rg * 16 + col) * 2 + tg] = top;
       }
-      __syncthreads();
+      if constexpr (MX) landed(min(kAhead - 1, tend - 2 - t));  // raw rows of tile t + 1
+      barrier();
 
-      // ---- running maxima of every row; numerators of this wave's rows
-      float alpha[MB], mu[MB];
+      // ---- running maxima and numerators; the next tile's rows
+      if (scores) {
+        const int r = rg * 16 + col;
+        if (TG == 2) top = fmaxf(sm.mx[2 * r], sm.mx[2 * r + 1]);
+        const float mn = fmaxf(m, top), mu = mn == -kInf ? 0.0f : mn;
+        const float al = __builtin_amdgcn_exp2f(m - mu);
+        m = mn;
+        l *= al;
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb) {
+          float e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[tb][k] - mu);
+          l += (e[0] + e[1]) + (e[2] + e[3]);
+          *(u32x2*)(sm.p + r * kPStride + 16 * TB * tg + 16 * tb + 4 * g) =
+              u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
+        }
+        if (tg == 0 && g == 0) sm.al[r] = al;
+      }
+      // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16; pieces
+      // 8 wave + 2 c + (lane % 4) / 2, which the row's swizzle permutes within 8
+      bf16x8 va[4];
+      const int vl = anew(lane), vtok = 8 * (vl >> 4) + ((vl & 15) >> 2);
+      const uint32_t vx = ((((vl & 3) >> 1) ^ swz(vtok)) << 4);
+      const uint32_t v_at = tile + vtok * (2 * kRow) + 128 * wave + 8 * (vl & 1);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        struct { i16x4 a, b; } both = {
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)))),
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)) + 4 * (2 * kRow)))};
+        va[c] = __builtin_bit_cast(bf16x8, both);
+      }
+      if constexpr (MX) {
+        if (t + 1 < tend) unpack(t + 1);
+        resolve(t + 1 + kAhead);
+      } else {
+        landed(min(kAhead - 2, tend - 2 - t));  // tile t + 1
+        resolve(t + kAhead);
+      }
+      barrier();
+      // ---- outputs: the numerators' reads, then the tile after next's requests, while they come
+      const uint32_t p_row = p_at + anew(col) * (2 * kPStride) + 16 * g;
+      constexpr int PB = MB < 8 ? MB : 2;  // (registers)
+      float alpha[MB];
+      bf16x8 pb[PB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) alpha[i] = sm.al[16 * i + col];
+#pragma unroll
+      for (int i = 0; i < PB; ++i) pb[i] = lds_read<bf16x8>(p_row + i * 16 * (2 * kPStride));
+      if constexpr (MX) {
+        if (t + 1 + kAhead < tend) {
+          entries(t + kAhead + 3);
+          issue(t + 1 + kAhead);
+        }
+      } else {
+        if (t + kAhead < tend) {
+          entries(t + kAhead + 2);
+          issue(t + kAhead);
+        }
+      }
+
       bool same = true;
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const f32x4 v = *(const f32x4*)(sm.mx + (16 * i + col) * 4);
-        const float mn = fmaxf(m[i], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-        mu[i] = mn == -kInf ? 0.0f : mn;
-        alpha[i] = __builtin_amdgcn_exp2f(m[i] - mu[i]);
-        same = same && mn == m[i];
-        m[i] = mn;
-      }
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float mr_ = mu[rb], al = alpha[rb];
-        if (rg == 1) mr_ = mu[RB + rb], al = alpha[RB + rb];
-        float e[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[rb][k] - mr_);
-        l[rb] = l[rb] * al + ((e[0] + e[1]) + (e[2] + e[3]));
-        *(u32x2*)(sm.p + ((rg * RB + rb) * 16 + col) * kPStride + 16 * tg + 4 * g) =
-            u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
-      }
+      for (int i = 0; i < MB; ++i) same = same && alpha[i] == 1.0f;
       if (!__all(same)) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c) o[c][i] *= alpha[i];
       }
-      __syncthreads();
-
-      // ---- outputs
 #pragma unroll
-      for (int ks = 0; ks < kN / 32; ++ks) {
-        bf16x8 pb[MB];
+      for (int i = 0; i < MB; ++i) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) pb[i] = *(const bf16x8*)(sm.p + (16 * i + col) * kPStride + 32 * ks + 8 * g);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int piece = 8 * wave + 2 * c + ((lane & 3) >> 1);
-          i16x4 lo, hi;
-          {
-            const int r = 32 * ks + vtok;
-            lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (MKMOE_LDS i16x4*)(tile + r * (2 * kRow) + ((piece ^ swz(r)) << 4) + 8 * (lane & 1)));
-            hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (MKMOE_LDS i16x4*)(tile + (r + 4) * (2 * kRow) + ((piece ^ swz(r + 4)) << 4) + 8 * (lane & 1)));
-          }
-          struct { i16x4 a, b; } both = {lo, hi};
-          const bf16x8 a = __builtin_bit_cast(bf16x8, both);
-#pragma unroll
-          for (int i = 0; i < MB; ++i) o[c][i] = mfma(a, pb[i], o[c][i]);
-        }
+        for (int c = 0; c < 4; ++c) o[c][i] = mfma(va[c], pb[i % PB], o[c][i]);
+        if (i + PB < MB) pb[i % PB] = lds_read<bf16x8>(p_row + (i + PB) * 16 * (2 * kPStride));
       }
-      if (more) unpack(buf ^ 1);
-      if (tid < kN) sm.rowid[buf][tid] = row_of(t + 2, next_page);
     }
+    if (lost) record(p.err, MKMOE_LATENT_ERR_PAGE, b);
 
     // ---- the row sums, then the rows out
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      l[rb] += __shfl_xor(l[rb], 16, 64);
-      l[rb] += __shfl_xor(l[rb], 32, 64);
-    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
     __syncthreads();
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-      if (g == 0) sm.mx[((rg * RB + rb) * 16 + col) * 4 + tg] = l[rb];
+    float* sums = (float*)sm.p;  // [row][token group]
+    if (scores && g == 0) {
+      sums[(rg * 16 + col) * TG + tg] = l;
+      if (tg == 0) sm.al[rg * 16 + col] = m;
+    }
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == kt;
     const int slot = 2 * blockIdx.x + (unit0 > w0 ? 1 : 0);
@@ -660,8 +744,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     for (int i = 0; i < MB; ++i) {
       const int r = 16 * i + col;
       if (r >= nrows) continue;
-      const f32x4 v = *(const f32x4*)(sm.mx + r * 4);
-      const float sum = (v.x + v.y) + (v.z + v.w);
+      const float sum = TG == 2 ? sums[2 * r] + sums[2 * r + 1] : sums[r], top = sm.al[r];
       if (whole) {
         const int qi = (r0 + r) / p.heads, h = (r0 + r) - qi * p.heads;
         const bool none = base + qi <= 0;
@@ -673,13 +756,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           *(u32x2*)(dst + 16 * c) = u32x2{pack_bf(x[0], x[1]), pack_bf(x[2], x[3])};
         }
         if (p.lse && wave == 0 && g == 0)
-          p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = none ? -kInf : (m[i] + log2f(sum)) * (1.0f / kLog2e);
+          p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
       } else {
         float* dst = p.part_o + ((int64_t)slot * M + r) * kL + 64 * wave + 4 * g;
 #pragma unroll
         for (int c = 0; c < 4; ++c) *(f32x4*)(dst + 16 * c) = o[c][i];
         if (wave == 0 && g == 0) {
-          p.part_ml[((int64_t)slot * M + r) * 2] = m[i];
+          p.part_ml[((int64_t)slot * M + r) * 2] = top;
           p.part_ml[((int64_t)slot * M + r) * 2 + 1] = sum;
         }
       }
@@ -963,7 +1046,7 @@ int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_by
   p.o_ts = io->out_token_stride;
   p.o_hs = io->out_head_stride;
   p.table_stride = io->table_stride;
-  p.pages = io->cache.pages;
+  p.pages = (int)io->cache.pages;
   p.seqs = io->seqs;
   p.tokens = io->tokens;
   p.heads = io->heads;
@@ -973,10 +1056,11 @@ int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_by
   p.scale2 = io->scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
   const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8;
-  // 32 query rows a tile where a sequence has no more of them on average, else 64
-  const bool small = (int64_t)io->tokens * io->heads <= (int64_t)32 * io->seqs;
-  if (small) return mx ? attend<32, true>(p, st) : attend<32, false>(p, st);
-  return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
+  // the fewest query rows a tile that hold a sequence's on average, at most 128
+  const int64_t rows = ((int64_t)io->tokens * io->heads + io->seqs - 1) / io->seqs;
+  if (rows <= 32) return mx ? attend<32, true>(p, st) : attend<32, false>(p, st);
+  if (rows <= 64) return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
+  return mx ? attend<128, true>(p, st) : attend<128, false>(p, st);
 }
 
 int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream) {
