@@ -260,6 +260,16 @@ constexpr int kEnts = 8;        // tiles whose page entries are in LDS
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
 
+// what the end of a share cut, for the merge: the row tile that goes on in the next share
+struct Cut {
+  int32_t parts;        // 0: nothing was cut there
+  int32_t share;        // the first share with a part of it
+  int32_t slot;         // that part's slot; the others are in slots 2 (share + 1), 2 (share + 2) ..
+  int32_t t0, r0, nrows;  // the sequence's first query token, the tile's rows of it
+  int32_t base;         // tokens that its first query sees (may be negative)
+  int32_t unused;
+};
+
 struct AttendParams {
   const uint16_t* ql;
   const uint16_t* qp;
@@ -270,7 +280,7 @@ struct AttendParams {
   uint16_t* out;
   float* lse;
   int32_t* err;
-  int32_t* plan;   // [0] tiles a share, [1 ..] each sequence's first tile of the work
+  Cut* cut;        // [kShares]
   float* part_o;   // [2 kShares][M][512]
   float* part_ml;  // [2 kShares][M][2]
   int64_t ql_ts, ql_hs, qp_ts, qp_hs, o_ts, o_hs;
@@ -434,10 +444,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   if (tid < p.seqs) {
     sm.start[tid] = from;
     if (w0 >= from && w0 < from + mine) sm.first = tid;
-    if (blockIdx.x == 0) p.plan[1 + tid] = from;
   }
-  if (tid == 0 && blockIdx.x == 0) p.plan[0] = share;
-  if (w0 >= w1) return;
+  if (w0 >= w1) {
+    if (tid == 0) p.cut[blockIdx.x].parts = 0;
+    return;
+  }
   __syncthreads();
 
   const uint32_t tiles = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)sm.tile[0];
@@ -740,6 +751,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == kt;
     const int slot = 2 * blockIdx.x + (unit0 > w0 ? 1 : 0);
+    if (tid == 0 && w >= w1) {
+      Cut c = {0, 0, 0, s.t0, r0, nrows, base, 0};
+      if (tile1 < kt) {
+        c.share = unit0 / share;
+        c.parts = (unit0 + kt - 1) / share - c.share + 1;
+        c.slot = 2 * c.share + (unit0 > c.share * share ? 1 : 0);
+      }
+      p.cut[blockIdx.x] = c;
+    }
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
       const int r = 16 * i + col;
@@ -771,51 +791,106 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 }
 
 // ---------------------------------------------------------------- merge
-// 128 threads a query row: the parts of the row's tile, in order, scaled to their common maximum
+// Row tiles that were cut, their parts joined in order at their common maximum. The work of a
+// tile is M rows by 4 quarters of the latent values; kMergeWgs workgroups at each of its cuts
+// share it, so that a long sequence's many parts are read by many. Few parts: 32 lanes a row's
+// quarter; many: the workgroup's 8 groups of 32 lanes take every eighth part and add up in LDS.
+constexpr int kMergeWgs = 8;
+constexpr int kFewParts = 16;
+
 template <int M>
 __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
-  __shared__ int s_b[2];
-  const int half = threadIdx.x >> 7, th = threadIdx.x & 127;
-  const int64_t row = (int64_t)blockIdx.x * 2 + half;
-  const bool in = row < (int64_t)p.tokens * p.heads;
-  const int t = in ? (int)(row / p.heads) : 0;
-  int b;
-  if (p.starts) {
-    if (th == 0) s_b[half] = -1;
+  __shared__ float s_w[kShares], s_red[8];
+  __shared__ f32x4 s_acc[8][32];
+  const Cut c = p.cut[blockIdx.x];
+  if (c.parts == 0) return;
+  const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5;
+  const int helper = (blockIdx.x - c.share) * kMergeWgs + blockIdx.y, helpers = (c.parts - 1) * kMergeWgs;
+  auto at = [&](int i, int r) { return (int64_t)(i == 0 ? c.slot : 2 * (c.share + i)) * M + r; };
+  auto store = [&](int r, int part, f32x4 acc, float top, float sum) {
+    const int qi = (c.r0 + r) / p.heads, h = (c.r0 + r) - qi * p.heads;
+    const bool none = c.base + qi <= 0;
+    acc *= none ? 0.0f : 1.0f / sum;
+    *(u32x2*)(p.out + (int64_t)(c.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 128 * part + 4 * lane) =
+        u32x2{pack_bf(acc[0], acc[1]), pack_bf(acc[2], acc[3])};
+    if (p.lse && part == 0 && lane == 0)
+      p.lse[(int64_t)(c.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
+  };
+  if (c.parts < kFewParts) {
+    for (int item = helper * 8 + grp; item < 4 * c.nrows; item += helpers * 8) {
+      const int r = item >> 2, part = item & 3;
+      float mi = -kInf, li = 0.0f;
+      if (lane < c.parts) {
+        mi = p.part_ml[at(lane, r) * 2];
+        li = p.part_ml[at(lane, r) * 2 + 1];
+      }
+      const float* src = p.part_o + 128 * part + 4 * lane;
+      f32x4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = *(const f32x4*)(src + at(min(i, c.parts - 1), r) * kL);
+      float top = mi;
+#pragma unroll
+      for (int d = 8; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
+      const float w = __builtin_amdgcn_exp2f(mi - (top == -kInf ? 0.0f : top));
+      float sum = w * li;
+#pragma unroll
+      for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 32);
+      f32x4 acc = {0, 0, 0, 0};
+      for (int i0 = 0; i0 < c.parts; i0 += 4) {
+        f32x4 next[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i0 + 4 < c.parts) next[i] = *(const f32x4*)(src + at(min(i0 + 4 + i, c.parts - 1), r) * kL);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i0 + i < c.parts) acc += __shfl(w, i0 + i, 32) * v[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = next[i];
+      }
+      top = __shfl(top, 0, 32);
+      sum = __shfl(sum, 0, 32);
+      store(r, part, acc, top, sum);
+    }
+    return;
+  }
+  for (int item = helper; item < 4 * c.nrows; item += helpers) {
+    const int r = item >> 2, part = item & 3;
+    float mi = -kInf, li = 0.0f;
+    if (tid < c.parts) {
+      mi = p.part_ml[at(tid, r) * 2];
+      li = p.part_ml[at(tid, r) * 2 + 1];
+    }
+    float top = mi;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
+    if (lane == 0) s_red[grp] = top;
     __syncthreads();
-    for (int i = th; i < p.seqs; i += 128) {
-      const Seq s = seq_of(p, i);
-      if (t >= s.t0 && t < s.t0 + s.n) s_b[half] = i;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, s_red[i]);
+    const float w = __builtin_amdgcn_exp2f(mi - (top == -kInf ? 0.0f : top));
+    s_w[tid] = w;
+    float sum = w * li;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 32);
+    __syncthreads();
+    if (lane == 0) s_red[grp] = sum;
+    const float* src = p.part_o + 128 * part + 4 * lane;
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int i = grp; i < c.parts; i += 8) acc += s_w[i] * *(const f32x4*)(src + at(i, r) * kL);
+    s_acc[grp][lane] = acc;
+    __syncthreads();
+    if (grp == 0) {
+      sum = s_red[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        acc += s_acc[i][lane];
+        sum += s_red[i];
+      }
+      store(r, part, acc, top, sum);
     }
     __syncthreads();
-    b = s_b[half];
-  } else {
-    b = t / p.n;
   }
-  if (!in || b < 0) return;  // (a row behind the last sequence stays as it was)
-  const Seq s = seq_of(p, b);
-  const int kt = kv_tiles(s), h = (int)(row - (int64_t)t * p.heads);
-  const int r = (t - s.t0) * p.heads + h, rt = r / M, rr = r % M;
-  const int share = p.plan[0], u0 = p.plan[1 + b] + rt * kt, u1 = u0 + kt - 1;
-  const int g0 = u0 / share, g1 = u1 / share;
-  if (g0 == g1) return;  // finished where it was computed
-  auto slot_of = [&](int gi) { return (int64_t)(2 * gi + (u0 > gi * share ? 1 : 0)) * M + rr; };
-  float top = -kInf;
-  for (int gi = g0; gi <= g1; ++gi) top = fmaxf(top, p.part_ml[slot_of(gi) * 2]);
-  const float mu = top == -kInf ? 0.0f : top;
-  float sum = 0.0f;
-  f32x4 acc = {0, 0, 0, 0};
-  for (int gi = g0; gi <= g1; ++gi) {
-    const int64_t at = slot_of(gi);
-    const float wgt = __builtin_amdgcn_exp2f(p.part_ml[at * 2] - mu);
-    sum += wgt * p.part_ml[at * 2 + 1];
-    acc += wgt * *(const f32x4*)(p.part_o + at * kL + 4 * th);
-  }
-  const bool none = s.len - s.n + 1 + (t - s.t0) <= 0;
-  const float inv = none ? 0.0f : 1.0f / sum;
-  acc *= inv;
-  *(u32x2*)(p.out + (int64_t)t * p.o_ts + (int64_t)h * p.o_hs + 4 * th) = u32x2{pack_bf(acc[0], acc[1]), pack_bf(acc[2], acc[3])};
-  if (p.lse && th == 0) p.lse[row] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
 }
 
 // ---------------------------------------------------------------- the heads' products
@@ -884,10 +959,10 @@ __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
 
 // ---------------------------------------------------------------- host
 constexpr size_t kCtlBytes = 256;
-constexpr size_t kPlanBytes = (1 + kMaxSeqs + 63) / 64 * 64 * 4;
+constexpr size_t kCutBytes = kShares * sizeof(Cut);
 constexpr size_t kMlBytes = (size_t)2 * kShares * kRowsMax * 2 * 4;
 constexpr size_t kPartBytes = (size_t)2 * kShares * kRowsMax * kL * 4;
-constexpr size_t kWsBytes = kCtlBytes + kPlanBytes + kMlBytes + kPartBytes;
+constexpr size_t kWsBytes = kCtlBytes + kCutBytes + kMlBytes + kPartBytes;
 constexpr int64_t kMaxRows = (int64_t)1 << 24;  // query rows (tokens x heads) and tokens a call
 
 inline bool aligned(const void* q, size_t a) { return ((uintptr_t)q % a) == 0; }
@@ -912,8 +987,7 @@ template <int M, bool MX>
 int attend(const AttendParams& p, hipStream_t st) {
   hipLaunchKernelGGL((k_latent_attend<M, MX>), dim3(kShares), dim3(kThreads), 0, st, p);
   if (int rc = launched()) return rc;
-  const int64_t rows = (int64_t)p.tokens * p.heads;
-  hipLaunchKernelGGL(k_latent_merge<M>, dim3((unsigned)((rows + 1) / 2)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(k_latent_merge<M>, dim3(kShares, kMergeWgs), dim3(256), 0, st, p);
   return launched();
 }
 
@@ -1036,8 +1110,8 @@ int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_by
   p.lse = io->lse;
   uint8_t* at = (uint8_t*)ws;
   p.err = (int32_t*)at;
-  p.plan = (int32_t*)(at += kCtlBytes);
-  p.part_ml = (float*)(at += kPlanBytes);
+  p.cut = (Cut*)(at += kCtlBytes);
+  p.part_ml = (float*)(at += kCutBytes);
   p.part_o = (float*)(at += kMlBytes);
   p.ql_ts = io->ql_token_stride;
   p.ql_hs = io->ql_head_stride;
