@@ -256,18 +256,19 @@ constexpr int kPStride = kN + 16;  // bf16 of a row of P: 96 bytes, whose 16-byt
 constexpr int kTileBytes = kN * kRow * 2;  // a tile's rows in LDS, bf16
 constexpr int kRing = 4;        // bf16 cache: tiles in LDS, one in use and three on their way
 constexpr int kMxRing = 3;      // MXFP8: raw tiles on their way
-constexpr int kEnts = 8;        // tiles whose page entries are in LDS
+constexpr int kSetup = 3;       // see setup()
+constexpr int kEnts = 4;        // tiles whose page entries are in LDS
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
 
 // what the end of a share cut, for the merge: the row tile that goes on in the next share
 struct Cut {
   int32_t parts;        // 0: nothing was cut there
-  int32_t share;        // the first share with a part of it
-  int32_t slot;         // that part's slot; the others are in slots 2 (share + 1), 2 (share + 2) ..
+  int32_t share;        // the first share with a part of it, in slot 2 share + 1; the others are in
+                        // slots 2 (share + 1), 2 (share + 2) ..
   int32_t t0, r0, nrows;  // the sequence's first query token, the tile's rows of it
   int32_t base;         // tokens that its first query sees (may be negative)
-  int32_t unused;
+  int32_t unused[2];
 };
 
 struct AttendParams {
@@ -286,8 +287,15 @@ struct AttendParams {
   int64_t ql_ts, ql_hs, qp_ts, qp_hs, o_ts, o_hs;
   int64_t table_stride;
   int pages, seqs, tokens, heads, n, max_len, page_shift;
-  float scale2;  // scale log2(e)
+  uint32_t per_head;  // 2^32 / heads, rounded up
+  float scale2;       // scale log2(e)
 };
+
+// a query row's token: exact for rows below 2^24 and up to 128 heads (the product is off by less
+// than rows x heads <= 2^31 of 2^32)
+__device__ __forceinline__ int over_heads(const AttendParams& p, int row) {
+  return p.heads == 1 ? row : (int)__umulhi((uint32_t)row, p.per_head);
+}
 
 // a sequence's query tokens and length, clamped to their bounds
 struct Seq {
@@ -311,13 +319,14 @@ __device__ __forceinline__ Seq seq_of(const AttendParams& p, int b) {
   }
   return s;
 }
-// tiles of a sequence: query row tiles times tiles of its cached tokens (an empty sequence has
-// one, which writes its rows)
+// a sequence's work: its query row tiles, each as long as its tiles of cached tokens and kSetup
+// more, about what starting and storing a row tile takes (an empty sequence only stores its rows)
 template <int M>
 __device__ __forceinline__ int row_tiles(const AttendParams& p, const Seq& s) {
   return (int)(((int64_t)s.n * p.heads + M - 1) / M);
 }
 __device__ __forceinline__ int kv_tiles(const Seq& s) { return max(1, (s.len + kN - 1) / kN); }
+__device__ __forceinline__ int setup(const Seq& s) { return s.len > 0 ? kSetup : 0; }
 
 // 16-byte pieces of LDS row r are stored at piece c ^ swz(r). The LDS has 64 banks (16 pieces);
 // rows are 72 pieces, so odd rows start half way round. A 16-byte read serves lanes 0 .. 3,
@@ -364,6 +373,14 @@ __device__ __forceinline__ int anew(int v) {
   asm volatile("" : "+v"(v));
   return v;
 }
+// a value joined over the four lanes of a column (lane % 16), in each of them
+template <class F>
+__device__ __forceinline__ float over_groups(float v, F join) {
+  const auto a = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
+  v = join(u2f(a[0]), u2f(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return join(u2f(b[0]), u2f(b[1]));
+}
 // LDS at a byte offset
 template <class T>
 __device__ __forceinline__ T lds_read(uint32_t at) {
@@ -381,7 +398,7 @@ struct __align__(128) AttendSmem {
   int ent[kEnts][kN];          // page entries of a tile's tokens
   int start[kMaxSeqs];         // first tile of each sequence in the work
   int scan[8];
-  int first;
+  int first[4];                // the share's first sequence: its number, t0, n, len
   uint8_t bad[kN];             // tokens of the tile with a non-finite latent value
 };
 
@@ -418,9 +435,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 
   // ---- the work list
   int mine = 0;
+  Seq own = {0, 0, 0, false};
   if (tid < p.seqs) {
-    const Seq s = seq_of(p, tid);
-    mine = row_tiles<M>(p, s) * kv_tiles(s);
+    const Seq s = own = seq_of(p, tid);
+    mine = row_tiles<M>(p, s) * (kv_tiles(s) + setup(s));
     if (s.bad && blockIdx.x == 0) record(p.err, MKMOE_LATENT_ERR_LENGTH, tid);
   }
   int inc = mine;
@@ -443,7 +461,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   const int from = before + inc - mine;
   if (tid < p.seqs) {
     sm.start[tid] = from;
-    if (w0 >= from && w0 < from + mine) sm.first = tid;
+    if (w0 >= from && w0 < from + mine) {
+      sm.first[0] = tid;
+      sm.first[1] = own.t0;
+      sm.first[2] = own.n;
+      sm.first[3] = own.len;
+    }
   }
   if (w0 >= w1) {
     if (tid == 0) p.cut[blockIdx.x].parts = 0;
@@ -454,50 +477,68 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   const uint32_t tiles = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)sm.tile[0];
   const uint32_t p_at = (uint32_t)(uintptr_t)(MKMOE_LDS uint16_t*)sm.p;
 
-  int b = __builtin_amdgcn_readfirstlane(sm.first);
+  int b = __builtin_amdgcn_readfirstlane(sm.first[0]);
+  Seq s = {__builtin_amdgcn_readfirstlane(sm.first[1]), __builtin_amdgcn_readfirstlane(sm.first[2]),
+           __builtin_amdgcn_readfirstlane(sm.first[3]), false};
   for (int w = w0; w < w1;) {
-    while (b + 1 < p.seqs && __builtin_amdgcn_readfirstlane(sm.start[b + 1]) <= w) ++b;
-    const Seq s = seq_of(p, b);
-    const int kt = kv_tiles(s), at = w - __builtin_amdgcn_readfirstlane(sm.start[b]);
-    const int rt = at / kt, tile0 = at - rt * kt;
-    const int tile1 = min(kt, tile0 + (w1 - w));
-    const int unit0 = w - tile0;
+    if (w > w0) {
+      const int last = b;
+      while (b + 1 < p.seqs && __builtin_amdgcn_readfirstlane(sm.start[b + 1]) <= w) ++b;
+      if (b != last) s = seq_of(p, b);
+    }
+    const int kt = kv_tiles(s), pre = setup(s), at = w - __builtin_amdgcn_readfirstlane(sm.start[b]);
+    const int rt = at / (kt + pre), unit0 = w - (at - rt * (kt + pre));  // the row tile's place in the list
+    const int tile0 = max(0, w - unit0 - pre), tile1 = min(kt, w1 - unit0 - pre);
     const int r0 = rt * M, nrows = min(M, s.n * p.heads - r0);
-    w += tile1 - tile0;
+    w = min(w1, unit0 + pre + kt);
+    if (tile1 <= 0) {  // the next share begins it
+      if (tid == 0 && w >= w1) p.cut[blockIdx.x].parts = 0;
+      continue;
+    }
 
     // each row's visible tokens: query token i of n sees len - n + 1 + i
     const int base = s.len - s.n + 1;
-    const int lim_lo = max(0, base + r0 / p.heads), lim_hi = max(0, base + (r0 + nrows - 1) / p.heads);
+    const int lim_lo = max(0, base + over_heads(p, r0)), lim_hi = max(0, base + over_heads(p, r0 + nrows - 1));
     const int tend = min(tile1, (lim_hi + kN - 1) / kN);
     const int32_t* table = p.table + (int64_t)b * p.table_stride;
+    if (lim_hi == 0) {  // nothing to see: rows of zeros, by every share that has a part of them
+      for (int i = tid; i < nrows * (kL / 8); i += kThreads) {
+        const int r = r0 + i / (kL / 8), qi = over_heads(p, r), h = r - qi * p.heads;
+        *(u32x4*)(p.out + (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 8 * (i % (kL / 8))) = u32x4{0, 0, 0, 0};
+        if (p.lse && i % (kL / 8) == 0) p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = -kInf;
+      }
+      if (tid == 0 && w >= w1) p.cut[blockIdx.x].parts = 0;
+      continue;
+    }
 
     // ---- a tile's rows on their way. Its page entries come first, to the last wave (whose other
     // loads are the fewest), which turns them into the rows' addresses a tile before the loads
     auto entries = [&](int t) {
-      const int tok = min(t * kN + lane, lim_hi - 1);
-      if (wave == 7 && lane < kN) lds_dma4(table + (tok >> p.page_shift), sm.ent[t % kEnts]);
+      const int ln = anew(lane), tok = min(t * kN + ln, lim_hi - 1);
+      if (wave == 7 && ln < kN) lds_dma4(table + (tok >> p.page_shift), sm.ent[t % kEnts]);
     };
     bool lost = false;  // a page outside the cache
+    auto address = [&](int tok, int pg) -> const uint8_t* {
+      const bool real = tok < lim_hi, in = (uint32_t)pg < (uint32_t)p.pages;
+      lost = lost || (real && !in);
+      const uint32_t row = ((uint32_t)pg << p.page_shift) + (tok & ((1 << p.page_shift) - 1));
+      return real && in ? p.cache + (uint64_t)row * (kPieces * 16) : (const uint8_t*)g_zero_row;
+    };
     auto resolve = [&](int t) {
-      if (t < tend && wave == 7 && lane < kN) {
-        const int tok = t * kN + lane, pg = sm.ent[t % kEnts][lane];
-        const bool real = tok < lim_hi, in = (uint32_t)pg < (uint32_t)p.pages;
-        lost = lost || (real && !in);
-        const uint32_t row = ((uint32_t)pg << p.page_shift) + (tok & ((1 << p.page_shift) - 1));
-        sm.addr[lane] = real && in ? p.cache + (uint64_t)row * (kPieces * 16) : (const uint8_t*)g_zero_row;
-      }
+      const int ln = anew(lane);
+      if (t < tend && wave == 7 && ln < kN) sm.addr[ln] = address(t * kN + ln, sm.ent[t % kEnts][ln]);
     };
     // load i of wave w is number 8 i + w of the tile
     const int mine_n = (kLoads - wave + 7) / 8;  // loads of this wave a tile
-    auto issue = [&](int t) {
+    auto issue = [&](int t, const uint8_t* const* addr) {
       constexpr int A = (kLoads + 7) / 8;
       uint8_t* dst = (MX ? sm.raw[(t - tile0) % kMxRing] : sm.tile[(t - tile0) % kRing]) + wave * 1024;
-      const int ln = (M < 128 ? lane : anew(lane)) + wave * 64;
+      const int ln = (M < 64 ? lane : anew(lane)) + wave * 64;
       const uint8_t* src[A];
 #pragma unroll
       for (int i = 0; i < A; ++i) {
         const uint32_t at = i * 512 + ln, r = at / kPieces, c = at - r * kPieces;
-        src[i] = sm.addr[min(r, (uint32_t)kN - 1)] + ((MX ? c : c ^ swz(r)) << 4);
+        src[i] = addr[min(r, (uint32_t)kN - 1)] + ((MX ? c : c ^ swz(r)) << 4);
       }
 #pragma unroll
       for (int i = 0; i < A; ++i)
@@ -507,9 +548,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     // the raw rows of tile t as bf16: 16 threads a row, each the codes 16 j .. and 256 + 16 j ..
     auto unpack = [&](int t) {
       if constexpr (MX) {
-        const uint8_t* src = sm.raw[(t - tile0) % kMxRing] + (tid >> 4) * kMxRow;
-        uint8_t* dst = sm.tile[(t - tile0) & 1] + (tid >> 4) * (2 * kRow);
-        const int x = swz(tid >> 4), j = tid & 15;
+        const int th = wave * 64 + anew(lane), r = th >> 4, x = swz(r), j = th & 15;
+        const uint8_t* src = sm.raw[(t - tile0) % kMxRing] + r * kMxRow;
+        uint8_t* dst = sm.tile[(t - tile0) & 1] + r * (2 * kRow);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int c = 16 * i + j;
@@ -530,35 +571,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       else { if (more) wait_loads<2 * A>(); else wait_loads<2 * B>(); }
     };
 
-    // ---- the first tiles, and the queries into registers
-    __syncthreads();  // the last row tile's reads of LDS are over
-    for (int i = tid; i < 5 * kN; i += kThreads) {
-      const int t = tile0 + i / kN, tok = t * kN + i % kN;
-      sm.ent[t % kEnts][i % kN] = tok < lim_hi ? table[tok >> p.page_shift] : 0;
-    }
-    // (a row past the tile's rows takes the first one's query: it sees no token and is not stored)
-    bf16x8 q[KS];
-    int lim = 0;
-    {
-      const int r = rg * 16 + col;
-      const bool real = scores && r < nrows;
-      const int i = (r0 + (real ? r : 0)) / p.heads, h = r0 + (real ? r : 0) - i * p.heads;
-      if (real) lim = max(0, base + i);
-      const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)h * p.ql_hs + 8 * g;
-      const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)h * p.qp_hs + 8 * g;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        q[ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
-    }
-    wait_queries();
-    __syncthreads();
-    for (int i = 0; i < kAhead && tile0 + i < tend; ++i) {
-      resolve(tile0 + i);
-      barrier();
-      issue(tile0 + i);
-      barrier();
-    }
-
     float m = -kInf, l = 0.0f;
     f32x4 o[4][MB];
 #pragma unroll
@@ -566,21 +578,49 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 #pragma unroll
       for (int i = 0; i < MB; ++i) o[c][i] = f32x4{0, 0, 0, 0};
 
-    if (tile0 < tend) {
-      landed(min(kAhead - 1, tend - 1 - tile0));
+    // ---- the first tiles' rows, and the queries into registers
+    __syncthreads();  // the last row tile's reads of LDS are over
+    const uint8_t** first = (const uint8_t**)sm.p;  // [kAhead][kN] (P is not in use yet)
+    static_assert(M * kPStride * 2 >= kAhead * kN * 8, "the first tiles' addresses fit into P");
+    const bool entry = tid < (kAhead + 2) * kN;
+    const int tok0 = tile0 * kN + tid;
+    const int pg0 = entry ? table[min(tok0, lim_hi - 1) >> p.page_shift] : 0;
+    // (a row past the tile's rows takes the first one's query: it sees no token and is not stored)
+    bf16x8 q[KS];
+    int lim = 0;
+    {
+      const int r = rg * 16 + col;
+      const bool real = scores && r < nrows;
+      const int i = over_heads(p, r0 + (real ? r : 0)), h = r0 + (real ? r : 0) - i * p.heads;
+      if (real) lim = max(0, base + i);
+      const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)h * p.ql_hs + 8 * g;
+      const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)h * p.qp_hs + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        q[ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
+    }
+    if (entry) {
+      const int t = tile0 + tid / kN;
+      if (tid < kAhead * kN) first[tid] = address(tok0, pg0);
+      else sm.ent[t % kEnts][tid % kN] = pg0;
+    }
+    barrier();
+    issue(tile0, first);
+    wait_queries();  // and the first tile
+    for (int i = 1; i < kAhead && tile0 + i < tend; ++i) issue(tile0 + i, first + i * kN);
+    barrier();
+    if constexpr (MX) {
+      unpack(tile0);
+      resolve(tile0 + kAhead);
       barrier();
-      if constexpr (MX) {
-        unpack(tile0);
-        resolve(tile0 + kAhead);
-        barrier();
-        if (tile0 + kAhead < tend) {
-          entries(tile0 + kAhead + 2);
-          issue(tile0 + kAhead);
-        }
+      if (tile0 + kAhead < tend) {
+        entries(tile0 + kAhead + 2);
+        issue(tile0 + kAhead, sm.addr);
       }
     }
 
     for (int t = tile0; t < tend; ++t) {
+      const int ln = anew(lane), col = ln & 15, g = ln >> 4;
       const uint32_t tile = tiles + (MX ? (t - tile0) & 1 : (t - tile0) % kRing) * kTileBytes;
 
       // tokens that only some of the rows see: their non-finite values must not reach the
@@ -613,7 +653,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 #pragma unroll
         for (int tb = 0; tb < TB; ++tb) sc[tb] = f32x4{0, 0, 0, 0};
         // keys: this lane's row of the wave's 16, pieces 4 ks + g
-        const int ktok = 16 * TB * tg + anew(col);
+        const int ktok = 16 * TB * tg + col;
         const uint32_t k_even = tile + ktok * (2 * kRow) + ((g ^ swz(ktok)) << 4), k_odd = k_even ^ 64;
         // (keys read a few steps ahead, and no further: the registers are the queries')
         bf16x8 a[G < KS ? 2 : 1][G][TB];
@@ -652,8 +692,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
             top = fmaxf(top, v);
           }
         }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
         if (TG == 2 && g == 0) sm.mx[(rg * 16 + col) * 2 + tg] = top;
       }
       if constexpr (MX) landed(min(kAhead - 1, tend - 2 - t));  // raw rows of tile t + 1
@@ -681,17 +720,20 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16; pieces
       // 8 wave + 2 c + (lane % 4) / 2, which the row's swizzle permutes within 8
       bf16x8 va[4];
-      const int vl = anew(lane), vtok = 8 * (vl >> 4) + ((vl & 15) >> 2);
-      const uint32_t vx = ((((vl & 3) >> 1) ^ swz(vtok)) << 4);
-      const uint32_t v_at = tile + vtok * (2 * kRow) + 128 * wave + 8 * (vl & 1);
+      auto values = [&]() {
+        const int vtok = 8 * g + (col >> 2);
+        const uint32_t vx = ((((col & 3) >> 1) ^ swz(vtok)) << 4);
+        const uint32_t v_at = tile + vtok * (2 * kRow) + 128 * wave + 8 * (col & 1);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        struct { i16x4 a, b; } both = {
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)))),
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)) + 4 * (2 * kRow)))};
-        va[c] = __builtin_bit_cast(bf16x8, both);
-      }
+        for (int c = 0; c < 4; ++c) {
+          struct { i16x4 a, b; } both = {
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)))),
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)) + 4 * (2 * kRow)))};
+          va[c] = __builtin_bit_cast(bf16x8, both);
+        }
+      };
+      if (M < 128) values();  // (with 128 rows there are no registers to hold them early)
       if constexpr (MX) {
         if (t + 1 < tend) unpack(t + 1);
         resolve(t + 1 + kAhead);
@@ -701,34 +743,36 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       }
       barrier();
       // ---- outputs: the numerators' reads, then the tile after next's requests, while they come
-      const uint32_t p_row = p_at + anew(col) * (2 * kPStride) + 16 * g;
-      constexpr int PB = MB < 8 ? MB : 2;  // (registers)
-      float alpha[MB];
+      const uint32_t p_row = p_at + col * (2 * kPStride) + 16 * g;
+      constexpr int PB = MB < 8 ? MB : 2;
+      float al = sm.al[min(ln, M - 1)];
+      if (M == 128) al = sm.al[64 + ln] == 1.0f ? al : 0.0f;
       bf16x8 pb[PB];
+      auto numerators = [&]() {
 #pragma unroll
-      for (int i = 0; i < MB; ++i) alpha[i] = sm.al[16 * i + col];
-#pragma unroll
-      for (int i = 0; i < PB; ++i) pb[i] = lds_read<bf16x8>(p_row + i * 16 * (2 * kPStride));
+        for (int i = 0; i < PB; ++i) pb[i] = lds_read<bf16x8>(p_row + i * 16 * (2 * kPStride));
+      };
+      if (M < 128) numerators();
       if constexpr (MX) {
         if (t + 1 + kAhead < tend) {
           entries(t + kAhead + 3);
-          issue(t + 1 + kAhead);
+          issue(t + 1 + kAhead, sm.addr);
         }
       } else {
         if (t + kAhead < tend) {
           entries(t + kAhead + 2);
-          issue(t + kAhead);
+          issue(t + kAhead, sm.addr);
         }
       }
 
-      bool same = true;
+      if (M == 128) values(), numerators();
+      if (!__all(al == 1.0f)) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i) same = same && alpha[i] == 1.0f;
-      if (!__all(same)) {
+        for (int i = 0; i < MB; ++i) {
+          const float alpha = sm.al[16 * i + col];
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[c][i] *= alpha[i];
+          for (int c = 0; c < 4; ++c) o[c][i] *= alpha;
+        }
       }
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
@@ -740,8 +784,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     if (lost) record(p.err, MKMOE_LATENT_ERR_PAGE, b);
 
     // ---- the row sums, then the rows out
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = over_groups(l, [](float a, float b) { return a + b; });
     __syncthreads();
     float* sums = (float*)sm.p;  // [row][token group]
     if (scores && g == 0) {
@@ -750,13 +793,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     }
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == kt;
-    const int slot = 2 * blockIdx.x + (unit0 > w0 ? 1 : 0);
+    const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
     if (tid == 0 && w >= w1) {
-      Cut c = {0, 0, 0, s.t0, r0, nrows, base, 0};
+      Cut c = {0, 0, s.t0, r0, nrows, base, 0, 0};
       if (tile1 < kt) {
-        c.share = unit0 / share;
-        c.parts = (unit0 + kt - 1) / share - c.share + 1;
-        c.slot = 2 * c.share + (unit0 > c.share * share ? 1 : 0);
+        c.share = (unit0 + pre) / share;
+        c.parts = (unit0 + pre + kt - 1) / share - c.share + 1;
       }
       p.cut[blockIdx.x] = c;
     }
@@ -766,7 +808,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       if (r >= nrows) continue;
       const float sum = TG == 2 ? sums[2 * r] + sums[2 * r + 1] : sums[r], top = sm.al[r];
       if (whole) {
-        const int qi = (r0 + r) / p.heads, h = (r0 + r) - qi * p.heads;
+        const int qi = over_heads(p, r0 + r), h = (r0 + r) - qi * p.heads;
         const bool none = base + qi <= 0;
         const float inv = none ? 0.0f : 1.0f / sum;
         uint16_t* dst = p.out + (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 64 * wave + 4 * g;
@@ -806,9 +848,9 @@ __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
   if (c.parts == 0) return;
   const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5;
   const int helper = (blockIdx.x - c.share) * kMergeWgs + blockIdx.y, helpers = (c.parts - 1) * kMergeWgs;
-  auto at = [&](int i, int r) { return (int64_t)(i == 0 ? c.slot : 2 * (c.share + i)) * M + r; };
+  auto at = [&](int i, int r) { return (int64_t)(2 * (c.share + i) + (i == 0 ? 1 : 0)) * M + r; };
   auto store = [&](int r, int part, f32x4 acc, float top, float sum) {
-    const int qi = (c.r0 + r) / p.heads, h = (c.r0 + r) - qi * p.heads;
+    const int qi = over_heads(p, c.r0 + r), h = (c.r0 + r) - qi * p.heads;
     const bool none = c.base + qi <= 0;
     acc *= none ? 0.0f : 1.0f / sum;
     *(u32x2*)(p.out + (int64_t)(c.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 128 * part + 4 * lane) =
@@ -1087,7 +1129,7 @@ int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_by
   const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
   if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
   // the work list's tiles are counted in 32 bits
-  const int64_t tiles = ((int64_t)io->tokens * io->heads / 32 + io->seqs) * ((max_len + kN - 1) / kN);
+  const int64_t tiles = ((int64_t)io->tokens * io->heads / 32 + io->seqs) * ((max_len + kN - 1) / kN + kSetup);
   if (tiles > 0x3fffffff) return MKMOE_ERR_ARG;
   const void* wide[] = {io->q_lat, io->q_pe, io->out};
   for (const void* q : wide)
@@ -1127,6 +1169,7 @@ int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_by
   p.n = io->q_starts ? 0 : io->tokens / io->seqs;
   p.max_len = (int)max_len;
   p.page_shift = __builtin_ctz((unsigned)io->cache.page_size);
+  p.per_head = (uint32_t)(((1ull << 32) + io->heads - 1) / io->heads);
   p.scale2 = io->scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
   const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8;
