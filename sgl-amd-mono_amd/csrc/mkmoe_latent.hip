@@ -251,13 +251,18 @@ constexpr int kN = 32;          // cached tokens a tile
 constexpr int kShares = 256;    // equal shares of the work, a workgroup each: one a CU
 constexpr int kThreads = 512;   // 8 waves
 constexpr int kMaxSeqs = MKMOE_LATENT_MAX_SEQS;
-constexpr int kRowsMax = 128;   // query rows a row tile holds at most
+constexpr int kRowsMax = 64;    // query rows a row tile holds at most
 constexpr int kPStride = kN + 16;  // bf16 of a row of P: 96 bytes, whose 16-byte reads meet every bank once
-constexpr int kTileBytes = kN * kRow * 2;  // a tile's rows in LDS, bf16
+constexpr int kTileBytes = kN * kRow * 2;  // a tile's rows in LDS, bf16: the latent parts, then the rope parts
+constexpr int kRopeAt = kN * kL * 2;
 constexpr int kRing = 4;        // bf16 cache: tiles in LDS, one in use and three on their way
 constexpr int kMxRing = 3;      // MXFP8: raw tiles on their way
 constexpr int kSetup = 3;       // see setup()
 constexpr int kEnts = 4;        // tiles whose page entries are in LDS
+// a row's maximum is moved where a score passes it by more than 2^kSlack: numerators then stay below
+// 2^kSlack (bf16 and fp32 keep their relative precision there), and after the first tiles almost no
+// tile rescales the outputs (with kSlack 0 the 64 rows' products were half of a tile's VALU work)
+constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
 
@@ -328,12 +333,14 @@ __device__ __forceinline__ int row_tiles(const AttendParams& p, const Seq& s) {
 __device__ __forceinline__ int kv_tiles(const Seq& s) { return max(1, (s.len + kN - 1) / kN); }
 __device__ __forceinline__ int setup(const Seq& s) { return s.len > 0 ? kSetup : 0; }
 
-// 16-byte pieces of LDS row r are stored at piece c ^ swz(r). The LDS has 64 banks (16 pieces);
-// rows are 72 pieces, so odd rows start half way round. A 16-byte read serves lanes 0 .. 3,
-// 12 .. 15, 20 .. 27 at once (and so on), which for the keys are 16 rows at pieces c and c ^ 1; a
-// transposing read serves 32 lanes, rows r .. r + 3 and r + 8 .. r + 11 by 32 bytes. With these
-// bits both meet every bank once (measured: no conflicts; with bits 0 .. 2 of r one of them has)
-__device__ __forceinline__ int swz(int r) { return ((r & 2) << 1) | ((r & 8) >> 2); }
+// 16-byte pieces c of LDS row r are stored at piece c ^ swz(r) (latent parts, rows of 64 pieces) or
+// c ^ swz_rope(r) (rope parts, rows of 8). The LDS has 64 banks, 16 pieces. A 16-byte read serves
+// lanes 0 .. 3, 12 .. 15, 20 .. 27 at once (and so on), which for the keys are 16 rows at pieces c and
+// c ^ 1; a transposing read serves 32 lanes, rows r .. r + 3 and r + 8 .. r + 11 by 32 bytes. With
+// these bits both meet every bank once (measured: without conflicts; with r % 16 in order, or other
+// bits, one of them has some)
+__device__ __forceinline__ int swz(int r) { return (r & 8) | ((r & 2) << 1) | ((r & 1) << 1); }
+__device__ __forceinline__ int swz_rope(int r) { return ((r & 2) << 1) | ((r & 8) >> 2); }
 
 // the row of tokens that are not there
 __device__ const u32x4 g_zero_row[kRow * 2 / 16] = {};
@@ -346,6 +353,10 @@ __device__ __forceinline__ uint32_t lds_at(const void* lds) {
 }
 __device__ __forceinline__ void lds_dma16(const void* g, const void* lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_at(lds)) : "memory", "m0");
+}
+// (lane l's from base + at)
+__device__ __forceinline__ void lds_dma16(const void* base, uint32_t at, const void* lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(lds_at(lds)) : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma4(const void* g, const void* lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_at(lds)) : "memory", "m0");
@@ -388,11 +399,11 @@ __device__ __forceinline__ T lds_read(uint32_t at) {
 }
 
 template <int M, bool MX>
-struct __align__(128) AttendSmem {
+struct __align__(256) AttendSmem {
   uint8_t tile[MX ? 2 : kRing][kTileBytes];  // cached rows, bf16, swizzled pieces
   uint8_t raw[MX ? kMxRing : 1][MX ? kN * kMxRow : 16];
   uint16_t p[M * kPStride];    // softmax numerators of the tile [row][token]
-  float mx[M < 128 ? M * 2 : 4];  // [row][token group]: tile maxima
+  float mx[M * 2];             // [row][token group]: tile maxima
   float al[M];                 // the tile's rescaling of each row; at the end the maxima
   const uint8_t* addr[kN];     // the rows of the tile that is requested next
   int ent[kEnts][kN];          // page entries of a tile's tokens
@@ -409,29 +420,30 @@ struct __align__(128) AttendSmem {
 // leaves its running maximum, sum and fp32 outputs in the workspace for k_latent_merge.
 //
 // A tile: 32 rows of 576 bf16 in LDS, read once from memory for all M query rows and used twice.
-//   S^T = K Q^T   wave (rg, tg): rows 16 rg .., 16 TB tokens from 16 TB tg: A = K (16-byte reads
-//                 of LDS), B = Q^T, which stays in registers
-//   P             exp2 of the scores less the rows' running maxima (joined over the token groups
-//                 in LDS), bf16, [row][token] in LDS; the sums stay fp32
+//   S^T = K Q^T   wave (rg, tg): rows 16 rg .., tokens 16 tg ..: A = K (16-byte reads of LDS),
+//                 B = Q^T, which stays in registers
+//   P             exp2 of the scores less the rows' running maxima (joined over the two token
+//                 groups in LDS), bf16, [row][token] in LDS; the sums stay fp32
 //   O^T += V^T P^T   wave w: latent values 64 w .. 64 w + 63 of every row: A = V^T by transposing
 //                 LDS reads of the same tile, B = P^T
 // bf16 rows go straight from memory to LDS, three tiles ahead; MXFP8 rows go there as they are,
 // and a pass of the workgroup turns the next tile's into bf16 (exact) beside the softmax.
 template <int M, bool MX>
 __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
+  static_assert(M == 32 || M == 64, "row blocks of 16 by two token groups on 4 or 8 waves");
   constexpr int MB = M / 16;             // row blocks
-  constexpr int TG = M < 128 ? 2 : 1;    // token groups
-  constexpr int TB = kN / 16 / TG;       // blocks of 16 tokens a wave scores
   constexpr int KS = kRow / 32;          // MFMA steps of a score: 18
-  constexpr int G = M == 32 ? 18 : M == 64 ? 6 : 2;     // of them whose keys are read at once
-  constexpr int kPieces = MX ? kMxRow / 16 : kRow * 2 / 16;  // 16-byte pieces of a row on its way: 41 or 72
-  constexpr int kLoads = (kN * kPieces + 63) / 64;           // wave loads of a tile: 21 or 36
-  constexpr int kAhead = MX ? kMxRing : kRing - 1;           // tiles on their way
+  constexpr int G = M == 32 ? 18 : 6;    // of them whose keys are read at once
+  constexpr int kPieces = kMxRow / 16;   // 16-byte pieces of an MXFP8 row: 41
+  constexpr int kMxLoads = (kN * kPieces + 63) / 64;  // wave loads of an MXFP8 tile: 21
+  constexpr int kLoads = MX ? (kMxLoads + 7) / 8 : 5;  // of a wave, at most
+  constexpr int kRowBytes = MX ? kMxRow : 2 * kRow;
+  constexpr int kAhead = MX ? kMxRing : kRing - 1;    // tiles on their way
   __shared__ AttendSmem<M, MX> sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int rg = wave % MB, tg = wave / MB;
-  const bool scores = wave < MB * TG;  // (M = 32: four waves score)
+  const bool scores = wave < 2 * MB;  // (M = 32: four waves score)
 
   // ---- the work list
   int mine = 0;
@@ -522,53 +534,72 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       const bool real = tok < lim_hi, in = (uint32_t)pg < (uint32_t)p.pages;
       lost = lost || (real && !in);
       const uint32_t row = ((uint32_t)pg << p.page_shift) + (tok & ((1 << p.page_shift) - 1));
-      return real && in ? p.cache + (uint64_t)row * (kPieces * 16) : (const uint8_t*)g_zero_row;
+      return real && in ? p.cache + (uint64_t)row * kRowBytes : (const uint8_t*)g_zero_row;
     };
     auto resolve = [&](int t) {
       const int ln = anew(lane);
       if (t < tend && wave == 7 && ln < kN) sm.addr[ln] = address(t * kN + ln, sm.ent[t % kEnts][ln]);
     };
-    // load i of wave w is number 8 i + w of the tile
-    const int mine_n = (kLoads - wave + 7) / 8;  // loads of this wave a tile
     auto issue = [&](int t, const uint8_t* const* addr) {
-      constexpr int A = (kLoads + 7) / 8;
-      uint8_t* dst = (MX ? sm.raw[(t - tile0) % kMxRing] : sm.tile[(t - tile0) % kRing]) + wave * 1024;
-      const int ln = (M < 64 ? lane : anew(lane)) + wave * 64;
-      const uint8_t* src[A];
+      if constexpr (MX) {  // load i of wave w is number 8 i + w of the tile's 1 KB pieces
+        uint8_t* dst = sm.raw[(t - tile0) % kMxRing] + wave * 1024;
+        const int ln = (M < 64 ? lane : anew(lane)) + wave * 64;
+        const uint8_t* src[kLoads];
 #pragma unroll
-      for (int i = 0; i < A; ++i) {
-        const uint32_t at = i * 512 + ln, r = at / kPieces, c = at - r * kPieces;
-        src[i] = addr[min(r, (uint32_t)kN - 1)] + ((MX ? c : c ^ swz(r)) << 4);
+        for (int i = 0; i < kLoads; ++i) {
+          const uint32_t at = i * 512 + ln, r = at / kPieces;
+          src[i] = addr[min(r, (uint32_t)kN - 1)] + ((at - r * kPieces) << 4);
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if ((i < kLoads - 1 || 8 * i + wave < kMxLoads) && i * 512 + ln < kN * kPieces)
+            lds_dma16(src[i], dst + i * 8192);
+      } else {  // wave w: the rows 4 w .. 4 w + 3, a load each and one for their rope parts
+        uint8_t* dst = sm.tile[(t - tile0) % kRing];
+        const int ln = anew(lane), own = ln & 31;
+        const uint64_t row = (uint64_t)addr[4 * wave + (own >> 3)];
+        const uint32_t lo = (uint32_t)row, hi = (uint32_t)(row >> 32);
+        const uint8_t* rope = (const uint8_t*)row + 2 * kL + (((own & 7) ^ swz_rope(4 * wave + (own >> 3))) << 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint64_t base = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, 8 * i) << 32) |
+                                (uint32_t)__builtin_amdgcn_readlane(lo, 8 * i);
+          lds_dma16((const void*)base, (ln ^ swz(4 * wave + i)) << 4, dst + (4 * wave + i) * (2 * kL));
+        }
+        if (ln < 32) lds_dma16(rope, dst + kRopeAt + 4 * wave * (2 * kR));
       }
-#pragma unroll
-      for (int i = 0; i < A; ++i)
-        if ((i < A - 1 || 8 * i + wave < kLoads) && (kN * kPieces % 64 == 0 || i * 512 + ln < kN * kPieces))
-          lds_dma16(src[i], dst + i * 8192);
     };
     // the raw rows of tile t as bf16: 16 threads a row, each the codes 16 j .. and 256 + 16 j ..
     auto unpack = [&](int t) {
       if constexpr (MX) {
-        const int th = wave * 64 + anew(lane), r = th >> 4, x = swz(r), j = th & 15;
+        const int th = wave * 64 + anew(lane), r = th >> 4, j = th & 15;
         const uint8_t* src = sm.raw[(t - tile0) % kMxRing] + r * kMxRow;
-        uint8_t* dst = sm.tile[(t - tile0) & 1] + r * (2 * kRow);
+        uint8_t* dst = sm.tile[(t - tile0) & 1];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int c = 16 * i + j;
           const u32x4 q = *(const u32x4*)(src + 16 * c);
           const float sc = e8m0(src[kL + (c >> 1)]);
-          *(u32x4*)(dst + (((2 * c) ^ x) << 4)) = fp8x8(q.x, q.y, sc);
-          *(u32x4*)(dst + (((2 * c + 1) ^ x) << 4)) = fp8x8(q.z, q.w, sc);
+          u32x4* to = (u32x4*)(dst + r * (2 * kL) + (((2 * c) ^ swz(r)) << 4));  // (swz is even)
+          to[0] = fp8x8(q.x, q.y, sc);
+          to[1] = fp8x8(q.z, q.w, sc);
         }
-        if (j < 8) *(u32x4*)(dst + (((64 + j) ^ x) << 4)) = *(const u32x4*)(src + kL + kMxScales + 16 * j);
+        if (j < 8)
+          *(u32x4*)(dst + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) =
+              *(const u32x4*)(src + kL + kMxScales + 16 * j);
       }
     };
     // waits until the tile after which `newer` more were requested has landed
     auto landed = [&](int newer) {
-      const bool more = mine_n == (kLoads + 7) / 8;
-      constexpr int A = (kLoads + 7) / 8, B = A - 1;
-      if (newer <= 0) wait_loads<0>();
-      else if (newer == 1) { if (more) wait_loads<A>(); else wait_loads<B>(); }
-      else { if (more) wait_loads<2 * A>(); else wait_loads<2 * B>(); }
+      if (newer <= 0) {
+        wait_loads<0>();
+      } else if (MX && wave >= kMxLoads % 8) {
+        if (newer == 1) wait_loads<kLoads - 1>();
+        else wait_loads<2 * (kLoads - 1)>();
+      } else {
+        if (newer == 1) wait_loads<kLoads>();
+        else wait_loads<2 * kLoads>();
+      }
     };
 
     float m = -kInf, l = 0.0f;
@@ -629,7 +660,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       if (edge) {
         for (int i = 0; i < kN / 8; ++i) {
           const int r = wave * (kN / 8) + i;
-          u32x4* at = (u32x4*)(sm.tile[0] + (tile - tiles) + r * (2 * kRow) + (lane << 4));
+          u32x4* at = (u32x4*)(sm.tile[0] + (tile - tiles) + r * (2 * kL) + (lane << 4));
           u32x4 v = *at;
           bool any = false;
 #pragma unroll
@@ -646,24 +677,22 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       }
 
       // ---- scores
-      f32x4 sc[TB];
+      f32x4 sc = {0, 0, 0, 0};
       float top = -kInf;
       if (scores) {
-        f32x4 odd = {0, 0, 0, 0};  // (a second chain of sums where one block leaves the MFMA waiting)
+        f32x4 odd = {0, 0, 0, 0};  // (a second chain of sums: one leaves the MFMA waiting)
+        // keys: this lane's row of the wave's 16, pieces 4 ks + g; read a few steps ahead, and no
+        // further: the registers are the queries'
+        const uint32_t k_at = tile + (16 * tg + col) * (2 * kL) + ((g ^ swz(col)) << 4);
+        const uint32_t r_at = tile + kRopeAt + (16 * tg + col) * (2 * kR) + ((g ^ swz_rope(col)) << 4);
+        bf16x8 a[G < KS ? 2 : 1][G];
+        auto keys = [&](int ks0, bf16x8(&to)[G]) {
 #pragma unroll
-        for (int tb = 0; tb < TB; ++tb) sc[tb] = f32x4{0, 0, 0, 0};
-        // keys: this lane's row of the wave's 16, pieces 4 ks + g
-        const int ktok = 16 * TB * tg + col;
-        const uint32_t k_even = tile + ktok * (2 * kRow) + ((g ^ swz(ktok)) << 4), k_odd = k_even ^ 64;
-        // (keys read a few steps ahead, and no further: the registers are the queries')
-        bf16x8 a[G < KS ? 2 : 1][G][TB];
-        auto keys = [&](int ks0, bf16x8(&to)[G][TB]) {
-#pragma unroll
-          for (int i = 0; i < G; ++i)
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-              to[i][tb] = lds_read<bf16x8>(((ks0 + i) & 1 ? k_odd : k_even) + ((ks0 + i) >> 1) * 128 +
-                                           tb * 16 * (2 * kRow));
+          for (int i = 0; i < G; ++i) {
+            const int ks = ks0 + i;
+            to[i] = ks < kL / 32 ? lds_read<bf16x8>((k_at ^ ((ks & 3) << 6)) + (ks >> 2) * 256)
+                                 : lds_read<bf16x8>(r_at ^ ((ks & 1) << 6));
+          }
         };
         keys(0, a[0]);
 #pragma unroll
@@ -671,29 +700,24 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           if (k0 + G < KS) keys(k0 + G, a[(k0 / G + 1) % 2]);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < G; ++i)
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb) {
-              f32x4& to = TB == 1 && ((k0 + i) & 1) ? odd : sc[tb];
-              to = mfma(a[(k0 / G) & 1][i][tb], q[k0 + i], to);
-            }
+          for (int i = 0; i < G; ++i) {
+            f32x4& to = (k0 + i) & 1 ? odd : sc;
+            to = mfma(a[(k0 / G) & 1][i], q[k0 + i], to);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (TB == 1) sc[0] += odd;
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb) {
-          const int r = 16 * TB * tg + 16 * tb + 4 * g;
+        sc = (sc + odd) * p.scale2;
+        if ((t + 1) * kN > lim_lo) {  // (rows past the tile's rows see every token before: not stored)
+          const int r = 16 * tg + 4 * g;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float v = sc[tb][k] * p.scale2;
-            if (edge && sm.bad[r + k]) v = __builtin_nanf("");
-            v = t * kN + r + k < lim ? v : -kInf;
-            sc[tb][k] = v;
-            top = fmaxf(top, v);
+            if (edge && sm.bad[r + k]) sc[k] = __builtin_nanf("");
+            if (t * kN + r + k >= lim) sc[k] = -kInf;
           }
         }
+        top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
         top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
-        if (TG == 2 && g == 0) sm.mx[(rg * 16 + col) * 2 + tg] = top;
+        if (g == 0) sm.mx[(rg * 16 + col) * 2 + tg] = top;
       }
       if constexpr (MX) landed(min(kAhead - 1, tend - 2 - t));  // raw rows of tile t + 1
       barrier();
@@ -701,39 +725,35 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       // ---- running maxima and numerators; the next tile's rows
       if (scores) {
         const int r = rg * 16 + col;
-        if (TG == 2) top = fmaxf(sm.mx[2 * r], sm.mx[2 * r + 1]);
-        const float mn = fmaxf(m, top), mu = mn == -kInf ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - mu);
-        m = mn;
-        l *= al;
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb) {
-          float e[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[tb][k] - mu);
-          l += (e[0] + e[1]) + (e[2] + e[3]);
-          *(u32x2*)(sm.p + r * kPStride + 16 * TB * tg + 16 * tb + 4 * g) =
-              u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
+        top = fmaxf(sm.mx[2 * r], sm.mx[2 * r + 1]);
+        float al = 1.0f;
+        if (top > m + kSlack) {
+          al = __builtin_amdgcn_exp2f(m - top);
+          m = top;
         }
+        const float mu = m == -kInf ? 0.0f : m;
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[k] - mu);
+        l = l * al + ((e[0] + e[1]) + (e[2] + e[3]));
+        *(u32x2*)(sm.p + r * kPStride + 16 * tg + 4 * g) = u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
         if (tg == 0 && g == 0) sm.al[r] = al;
       }
-      // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16; pieces
-      // 8 wave + 2 c + (lane % 4) / 2, which the row's swizzle permutes within 8
+      // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16, pieces
+      // 8 wave + 2 c + (lane % 4) / 2
       bf16x8 va[4];
-      auto values = [&]() {
+      {
         const int vtok = 8 * g + (col >> 2);
-        const uint32_t vx = ((((col & 3) >> 1) ^ swz(vtok)) << 4);
-        const uint32_t v_at = tile + vtok * (2 * kRow) + 128 * wave + 8 * (col & 1);
+        const uint32_t v_at = tile + vtok * (2 * kL) + (wave >> 1) * 256 + 8 * (col & 1) +
+                              (((((wave & 1) << 3) | ((col & 3) >> 1)) ^ swz(vtok)) << 4);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           struct { i16x4 a, b; } both = {
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)))),
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (MKMOE_LDS i16x4*)(uintptr_t)(v_at + (vx ^ (c << 5)) + 4 * (2 * kRow)))};
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)(v_at ^ (c << 5))),
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)((v_at ^ (c << 5)) + 4 * (2 * kL)))};
           va[c] = __builtin_bit_cast(bf16x8, both);
         }
-      };
-      if (M < 128) values();  // (with 128 rows there are no registers to hold them early)
+      }
       if constexpr (MX) {
         if (t + 1 < tend) unpack(t + 1);
         resolve(t + 1 + kAhead);
@@ -744,15 +764,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       barrier();
       // ---- outputs: the numerators' reads, then the tile after next's requests, while they come
       const uint32_t p_row = p_at + col * (2 * kPStride) + 16 * g;
-      constexpr int PB = MB < 8 ? MB : 2;
-      float al = sm.al[min(ln, M - 1)];
-      if (M == 128) al = sm.al[64 + ln] == 1.0f ? al : 0.0f;
-      bf16x8 pb[PB];
-      auto numerators = [&]() {
+      const float al = sm.al[min(ln, M - 1)];
+      bf16x8 pb[MB];
 #pragma unroll
-        for (int i = 0; i < PB; ++i) pb[i] = lds_read<bf16x8>(p_row + i * 16 * (2 * kPStride));
-      };
-      if (M < 128) numerators();
+      for (int i = 0; i < MB; ++i) pb[i] = lds_read<bf16x8>(p_row + i * 16 * (2 * kPStride));
       if constexpr (MX) {
         if (t + 1 + kAhead < tend) {
           entries(t + kAhead + 3);
@@ -765,7 +780,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         }
       }
 
-      if (M == 128) values(), numerators();
       if (!__all(al == 1.0f)) {
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
@@ -777,8 +791,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c][i] = mfma(va[c], pb[i % PB], o[c][i]);
-        if (i + PB < MB) pb[i % PB] = lds_read<bf16x8>(p_row + (i + PB) * 16 * (2 * kPStride));
+        for (int c = 0; c < 4; ++c) o[c][i] = mfma(va[c], pb[i], o[c][i]);
       }
     }
     if (lost) record(p.err, MKMOE_LATENT_ERR_PAGE, b);
@@ -788,7 +801,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     __syncthreads();
     float* sums = (float*)sm.p;  // [row][token group]
     if (scores && g == 0) {
-      sums[(rg * 16 + col) * TG + tg] = l;
+      sums[(rg * 16 + col) * 2 + tg] = l;
       if (tg == 0) sm.al[rg * 16 + col] = m;
     }
     __syncthreads();
@@ -806,7 +819,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     for (int i = 0; i < MB; ++i) {
       const int r = 16 * i + col;
       if (r >= nrows) continue;
-      const float sum = TG == 2 ? sums[2 * r] + sums[2 * r + 1] : sums[r], top = sm.al[r];
+      const float sum = sums[2 * r] + sums[2 * r + 1], top = sm.al[r];
       if (whole) {
         const int qi = over_heads(p, r0 + r), h = (r0 + r) - qi * p.heads;
         const bool none = base + qi <= 0;
@@ -1173,11 +1186,10 @@ int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_by
   p.scale2 = io->scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
   const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8;
-  // the fewest query rows a tile that hold a sequence's on average, at most 128
+  // 32 query rows a tile where a sequence has no more of them on average, else 64
   const int64_t rows = ((int64_t)io->tokens * io->heads + io->seqs - 1) / io->seqs;
   if (rows <= 32) return mx ? attend<32, true>(p, st) : attend<32, false>(p, st);
-  if (rows <= 64) return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
-  return mx ? attend<128, true>(p, st) : attend<128, false>(p, st);
+  return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
 }
 
 int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream) {
