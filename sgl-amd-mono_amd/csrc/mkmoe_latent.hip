@@ -18,6 +18,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/mkmoe.h"
 #include "mkmoe_numerics.h"
 
@@ -259,9 +261,9 @@ constexpr int kRing = 4;        // bf16 cache: tiles in LDS, one in use and thre
 constexpr int kMxRing = 3;      // MXFP8: raw tiles on their way
 constexpr int kSetup = 3;       // see setup()
 constexpr int kEnts = 4;        // tiles whose page entries are in LDS
-// a row's maximum is moved where a score passes it by more than 2^kSlack: numerators then stay below
-// 2^kSlack (bf16 and fp32 keep their relative precision there), and after the first tiles almost no
-// tile rescales the outputs (with kSlack 0 the 64 rows' products were half of a tile's VALU work)
+// A row's maximum is moved only where a score passes it by more than 2^kSlack: numerators then stay
+// below 2^kSlack (bf16 and fp32 keep their relative precision there). After the first tiles almost
+// none does, so that the waves need not agree on a tile's maxima before its numerators, nor rescale
 constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
@@ -402,14 +404,15 @@ template <int M, bool MX>
 struct __align__(256) AttendSmem {
   uint8_t tile[MX ? 2 : kRing][kTileBytes];  // cached rows, bf16, swizzled pieces
   uint8_t raw[MX ? kMxRing : 1][MX ? kN * kMxRow : 16];
-  uint16_t p[M * kPStride];    // softmax numerators of the tile [row][token]
+  uint16_t p[MX ? 1 : 2][M * kPStride];  // softmax numerators of a tile [row][token]
   float mx[M * 2];             // [row][token group]: tile maxima
   float al[M];                 // the tile's rescaling of each row; at the end the maxima
-  const uint8_t* addr[kN];     // the rows of the tile that is requested next
+  const uint8_t* addr[2][kN];  // the rows of the tile that is requested next
   int ent[kEnts][kN];          // page entries of a tile's tokens
   int start[kMaxSeqs];         // first tile of each sequence in the work
   int scan[8];
   int first[4];                // the share's first sequence: its number, t0, n, len
+  int moved[3];                // a tile's flag: some row's maximum has to move
   uint8_t bad[kN];             // tokens of the tile with a non-finite latent value
 };
 
@@ -487,7 +490,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   __syncthreads();
 
   const uint32_t tiles = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)sm.tile[0];
-  const uint32_t p_at = (uint32_t)(uintptr_t)(MKMOE_LDS uint16_t*)sm.p;
+  const uint32_t p_at = (uint32_t)(uintptr_t)(MKMOE_LDS uint16_t*)sm.p[0];
 
   int b = __builtin_amdgcn_readfirstlane(sm.first[0]);
   Seq s = {__builtin_amdgcn_readfirstlane(sm.first[1]), __builtin_amdgcn_readfirstlane(sm.first[2]),
@@ -524,7 +527,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     }
 
     // ---- a tile's rows on their way. Its page entries come first, to the last wave (whose other
-    // loads are the fewest), which turns them into the rows' addresses a tile before the loads
+    // loads are the fewest), which turns them into the rows' addresses well before the loads
     auto entries = [&](int t) {
       const int ln = anew(lane), tok = min(t * kN + ln, lim_hi - 1);
       if (wave == 7 && ln < kN) lds_dma4(table + (tok >> p.page_shift), sm.ent[t % kEnts]);
@@ -538,7 +541,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     };
     auto resolve = [&](int t) {
       const int ln = anew(lane);
-      if (t < tend && wave == 7 && ln < kN) sm.addr[ln] = address(t * kN + ln, sm.ent[t % kEnts][ln]);
+      if (wave == 7 && ln < kN) sm.addr[t & 1][ln] = address(t * kN + ln, sm.ent[t % kEnts][ln]);
     };
     auto issue = [&](int t, const uint8_t* const* addr) {
       if constexpr (MX) {  // load i of wave w is number 8 i + w of the tile's 1 KB pieces
@@ -569,24 +572,32 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         if (ln < 32) lds_dma16(rope, dst + kRopeAt + 4 * wave * (2 * kR));
       }
     };
-    // the raw rows of tile t as bf16: 16 threads a row, each the codes 16 j .. and 256 + 16 j ..
-    auto unpack = [&](int t) {
+    // the raw rows of tile t as bf16, by kBy threads (numbered th): kBy / 32 a row, the codes
+    // 16 j .. of every kBy / 32 pieces each
+    auto unpack = [&](int t, int th, auto by) {
       if constexpr (MX) {
-        const int th = wave * 64 + anew(lane), r = th >> 4, j = th & 15;
+        constexpr int A = decltype(by)::value / kN;
+        const int r = th / A, j = th % A;
         const uint8_t* src = sm.raw[(t - tile0) % kMxRing] + r * kMxRow;
         uint8_t* dst = sm.tile[(t - tile0) & 1];
+        u32x4 q[32 / A], pe;
+        float sc[32 / A];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = 16 * i + j;
-          const u32x4 q = *(const u32x4*)(src + 16 * c);
-          const float sc = e8m0(src[kL + (c >> 1)]);
-          u32x4* to = (u32x4*)(dst + r * (2 * kL) + (((2 * c) ^ swz(r)) << 4));  // (swz is even)
-          to[0] = fp8x8(q.x, q.y, sc);
-          to[1] = fp8x8(q.z, q.w, sc);
+        for (int i = 0; i < 32 / A; ++i) {
+          q[i] = *(const u32x4*)(src + 16 * (A * i + j));
+          sc[i] = e8m0(src[kL + ((A * i + j) >> 1)]);
         }
-        if (j < 8)
-          *(u32x4*)(dst + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) =
-              *(const u32x4*)(src + kL + kMxScales + 16 * j);
+        pe = *(const u32x4*)(src + kL + kMxScales + 16 * (j & 7));
+#pragma unroll
+        for (int i = 0; i < 32 / A; ++i) {
+          u32x4* to = (u32x4*)(dst + r * (2 * kL) + (((2 * (A * i + j)) ^ swz(r)) << 4));  // (swz is even)
+          const u32x4 v0 = fp8x8(q[i].x, q[i].y, sc[i]), v1 = fp8x8(q[i].z, q[i].w, sc[i]);
+          // (odd lanes store their second half first: either store then meets every bank once)
+          const bool odd = j & 1;
+          to[odd] = odd ? v1 : v0;
+          to[!odd] = odd ? v0 : v1;
+        }
+        if (j < 8) *(u32x4*)(dst + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) = pe;
       }
     };
     // waits until the tile after which `newer` more were requested has landed
@@ -611,9 +622,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 
     // ---- the first tiles' rows, and the queries into registers
     __syncthreads();  // the last row tile's reads of LDS are over
-    const uint8_t** first = (const uint8_t**)sm.p;  // [kAhead][kN] (P is not in use yet)
+    const uint8_t** first = (const uint8_t**)sm.p[0];  // [kAhead][kN] (P is not in use yet)
     static_assert(M * kPStride * 2 >= kAhead * kN * 8, "the first tiles' addresses fit into P");
-    const bool entry = tid < (kAhead + 2) * kN;
+    const bool entry = tid < (kAhead + 3) * kN;
     const int tok0 = tile0 * kN + tid;
     const int pg0 = entry ? table[min(tok0, lim_hi - 1) >> p.page_shift] : 0;
     // (a row past the tile's rows takes the first one's query: it sees no token and is not stored)
@@ -635,28 +646,33 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       if (tid < kAhead * kN) first[tid] = address(tok0, pg0);
       else sm.ent[t % kEnts][tid % kN] = pg0;
     }
+    if (tid < 3) sm.moved[tid] = 0;
     barrier();
     issue(tile0, first);
-    wait_queries();  // and the first tile
-    for (int i = 1; i < kAhead && tile0 + i < tend; ++i) issue(tile0 + i, first + i * kN);
+    if (MX && tile0 + 1 < tend) issue(tile0 + 1, first + kN);
+    wait_queries();  // and the first tile (MXFP8: two)
+    for (int i = MX ? 2 : 1; i < kAhead && tile0 + i < tend; ++i) issue(tile0 + i, first + i * kN);
+    if (tile0 + kAhead < tend) resolve(tile0 + kAhead);
+    if (MX && tile0 + kAhead + 1 < tend) resolve(tile0 + kAhead + 1);
     barrier();
     if constexpr (MX) {
-      unpack(tile0);
-      resolve(tile0 + kAhead);
+      unpack(tile0, tid, std::integral_constant<int, kThreads>{});
       barrier();
       if (tile0 + kAhead < tend) {
-        entries(tile0 + kAhead + 2);
-        issue(tile0 + kAhead, sm.addr);
+        entries(tile0 + kAhead + 3);
+        issue(tile0 + kAhead, sm.addr[(tile0 + kAhead) & 1]);
       }
     }
 
-    for (int t = tile0; t < tend; ++t) {
+    // One tile. Steady: every row sees all of it, and the tiles that its requests are for exist
+    auto step = [&](int t, auto is_steady) __attribute__((always_inline)) {
+      constexpr bool steady = decltype(is_steady)::value;
       const int ln = anew(lane), col = ln & 15, g = ln >> 4;
       const uint32_t tile = tiles + (MX ? (t - tile0) & 1 : (t - tile0) % kRing) * kTileBytes;
 
       // tokens that only some of the rows see: their non-finite values must not reach the
       // others through 0 * V. They are cleared, and the rows that see them become NaN below
-      const bool edge = lim_lo < lim_hi && (t + 1) * kN > lim_lo;
+      const bool edge = !steady && lim_lo < lim_hi && (t + 1) * kN > lim_lo;
       if (edge) {
         for (int i = 0; i < kN / 8; ++i) {
           const int r = wave * (kN / 8) + i;
@@ -676,9 +692,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         barrier();
       }
 
-      // ---- scores
+      // ---- scores, and the numerators under the maximum so far
+      const uint32_t p_to = p_at + (MX ? 0 : (t & 1) * (M * kPStride * 2));
       f32x4 sc = {0, 0, 0, 0};
-      float top = -kInf;
+      float top = -kInf, sum = 0.0f;
+      auto numerators = [&]() {
+        const float mu = m == -kInf ? 0.0f : m;
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[k] - mu);
+        sum = (e[0] + e[1]) + (e[2] + e[3]);
+        *(MKMOE_LDS u32x2*)(uintptr_t)(p_to + (rg * 16 + col) * (2 * kPStride) + 32 * tg + 8 * g) =
+            u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
+      };
       if (scores) {
         f32x4 odd = {0, 0, 0, 0};  // (a second chain of sums: one leaves the MFMA waiting)
         // keys: this lane's row of the wave's 16, pieces 4 ks + g; read a few steps ahead, and no
@@ -707,7 +733,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           __builtin_amdgcn_sched_barrier(0);
         }
         sc = (sc + odd) * p.scale2;
-        if ((t + 1) * kN > lim_lo) {  // (rows past the tile's rows see every token before: not stored)
+        if (!steady && (t + 1) * kN > lim_lo) {  // (rows past the tile's rows see every token before: not stored)
           const int r = 16 * tg + 4 * g;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -716,28 +742,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           }
         }
         top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-        top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
-        if (g == 0) sm.mx[(rg * 16 + col) * 2 + tg] = top;
+        numerators();
+        if (__any(top > m + kSlack) && lane == 0) sm.moved[t % 3] = 1;
       }
-      if constexpr (MX) landed(min(kAhead - 1, tend - 2 - t));  // raw rows of tile t + 1
-      barrier();
-
-      // ---- running maxima and numerators; the next tile's rows
-      if (scores) {
-        const int r = rg * 16 + col;
-        top = fmaxf(sm.mx[2 * r], sm.mx[2 * r + 1]);
-        float al = 1.0f;
-        if (top > m + kSlack) {
-          al = __builtin_amdgcn_exp2f(m - top);
-          m = top;
-        }
-        const float mu = m == -kInf ? 0.0f : m;
-        float e[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[k] - mu);
-        l = l * al + ((e[0] + e[1]) + (e[2] + e[3]));
-        *(u32x2*)(sm.p + r * kPStride + 16 * tg + 4 * g) = u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
-        if (tg == 0 && g == 0) sm.al[r] = al;
+      if (tid == 0) sm.moved[(t + 1) % 3] = 0;  // (last read before the last barrier)
+      // MXFP8: the next tile takes the place of t - 1; with 32 query rows the waves that score nothing
+      // unpack it meanwhile
+      if (MX && (steady || t + 1 < tend)) {
+        if (M == 64) unpack(t + 1, wave * 64 + ln, std::integral_constant<int, kThreads>{});
+        else if (!scores) unpack(t + 1, (wave - 4) * 64 + ln, std::integral_constant<int, kThreads / 2>{});
       }
       // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16, pieces
       // 8 wave + 2 c + (lane % 4) / 2
@@ -754,33 +767,31 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           va[c] = __builtin_bit_cast(bf16x8, both);
         }
       }
-      if constexpr (MX) {
-        if (t + 1 < tend) unpack(t + 1);
-        resolve(t + 1 + kAhead);
-      } else {
-        landed(min(kAhead - 2, tend - 2 - t));  // tile t + 1
-        resolve(t + kAhead);
-      }
+      // tile t + 1 is there at the barrier, and the one that takes the place of t - 1 (MXFP8: of the raw
+      // t + 1) is requested after it
+      if (!MX) landed(steady ? kAhead - 2 : min(kAhead - 2, tend - 2 - t));
       barrier();
-      // ---- outputs: the numerators' reads, then the tile after next's requests, while they come
-      const uint32_t p_row = p_at + col * (2 * kPStride) + 16 * g;
-      const float al = sm.al[min(ln, M - 1)];
-      bf16x8 pb[MB];
-#pragma unroll
-      for (int i = 0; i < MB; ++i) pb[i] = lds_read<bf16x8>(p_row + i * 16 * (2 * kPStride));
-      if constexpr (MX) {
-        if (t + 1 + kAhead < tend) {
-          entries(t + kAhead + 3);
-          issue(t + 1 + kAhead, sm.addr);
-        }
-      } else {
-        if (t + kAhead < tend) {
-          entries(t + kAhead + 2);
-          issue(t + kAhead, sm.addr);
-        }
-      }
+      if (steady || t + kAhead + (MX ? 2 : 1) < tend) resolve(t + kAhead + (MX ? 2 : 1));
 
-      if (!__all(al == 1.0f)) {
+      if (__builtin_amdgcn_readfirstlane(sm.moved[t % 3])) {  // maxima move: the numerators again
+        if (scores) {
+          top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
+          if (g == 0) sm.mx[(rg * 16 + col) * 2 + tg] = top;
+        }
+        barrier();
+        if (scores) {
+          const int r = rg * 16 + col;
+          top = fmaxf(sm.mx[2 * r], sm.mx[2 * r + 1]);
+          float al = 1.0f;
+          if (top > m + kSlack) {
+            al = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+          }
+          l *= al;
+          numerators();
+          if (tg == 0 && g == 0) sm.al[r] = al;
+        }
+        barrier();
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           const float alpha = sm.al[16 * i + col];
@@ -788,18 +799,38 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           for (int c = 0; c < 4; ++c) o[c][i] *= alpha;
         }
       }
+
+      l += sum;
+
+      // ---- outputs; the next rows' requests while the numerators come
+      bf16x8 pb[MB];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) pb[i] = lds_read<bf16x8>(p_to + col * (2 * kPStride) + 16 * g + i * 16 * (2 * kPStride));
+      constexpr int kNext = kAhead + (MX ? 1 : 0);
+      if (steady || t + kNext < tend) {
+        entries(t + kNext + 3);
+        issue(t + kNext, sm.addr[(t + kNext) & 1]);
+      }
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[c][i] = mfma(va[c], pb[i], o[c][i]);
       }
-    }
+      if constexpr (MX) {  // the raw rows of t + 2 are there at the barrier
+        landed(steady ? kAhead - 1 : min(kAhead - 1, tend - 3 - t));
+        barrier();
+      }
+    };
+    const int steady_end = min(tend - kAhead - 1, lim_lo / kN);
+    int t = tile0;
+    for (; t < steady_end; ++t) step(t, std::true_type{});
+    for (; t < tend; ++t) step(t, std::false_type{});
     if (lost) record(p.err, MKMOE_LATENT_ERR_PAGE, b);
 
     // ---- the row sums, then the rows out
     l = over_groups(l, [](float a, float b) { return a + b; });
     __syncthreads();
-    float* sums = (float*)sm.p;  // [row][token group]
+    float* sums = (float*)sm.p[0];  // [row][token group]
     if (scores && g == 0) {
       sums[(rg * 16 + col) * 2 + tg] = l;
       if (tg == 0) sm.al[rg * 16 + col] = m;
