@@ -423,30 +423,37 @@ struct __align__(256) AttendSmem {
 // leaves its running maximum, sum and fp32 outputs in the workspace for k_latent_merge.
 //
 // A tile: 32 rows of 576 bf16 in LDS, read once from memory for all M query rows and used twice.
-//   S^T = K Q^T   wave (rg, tg): rows 16 rg .., tokens 16 tg ..: A = K (16-byte reads of LDS),
+// Waves 0 .. 3 score, waves 4 .. 7 bring the tiles; both share the outputs' columns so that the
+// registers hold (a scoring wave has the queries there) and the MFMA has as much of either:
+//   S^T = K Q^T   scoring wave (rg, tg): the rows of half rg, tokens 16 tg ..: A = K (16-byte
+//                 reads of LDS, which bound this step: with 64 rows each serves two row blocks),
 //                 B = Q^T, which stays in registers
-//   P             exp2 of the scores less the rows' running maxima (joined over the two token
-//                 groups in LDS), bf16, [row][token] in LDS; the sums stay fp32
-//   O^T += V^T P^T   wave w: latent values 64 w .. 64 w + 63 of every row: A = V^T by transposing
-//                 LDS reads of the same tile, B = P^T
+//   P             exp2 of the scores less the rows' running maxima (moved for both token groups
+//                 at once), bf16, [row][token] in LDS; the sums stay fp32
+//   O^T += V^T P^T   latent values 32 w .. of a scoring wave (32 of them), 128 + 96 l .. of the others
+//                 (96), for every row: A = V^T by transposing LDS reads of the same tile, B = P^T
 // bf16 rows go straight from memory to LDS, three tiles ahead; MXFP8 rows go there as they are,
-// and a pass of the workgroup turns the next tile's into bf16 (exact) beside the softmax.
-template <int M, bool MX>
+// and waves 4 .. 7 turn the next tile's into bf16 (exact) while waves 0 .. 3 score.
+// PAGED: pages of kN tokens or more, so that a tile lies in one and its rows follow each other;
+// without it each token's page entry is looked up.
+template <int M, bool MX, bool PAGED>
 __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   static_assert(M == 32 || M == 64, "row blocks of 16 by two token groups on 4 or 8 waves");
   constexpr int MB = M / 16;             // row blocks
+  constexpr int RB = MB / 2;             // row blocks of a scoring wave
   constexpr int KS = kRow / 32;          // MFMA steps of a score: 18
-  constexpr int G = M == 32 ? 18 : 6;    // of them whose keys are read at once
+  constexpr int G = M == 32 ? 9 : 3;     // of them whose keys are read at once
   constexpr int kPieces = kMxRow / 16;   // 16-byte pieces of an MXFP8 row: 41
   constexpr int kMxLoads = (kN * kPieces + 63) / 64;  // wave loads of an MXFP8 tile: 21
-  constexpr int kLoads = MX ? (kMxLoads + 7) / 8 : 5;  // of a wave, at most
+  constexpr int kLoads = MX ? (kMxLoads + 3) / 4 : 9;  // of a wave, at most
   constexpr int kRowBytes = MX ? kMxRow : 2 * kRow;
   constexpr int kAhead = MX ? kMxRing : kRing - 1;    // tiles on their way
   __shared__ AttendSmem<M, MX> sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int rg = wave % MB, tg = wave / MB;
-  const bool scores = wave < 2 * MB;  // (M = 32: four waves score)
+  const bool scores = wave < 4;
+  const int rg = wave & 1, tg = (wave >> 1) & 1;  // of a scoring wave
+  const int lw = wave & 3;                        // of the others: their number
 
   // ---- the work list
   int mine = 0;
@@ -529,8 +536,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     // ---- a tile's rows on their way. Its page entries come first, to the last wave (whose other
     // loads are the fewest), which turns them into the rows' addresses well before the loads
     auto entries = [&](int t) {
-      const int ln = anew(lane), tok = min(t * kN + ln, lim_hi - 1);
-      if (wave == 7 && ln < kN) lds_dma4(table + (tok >> p.page_shift), sm.ent[t % kEnts]);
+      if constexpr (!PAGED) {
+        const int ln = anew(lane), tok = min(t * kN + ln, lim_hi - 1);
+        if (wave == 7 && ln < kN) lds_dma4(table + (tok >> p.page_shift), sm.ent[t % kEnts]);
+      }
     };
     bool lost = false;  // a page outside the cache
     auto address = [&](int tok, int pg) -> const uint8_t* {
@@ -540,71 +549,106 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       return real && in ? p.cache + (uint64_t)row * kRowBytes : (const uint8_t*)g_zero_row;
     };
     auto resolve = [&](int t) {
-      const int ln = anew(lane);
-      if (wave == 7 && ln < kN) sm.addr[t & 1][ln] = address(t * kN + ln, sm.ent[t % kEnts][ln]);
-    };
-    auto issue = [&](int t, const uint8_t* const* addr) {
-      if constexpr (MX) {  // load i of wave w is number 8 i + w of the tile's 1 KB pieces
-        uint8_t* dst = sm.raw[(t - tile0) % kMxRing] + wave * 1024;
-        const int ln = (M < 64 ? lane : anew(lane)) + wave * 64;
-        const uint8_t* src[kLoads];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const uint32_t at = i * 512 + ln, r = at / kPieces;
-          src[i] = addr[min(r, (uint32_t)kN - 1)] + ((at - r * kPieces) << 4);
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          if ((i < kLoads - 1 || 8 * i + wave < kMxLoads) && i * 512 + ln < kN * kPieces)
-            lds_dma16(src[i], dst + i * 8192);
-      } else {  // wave w: the rows 4 w .. 4 w + 3, a load each and one for their rope parts
-        uint8_t* dst = sm.tile[(t - tile0) % kRing];
-        const int ln = anew(lane), own = ln & 31;
-        const uint64_t row = (uint64_t)addr[4 * wave + (own >> 3)];
-        const uint32_t lo = (uint32_t)row, hi = (uint32_t)(row >> 32);
-        const uint8_t* rope = (const uint8_t*)row + 2 * kL + (((own & 7) ^ swz_rope(4 * wave + (own >> 3))) << 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint64_t base = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, 8 * i) << 32) |
-                                (uint32_t)__builtin_amdgcn_readlane(lo, 8 * i);
-          lds_dma16((const void*)base, (ln ^ swz(4 * wave + i)) << 4, dst + (4 * wave + i) * (2 * kL));
-        }
-        if (ln < 32) lds_dma16(rope, dst + kRopeAt + 4 * wave * (2 * kR));
+      if constexpr (!PAGED) {
+        const int ln = anew(lane);
+        if (wave == 7 && ln < kN) sm.addr[t & 1][ln] = address(t * kN + ln, sm.ent[t % kEnts][ln]);
       }
     };
-    // the raw rows of tile t as bf16, by kBy threads (numbered th): kBy / 32 a row, the codes
-    // 16 j .. of every kBy / 32 pieces each
-    auto unpack = [&](int t, int th, auto by) {
+    // (PAGED) the page of tile t, by a scalar load
+    typedef const int32_t __attribute__((address_space(4))) scalar_int;
+    scalar_int* s_table = (scalar_int*)(uintptr_t)table;
+    auto page_of = [&](int t) -> int {
+      return PAGED ? s_table[min(t * kN, lim_hi - 1) >> p.page_shift] : 0;
+    };
+    // requests tile t: PAGED by its page, else by its rows' addresses in addr. whole: all its tokens
+    // are there
+    auto issue = [&](int t, int pg, const uint8_t* const* addr, bool whole) {
+      const bool in = !PAGED || (uint32_t)pg < (uint32_t)p.pages;
+      const uint8_t* base = nullptr;
+      const int left = whole ? kN : lim_hi - t * kN;
+      if (PAGED) {
+        lost = lost || !in;
+        const uint32_t row = ((uint32_t)pg << p.page_shift) + ((t * kN) & ((1 << p.page_shift) - 1));
+        base = p.cache + (uint64_t)row * kRowBytes;
+      }
+      if constexpr (MX) {  // load i of wave l is number 4 i + l of the tile's 1 KB pieces
+        uint8_t* dst = sm.raw[(t - tile0) % kMxRing] + lw * 1024;
+        const int ln = anew(lane) + lw * 64;
+        if (PAGED && whole && in) {
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i)
+            if ((i < kLoads - 1 || 4 * i + lw < kMxLoads) && i * 256 + ln < kN * kPieces)
+              lds_dma16(base, (i * 256 + ln) << 4, dst + i * 4096);
+        } else {
+          const uint8_t* src[kLoads];
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const uint32_t at = i * 256 + ln, r = min(at / kPieces, (uint32_t)kN - 1);
+            const uint8_t* row = !PAGED ? addr[r] : in && (int)r < left ? base + r * kRowBytes : (const uint8_t*)g_zero_row;
+            src[i] = row + ((at - r * kPieces) << 4);
+          }
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i)
+            if ((i < kLoads - 1 || 4 * i + lw < kMxLoads) && i * 256 + ln < kN * kPieces)
+              lds_dma16(src[i], dst + i * 4096);
+        }
+      } else {  // wave l: the rows 8 l .. 8 l + 7, a load each and one for their rope parts
+        uint8_t* dst = sm.tile[(t - tile0) % kRing];
+        const int ln = anew(lane), r = 8 * lw + (ln >> 3);
+        const uint32_t rope_at = 2 * kL + (((ln & 7) ^ swz_rope(r)) << 4);
+        const uint64_t row = PAGED ? 0 : (uint64_t)addr[r];
+        const uint32_t lo = (uint32_t)row, hi = (uint32_t)(row >> 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint8_t* from;
+          if (PAGED)
+            from = in && 8 * lw + i < left ? base + (8 * lw + i) * kRowBytes : (const uint8_t*)g_zero_row;
+          else
+            from = (const uint8_t*)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, 8 * i) << 32) |
+                                    (uint32_t)__builtin_amdgcn_readlane(lo, 8 * i));
+          lds_dma16(from, (ln ^ swz(8 * lw + i)) << 4, dst + (8 * lw + i) * (2 * kL));
+        }
+        uint8_t* rope_to = dst + kRopeAt + 8 * lw * (2 * kR);
+        if (PAGED && whole && in) {
+          lds_dma16(base, r * kRowBytes + rope_at, rope_to);
+        } else {
+          const uint8_t* from = !PAGED ? (const uint8_t*)row : in && r < left ? base + r * kRowBytes : (const uint8_t*)g_zero_row;
+          lds_dma16(from + rope_at, rope_to);
+        }
+      }
+    };
+    // (waves 4 .. 7) the raw rows of tile t as bf16: 8 threads a row, the codes 16 j .. of every 8
+    // pieces each
+    auto unpack = [&](int t) {
       if constexpr (MX) {
-        constexpr int A = decltype(by)::value / kN;
-        const int r = th / A, j = th % A;
+        const int th = lw * 64 + anew(lane), r = th >> 3, j = th & 7;
         const uint8_t* src = sm.raw[(t - tile0) % kMxRing] + r * kMxRow;
         uint8_t* dst = sm.tile[(t - tile0) & 1];
-        u32x4 q[32 / A], pe;
-        float sc[32 / A];
+        u32x4 q[4];
+        float sc[4];
 #pragma unroll
-        for (int i = 0; i < 32 / A; ++i) {
-          q[i] = *(const u32x4*)(src + 16 * (A * i + j));
-          sc[i] = e8m0(src[kL + ((A * i + j) >> 1)]);
+        for (int i = 0; i < 4; ++i) {
+          q[i] = *(const u32x4*)(src + 16 * (8 * i + j));
+          sc[i] = e8m0(src[kL + 4 * i + (j >> 1)]);
         }
-        pe = *(const u32x4*)(src + kL + kMxScales + 16 * (j & 7));
+        const u32x4 pe = *(const u32x4*)(src + kL + kMxScales + 16 * j);
 #pragma unroll
-        for (int i = 0; i < 32 / A; ++i) {
-          u32x4* to = (u32x4*)(dst + r * (2 * kL) + (((2 * (A * i + j)) ^ swz(r)) << 4));  // (swz is even)
+        for (int i = 0; i < 4; ++i) {
+          u32x4* to = (u32x4*)(dst + r * (2 * kL) + (((2 * (8 * i + j)) ^ swz(r)) << 4));  // (swz is even)
           const u32x4 v0 = fp8x8(q[i].x, q[i].y, sc[i]), v1 = fp8x8(q[i].z, q[i].w, sc[i]);
           // (odd lanes store their second half first: either store then meets every bank once)
           const bool odd = j & 1;
           to[odd] = odd ? v1 : v0;
           to[!odd] = odd ? v0 : v1;
         }
-        if (j < 8) *(u32x4*)(dst + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) = pe;
+        *(u32x4*)(dst + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) = pe;
       }
     };
     // waits until the tile after which `newer` more were requested has landed
     auto landed = [&](int newer) {
       if (newer <= 0) {
         wait_loads<0>();
-      } else if (MX && wave >= kMxLoads % 8) {
+      } else if (MX && lw >= kMxLoads % 4) {
         if (newer == 1) wait_loads<kLoads - 1>();
         else wait_loads<2 * (kLoads - 1)>();
       } else {
@@ -613,105 +657,165 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       }
     };
 
-    float m = -kInf, l = 0.0f;
-    f32x4 o[4][MB];
+    // ---- what both kinds of wave do with a tile
+    auto tile_at = [&](int t) { return tiles + (MX ? (t - tile0) & 1 : (t - tile0) % kRing) * kTileBytes; };
+    auto p_of = [&](int t) { return p_at + (MX ? 0 : (t & 1) * (M * kPStride * 2)); };
+    // tokens that only some of the rows see: their non-finite values must not reach the others
+    // through 0 * V. They are cleared, and the rows that see them become NaN
+    const bool edges = lim_lo < lim_hi;
+    auto sanitize = [&](int t) {
+      for (int i = 0; i < kN / 8; ++i) {
+        const int r = wave * (kN / 8) + i;
+        u32x4* at = (u32x4*)(sm.tile[0] + (tile_at(t) - tiles) + r * (2 * kL) + (lane << 4));
+        u32x4 v = *at;
+        bool any = false;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < MB; ++i) o[c][i] = f32x4{0, 0, 0, 0};
-
-    // ---- the first tiles' rows, and the queries into registers
-    __syncthreads();  // the last row tile's reads of LDS are over
-    const uint8_t** first = (const uint8_t**)sm.p[0];  // [kAhead][kN] (P is not in use yet)
-    static_assert(M * kPStride * 2 >= kAhead * kN * 8, "the first tiles' addresses fit into P");
-    const bool entry = tid < (kAhead + 3) * kN;
-    const int tok0 = tile0 * kN + tid;
-    const int pg0 = entry ? table[min(tok0, lim_hi - 1) >> p.page_shift] : 0;
-    // (a row past the tile's rows takes the first one's query: it sees no token and is not stored)
-    bf16x8 q[KS];
-    int lim = 0;
-    {
-      const int r = rg * 16 + col;
-      const bool real = scores && r < nrows;
-      const int i = over_heads(p, r0 + (real ? r : 0)), h = r0 + (real ? r : 0) - i * p.heads;
-      if (real) lim = max(0, base + i);
-      const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)h * p.ql_hs + 8 * g;
-      const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)h * p.qp_hs + 8 * g;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        q[ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
-    }
-    if (entry) {
-      const int t = tile0 + tid / kN;
-      if (tid < kAhead * kN) first[tid] = address(tok0, pg0);
-      else sm.ent[t % kEnts][tid % kN] = pg0;
-    }
-    if (tid < 3) sm.moved[tid] = 0;
-    barrier();
-    issue(tile0, first);
-    if (MX && tile0 + 1 < tend) issue(tile0 + 1, first + kN);
-    wait_queries();  // and the first tile (MXFP8: two)
-    for (int i = MX ? 2 : 1; i < kAhead && tile0 + i < tend; ++i) issue(tile0 + i, first + i * kN);
-    if (tile0 + kAhead < tend) resolve(tile0 + kAhead);
-    if (MX && tile0 + kAhead + 1 < tend) resolve(tile0 + kAhead + 1);
-    barrier();
-    if constexpr (MX) {
-      unpack(tile0, tid, std::integral_constant<int, kThreads>{});
-      barrier();
-      if (tile0 + kAhead < tend) {
-        entries(tile0 + kAhead + 3);
-        issue(tile0 + kAhead, sm.addr[(tile0 + kAhead) & 1]);
-      }
-    }
-
-    // One tile. Steady: every row sees all of it, and the tiles that its requests are for exist
-    auto step = [&](int t, auto is_steady) __attribute__((always_inline)) {
-      constexpr bool steady = decltype(is_steady)::value;
-      const int ln = anew(lane), col = ln & 15, g = ln >> 4;
-      const uint32_t tile = tiles + (MX ? (t - tile0) & 1 : (t - tile0) % kRing) * kTileBytes;
-
-      // tokens that only some of the rows see: their non-finite values must not reach the
-      // others through 0 * V. They are cleared, and the rows that see them become NaN below
-      const bool edge = !steady && lim_lo < lim_hi && (t + 1) * kN > lim_lo;
-      if (edge) {
-        for (int i = 0; i < kN / 8; ++i) {
-          const int r = wave * (kN / 8) + i;
-          u32x4* at = (u32x4*)(sm.tile[0] + (tile - tiles) + r * (2 * kL) + (lane << 4));
-          u32x4 v = *at;
-          bool any = false;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if ((v[k] & 0x7f80u) == 0x7f80u) any = true, v[k] &= 0xffff0000u;
-            if ((v[k] & 0x7f800000u) == 0x7f800000u) any = true, v[k] &= 0x0000ffffu;
-          }
-          if (t * kN + r < lim_lo) any = false;
-          if (any) *at = v;
-          const bool some = __any(any);
-          if (lane == 0) sm.bad[r] = some;
+        for (int k = 0; k < 4; ++k) {
+          if ((v[k] & 0x7f80u) == 0x7f80u) any = true, v[k] &= 0xffff0000u;
+          if ((v[k] & 0x7f800000u) == 0x7f800000u) any = true, v[k] &= 0x0000ffffu;
         }
-        barrier();
+        if (t * kN + r < lim_lo) any = false;
+        if (any) *at = v;
+        const bool some = __any(any);
+        if (lane == 0) sm.bad[r] = some;
       }
-
-      // ---- scores, and the numerators under the maximum so far
-      const uint32_t p_to = p_at + (MX ? 0 : (t & 1) * (M * kPStride * 2));
-      f32x4 sc = {0, 0, 0, 0};
-      float top = -kInf, sum = 0.0f;
-      auto numerators = [&]() {
-        const float mu = m == -kInf ? 0.0f : m;
-        float e[4];
+      barrier();
+    };
+    // V^T of 16 C latent values from piece first (a multiple of 4): rows 8 g + col / 4 (and + 4), 4 values
+    // from 4 (lane % 4) of each 16
+    auto values = [&](uint32_t tile, int first, auto& va) {
+      const int ln = anew(lane), vtok = 8 * (ln >> 4) + ((ln & 15) >> 2);
+      const uint32_t x = (((ln & 3) >> 1) ^ swz(vtok)) << 4, row = tile + vtok * (2 * kL) + 8 * (ln & 1);
+      constexpr int C = sizeof(va) / sizeof(va[0]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[k] - mu);
-        sum = (e[0] + e[1]) + (e[2] + e[3]);
-        *(MKMOE_LDS u32x2*)(uintptr_t)(p_to + (rg * 16 + col) * (2 * kPStride) + 32 * tg + 8 * g) =
-            u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
-      };
-      if (scores) {
-        f32x4 odd = {0, 0, 0, 0};  // (a second chain of sums: one leaves the MFMA waiting)
+      for (int c = 0; c < C; ++c) {
+        const int piece = first + 2 * c;
+        const uint32_t at = (x ^ ((piece & 15) << 4)) + (row + (piece >> 4) * 256);
+        struct { i16x4 a, b; } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)at),
+                                       __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (MKMOE_LDS i16x4*)(uintptr_t)(at + 4 * (2 * kL)))};
+        va[c] = __builtin_bit_cast(bf16x8, both);
+      }
+    };
+    auto numerators_of = [&](int t, bf16x8(&pb)[MB]) {
+      const int ln = anew(lane);
+      const uint32_t at = p_of(t) + (ln & 15) * (2 * kPStride) + ((ln >> 4) << 4);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) pb[i] = lds_read<bf16x8>(at + i * 16 * (2 * kPStride));
+    };
+    auto rescale = [&](auto& o) {
+      constexpr int C = sizeof(o) / sizeof(o[0]);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const float alpha = sm.al[16 * i + col];
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c][i] *= alpha;
+      }
+    };
+    auto add = [&](auto& o, auto& va, bf16x8(&pb)[MB]) {
+      constexpr int C = sizeof(o) / sizeof(o[0]);
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c][i] = mfma(va[c], pb[i], o[c][i]);
+    };
+    const bool whole = tile0 == 0 && tile1 == kt;
+    const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
+    float* sums = (float*)sm.p[0];  // at the end: [row][token group]
+    // the rows out: latent values first .. of every row
+    auto store = [&](auto& o, int first, bool lead) {
+      constexpr int C = sizeof(o) / sizeof(o[0]);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const int ln = anew(lane), g = ln >> 4, r = 16 * i + (ln & 15);
+        if (r >= nrows) continue;
+        const float sum = sums[2 * r] + sums[2 * r + 1], top = sm.al[r];
+        if (whole) {
+          const int qi = over_heads(p, r0 + r), h = (r0 + r) - qi * p.heads;
+          const bool none = base + qi <= 0;
+          const float inv = none ? 0.0f : 1.0f / sum;
+          uint16_t* dst = p.out + (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + first + 4 * g;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const f32x4 x = o[c][i] * inv;
+            *(u32x2*)(dst + 16 * c) = u32x2{pack_bf(x[0], x[1]), pack_bf(x[2], x[3])};
+          }
+          if (p.lse && lead && g == 0)
+            p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
+        } else {
+          float* dst = p.part_o + ((int64_t)slot * M + r) * kL + first + 4 * g;
+#pragma unroll
+          for (int c = 0; c < C; ++c) *(f32x4*)(dst + 16 * c) = o[c][i];
+          if (lead && g == 0) {
+            p.part_ml[((int64_t)slot * M + r) * 2] = top;
+            p.part_ml[((int64_t)slot * M + r) * 2 + 1] = sum;
+          }
+        }
+      }
+    };
+    // Steady tiles: every row sees all of them, and the tiles that their requests are for exist
+    const int steady_end = min(min(tend, lim_hi / kN) - kAhead - 1, lim_lo / kN);
+    __syncthreads();  // the last row tile's reads of LDS are over
+
+    if (scores) {
+      // ---- the queries into registers (a row past the tile's rows takes the first one's: it is
+      // not stored)
+      bf16x8 q[RB][KS];
+      int lim[RB];
+      float m[RB], l[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const int r = (rg * RB + rb) * 16 + col;
+        const bool real = r < nrows;
+        const int i = over_heads(p, r0 + (real ? r : 0)), h = r0 + (real ? r : 0) - i * p.heads;
+        lim[rb] = real ? max(0, base + i) : 0;
+        m[rb] = -kInf;
+        l[rb] = 0.0f;
+        const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)h * p.ql_hs + 8 * g;
+        const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)h * p.qp_hs + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          q[rb][ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
+      }
+      if (tid < 3) sm.moved[tid] = 0;
+      f32x4 o[2][MB];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) o[c][i] = f32x4{0, 0, 0, 0};
+      if (!PAGED) barrier();
+      wait_queries();
+      barrier();
+      if (MX) barrier();
+
+      auto step = [&](int t, auto is_steady) __attribute__((always_inline)) {
+        constexpr bool steady = decltype(is_steady)::value;
+        const int ln = anew(lane), col = ln & 15, g = ln >> 4;
+        const uint32_t tile = tile_at(t);
+        const bool edge = !steady && edges && (t + 1) * kN > lim_lo;
+        if (edge) sanitize(t);
+
+        // scores, and the numerators under the maximum so far
+        f32x4 sc[RB];
+        float top[RB], sum[RB];
+        auto numerators = [&]() {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            const float mu = m[rb] == -kInf ? 0.0f : m[rb];
+            float e[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[rb][k] - mu);
+            sum[rb] = (e[0] + e[1]) + (e[2] + e[3]);
+            *(MKMOE_LDS u32x2*)(uintptr_t)(p_of(t) + ((rg * RB + rb) * 16 + col) * (2 * kPStride) + 32 * tg + 8 * g) =
+                u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
+          }
+        };
         // keys: this lane's row of the wave's 16, pieces 4 ks + g; read a few steps ahead, and no
-        // further: the registers are the queries'
+        // further: the registers are the queries'. Two chains of sums, so that the MFMA need not wait
+        f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         const uint32_t k_at = tile + (16 * tg + col) * (2 * kL) + ((g ^ swz(col)) << 4);
         const uint32_t r_at = tile + kRopeAt + (16 * tg + col) * (2 * kR) + ((g ^ swz_rope(col)) << 4);
-        bf16x8 a[G < KS ? 2 : 1][G];
+        bf16x8 a[2][G];
         auto keys = [&](int ks0, bf16x8(&to)[G]) {
 #pragma unroll
           for (int i = 0; i < G; ++i) {
@@ -726,152 +830,170 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           if (k0 + G < KS) keys(k0 + G, a[(k0 / G + 1) % 2]);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < G; ++i) {
-            f32x4& to = (k0 + i) & 1 ? odd : sc;
-            to = mfma(a[(k0 / G) & 1][i], q[k0 + i], to);
-          }
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              f32x4& to = acc[RB == 2 ? rb : (k0 + i) & 1];
+              to = mfma(a[(k0 / G) & 1][i], q[rb][k0 + i], to);
+            }
           __builtin_amdgcn_sched_barrier(0);
         }
-        sc = (sc + odd) * p.scale2;
-        if (!steady && (t + 1) * kN > lim_lo) {  // (rows past the tile's rows see every token before: not stored)
-          const int r = 16 * tg + 4 * g;
+        if (RB == 1) acc[0] += acc[1];
+        bf16x8 va[2], pb[MB];
+        values(tile, 4 * wave, va);
+        bool move = false;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (edge && sm.bad[r + k]) sc[k] = __builtin_nanf("");
-            if (t * kN + r + k >= lim) sc[k] = -kInf;
+        for (int rb = 0; rb < RB; ++rb) {
+          sc[rb] = acc[rb] * p.scale2;
+          if (!steady && (t + 1) * kN > lim_lo) {  // (rows past the tile's see every token before)
+            const int r = 16 * tg + 4 * g;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (edge && sm.bad[r + k]) sc[rb][k] = __builtin_nanf("");
+              if (t * kN + r + k >= lim[rb]) sc[rb][k] = -kInf;
+            }
           }
+          top[rb] = fmaxf(fmaxf(sc[rb][0], sc[rb][1]), fmaxf(sc[rb][2], sc[rb][3]));
+          move = move || top[rb] > m[rb] + kSlack;
         }
-        top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
         numerators();
-        if (__any(top > m + kSlack) && lane == 0) sm.moved[t % 3] = 1;
-      }
-      if (tid == 0) sm.moved[(t + 1) % 3] = 0;  // (last read before the last barrier)
-      // MXFP8: the next tile takes the place of t - 1; with 32 query rows the waves that score nothing
-      // unpack it meanwhile
-      if (MX && (steady || t + 1 < tend)) {
-        if (M == 64) unpack(t + 1, wave * 64 + ln, std::integral_constant<int, kThreads>{});
-        else if (!scores) unpack(t + 1, (wave - 4) * 64 + ln, std::integral_constant<int, kThreads / 2>{});
-      }
-      // values: rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each 16, pieces
-      // 8 wave + 2 c + (lane % 4) / 2
-      bf16x8 va[4];
-      {
-        const int vtok = 8 * g + (col >> 2);
-        const uint32_t v_at = tile + vtok * (2 * kL) + (wave >> 1) * 256 + 8 * (col & 1) +
-                              (((((wave & 1) << 3) | ((col & 3) >> 1)) ^ swz(vtok)) << 4);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          struct { i16x4 a, b; } both = {
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)(v_at ^ (c << 5))),
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)((v_at ^ (c << 5)) + 4 * (2 * kL)))};
-          va[c] = __builtin_bit_cast(bf16x8, both);
-        }
-      }
-      // tile t + 1 is there at the barrier, and the one that takes the place of t - 1 (MXFP8: of the raw
-      // t + 1) is requested after it
-      if (!MX) landed(steady ? kAhead - 2 : min(kAhead - 2, tend - 2 - t));
-      barrier();
-      if (steady || t + kAhead + (MX ? 2 : 1) < tend) resolve(t + kAhead + (MX ? 2 : 1));
-
-      if (__builtin_amdgcn_readfirstlane(sm.moved[t % 3])) {  // maxima move: the numerators again
-        if (scores) {
-          top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
-          if (g == 0) sm.mx[(rg * 16 + col) * 2 + tg] = top;
-        }
+        if (__any(move) && ln == 0) sm.moved[t % 3] = 1;
+        if (tid == 0) sm.moved[(t + 1) % 3] = 0;  // (last read before the last barrier)
         barrier();
-        if (scores) {
-          const int r = rg * 16 + col;
-          top = fmaxf(sm.mx[2 * r], sm.mx[2 * r + 1]);
-          float al = 1.0f;
-          if (top > m + kSlack) {
-            al = __builtin_amdgcn_exp2f(m - top);
-            m = top;
+
+        numerators_of(t, pb);
+        if (__builtin_amdgcn_readfirstlane(sm.moved[t % 3])) {  // maxima move: the numerators again
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            top[rb] = over_groups(top[rb], [](float a, float b) { return fmaxf(a, b); });
+            if (g == 0) sm.mx[((rg * RB + rb) * 16 + col) * 2 + tg] = top[rb];
           }
-          l *= al;
+          barrier();
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            const int r = (rg * RB + rb) * 16 + col;
+            const float both = fmaxf(sm.mx[2 * r], sm.mx[2 * r + 1]);
+            float al = 1.0f;
+            if (both > m[rb] + kSlack) {
+              al = __builtin_amdgcn_exp2f(m[rb] - both);
+              m[rb] = both;
+            }
+            l[rb] *= al;
+            if (tg == 0 && g == 0) sm.al[r] = al;
+          }
           numerators();
-          if (tg == 0 && g == 0) sm.al[r] = al;
+          barrier();
+          rescale(o);
+          numerators_of(t, pb);
         }
-        barrier();
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          const float alpha = sm.al[16 * i + col];
+        for (int rb = 0; rb < RB; ++rb) l[rb] += sum[rb];
+        add(o, va, pb);
+        if (MX) barrier();
+      };
+      int t = tile0;
+      for (; t < steady_end; ++t) step(t, std::true_type{});
+      for (; t < tend; ++t) step(t, std::false_type{});
+
+      // ---- the row sums, then the rows out
+      __syncthreads();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) o[c][i] *= alpha;
+      for (int rb = 0; rb < RB; ++rb) {
+        const int r = (rg * RB + rb) * 16 + col;
+        const float v = over_groups(l[rb], [](float a, float b) { return a + b; });
+        if (g == 0) sums[2 * r + tg] = v;
+        if (g == 0 && tg == 0) sm.al[r] = m[rb];
+      }
+      __syncthreads();
+      if (tid == 0 && w >= w1) {
+        Cut c = {0, 0, s.t0, r0, nrows, base, 0, 0};
+        if (tile1 < kt) {
+          c.share = (unit0 + pre) / share;
+          c.parts = (unit0 + pre + kt - 1) / share - c.share + 1;
         }
+        p.cut[blockIdx.x] = c;
       }
-
-      l += sum;
-
-      // ---- outputs; the next rows' requests while the numerators come
-      bf16x8 pb[MB];
+      store(o, 32 * wave, wave == 0);
+    } else {
+      // ---- the first tiles' rows
+      const uint8_t** first = (const uint8_t**)sm.p[0];  // [kAhead][kN] (P is not in use yet)
+      static_assert(M * kPStride * 2 >= kAhead * kN * 8, "the first tiles' addresses fit into P");
+      int pg[kAhead + 1];
+      if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i) pb[i] = lds_read<bf16x8>(p_to + col * (2 * kPStride) + 16 * g + i * 16 * (2 * kPStride));
-      constexpr int kNext = kAhead + (MX ? 1 : 0);
-      if (steady || t + kNext < tend) {
-        entries(t + kNext + 3);
-        issue(t + kNext, sm.addr[(t + kNext) & 1]);
-      }
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c][i] = mfma(va[c], pb[i], o[c][i]);
-      }
-      if constexpr (MX) {  // the raw rows of t + 2 are there at the barrier
-        landed(steady ? kAhead - 1 : min(kAhead - 1, tend - 3 - t));
-        barrier();
-      }
-    };
-    const int steady_end = min(tend - kAhead - 1, lim_lo / kN);
-    int t = tile0;
-    for (; t < steady_end; ++t) step(t, std::true_type{});
-    for (; t < tend; ++t) step(t, std::false_type{});
-    if (lost) record(p.err, MKMOE_LATENT_ERR_PAGE, b);
-
-    // ---- the row sums, then the rows out
-    l = over_groups(l, [](float a, float b) { return a + b; });
-    __syncthreads();
-    float* sums = (float*)sm.p[0];  // [row][token group]
-    if (scores && g == 0) {
-      sums[(rg * 16 + col) * 2 + tg] = l;
-      if (tg == 0) sm.al[rg * 16 + col] = m;
-    }
-    __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == kt;
-    const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
-    if (tid == 0 && w >= w1) {
-      Cut c = {0, 0, s.t0, r0, nrows, base, 0, 0};
-      if (tile1 < kt) {
-        c.share = (unit0 + pre) / share;
-        c.parts = (unit0 + pre + kt - 1) / share - c.share + 1;
-      }
-      p.cut[blockIdx.x] = c;
-    }
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      const int r = 16 * i + col;
-      if (r >= nrows) continue;
-      const float sum = sums[2 * r] + sums[2 * r + 1], top = sm.al[r];
-      if (whole) {
-        const int qi = over_heads(p, r0 + r), h = (r0 + r) - qi * p.heads;
-        const bool none = base + qi <= 0;
-        const float inv = none ? 0.0f : 1.0f / sum;
-        uint16_t* dst = p.out + (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 64 * wave + 4 * g;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const f32x4 x = o[c][i] * inv;
-          *(u32x2*)(dst + 16 * c) = u32x2{pack_bf(x[0], x[1]), pack_bf(x[2], x[3])};
-        }
-        if (p.lse && wave == 0 && g == 0)
-          p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
+        for (int i = 0; i <= kAhead; ++i) pg[i] = page_of(tile0 + i);
       } else {
-        float* dst = p.part_o + ((int64_t)slot * M + r) * kL + 64 * wave + 4 * g;
+        const int i = tid - 256;
+        if (i < (kAhead + 3) * kN) {
+          const int e = table[min(tile0 * kN + i, lim_hi - 1) >> p.page_shift];
+          if (i < kAhead * kN) first[i] = address(tile0 * kN + i, e);
+          else sm.ent[(tile0 + i / kN) % kEnts][i % kN] = e;
+        }
+        wait_queries();  // (the entries)
+        barrier();
+      }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) *(f32x4*)(dst + 16 * c) = o[c][i];
-        if (wave == 0 && g == 0) {
-          p.part_ml[((int64_t)slot * M + r) * 2] = top;
-          p.part_ml[((int64_t)slot * M + r) * 2 + 1] = sum;
+      for (int i = 0; i < kAhead; ++i)
+        if (tile0 + i < tend) issue(tile0 + i, pg[i], first + i * kN, false);
+      int pg_next = pg[kAhead];  // the page of the tile that is requested next
+      if (tile0 + kAhead < tend) resolve(tile0 + kAhead);
+      if (MX && tile0 + kAhead + 1 < tend) resolve(tile0 + kAhead + 1);
+      f32x4 o[6][MB];
+#pragma unroll
+      for (int c = 0; c < 6; ++c)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) o[c][i] = f32x4{0, 0, 0, 0};
+      landed(min(tend - 1 - tile0, kAhead - 1) - (MX ? 1 : 0));  // the first tile (MXFP8: two)
+      barrier();
+      if constexpr (MX) {
+        if (tile0 < tend) unpack(tile0);
+        barrier();
+        if (tile0 + kAhead < tend) {
+          entries(tile0 + kAhead + 3);
+          issue(tile0 + kAhead, pg_next, sm.addr[(tile0 + kAhead) & 1], false);
+          pg_next = page_of(tile0 + kAhead + 1);
         }
       }
+
+      auto step = [&](int t, auto is_steady) __attribute__((always_inline)) {
+        constexpr bool steady = decltype(is_steady)::value;
+        if (!steady && edges && (t + 1) * kN > lim_lo) sanitize(t);
+        bf16x8 va[6], pb[MB];
+        // MXFP8: the next tile takes the place of t - 1
+        if (MX && (steady || t + 1 < tend)) unpack(t + 1);
+        values(tile_at(t), 16 + 12 * lw, va);
+        // tile t + 1 is there at the barrier, and the one that takes the place of t - 1 (MXFP8: of the raw
+        // t + 1) is requested after it
+        if (!MX) landed(steady ? kAhead - 2 : min(kAhead - 2, tend - 2 - t));
+        barrier();
+
+        numerators_of(t, pb);
+        if (__builtin_amdgcn_readfirstlane(sm.moved[t % 3])) {
+          barrier();
+          barrier();
+          rescale(o);
+          numerators_of(t, pb);
+        }
+        if (steady || t + kAhead + (MX ? 2 : 1) < tend) resolve(t + kAhead + (MX ? 2 : 1));
+        constexpr int kNext = kAhead + (MX ? 1 : 0);
+        if (steady || t + kNext < tend) {
+          entries(t + kNext + 3);
+          issue(t + kNext, pg_next, sm.addr[(t + kNext) & 1], steady);
+          pg_next = page_of(t + kNext + 1);
+        }
+        add(o, va, pb);
+        if constexpr (MX) {  // the raw rows of t + 2 are there at the barrier
+          landed(steady ? kAhead - 1 : min(kAhead - 1, tend - 3 - t));
+          barrier();
+        }
+      };
+      int t = tile0;
+      for (; t < steady_end; ++t) step(t, std::true_type{});
+      for (; t < tend; ++t) step(t, std::false_type{});
+      if (lost) record(p.err, MKMOE_LATENT_ERR_PAGE, b);
+      __syncthreads();
+      __syncthreads();
+      store(o, 128 + 96 * lw, false);
     }
   }
 }
@@ -1071,7 +1193,10 @@ inline int launched() { return hipGetLastError() == hipSuccess ? MKMOE_OK : MKMO
 
 template <int M, bool MX>
 int attend(const AttendParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((k_latent_attend<M, MX>), dim3(kShares), dim3(kThreads), 0, st, p);
+  if ((1 << p.page_shift) >= kN)
+    hipLaunchKernelGGL((k_latent_attend<M, MX, true>), dim3(kShares), dim3(kThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((k_latent_attend<M, MX, false>), dim3(kShares), dim3(kThreads), 0, st, p);
   if (int rc = launched()) return rc;
   hipLaunchKernelGGL(k_latent_merge<M>, dim3(kShares, kMergeWgs), dim3(256), 0, st, p);
   return launched();
