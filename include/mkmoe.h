@@ -343,23 +343,24 @@ typedef struct mkmoe_latent_attend_io {
   const int32_t* table;    /* [seqs][max_pages] pages */
   const int32_t* lens;     /* [seqs] cached tokens, the queries' own among them; 0: none */
   const int32_t* q_starts; /* [seqs + 1] first query token of each sequence, or NULL: equal counts */
-  void* out;               /* [tokens][heads][512] bf16; 0 for a query that sees nothing */
+  void* out;               /* [tokens][heads][512] bf16 (fp32: out_f32); 0 for a query that sees nothing */
   float* lse;              /* [tokens][heads] log of the sum of exp(s), or NULL; -inf there */
   float scale;
-  int32_t reserved;
+  int32_t out_f32;         /* 1: out is fp32 */
 } mkmoe_latent_attend_io;
 
 /* y = W_UK^T x ([tokens][heads][128] -> 512, expand 0) or W_UV x (512 -> 128, expand 1), each head
- * by its own weights; fp32 sums */
+ * by its own weights; fp32 sums, y in bf16 */
 typedef struct mkmoe_latent_project_io {
-  int32_t tokens, heads, expand, reserved;
+  int32_t tokens, heads, expand;
+  int32_t x_f32; /* 1 (expand only): x is fp32 */
   int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
-  const void* x;
+  const void* x; /* bf16 */
   const void* w; /* [heads][256][512] bf16 (kv_b): W_UK rows 0 .. 127, W_UV rows 128 .. 255 */
   void* y;
 } mkmoe_latent_project_io;
 
-/* Workspace bytes of every latent call (256-byte aligned; zeroed once by the caller). */
+/* Workspace bytes of every latent call (256-byte aligned; its error words zeroed once by the caller). */
 int mkmoe_latent_workspace_bytes(size_t* bytes);
 /* Norm, rotate and store the step's rows; rotate the query's rope part. One launch. */
 int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_bytes, void* stream);
@@ -370,6 +371,12 @@ int mkmoe_latent_rows(const mkmoe_latent_cache* cache, const void* slots, int32_
  * Rows of out behind the last sequence's queries stay as they were. Two launches. */
 int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_bytes, void* stream);
 int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream);
+/* A layer's whole step: append and absorb (expand 0) in one launch, attend, expand (1), with the same
+ * tokens in each. All four are checked before the first launch; each one's outputs are the next
+ * one's inputs as the caller set them. */
+int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_project_io* absorb,
+                      const mkmoe_latent_attend_io* attend, const mkmoe_latent_project_io* expand, void* ws,
+                      size_t ws_bytes, void* stream);
 /* Copy n error words to host memory (synchronises stream). */
 int mkmoe_latent_read_errors(const void* ws, int32_t* words, int32_t n, void* stream);
 

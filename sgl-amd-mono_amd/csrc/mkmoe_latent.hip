@@ -133,10 +133,10 @@ __device__ __forceinline__ u32x4 rotate8(u32x4 v, const float* cs, int j, int ha
 // values. Bytes: each value is read and written once; a decode step's few rows are one trip to
 // memory and back.
 template <bool MX>
-__global__ __launch_bounds__(256) void k_latent_append(AppendParams p) {
+__device__ __forceinline__ void append_block(const AppendParams& p, int block) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if ((int)blockIdx.x < p.kv_blocks) {
-    const int t = blockIdx.x * 4 + wave;
+  if (block < p.kv_blocks) {
+    const int t = block * 4 + wave;
     if (t >= p.tokens) return;
     const int64_t slot = index_at(p.slots, t, p.wide), pos = index_at(p.positions, t, p.wide);
     if (slot < 0) return;  // a padded row
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256) void k_latent_append(AppendParams p) {
     }
     return;
   }
-  const int64_t r = ((int64_t)(blockIdx.x - p.kv_blocks) * 4 + wave) * 8 + (lane >> 3);
+  const int64_t r = ((int64_t)(block - p.kv_blocks) * 4 + wave) * 8 + (lane >> 3);
   if (r >= (int64_t)p.tokens * p.heads) return;
   const int t = (int)(r / p.heads), h = (int)(r - (int64_t)t * p.heads), j = lane & 7;
   const int64_t pos = index_at(p.positions, t, p.wide);
@@ -212,6 +212,11 @@ __global__ __launch_bounds__(256) void k_latent_append(AppendParams p) {
   }
   const u32x4 v = *(const u32x4*)(p.q + t * p.q_ts + h * p.q_hs + 8 * j);
   *(u32x4*)(p.q_out + t * p.o_ts + h * p.o_hs + 8 * j) = rotate8(v, p.cos_sin + pos * kR, j, p.half);
+}
+
+template <bool MX>
+__global__ __launch_bounds__(256) void k_latent_append(AppendParams p) {
+  append_block<MX>(p, blockIdx.x);
 }
 
 // ---------------------------------------------------------------- rows as values
@@ -285,7 +290,7 @@ struct AttendParams {
   const int32_t* table;
   const int32_t* lens;
   const int32_t* starts;  // NULL: n query tokens a sequence
-  uint16_t* out;
+  void* out;  // bf16, or fp32 (f32)
   float* lse;
   int32_t* err;
   Cut* cut;        // [kShares]
@@ -293,10 +298,18 @@ struct AttendParams {
   float* part_ml;  // [2 kShares][M][2]
   int64_t ql_ts, ql_hs, qp_ts, qp_hs, o_ts, o_hs;
   int64_t table_stride;
-  int pages, seqs, tokens, heads, n, max_len, page_shift;
+  int pages, seqs, tokens, heads, n, max_len, page_shift, f32;
   uint32_t per_head;  // 2^32 / heads, rounded up
   float scale2;       // scale log2(e)
 };
+
+// four attended values, rounded where the caller takes bf16
+__device__ __forceinline__ void store4(const AttendParams& p, int64_t to, f32x4 v) {
+  if (p.f32)
+    *(f32x4*)((float*)p.out + to) = v;
+  else
+    *(u32x2*)((uint16_t*)p.out + to) = u32x2{pack_bf(v[0], v[1]), pack_bf(v[2], v[3])};
+}
 
 // a query row's token: exact for rows below 2^24 and up to 128 heads (the product is off by less
 // than rows x heads <= 2^31 of 2^32)
@@ -526,7 +539,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     if (lim_hi == 0) {  // nothing to see: rows of zeros, by every share that has a part of them
       for (int i = tid; i < nrows * (kL / 8); i += kThreads) {
         const int r = r0 + i / (kL / 8), qi = over_heads(p, r), h = r - qi * p.heads;
-        *(u32x4*)(p.out + (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 8 * (i % (kL / 8))) = u32x4{0, 0, 0, 0};
+        const int64_t to = (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 8 * (i % (kL / 8));
+        store4(p, to, f32x4{0, 0, 0, 0});
+        store4(p, to + 4, f32x4{0, 0, 0, 0});
         if (p.lse && i % (kL / 8) == 0) p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = -kInf;
       }
       if (tid == 0 && w >= w1) p.cut[blockIdx.x].parts = 0;
@@ -734,12 +749,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           const int qi = over_heads(p, r0 + r), h = (r0 + r) - qi * p.heads;
           const bool none = base + qi <= 0;
           const float inv = none ? 0.0f : 1.0f / sum;
-          uint16_t* dst = p.out + (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + first + 4 * g;
+          const int64_t to = (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + first + 4 * g;
 #pragma unroll
-          for (int c = 0; c < C; ++c) {
-            const f32x4 x = o[c][i] * inv;
-            *(u32x2*)(dst + 16 * c) = u32x2{pack_bf(x[0], x[1]), pack_bf(x[2], x[3])};
-          }
+          for (int c = 0; c < C; ++c) store4(p, to + 16 * c, o[c][i] * inv);
           if (p.lse && lead && g == 0)
             p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
         } else {
@@ -1019,8 +1031,7 @@ __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
     const int qi = over_heads(p, c.r0 + r), h = (c.r0 + r) - qi * p.heads;
     const bool none = c.base + qi <= 0;
     acc *= none ? 0.0f : 1.0f / sum;
-    *(u32x2*)(p.out + (int64_t)(c.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 128 * part + 4 * lane) =
-        u32x2{pack_bf(acc[0], acc[1]), pack_bf(acc[2], acc[3])};
+    store4(p, (int64_t)(c.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 128 * part + 4 * lane, acc);
     if (p.lse && part == 0 && lane == 0)
       p.lse[(int64_t)(c.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
   };
@@ -1103,20 +1114,25 @@ __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
 
 // ---------------------------------------------------------------- the heads' products
 struct ProjectParams {
-  const uint16_t* x;
+  const void* x;      // bf16; fp32 (f32) where the attended latents come unrounded
   const uint16_t* w;  // [heads][256][512]: rows 0 .. 127 W_UK, 128 .. 255 W_UV
   uint16_t* y;
   int64_t x_ts, x_hs, y_ts, y_hs;
-  int tokens;
+  int tokens, heads, f32;
 };
 
+// what bf16's rounding left of a value, nothing where that is not finite
+__device__ __forceinline__ float rest(float x, float rounded) { return fabsf(rounded) < kInf ? x - rounded : 0.0f; }
+
 // y[t, h, l] = sum_d x[t, h, d] W_UK[h, d, l]: a workgroup a head, 64 columns and 64 tokens; the
-// 128 x 64 weight block in LDS, its transposing reads the A operand, 16 tokens a wave
-__global__ __launch_bounds__(256) void k_latent_absorb(ProjectParams p) {
-  constexpr int S = 144;  // bytes an LDS row of 64 values: 16 past the banks' period
-  __shared__ __align__(16) uint8_t wl[kNope * S];
+// 128 x 64 weight block in LDS, its transposing reads the A operand, 16 tokens a wave. The result
+// is rounded to bf16 because it is the scores' matrix operand
+constexpr int kAbsorbStride = 144;  // bytes an LDS row of 64 values: 16 past the banks' period
+__device__ __forceinline__ void absorb_block(const ProjectParams& p, int block, uint8_t* wl) {
+  constexpr int S = kAbsorbStride;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-  const int c0 = blockIdx.x * 64, h = blockIdx.y, t = blockIdx.z * 64 + 16 * wave + col;
+  const int c0 = (block % (kL / 64)) * 64, h = block / (kL / 64) % p.heads;
+  const int t = block / (kL / 64) / p.heads * 64 + 16 * wave + col;
   const uint16_t* w = p.w + (int64_t)h * (kNope + kV) * kL + c0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -1124,11 +1140,12 @@ __global__ __launch_bounds__(256) void k_latent_absorb(ProjectParams p) {
     *(u32x4*)(wl + d * S + 16 * c) = *(const u32x4*)(w + (int64_t)d * kL + 8 * c);
   }
   const bool real = t < p.tokens;
-  const uint16_t* x = p.x + (int64_t)(real ? t : 0) * p.x_ts + (int64_t)h * p.x_hs + 8 * g;
+  const uint16_t* x = (const uint16_t*)p.x + (int64_t)(real ? t : 0) * p.x_ts + (int64_t)h * p.x_hs + 8 * g;
   bf16x8 xb[4];
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) xb[ks] = real ? *(const bf16x8*)(x + 32 * ks) : bf16x8{};
   __syncthreads();
+  if (t - col >= p.tokens) return;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     f32x4 acc = {0, 0, 0, 0};
@@ -1145,24 +1162,66 @@ __global__ __launch_bounds__(256) void k_latent_absorb(ProjectParams p) {
   }
 }
 
-// y[t, h, j] = sum_l x[t, h, l] W_UV[h, j, l]: a workgroup a head, 16 columns and 64 tokens, 16
-// tokens a wave; both operands are contiguous along l and come straight from memory
+__global__ __launch_bounds__(256) void k_latent_absorb(ProjectParams p) {
+  __shared__ __align__(16) uint8_t wl[kNope * kAbsorbStride];
+  absorb_block(p, blockIdx.x, wl);
+}
+
+// A step's first launch: the two that need nothing of each other, append and absorb
+template <bool MX>
+__global__ __launch_bounds__(256) void k_latent_front(AppendParams a, ProjectParams p, int absorb_blocks) {
+  __shared__ __align__(16) uint8_t wl[kNope * kAbsorbStride];
+  if ((int)blockIdx.x < absorb_blocks)
+    absorb_block(p, blockIdx.x, wl);
+  else
+    append_block<MX>(a, blockIdx.x - absorb_blocks);
+}
+
+// y[t, h, j] = sum_l x[t, h, l] W_UV[h, j, l]: a workgroup a head, 16 columns and 64 tokens. The
+// four waves split l, so that few tokens keep them all busy and no weight is read twice, and add up
+// in LDS; both operands are contiguous along l and come straight from memory. x in fp32 is taken as
+// the sum of two bf16 parts (2^-17 of it is left out) against the same weights
+template <bool F32>
 __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
+  constexpr int KS = kL / 32 / 4;  // MFMA steps of a wave
+  __shared__ f32x4 sums[4][4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int j0 = blockIdx.x * 16, h = blockIdx.y, t = blockIdx.z * 64 + 16 * wave + col;
-  if (blockIdx.z * 64 + 16 * wave >= p.tokens) return;
-  const bool real = t < p.tokens;
-  const uint16_t* w = p.w + ((int64_t)h * (kNope + kV) + kNope + j0 + col) * kL + 8 * g;
-  const uint16_t* x = p.x + (int64_t)(real ? t : 0) * p.x_ts + (int64_t)h * p.x_hs + 8 * g;
-  f32x4 acc = {0, 0, 0, 0};
+  const int j0 = blockIdx.x * 16, h = blockIdx.y, t0 = blockIdx.z * 64, l0 = wave * (kL / 4) + 8 * g;
+  const uint16_t* w = p.w + ((int64_t)h * (kNope + kV) + kNope + j0 + col) * kL + l0;
+  bf16x8 a[KS];
 #pragma unroll
-  for (int ks = 0; ks < kL / 32; ++ks) {
-    const bf16x8 b = real ? *(const bf16x8*)(x + 32 * ks) : bf16x8{};
-    acc = mfma(*(const bf16x8*)(w + 32 * ks), b, acc);
+  for (int ks = 0; ks < KS; ++ks) a[ks] = *(const bf16x8*)(w + 32 * ks);
+#pragma unroll
+  for (int tb = 0; tb < 4; ++tb) {
+    if (t0 + 16 * tb >= p.tokens) break;
+    const int t = min(t0 + 16 * tb + col, p.tokens - 1);
+    const int64_t at = (int64_t)t * p.x_ts + (int64_t)h * p.x_hs + l0;
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if constexpr (F32) {
+        const float* x = (const float*)p.x + at + 32 * ks;
+        const f32x4 v[2] = {*(const f32x4*)x, *(const f32x4*)(x + 4)};
+        u32x4 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a0 = v[i >> 1][2 * (i & 1)], a1 = v[i >> 1][2 * (i & 1) + 1];
+          hi[i] = pack_bf(a0, a1);
+          lo[i] = pack_bf(rest(a0, bf_lo(hi[i])), rest(a1, bf_hi(hi[i])));
+        }
+        acc = mfma(a[ks], __builtin_bit_cast(bf16x8, lo), acc);
+        acc = mfma(a[ks], __builtin_bit_cast(bf16x8, hi), acc);
+      } else {
+        acc = mfma(a[ks], *(const bf16x8*)((const uint16_t*)p.x + at + 32 * ks), acc);
+      }
+    }
+    sums[tb][wave][lane] = acc;
   }
-  if (real)
-    *(u32x2*)(p.y + (int64_t)t * p.y_ts + (int64_t)h * p.y_hs + j0 + 4 * g) =
-        u32x2{pack_bf(acc[0], acc[1]), pack_bf(acc[2], acc[3])};
+  __syncthreads();
+  const int t = t0 + 16 * wave + col;
+  if (t >= p.tokens) return;
+  const f32x4 v = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
+  *(u32x2*)(p.y + (int64_t)t * p.y_ts + (int64_t)h * p.y_hs + j0 + 4 * g) = u32x2{pack_bf(v[0], v[1]), pack_bf(v[2], v[3])};
 }
 
 // ---------------------------------------------------------------- host
@@ -1202,18 +1261,8 @@ int attend(const AttendParams& p, hipStream_t st) {
   return launched();
 }
 
-}  // namespace mkmoe_latent
-
-extern "C" {
-
-int mkmoe_latent_workspace_bytes(size_t* bytes) {
-  if (!bytes) return MKMOE_ERR_NULL;
-  *bytes = mkmoe_latent::kWsBytes;
-  return MKMOE_OK;
-}
-
-int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_bytes, void* stream) {
-  using namespace mkmoe_latent;
+// the checks of each call and, where they pass, its kernel's parameters
+inline int append_params(const mkmoe_latent_append_io* io, void* ws, size_t ws_bytes, AppendParams& p) {
   if (!io) return MKMOE_ERR_NULL;
   if (int rc = check_ws(ws, ws_bytes)) return rc;
   if (int rc = check_cache(io->cache)) return rc;
@@ -1231,8 +1280,6 @@ int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_by
                         !strides8(io->q_token_stride, io->q_head_stride) ||
                         !strides8(io->out_token_stride, io->out_head_stride)))
     return MKMOE_ERR_ALIGN;
-  if (io->tokens == 0) return MKMOE_OK;
-  AppendParams p;
   p.kv = (const uint16_t*)io->kv;
   p.norm_w = (const uint16_t*)io->norm_w;
   p.cos_sin = (const float*)io->cos_sin;
@@ -1255,12 +1302,121 @@ int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_by
   p.wide = io->index_bytes == 8;
   p.kv_blocks = (io->tokens + 3) / 4;
   p.eps = io->norm_eps;
-  const unsigned blocks = (unsigned)(p.kv_blocks + ((int64_t)io->tokens * io->heads + 31) / 32);
+  return MKMOE_OK;
+}
+inline unsigned append_blocks(const AppendParams& p) {
+  return (unsigned)(p.kv_blocks + ((int64_t)p.tokens * p.heads + 31) / 32);
+}
+inline int attend_params(const mkmoe_latent_attend_io* io, void* ws, size_t ws_bytes, AttendParams& p) {
+  if (!io) return MKMOE_ERR_NULL;
+  if (int rc = check_ws(ws, ws_bytes)) return rc;
+  if (int rc = check_cache(io->cache)) return rc;
+  if (!io->q_lat || !io->q_pe || !io->table || !io->lens || !io->out) return MKMOE_ERR_NULL;
+  if (io->seqs < 1 || io->seqs > kMaxSeqs || io->tokens < 0) return MKMOE_ERR_ROWS;
+  if (io->heads < 1 || io->heads > MKMOE_LATENT_MAX_HEADS) return MKMOE_ERR_ARG;
+  if ((int64_t)io->tokens * io->heads > kMaxRows) return MKMOE_ERR_ROWS;
+  if (!io->q_starts && io->tokens % io->seqs != 0) return MKMOE_ERR_ROWS;
+  if ((io->out_f32 & ~1) != 0) return MKMOE_ERR_ARG;
+  if (!isfinite(io->scale) || io->max_pages < 1 || io->table_stride < io->max_pages) return MKMOE_ERR_ARG;
+  const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
+  if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
+  // the work list's tiles are counted in 32 bits
+  const int64_t tiles = ((int64_t)io->tokens * io->heads / 32 + io->seqs) * ((max_len + kN - 1) / kN + kSetup);
+  if (tiles > 0x3fffffff) return MKMOE_ERR_ARG;
+  const void* wide[] = {io->q_lat, io->q_pe, io->out};
+  for (const void* q : wide)
+    if (!aligned(q, 16)) return MKMOE_ERR_ALIGN;
+  const void* narrow[] = {io->table, io->lens, io->q_starts, io->lse};
+  for (const void* q : narrow)
+    if (!aligned(q, 4)) return MKMOE_ERR_ALIGN;
+  if (!strides8(io->ql_token_stride, io->ql_head_stride) || !strides8(io->qp_token_stride, io->qp_head_stride) ||
+      !strides8(io->out_token_stride, io->out_head_stride))
+    return MKMOE_ERR_ALIGN;
+  p.ql = (const uint16_t*)io->q_lat;
+  p.qp = (const uint16_t*)io->q_pe;
+  p.cache = (const uint8_t*)io->cache.data;
+  p.table = io->table;
+  p.lens = io->lens;
+  p.starts = io->q_starts;
+  p.out = io->out;
+  p.f32 = io->out_f32;
+  p.lse = io->lse;
+  uint8_t* at = (uint8_t*)ws;
+  p.err = (int32_t*)at;
+  p.cut = (Cut*)(at += kCtlBytes);
+  p.part_ml = (float*)(at += kCutBytes);
+  p.part_o = (float*)(at += kMlBytes);
+  p.ql_ts = io->ql_token_stride;
+  p.ql_hs = io->ql_head_stride;
+  p.qp_ts = io->qp_token_stride;
+  p.qp_hs = io->qp_head_stride;
+  p.o_ts = io->out_token_stride;
+  p.o_hs = io->out_head_stride;
+  p.table_stride = io->table_stride;
+  p.pages = (int)io->cache.pages;
+  p.seqs = io->seqs;
+  p.tokens = io->tokens;
+  p.heads = io->heads;
+  p.n = io->q_starts ? 0 : io->tokens / io->seqs;
+  p.max_len = (int)max_len;
+  p.page_shift = __builtin_ctz((unsigned)io->cache.page_size);
+  p.per_head = (uint32_t)(((1ull << 32) + io->heads - 1) / io->heads);
+  p.scale2 = io->scale * kLog2e;
+  return MKMOE_OK;
+}
+inline int attend_launch(const mkmoe_latent_attend_io* io, const AttendParams& p, hipStream_t st) {
+  if (io->tokens == 0) return MKMOE_OK;
+  const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8;
+  // 32 query rows a tile where a sequence has no more of them on average, else 64
+  const int64_t rows = ((int64_t)io->tokens * io->heads + io->seqs - 1) / io->seqs;
+  if (rows <= 32) return mx ? attend<32, true>(p, st) : attend<32, false>(p, st);
+  return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
+}
+inline int project_params(const mkmoe_latent_project_io* io, ProjectParams& p) {
+  if (!io || !io->x || !io->w || !io->y) return MKMOE_ERR_NULL;
+  if (io->tokens < 0 || io->tokens > (1 << 20)) return MKMOE_ERR_ROWS;
+  if (io->heads < 1 || io->heads > MKMOE_LATENT_MAX_HEADS || (io->expand & ~1) != 0 || (io->x_f32 & ~1) != 0 ||
+      (io->x_f32 && !io->expand))
+    return MKMOE_ERR_ARG;
+  if (!aligned(io->x, 16) || !aligned(io->w, 16) || !aligned(io->y, 16) ||
+      !strides8(io->x_token_stride, io->x_head_stride) || !strides8(io->y_token_stride, io->y_head_stride))
+    return MKMOE_ERR_ALIGN;
+  p = ProjectParams{io->x, (const uint16_t*)io->w, (uint16_t*)io->y, io->x_token_stride, io->x_head_stride,
+                    io->y_token_stride, io->y_head_stride, io->tokens, io->heads, io->x_f32};
+  return MKMOE_OK;
+}
+inline unsigned absorb_blocks(const ProjectParams& p) {
+  return (unsigned)(kL / 64) * p.heads * ((p.tokens + 63) / 64);
+}
+inline int expand_launch(const ProjectParams& p, hipStream_t st) {
+  const dim3 grid(kV / 16, p.heads, (p.tokens + 63) / 64);
+  if (p.f32)
+    hipLaunchKernelGGL(k_latent_expand<true>, grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL(k_latent_expand<false>, grid, dim3(256), 0, st, p);
+  return launched();
+}
+
+}  // namespace mkmoe_latent
+
+extern "C" {
+
+int mkmoe_latent_workspace_bytes(size_t* bytes) {
+  if (!bytes) return MKMOE_ERR_NULL;
+  *bytes = mkmoe_latent::kWsBytes;
+  return MKMOE_OK;
+}
+
+int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_bytes, void* stream) {
+  using namespace mkmoe_latent;
+  AppendParams p;
+  if (int rc = append_params(io, ws, ws_bytes, p)) return rc;
+  if (p.tokens == 0) return MKMOE_OK;
   hipStream_t st = (hipStream_t)stream;
   if (io->cache.fmt == MKMOE_LATENT_MXFP8)
-    hipLaunchKernelGGL(k_latent_append<true>, dim3(blocks), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(k_latent_append<true>, dim3(append_blocks(p)), dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL(k_latent_append<false>, dim3(blocks), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(k_latent_append<false>, dim3(append_blocks(p)), dim3(256), 0, st, p);
   return launched();
 }
 
@@ -1286,85 +1442,46 @@ int mkmoe_latent_rows(const mkmoe_latent_cache* cache, const void* slots, int32_
 
 int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_bytes, void* stream) {
   using namespace mkmoe_latent;
-  if (!io) return MKMOE_ERR_NULL;
-  if (int rc = check_ws(ws, ws_bytes)) return rc;
-  if (int rc = check_cache(io->cache)) return rc;
-  if (!io->q_lat || !io->q_pe || !io->table || !io->lens || !io->out) return MKMOE_ERR_NULL;
-  if (io->seqs < 1 || io->seqs > kMaxSeqs || io->tokens < 0) return MKMOE_ERR_ROWS;
-  if (io->heads < 1 || io->heads > MKMOE_LATENT_MAX_HEADS) return MKMOE_ERR_ARG;
-  if ((int64_t)io->tokens * io->heads > kMaxRows) return MKMOE_ERR_ROWS;
-  if (!io->q_starts && io->tokens % io->seqs != 0) return MKMOE_ERR_ROWS;
-  if (!isfinite(io->scale) || io->max_pages < 1 || io->table_stride < io->max_pages) return MKMOE_ERR_ARG;
-  const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
-  if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
-  // the work list's tiles are counted in 32 bits
-  const int64_t tiles = ((int64_t)io->tokens * io->heads / 32 + io->seqs) * ((max_len + kN - 1) / kN + kSetup);
-  if (tiles > 0x3fffffff) return MKMOE_ERR_ARG;
-  const void* wide[] = {io->q_lat, io->q_pe, io->out};
-  for (const void* q : wide)
-    if (!aligned(q, 16)) return MKMOE_ERR_ALIGN;
-  const void* narrow[] = {io->table, io->lens, io->q_starts, io->lse};
-  for (const void* q : narrow)
-    if (!aligned(q, 4)) return MKMOE_ERR_ALIGN;
-  if (!strides8(io->ql_token_stride, io->ql_head_stride) || !strides8(io->qp_token_stride, io->qp_head_stride) ||
-      !strides8(io->out_token_stride, io->out_head_stride))
-    return MKMOE_ERR_ALIGN;
-  if (io->tokens == 0) return MKMOE_OK;
   AttendParams p;
-  p.ql = (const uint16_t*)io->q_lat;
-  p.qp = (const uint16_t*)io->q_pe;
-  p.cache = (const uint8_t*)io->cache.data;
-  p.table = io->table;
-  p.lens = io->lens;
-  p.starts = io->q_starts;
-  p.out = (uint16_t*)io->out;
-  p.lse = io->lse;
-  uint8_t* at = (uint8_t*)ws;
-  p.err = (int32_t*)at;
-  p.cut = (Cut*)(at += kCtlBytes);
-  p.part_ml = (float*)(at += kCutBytes);
-  p.part_o = (float*)(at += kMlBytes);
-  p.ql_ts = io->ql_token_stride;
-  p.ql_hs = io->ql_head_stride;
-  p.qp_ts = io->qp_token_stride;
-  p.qp_hs = io->qp_head_stride;
-  p.o_ts = io->out_token_stride;
-  p.o_hs = io->out_head_stride;
-  p.table_stride = io->table_stride;
-  p.pages = (int)io->cache.pages;
-  p.seqs = io->seqs;
-  p.tokens = io->tokens;
-  p.heads = io->heads;
-  p.n = io->q_starts ? 0 : io->tokens / io->seqs;
-  p.max_len = (int)max_len;
-  p.page_shift = __builtin_ctz((unsigned)io->cache.page_size);
-  p.per_head = (uint32_t)(((1ull << 32) + io->heads - 1) / io->heads);
-  p.scale2 = io->scale * kLog2e;
-  hipStream_t st = (hipStream_t)stream;
-  const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8;
-  // 32 query rows a tile where a sequence has no more of them on average, else 64
-  const int64_t rows = ((int64_t)io->tokens * io->heads + io->seqs - 1) / io->seqs;
-  if (rows <= 32) return mx ? attend<32, true>(p, st) : attend<32, false>(p, st);
-  return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
+  if (int rc = attend_params(io, ws, ws_bytes, p)) return rc;
+  return attend_launch(io, p, (hipStream_t)stream);
 }
 
 int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream) {
   using namespace mkmoe_latent;
-  if (!io || !io->x || !io->w || !io->y) return MKMOE_ERR_NULL;
-  if (io->tokens < 0 || io->tokens > (1 << 20)) return MKMOE_ERR_ROWS;
-  if (io->heads < 1 || io->heads > MKMOE_LATENT_MAX_HEADS || (io->expand & ~1) != 0) return MKMOE_ERR_ARG;
-  if (!aligned(io->x, 16) || !aligned(io->w, 16) || !aligned(io->y, 16) ||
-      !strides8(io->x_token_stride, io->x_head_stride) || !strides8(io->y_token_stride, io->y_head_stride))
-    return MKMOE_ERR_ALIGN;
+  ProjectParams p;
+  if (int rc = project_params(io, p)) return rc;
   if (io->tokens == 0) return MKMOE_OK;
-  ProjectParams p{(const uint16_t*)io->x, (const uint16_t*)io->w, (uint16_t*)io->y, io->x_token_stride,
-                  io->x_head_stride, io->y_token_stride, io->y_head_stride, io->tokens};
-  const unsigned tb = (io->tokens + 63) / 64;
-  if (io->expand)
-    hipLaunchKernelGGL(k_latent_expand, dim3(kV / 16, io->heads, tb), dim3(256), 0, (hipStream_t)stream, p);
-  else
-    hipLaunchKernelGGL(k_latent_absorb, dim3(kL / 64, io->heads, tb), dim3(256), 0, (hipStream_t)stream, p);
+  hipStream_t st = (hipStream_t)stream;
+  if (io->expand) return expand_launch(p, st);
+  hipLaunchKernelGGL(k_latent_absorb, dim3(absorb_blocks(p)), dim3(256), 0, st, p);
   return launched();
+}
+
+int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_project_io* absorb,
+                      const mkmoe_latent_attend_io* attend, const mkmoe_latent_project_io* expand, void* ws,
+                      size_t ws_bytes, void* stream) {
+  using namespace mkmoe_latent;
+  AppendParams a;
+  ProjectParams k, v;
+  AttendParams s;
+  if (int rc = append_params(append, ws, ws_bytes, a)) return rc;
+  if (int rc = project_params(absorb, k)) return rc;
+  if (int rc = attend_params(attend, ws, ws_bytes, s)) return rc;
+  if (int rc = project_params(expand, v)) return rc;
+  if (absorb->expand || !expand->expand) return MKMOE_ERR_ARG;
+  if (append->tokens != attend->tokens || absorb->tokens != attend->tokens || expand->tokens != attend->tokens)
+    return MKMOE_ERR_ROWS;
+  if (s.tokens == 0) return MKMOE_OK;
+  hipStream_t st = (hipStream_t)stream;
+  const int first = (int)absorb_blocks(k);
+  if (append->cache.fmt == MKMOE_LATENT_MXFP8)
+    hipLaunchKernelGGL(k_latent_front<true>, dim3(first + append_blocks(a)), dim3(256), 0, st, a, k, first);
+  else
+    hipLaunchKernelGGL(k_latent_front<false>, dim3(first + append_blocks(a)), dim3(256), 0, st, a, k, first);
+  if (int rc = launched()) return rc;
+  if (int rc = attend_launch(attend, s, st)) return rc;
+  return expand_launch(v, st);
 }
 
 int mkmoe_latent_read_errors(const void* ws, int32_t* words, int32_t n, void* stream) {

@@ -8,7 +8,7 @@ stream without a host synchronisation (``include/mkmoe.h``, latent attention):
 - ``rows``: the values that cache rows stand for
 - ``absorb`` / ``expand``: every head's query through W_UK, its result through W_UV
 - ``attend``: the absorbed attention over the cached rows
-- ``attention``: a layer's whole step, the four in turn
+- ``attention``: a layer's whole step in one call: the first two in one launch, then the others
 
 Caches (``cache_like``): bf16 [pages, page_size, 576], or MXFP8 as uint8 [pages, page_size, 656]
 (512 e4m3 codes, 16 E8M0 scales, one per 32 latent values, and the 64 rope values in bf16). The
@@ -53,12 +53,12 @@ class LatentWeights:
 
     def check(self, heads: int, device=None) -> None:
         """Raise unless each tensor has its shape and dtype and is contiguous on one GPU."""
-        for name, shape in (("norm", (LATENT,)), ("kv_b", (heads * (NOPE + V), LATENT))):
-            t = getattr(self, name)
+        at = None if device is None else torch.device(device)
+        for name, t, shape in (("norm", self.norm, (LATENT,)), ("kv_b", self.kv_b, (heads * (NOPE + V), LATENT))):
             if t is None:
                 raise RuntimeError(f"latent {name}: missing, want {shape} {BF}")
-            dev_ok = t.is_cuda and (device is None or t.device == torch.device(device))
-            if not (tuple(t.shape) == shape and t.dtype == BF and t.is_contiguous() and dev_ok):
+            dev_ok = t.is_cuda and (at is None or t.device == at)
+            if not (t.shape == shape and t.dtype == BF and t.is_contiguous() and dev_ok):
                 raise RuntimeError(
                     f"latent {name}: {tuple(t.shape)} {t.dtype} {t.device} contiguous={t.is_contiguous()}, "
                     f"want {shape} {BF} contiguous on the GPU"
@@ -95,44 +95,51 @@ class LatentRunner:
         self.device = torch.device("cuda", torch.cuda.current_device() if dev.index is None else dev.index)
         no_capture("the latent workspace")
         with torch.cuda.device(self.device):
-            self.ws = torch.zeros(n.value, dtype=torch.uint8, device=self.device)
-            mk = lambda w: torch.empty(self.max_tokens, self.heads, w, dtype=BF, device=self.device)  # noqa: E731
-            self._q_lat, self._q_pe, self._o_lat = mk(LATENT), mk(ROPE), mk(LATENT)
-            torch.cuda.current_stream().synchronize()  # whichever stream comes first finds it zeroed
+            self.ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+            self.clear_errors()
+            mk = lambda w, t: torch.empty(self.max_tokens, self.heads, w, dtype=t, device=self.device)  # noqa: E731
+            # (the attended latents stay in fp32: one rounding less before the output's own)
+            self._q_lat, self._q_pe, self._o_lat = mk(LATENT, BF), mk(ROPE, BF), mk(LATENT, torch.float32)
+            torch.cuda.current_stream().synchronize()  # whichever stream comes first finds them cleared
+        self._index = self.device.index
+        self._append_io, self._attend_io = _lib.LatentAppendIO(), _lib.LatentAttendIO()
+        self._absorb_io, self._expand_io = _lib.LatentProjectIO(), _lib.LatentProjectIO()
+        self._ws = (self.ws.data_ptr(), self.ws.numel())
 
     # ---- argument checks
     def _bad(self, name: str, t, want: str):
         got = "missing" if t is None else f"{tuple(t.shape)} {t.dtype} {t.device} strides {t.stride()}"
         return RuntimeError(f"mkmoe latent {name}: {got}, want {want} on {self.device}")
 
-    def _rows3(self, name: str, t, tokens: int, width: int, written: bool = False) -> tuple:
-        """(pointer, token stride, head stride) of a bf16 [tokens, heads, width] tensor whose last
-        axis is contiguous and whose rows start on 16 bytes."""
+    def _rows3(self, name: str, t, tokens: int, width: int, written: bool = False, dtype=BF) -> tuple:
+        """(pointer, token stride, head stride) of a [tokens, heads, width] tensor whose last axis is
+        contiguous and whose rows start on 16 bytes."""
         h = self.heads
-        if t is not None and t.dtype == BF and t.device == self.device and t.shape == (tokens, h, width):
+        if t is not None and t.dtype == dtype and t.get_device() == self._index and t.shape == (tokens, h, width):
             ts, hs, last = t.stride()
             ts, hs = ts if tokens > 1 else 0, hs if h > 1 else 0
-            ok = last == 1 and ts % 8 == 0 and hs % 8 == 0 and t.data_ptr() % 16 == 0
+            at = t.data_ptr()
+            ok = last == 1 and ts % 8 == 0 and hs % 8 == 0 and at % 16 == 0
             if ok and written:  # no two rows of an output share a place
-                a, b = (ts, tokens), (hs, h)
-                (s0, n0), (s1, n1) = (a, b) if ts >= hs else (b, a)
+                s0, n0, s1, n1 = (ts, tokens, hs, h) if ts >= hs else (hs, h, ts, tokens)
                 ok = (n1 == 1 or s1 >= width) and (n0 == 1 or s0 >= (n1 - 1) * s1 + width)
             if ok:
-                return t.data_ptr(), ts, hs
-        raise self._bad(name, t, f"[{tokens}, {h}, {width}] {BF}, rows of whole 16-byte pieces")
+                return at, ts, hs
+        raise self._bad(name, t, f"[{tokens}, {h}, {width}] {dtype}, rows of whole 16-byte pieces")
 
-    def _vec(self, name: str, t, n: int, dtypes: tuple) -> int:
-        if t is None or t.device != self.device or t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous():
-            raise self._bad(name, t, f"[{n}] {dtypes[0]} contiguous")
-        return t.data_ptr()
+    def _vec(self, name: str, t, n: int, *dtypes) -> int:
+        if (t is not None and t.dtype in dtypes and t.get_device() == self._index and t.shape == (n,)
+                and t.is_contiguous()):  # fmt: skip
+            return t.data_ptr()
+        raise self._bad(name, t, f"[{n}] {dtypes[0]} contiguous")
 
-    def _cache(self, t) -> _lib.LatentCache:
-        if t is not None and t.dim() == 3 and t.device == self.device and t.is_contiguous():
+    def _cache(self, t) -> tuple:
+        if t is not None and t.dim() == 3 and t.get_device() == self._index and t.is_contiguous():
             pages, page, row = t.shape
-            if (t.dtype, row) == (BF, ROW):
-                return _lib.LatentCache(t.data_ptr(), pages, page, _lib.LATENT_BF16)
-            if (t.dtype, row) == (torch.uint8, MX_ROW):
-                return _lib.LatentCache(t.data_ptr(), pages, page, _lib.LATENT_MXFP8)
+            if row == ROW and t.dtype == BF:
+                return t.data_ptr(), pages, page, _lib.LATENT_BF16
+            if row == MX_ROW and t.dtype == torch.uint8:
+                return t.data_ptr(), pages, page, _lib.LATENT_MXFP8
         raise self._bad("cache", t, f"[pages, page_size, {ROW}] {BF} or [pages, page_size, {MX_ROW}] torch.uint8 contiguous")
 
     def _new(self, what: str, *shape) -> torch.Tensor:
@@ -141,13 +148,61 @@ class LatentRunner:
 
     def _call(self, fn, *args) -> None:
         """``fn`` on the current stream of this runner's GPU."""
-        if torch.cuda.current_device() != self.device.index:
+        stream = torch._C._cuda_getCurrentRawStream(self._index)  # (current_stream()'s, without its object)
+        if torch.cuda.current_device() != self._index:
             with torch.cuda.device(self.device):
-                rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+                rc = fn(*args, stream)
         else:
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, stream)
         if rc:
             _lib.check(rc, fn.__name__)
+
+    # ---- the calls' arguments, checked and written into their structures
+    def _set_append(self, cache, kv, norm, cos_sin, positions, slots, heads: int, q: tuple, q_out: tuple) -> int:
+        c = self._cache(cache)
+        if kv is None or kv.dim() != 2 or kv.shape[1] != ROW or kv.dtype != BF or kv.get_device() != self._index:
+            raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}")
+        tokens, at = kv.shape[0], kv.data_ptr()
+        stride, last = kv.stride()
+        if tokens <= 1:
+            stride = ROW
+        if last != 1 or stride % 8 or stride < ROW or at % 16:
+            raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}, rows of whole 16-byte pieces")
+        w = 0 if norm is None else self._vec("norm", norm, LATENT, BF)
+        if (cos_sin is None or cos_sin.dim() != 2 or cos_sin.shape[1] != ROPE or cos_sin.dtype != torch.float32
+                or cos_sin.get_device() != self._index or not cos_sin.is_contiguous()):  # fmt: skip
+            raise self._bad("cos_sin", cos_sin, f"[positions, {ROPE}] torch.float32 contiguous")
+        pos = self._vec("positions", positions, tokens, torch.int64, torch.int32)
+        slot = self._vec("slots", slots, tokens, positions.dtype)
+        _lib.LATENT_APPEND.pack_into(
+            self._append_io, 0, *c, tokens, heads, self.rope, 8 if positions.dtype == torch.int64 else 4,
+            cos_sin.shape[0], stride, q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot,
+            q[0], q_out[0], self.norm_eps, 0,
+        )  # fmt: skip
+        return tokens
+
+    def _set_attend(self, cache, tokens: int, q_lat: tuple, q_pe: tuple, table, lens, q_starts, out: tuple,
+                    f32: int, lse: int) -> None:  # fmt: skip
+        c = self._cache(cache)
+        if (table is None or table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != self._index
+                or table.stride(1) != 1 and table.shape[1] > 1):  # fmt: skip
+            raise self._bad("table", table, "[seqs, max_pages] torch.int32")
+        seqs, max_pages = table.shape
+        stride = table.stride(0) if seqs > 1 else max_pages
+        at_lens = self._vec("lens", lens, seqs, torch.int32)
+        at_starts = 0 if q_starts is None else self._vec("q_starts", q_starts, seqs + 1, torch.int32)
+        if not 1 <= seqs <= _lib.LATENT_MAX_SEQS or (q_starts is None and tokens % seqs):
+            raise RuntimeError(
+                f"mkmoe latent: {seqs} sequences of {tokens} query tokens, want 1 .. {_lib.LATENT_MAX_SEQS} sequences "
+                "and, without q_starts, as many tokens in each"
+            )
+        _lib.LATENT_ATTEND.pack_into(
+            self._attend_io, 0, *c, seqs, tokens, self.heads, max_pages, stride, q_lat[1], q_lat[2], q_pe[1], q_pe[2],
+            out[1], out[2], q_lat[0], q_pe[0], table.data_ptr(), at_lens, at_starts, out[0], lse, self.scale, f32,
+        )  # fmt: skip
+
+    def _set_project(self, io, tokens: int, expand: int, f32: int, x: tuple, w: int, y: tuple) -> None:
+        _lib.LATENT_PROJECT.pack_into(io, 0, tokens, self.heads, expand, f32, x[1], x[2], y[1], y[2], x[0], w, y[0])
 
     # ---- the calls
     def append(
@@ -165,51 +220,37 @@ class LatentRunner:
         ``q_pe`` itself). A token with a negative slot is not stored. A slot outside the cache or
         a position outside ``cos_sin`` leaves the token unwritten and is recorded
         (``raise_on_device_error``)."""
-        c = self._cache(cache)
-        if kv is None or kv.dim() != 2 or kv.shape[1] != ROW or kv.dtype != BF or kv.device != self.device:
-            raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}")
-        tokens = kv.shape[0]
-        stride = kv.stride(0) if tokens > 1 else ROW
-        if kv.stride(1) != 1 or stride % 8 or stride < ROW or kv.data_ptr() % 16:
-            raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}, rows of whole 16-byte pieces")
-        if norm is not None:
-            self._vec("norm", norm, LATENT, (BF,))
-        if (cos_sin is None or cos_sin.dim() != 2 or cos_sin.shape[1] != ROPE or cos_sin.dtype != torch.float32
-                or cos_sin.device != self.device or not cos_sin.is_contiguous()):  # fmt: skip
-            raise self._bad("cos_sin", cos_sin, f"[positions, {ROPE}] torch.float32 contiguous")
-        pos = self._vec("positions", positions, tokens, (torch.int64, torch.int32))
-        slot = self._vec("slots", slots, tokens, (positions.dtype,))
-        qp = qts = qhs = op = ots = ohs = 0
+        qp = op = (0, 0, 0)
         if q_pe is not None:
-            qp, qts, qhs = self._rows3("q_pe", q_pe, tokens, ROPE)
+            if kv is None:
+                raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}")
+            tokens = kv.shape[0]
+            qp = self._rows3("q_pe", q_pe, tokens, ROPE)
             if q_out is None:
                 q_out = self._new("the rotated query", tokens, self.heads, ROPE)
-            op, ots, ohs = self._rows3("q_out", q_out, tokens, ROPE, written=True)
+            op = self._rows3("q_out", q_out, tokens, ROPE, written=True)
         elif q_out is not None:
             raise RuntimeError("mkmoe latent q_out: given without q_pe")
-        io = _lib.LatentAppendIO(
-            c, tokens, self.heads if q_pe is not None else 0, self.rope, 8 if positions.dtype == torch.int64 else 4,
-            cos_sin.shape[0], stride, qts, qhs, ots, ohs, kv.data_ptr(), None if norm is None else norm.data_ptr(),
-            cos_sin.data_ptr(), pos, slot, qp or None, op or None, self.norm_eps, 0,
-        )  # fmt: skip
-        if tokens:
-            self._call(self.lib.mkmoe_latent_append, ctypes.byref(io), self.ws.data_ptr(), self.ws.numel())
+        if self._set_append(cache, kv, norm, cos_sin, positions, slots, 0 if q_pe is None else self.heads, qp, op):
+            self._call(self.lib.mkmoe_latent_append, self._append_io, *self._ws)
         return q_out
 
     def rows(self, cache: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """-> bf16 [T, 576]: the values that the cache rows ``slots`` stand for (a negative slot's
         are 0), exactly."""
-        c = self._cache(cache)
+        c = _lib.LatentCache(*self._cache(cache))
+        if slots is None or slots.dim() != 1:
+            raise self._bad("slots", slots, "[tokens] torch.int64 contiguous")
         tokens = slots.shape[0]
-        at = self._vec("slots", slots, tokens, (torch.int64, torch.int32))
+        at = self._vec("slots", slots, tokens, torch.int64, torch.int32)
         if out is None:
             out = self._new("the rows", tokens, ROW)
         if out.shape != (tokens, ROW) or out.dtype != BF or out.device != self.device or not out.is_contiguous():
             raise self._bad("out", out, f"[{tokens}, {ROW}] {BF} contiguous")
         if tokens:
             self._call(
-                self.lib.mkmoe_latent_rows, ctypes.byref(c), at, 8 if slots.dtype == torch.int64 else 4, tokens,
-                out.data_ptr(), self.ws.data_ptr(), self.ws.numel(),
+                self.lib.mkmoe_latent_rows, c, at, 8 if slots.dtype == torch.int64 else 4, tokens, out.data_ptr(),
+                *self._ws,
             )  # fmt: skip
         return out
 
@@ -219,13 +260,15 @@ class LatentRunner:
         if x is None or x.dim() != 3:
             raise self._bad(what, x, f"[tokens, {self.heads}, {width}] {BF}")
         tokens = x.shape[0]
-        xp, xts, xhs = self._rows3(what, x, tokens, width)
+        f32 = expand and x.dtype == torch.float32
+        x = self._rows3(what, x, tokens, width, dtype=torch.float32 if f32 else BF)
         if out is None:
             out = self._new("an output", tokens, self.heads, wide)
-        yp, yts, yhs = self._rows3("out", out, tokens, wide, written=True)
-        io = _lib.LatentProjectIO(tokens, self.heads, expand, 0, xts, xhs, yts, yhs, xp, w.kv_b.data_ptr(), yp)
+        io = self._expand_io if expand else self._absorb_io
+        y = self._rows3("out", out, tokens, wide, written=True)
+        self._set_project(io, tokens, expand, int(f32), x, w.kv_b.data_ptr(), y)
         if tokens:
-            self._call(self.lib.mkmoe_latent_project, ctypes.byref(io))
+            self._call(self.lib.mkmoe_latent_project, io)
         return out
 
     def absorb(self, w: LatentWeights, q_nope: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -233,7 +276,7 @@ class LatentRunner:
         return self._project("q_nope", w, q_nope, out, 0)
 
     def expand(self, w: LatentWeights, o_lat: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        """The attended latents [T, heads, 512] -> [T, heads, 128]: each head's through W_UV."""
+        """The attended latents [T, heads, 512], bf16 or fp32 -> bf16 [T, heads, 128]: each head's through W_UV."""
         return self._project("o_lat", w, o_lat, out, 1)
 
     def attend(
@@ -247,44 +290,28 @@ class LatentRunner:
         out: torch.Tensor | None = None,
         lse: torch.Tensor | None = None,  # [T, heads] fp32: receives log sum exp
     ) -> torch.Tensor:
-        """-> bf16 [T, heads, 512]. A sequence's queries are its last tokens: of n, query i sees the
+        """-> [T, heads, 512], bf16 or, where ``out`` is, fp32. A sequence's queries are its last tokens: of n, query i sees the
         first ``len - n + 1 + i`` tokens; one that sees none gives 0 (``lse`` -inf). Rows of ``out``
         behind the last sequence's queries stay as they were. Pages outside the cache and lengths
         or starts outside their bounds are recorded (``raise_on_device_error``)."""
-        c = self._cache(cache)
         if q_lat is None or q_lat.dim() != 3:
             raise self._bad("q_lat", q_lat, f"[tokens, {self.heads}, {LATENT}] {BF}")
         tokens = q_lat.shape[0]
-        ql, ql_ts, ql_hs = self._rows3("q_lat", q_lat, tokens, LATENT)
-        qp, qp_ts, qp_hs = self._rows3("q_pe", q_pe, tokens, ROPE)
-        i32 = torch.int32
-        if (table is None or table.dim() != 2 or table.dtype != i32 or table.device != self.device
-                or table.stride(1) != 1 and table.shape[1] > 1):  # fmt: skip
-            raise self._bad("table", table, "[seqs, max_pages] torch.int32")
-        seqs, max_pages = table.shape
-        t_stride = table.stride(0) if seqs > 1 else max_pages
-        at_lens = self._vec("lens", lens, seqs, (i32,))
-        at_starts = None if q_starts is None else self._vec("q_starts", q_starts, seqs + 1, (i32,))
-        if not 1 <= seqs <= _lib.LATENT_MAX_SEQS or (q_starts is None and tokens % seqs):
-            raise RuntimeError(
-                f"mkmoe latent: {seqs} sequences of {tokens} query tokens, want 1 .. {_lib.LATENT_MAX_SEQS} sequences "
-                "and, without q_starts, as many tokens in each"
-            )
+        ql = self._rows3("q_lat", q_lat, tokens, LATENT)
+        qp = self._rows3("q_pe", q_pe, tokens, ROPE)
         if out is None:
             out = self._new("the attended rows", tokens, self.heads, LATENT)
-        op, o_ts, o_hs = self._rows3("out", out, tokens, LATENT, written=True)
-        at_lse = None
+        f32 = out.dtype == torch.float32
+        op = self._rows3("out", out, tokens, LATENT, written=True, dtype=torch.float32 if f32 else BF)
+        at_lse = 0
         if lse is not None:
             if (lse.dtype != torch.float32 or lse.shape != (tokens, self.heads) or lse.device != self.device
                     or not lse.is_contiguous()):  # fmt: skip
                 raise self._bad("lse", lse, f"[{tokens}, {self.heads}] torch.float32 contiguous")
             at_lse = lse.data_ptr()
-        io = _lib.LatentAttendIO(
-            c, seqs, tokens, self.heads, max_pages, t_stride, ql_ts, ql_hs, qp_ts, qp_hs, o_ts, o_hs, ql, qp,
-            table.data_ptr(), at_lens, at_starts, op, at_lse, self.scale, 0,
-        )  # fmt: skip
+        self._set_attend(cache, tokens, ql, qp, table, lens, q_starts, op, int(f32), at_lse)
         if tokens:
-            self._call(self.lib.mkmoe_latent_attend, ctypes.byref(io), self.ws.data_ptr(), self.ws.numel())
+            self._call(self.lib.mkmoe_latent_attend, self._attend_io, *self._ws)
         return out
 
     def attention(
@@ -306,23 +333,32 @@ class LatentRunner:
         of ``append`` and ``attend``; ``lens`` counts the appended tokens."""
         if q is None or q.dim() != 3 or q.shape[0] > self.max_tokens:
             raise self._bad("q", q, f"[tokens <= {self.max_tokens}, {self.heads}, {NOPE + ROPE}] {BF}")
-        tokens = q.shape[0]
-        self._rows3("q", q, tokens, NOPE + ROPE)
-        w.check(self.heads, self.device)
+        tokens, h = q.shape[0], self.heads
+        at, ts, hs = self._rows3("q", q, tokens, NOPE + ROPE)
+        w.check(h, self.device)
         if out is None:
-            out = self._new("the attention's output", tokens, self.heads, V)
-        self._rows3("out", out, tokens, V, written=True)
-        q_lat, q_pe, o_lat = self._q_lat[:tokens], self._q_pe[:tokens], self._o_lat[:tokens]
-        self.append(cache, kv, w.norm, cos_sin, positions, slots, q_pe=q[..., NOPE:], q_out=q_pe)
-        self.absorb(w, q[..., :NOPE], out=q_lat)
-        self.attend(cache, q_lat, q_pe, table, lens, q_starts=q_starts, out=o_lat)
-        return self.expand(w, o_lat, out=out)
+            out = self._new("the attention's output", tokens, h, V)
+        y = self._rows3("out", out, tokens, V, written=True)
+        if kv is None or kv.shape[0] != tokens:
+            raise self._bad("kv", kv, f"[{tokens}, {ROW}] {BF}")
+        q_lat, q_pe, o_lat = ((t.data_ptr(), h * n, n) for t, n in ((self._q_lat, LATENT), (self._q_pe, ROPE), (self._o_lat, LATENT)))
+        kv_b = w.kv_b.data_ptr()
+        self._set_append(cache, kv, w.norm, cos_sin, positions, slots, h, (at + 2 * NOPE, ts, hs), q_pe)
+        self._set_project(self._absorb_io, tokens, 0, 0, (at, ts, hs), kv_b, q_lat)
+        self._set_attend(cache, tokens, q_lat, q_pe, table, lens, q_starts, o_lat, 1, 0)
+        self._set_project(self._expand_io, tokens, 1, 1, o_lat, kv_b, y)
+        if tokens:
+            self._call(
+                self.lib.mkmoe_latent_step, self._append_io, self._absorb_io, self._attend_io, self._expand_io,
+                *self._ws,
+            )  # fmt: skip
+        return out
 
     # ---- device errors
     def read_errors(self) -> list[int]:
         """The device error words (synchronises the stream)."""
         words = (ctypes.c_int32 * _lib.LATENT_ERRW_WORDS)()
-        self._call(self.lib.mkmoe_latent_read_errors, self.ws.data_ptr(), words, _lib.LATENT_ERRW_WORDS)
+        self._call(self.lib.mkmoe_latent_read_errors, self._ws[0], words, _lib.LATENT_ERRW_WORDS)
         return list(words)
 
     def raise_on_device_error(self) -> None:

@@ -416,10 +416,10 @@ def _layer(fmt, heads, lens, n, page=16, seed=0):
 def test_attention_is_its_parts(fmt, heads, lens, n):
     """One call against append, absorb, attend and expand, bit for bit, and against 64 bits.
 
-    Five bf16 roundings lie on the way (absorbed query, rotated query, numerators, attended
-    latents, output), each off by at most 2^-8 of its value and 2^-8 / sqrt(3) in the mean square;
-    those of the query reach the output through scores of spread about 1. Their root mean square
-    is below sqrt(5 / 3) 2^-8 = 1.3 2^-8 of the output's; twice that is asked for."""
+    Four bf16 roundings lie on the way (absorbed query, rotated query, numerators, output; the
+    attended latents stay in fp32), each off by at most 2^-8 of its value and 2^-8 / sqrt(3) in the
+    mean square; those of the query reach the output through scores of spread about 1. Their root
+    mean square is below sqrt(4 / 3) 2^-8 = 1.16 2^-8 of the output's; twice that is asked for."""
     print(f"\nattention {fmt} heads={heads} lens={lens} n={n}", flush=True)
     d = _layer(fmt, heads, lens, n, seed=heads)
     run = _runner(heads)
@@ -429,7 +429,8 @@ def test_attention_is_its_parts(fmt, heads, lens, n):
     run.raise_on_device_error()
     w, q = d["w"], d["q"]
     q_pe = run.append(c2, d["kv"], w.norm, d["cos_sin"], d["positions"], d["slots"], q_pe=q[..., 128:])
-    o = run.attend(c2, run.absorb(w, q[..., :128]), q_pe, d["table"], d["lens"])
+    o = torch.empty(q.shape[0], heads, 512, device="cuda")
+    run.attend(c2, run.absorb(w, q[..., :128]), q_pe, d["table"], d["lens"], out=o)
     assert torch.equal(c2, d["cache"])
     assert torch.equal(run.expand(w, o), out)
     wk = w.kv_b.double().view(heads, 256, 512)
@@ -438,7 +439,29 @@ def test_attention_is_its_parts(fmt, heads, lens, n):
     want, *_ = ref.attend(d["cache"], ql, qr, d["table"], lens, SCALE)
     want = (want.transpose(0, 1) @ wk[:, 128:].transpose(1, 2)).transpose(0, 1)
     err = float((out.double() - want).norm() / want.norm())
-    assert err <= 2 * 1.3 * ref.U16, err
+    assert err <= 2 * 1.16 * ref.U16, err
+
+
+@pytest.mark.parametrize("fmt,page", [("bf16", 64), ("mxfp8", 1)])
+@pytest.mark.parametrize("heads,lens,n", [(32, [1, 70, 0, 4000], 1), (64, [500, 33], 4)])
+def test_attend_in_fp32(fmt, page, heads, lens, n):
+    """fp32 outputs, cut sequences' among them, round to the bf16 ones bit for bit; W_UV of them is
+    off by the output's rounding 2^-8, the 2^-17 that two bf16 parts leave of a value (each part's
+    rounding is within 2^-8 of what it rounds: 2^-16), and 512 fp32 sums."""
+    print(f"\nattend fp32 {fmt} page={page} heads={heads} lens={lens} n={n}", flush=True)
+    d, run = _layer(fmt, heads, lens, n, seed=3, page=page), _runner(heads)
+    w, q_pe = d["w"], d["q"][..., 128:]
+    ql = run.absorb(w, d["q"][..., :128])
+    wide = torch.full((q_pe.shape[0], heads, 520), 7.0, device="cuda")
+    o = run.attend(d["cache"], ql, q_pe, d["table"], d["lens"], out=wide[..., :512])
+    assert o.dtype == torch.float32 and bool((wide[..., 512:] == 7).all())
+    assert torch.equal(o.to(BF), run.attend(d["cache"], ql, q_pe, d["table"], d["lens"]))
+    wv = w.kv_b.double().view(heads, 256, 512)[:, 128:].transpose(1, 2)
+    want = (o.double().transpose(0, 1) @ wv).transpose(0, 1)
+    size = (o.double().abs().transpose(0, 1) @ wv.abs()).transpose(0, 1)
+    bound = (ref.U16 * want.abs() + (2.0**-16 + 520 * ref.U32) * size) * 1.01
+    ref.assert_within(run.expand(w, o), want, bound, "expand of fp32")
+    run.raise_on_device_error()
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
