@@ -363,18 +363,15 @@ __device__ const u32x4 g_zero_row[kRow * 2 / 16] = {};
 // Bytes from global memory straight into LDS: lane l's land at lds + 16 l (4 l). One asm
 // statement, so that the compiler does not wait for it before other reads of LDS; the caller
 // waits (wait_loads) before the bytes are read
-__device__ __forceinline__ uint32_t lds_at(const void* lds) {
-  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)(uint8_t*)const_cast<void*>(lds));
-}
-__device__ __forceinline__ void lds_dma16(const void* g, const void* lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_at(lds)) : "memory", "m0");
+__device__ __forceinline__ void lds_dma16(const void* g, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
 }
 // (lane l's from base + at)
-__device__ __forceinline__ void lds_dma16(const void* base, uint32_t at, const void* lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(lds_at(lds)) : "memory", "m0");
+__device__ __forceinline__ void lds_dma16(const void* base, uint32_t at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(lds) : "memory", "m0");
 }
-__device__ __forceinline__ void lds_dma4(const void* g, const void* lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_at(lds)) : "memory", "m0");
+__device__ __forceinline__ void lds_dma4(const void* g, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
 }
 // waits until at most N of the wave's loads are on their way (they complete in order)
 template <int N>
@@ -425,7 +422,7 @@ struct __align__(256) AttendSmem {
   int start[kMaxSeqs];         // first tile of each sequence in the work
   int scan[8];
   int first[4];                // the share's first sequence: its number, t0, n, len
-  int moved[3];                // a tile's flag: some row's maximum has to move
+  int moved[4];                // a tile's flag: some row's maximum has to move
   uint8_t bad[kN];             // tokens of the tile with a non-finite latent value
 };
 
@@ -443,8 +440,8 @@ struct __align__(256) AttendSmem {
 //                 B = Q^T, which stays in registers
 //   P             exp2 of the scores less the rows' running maxima (moved for both token groups
 //                 at once), bf16, [row][token] in LDS; the sums stay fp32
-//   O^T += V^T P^T   latent values 32 w .. of a scoring wave (32 of them), 128 + 96 l .. of the others
-//                 (96), for every row: A = V^T by transposing LDS reads of the same tile, B = P^T
+//   O^T += V^T P^T   latent values 32 w .. of a scoring wave (32 of them), 16 of every 64 past 128 of the
+//                 others (96), for every row: A = V^T by transposing LDS reads of the same tile, B = P^T
 // bf16 rows go straight from memory to LDS, three tiles ahead; MXFP8 rows go there as they are,
 // and waves 4 .. 7 turn the next tile's into bf16 (exact) while waves 0 .. 3 score.
 // PAGED: pages of kN tokens or more, so that a tile lies in one and its rows follow each other;
@@ -511,6 +508,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 
   const uint32_t tiles = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)sm.tile[0];
   const uint32_t p_at = (uint32_t)(uintptr_t)(MKMOE_LDS uint16_t*)sm.p[0];
+  const uint32_t raws = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)sm.raw[0];
+  const uint32_t ents = (uint32_t)(uintptr_t)(MKMOE_LDS int*)sm.ent[0];
+  // the lane, in the wide variant formed anew where it is used
+  auto own_lane = [&]() { return M == 32 ? lane : anew(lane); };
 
   int b = __builtin_amdgcn_readfirstlane(sm.first[0]);
   Seq s = {__builtin_amdgcn_readfirstlane(sm.first[1]), __builtin_amdgcn_readfirstlane(sm.first[2]),
@@ -553,7 +554,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     auto entries = [&](int t) {
       if constexpr (!PAGED) {
         const int ln = anew(lane), tok = min(t * kN + ln, lim_hi - 1);
-        if (wave == 7 && ln < kN) lds_dma4(table + (tok >> p.page_shift), sm.ent[t % kEnts]);
+        if (wave == 7 && ln < kN) lds_dma4(table + (tok >> p.page_shift), ents + (t % kEnts) * (4 * kN));
       }
     };
     bool lost = false;  // a page outside the cache
@@ -587,76 +588,70 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         base = p.cache + (uint64_t)row * kRowBytes;
       }
       if constexpr (MX) {  // load i of wave l is number 4 i + l of the tile's 1 KB pieces
-        uint8_t* dst = sm.raw[(t - tile0) % kMxRing] + lw * 1024;
-        const int ln = anew(lane) + lw * 64;
+        const uint32_t dst = raws + (t - tile0) % kMxRing * (kN * kMxRow) + lw * 1024;
+        const int ln = own_lane();
+        const bool ends = lw < kMxLoads % 4 && ln < kN * kPieces % 64;  // the last load, not a whole one
         if (PAGED && whole && in) {
+          const uint32_t at = (lw * 64 + ln) << 4;
 #pragma unroll
-          for (int i = 0; i < kLoads; ++i)
-            if ((i < kLoads - 1 || 4 * i + lw < kMxLoads) && i * 256 + ln < kN * kPieces)
-              lds_dma16(base, (i * 256 + ln) << 4, dst + i * 4096);
+          for (int i = 0; i < kLoads - 1; ++i) lds_dma16(base, at + i * 4096, dst + i * 4096);
+          if (ends) lds_dma16(base, at + (kLoads - 1) * 4096, dst + (kLoads - 1) * 4096);
         } else {
-          const uint8_t* src[kLoads];
 #pragma unroll
           for (int i = 0; i < kLoads; ++i) {
-            const uint32_t at = i * 256 + ln, r = min(at / kPieces, (uint32_t)kN - 1);
+            const uint32_t at = i * 256 + lw * 64 + ln, r = min(at / kPieces, (uint32_t)kN - 1);
             const uint8_t* row = !PAGED ? addr[r] : in && (int)r < left ? base + r * kRowBytes : (const uint8_t*)g_zero_row;
-            src[i] = row + ((at - r * kPieces) << 4);
+            if (i < kLoads - 1 || ends) lds_dma16(row + ((at - r * kPieces) << 4), dst + i * 4096);
           }
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i)
-            if ((i < kLoads - 1 || 4 * i + lw < kMxLoads) && i * 256 + ln < kN * kPieces)
-              lds_dma16(src[i], dst + i * 4096);
         }
       } else {  // wave l: the rows 8 l .. 8 l + 7, a load each and one for their rope parts
-        uint8_t* dst = sm.tile[(t - tile0) % kRing];
-        const int ln = anew(lane), r = 8 * lw + (ln >> 3);
-        const uint32_t rope_at = 2 * kL + (((ln & 7) ^ swz_rope(r)) << 4);
-        const uint64_t row = PAGED ? 0 : (uint64_t)addr[r];
-        const uint32_t lo = (uint32_t)row, hi = (uint32_t)(row >> 32);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint8_t* from;
-          if (PAGED)
-            from = in && 8 * lw + i < left ? base + (8 * lw + i) * kRowBytes : (const uint8_t*)g_zero_row;
-          else
-            from = (const uint8_t*)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, 8 * i) << 32) |
-                                    (uint32_t)__builtin_amdgcn_readlane(lo, 8 * i));
-          lds_dma16(from, (ln ^ swz(8 * lw + i)) << 4, dst + (8 * lw + i) * (2 * kL));
-        }
-        uint8_t* rope_to = dst + kRopeAt + 8 * lw * (2 * kR);
+        const uint32_t dst = tiles + (t - tile0) % kRing * kTileBytes, to = dst + 8 * lw * (2 * kL);
+        const uint32_t rope_to = dst + kRopeAt + 8 * lw * (2 * kR);
+        const int ln = own_lane(), r = 8 * lw + (ln >> 3);
+        const uint32_t at = (ln ^ swz(8 * (lw & 1))) << 4, rope_at = 2 * kL + (((ln & 7) ^ swz_rope(r)) << 4);
         if (PAGED && whole && in) {
-          lds_dma16(base, r * kRowBytes + rope_at, rope_to);
+          base += 8 * lw * kRowBytes;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) lds_dma16(base, (at ^ (swz(i) << 4)) + i * kRowBytes, to + i * (2 * kL));
+          lds_dma16(base, (ln >> 3) * kRowBytes + rope_at, rope_to);
         } else {
+          const uint64_t row = PAGED ? 0 : (uint64_t)addr[r];
+          const uint32_t lo = (uint32_t)row, hi = (uint32_t)(row >> 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint8_t* from;
+            if (PAGED)
+              from = in && 8 * lw + i < left ? base + (8 * lw + i) * kRowBytes : (const uint8_t*)g_zero_row;
+            else
+              from = (const uint8_t*)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, 8 * i) << 32) |
+                                      (uint32_t)__builtin_amdgcn_readlane(lo, 8 * i));
+            lds_dma16(from, at ^ (swz(i) << 4), to + i * (2 * kL));
+          }
           const uint8_t* from = !PAGED ? (const uint8_t*)row : in && r < left ? base + r * kRowBytes : (const uint8_t*)g_zero_row;
           lds_dma16(from + rope_at, rope_to);
         }
       }
     };
-    // (waves 4 .. 7) the raw rows of tile t as bf16: 8 threads a row, the codes 16 j .. of every 8
-    // pieces each
+    // (waves 4 .. 7) the raw rows of tile t as bf16: 8 threads a row, the codes 8 j .. of every 64 each
     auto unpack = [&](int t) {
       if constexpr (MX) {
-        const int th = lw * 64 + anew(lane), r = th >> 3, j = th & 7;
-        const uint8_t* src = sm.raw[(t - tile0) % kMxRing] + r * kMxRow;
-        uint8_t* dst = sm.tile[(t - tile0) & 1];
-        u32x4 q[4];
-        float sc[4];
+        const int ln = own_lane(), r = 8 * lw + (ln >> 3), j = ln & 7;
+        const uint32_t src = raws + (t - tile0) % kMxRing * (kN * kMxRow) + r * kMxRow;
+        const uint32_t tile = tiles + ((t - tile0) & 1) * kTileBytes;
+        const u32x4 scales = lds_read<u32x4>(src + kL);
+        u32x2 q[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          q[i] = *(const u32x4*)(src + 16 * (8 * i + j));
-          sc[i] = e8m0(src[kL + 4 * i + (j >> 1)]);
-        }
-        const u32x4 pe = *(const u32x4*)(src + kL + kMxScales + 16 * j);
+        for (int i = 0; i < 8; ++i) q[i] = lds_read<u32x2>(src + 64 * i + 8 * j);
+        const u32x4 pe = lds_read<u32x4>(src + kL + kMxScales + 16 * j);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t at = ((j ^ swz(r)) << 4), dst = tile + r * (2 * kL);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          u32x4* to = (u32x4*)(dst + r * (2 * kL) + (((2 * (8 * i + j)) ^ swz(r)) << 4));  // (swz is even)
-          const u32x4 v0 = fp8x8(q[i].x, q[i].y, sc[i]), v1 = fp8x8(q[i].z, q[i].w, sc[i]);
-          // (odd lanes store their second half first: either store then meets every bank once)
-          const bool odd = j & 1;
-          to[odd] = odd ? v1 : v0;
-          to[!odd] = odd ? v0 : v1;
+        for (int i = 0; i < 8; ++i) {  // (the scale's byte, 2 i + j / 4, to the exponent's place)
+          const uint32_t two = scales[i >> 1] >> (8 * (j >> 2));
+          const uint32_t e = (i & 1 ? two << 7 : two << 23) & 0x7f800000u;
+          *(MKMOE_LDS u32x4*)(uintptr_t)((at ^ ((i & 1) << 7)) + dst + (i >> 1) * 256) = fp8x8(q[i].x, q[i].y, u2f(e));
         }
-        *(u32x4*)(dst + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) = pe;
+        *(MKMOE_LDS u32x4*)(uintptr_t)(tile + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) = pe;
       }
     };
     // waits until the tile after which `newer` more were requested has landed
@@ -696,16 +691,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       }
       barrier();
     };
-    // V^T of 16 C latent values from piece first (a multiple of 4): rows 8 g + col / 4 (and + 4), 4 values
-    // from 4 (lane % 4) of each 16
-    auto values = [&](uint32_t tile, int first, auto& va) {
-      const int ln = anew(lane), vtok = 8 * (ln >> 4) + ((ln & 15) >> 2);
-      const uint32_t x = (((ln & 3) >> 1) ^ swz(vtok)) << 4, row = tile + vtok * (2 * kL) + 8 * (ln & 1);
+    // V^T of the blocks of 16 latent values own + k + step c (k a multiple of what own stays under):
+    // rows 8 g + col / 4 (and + 4), 4 values from 4 (lane % 4) of each block
+    auto values = [&](uint32_t tile, int own, auto first, auto step, auto& va) __attribute__((always_inline)) {
+      constexpr int k = decltype(first)::value, by = decltype(step)::value;
+      const int ln = own_lane(), vtok = 8 * (ln >> 4) + ((ln & 15) >> 2);
+      const uint32_t x = ((((ln & 3) >> 1) ^ swz(vtok)) ^ (2 * own)) << 4, row = tile + vtok * (2 * kL) + 8 * (ln & 1);
       constexpr int C = sizeof(va) / sizeof(va[0]);
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int piece = first + 2 * c;
-        const uint32_t at = (x ^ ((piece & 15) << 4)) + (row + (piece >> 4) * 256);
+        const int n = k + by * c;
+        const uint32_t at = (x ^ ((n & 7) << 5)) + row + (n >> 3) * 256;
         struct { i16x4 a, b; } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((MKMOE_LDS i16x4*)(uintptr_t)at),
                                        __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                            (MKMOE_LDS i16x4*)(uintptr_t)(at + 4 * (2 * kL)))};
@@ -713,7 +709,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       }
     };
     auto numerators_of = [&](int t, bf16x8(&pb)[MB]) {
-      const int ln = anew(lane);
+      const int ln = own_lane();
       const uint32_t at = p_of(t) + (ln & 15) * (2 * kPStride) + ((ln >> 4) << 4);
 #pragma unroll
       for (int i = 0; i < MB; ++i) pb[i] = lds_read<bf16x8>(at + i * 16 * (2 * kPStride));
@@ -737,8 +733,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     const bool whole = tile0 == 0 && tile1 == kt;
     const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
     float* sums = (float*)sm.p[0];  // at the end: [row][token group]
-    // the rows out: latent values first .. of every row
-    auto store = [&](auto& o, int first, bool lead) {
+    // the rows out: latent values first + by c .. of every row
+    auto store = [&](auto& o, int first, int by, bool lead) {
       constexpr int C = sizeof(o) / sizeof(o[0]);
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
@@ -751,13 +747,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           const float inv = none ? 0.0f : 1.0f / sum;
           const int64_t to = (int64_t)(s.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + first + 4 * g;
 #pragma unroll
-          for (int c = 0; c < C; ++c) store4(p, to + 16 * c, o[c][i] * inv);
+          for (int c = 0; c < C; ++c) store4(p, to + by * c, o[c][i] * inv);
           if (p.lse && lead && g == 0)
             p.lse[(int64_t)(s.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
         } else {
           float* dst = p.part_o + ((int64_t)slot * M + r) * kL + first + 4 * g;
 #pragma unroll
-          for (int c = 0; c < C; ++c) *(f32x4*)(dst + 16 * c) = o[c][i];
+          for (int c = 0; c < C; ++c) *(f32x4*)(dst + by * c) = o[c][i];
           if (lead && g == 0) {
             p.part_ml[((int64_t)slot * M + r) * 2] = top;
             p.part_ml[((int64_t)slot * M + r) * 2 + 1] = sum;
@@ -789,7 +785,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         for (int ks = 0; ks < KS; ++ks)
           q[rb][ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
       }
-      if (tid < 3) sm.moved[tid] = 0;
+      if (tid < 4) sm.moved[tid] = 0;
       f32x4 o[2][MB];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
@@ -802,7 +798,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 
       auto step = [&](int t, auto is_steady) __attribute__((always_inline)) {
         constexpr bool steady = decltype(is_steady)::value;
-        const int ln = anew(lane), col = ln & 15, g = ln >> 4;
+        const int ln = own_lane(), col = ln & 15, g = ln >> 4;
         const uint32_t tile = tile_at(t);
         const bool edge = !steady && edges && (t + 1) * kN > lim_lo;
         if (edge) sanitize(t);
@@ -852,7 +848,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         }
         if (RB == 1) acc[0] += acc[1];
         bf16x8 va[2], pb[MB];
-        values(tile, 4 * wave, va);
+        values(tile, 2 * wave, std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{}, va);
         bool move = false;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -869,12 +865,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           move = move || top[rb] > m[rb] + kSlack;
         }
         numerators();
-        if (__any(move) && ln == 0) sm.moved[t % 3] = 1;
-        if (tid == 0) sm.moved[(t + 1) % 3] = 0;  // (last read before the last barrier)
+        if (__any(move) && ln == 0) sm.moved[t & 3] = 1;
+        if (tid == 0) sm.moved[(t + 1) & 3] = 0;  // (last read before the last barrier)
         barrier();
 
         numerators_of(t, pb);
-        if (__builtin_amdgcn_readfirstlane(sm.moved[t % 3])) {  // maxima move: the numerators again
+        if (__builtin_amdgcn_readfirstlane(sm.moved[t & 3])) {  // maxima move: the numerators again
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
             top[rb] = over_groups(top[rb], [](float a, float b) { return fmaxf(a, b); });
@@ -925,7 +921,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         }
         p.cut[blockIdx.x] = c;
       }
-      store(o, 32 * wave, wave == 0);
+      store(o, 32 * wave, 16, wave == 0);
     } else {
       // ---- the first tiles' rows
       const uint8_t** first = (const uint8_t**)sm.p[0];  // [kAhead][kN] (P is not in use yet)
@@ -973,14 +969,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
         bf16x8 va[6], pb[MB];
         // MXFP8: the next tile takes the place of t - 1
         if (MX && (steady || t + 1 < tend)) unpack(t + 1);
-        values(tile_at(t), 16 + 12 * lw, va);
+        values(tile_at(t), lw, std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}, va);
         // tile t + 1 is there at the barrier, and the one that takes the place of t - 1 (MXFP8: of the raw
         // t + 1) is requested after it
         if (!MX) landed(steady ? kAhead - 2 : min(kAhead - 2, tend - 2 - t));
         barrier();
 
         numerators_of(t, pb);
-        if (__builtin_amdgcn_readfirstlane(sm.moved[t % 3])) {
+        if (__builtin_amdgcn_readfirstlane(sm.moved[t & 3])) {
           barrier();
           barrier();
           rescale(o);
@@ -1005,7 +1001,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       if (lost) record(p.err, MKMOE_LATENT_ERR_PAGE, b);
       __syncthreads();
       __syncthreads();
-      store(o, 128 + 96 * lw, false);
+      store(o, 128 + 16 * lw, 64, false);
     }
   }
 }
