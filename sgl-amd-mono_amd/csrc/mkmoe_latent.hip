@@ -452,7 +452,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   constexpr int MB = M / 16;             // row blocks
   constexpr int RB = MB / 2;             // row blocks of a scoring wave
   constexpr int KS = kRow / 32;          // MFMA steps of a score: 18
-  constexpr int G = M == 32 ? 9 : 3;     // of them whose keys are read at once
+  constexpr int G = 3;                   // of them whose keys are read at once
   constexpr int kPieces = kMxRow / 16;   // 16-byte pieces of an MXFP8 row: 41
   constexpr int kMxLoads = (kN * kPieces + 63) / 64;  // wave loads of an MXFP8 tile: 21
   constexpr int kLoads = MX ? (kMxLoads + 3) / 4 : 9;  // of a wave, at most
