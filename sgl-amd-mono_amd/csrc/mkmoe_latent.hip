@@ -37,6 +37,7 @@ constexpr int kMxRow = MKMOE_LATENT_MX_ROW;
 constexpr int kNope = MKMOE_LATENT_NOPE, kV = MKMOE_LATENT_V;
 static_assert(kMxRow == kL + kMxScales + 2 * kR && kMxRow % 16 == 0, "MXFP8 rows in whole 16-byte pieces");
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -264,7 +265,7 @@ constexpr int kTileBytes = kN * kRow * 2;  // a tile's rows in LDS, bf16: the la
 constexpr int kRopeAt = kN * kL * 2;
 constexpr int kRing = 4;        // bf16 cache: tiles in LDS, one in use and three on their way
 constexpr int kMxRing = 3;      // MXFP8: raw tiles on their way
-constexpr int kSetup = 3;       // see setup()
+constexpr int kSetup = 8;       // see setup()
 constexpr int kEnts = 4;        // tiles whose page entries are in LDS
 // A row's maximum is moved only where a score passes it by more than 2^kSlack: numerators then stay
 // below 2^kSlack (bf16 and fp32 keep their relative precision there). After the first tiles almost
@@ -379,8 +380,8 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 // the same for all of them, as the compiler's own wait: it would otherwise place a wait for the
-// queries' registers in the tile loop, which counts the tiles' loads too
-__device__ __forceinline__ void wait_queries() {
+// registers that page entries or queries went to in the tile loop, which counts the tiles' loads too
+__device__ __forceinline__ void wait_all() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0, expcnt 7 (none), lgkmcnt 15 (none)
   asm volatile("" ::: "memory");
@@ -766,24 +767,46 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     __syncthreads();  // the last row tile's reads of LDS are over
 
     if (scores) {
-      // ---- the queries into registers (a row past the tile's rows takes the first one's: it is
-      // not stored)
+      // ---- the queries into registers (a row past the tile's takes the first one's: it is not stored).
+      // 32 rows a tile: by way of LDS, in the place of tiles that come later, as whole rows in order.
+      // Their pieces by 16 rows, straight into the registers, take 2 us, twice as long (one sequence of 1025
+      // tokens 16.2 us against 14.8); 64 rows a tile gain nothing by it (verify 65 us against 73)
+      constexpr bool kByLds = M == 32;
+      const uint32_t place = tiles + (MX ? 0 : kRing - 1) * kTileBytes;
+      if constexpr (kByLds) {
+        auto row_of = [&](int j, const uint16_t* q, int64_t ts, int64_t hs) {
+          const int r = 8 * wave + j, row = r0 + (r < nrows ? r : 0), i = over_heads(p, row);
+          return q + (int64_t)(s.t0 + i) * ts + (int64_t)(row - i * p.heads) * hs;
+        };
+        const uint64_t mine = (uint64_t)row_of(lane & 7, p.ql, p.ql_ts, p.ql_hs);
+        const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint8_t* row = (const uint8_t*)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, j) << 32) |
+                                                (uint32_t)__builtin_amdgcn_readlane(lo, j));
+          lds_dma16(row, (lane ^ swz(8 * wave + j)) << 4, place + (8 * wave + j) * (2 * kL));
+        }
+        const int r = 8 * wave + (lane >> 3);
+        lds_dma16((const uint8_t*)row_of(lane >> 3, p.qp, p.qp_ts, p.qp_hs) + (((lane & 7) ^ swz_rope(r)) << 4),
+                  place + kRopeAt + 8 * wave * (2 * kR));
+      }
       bf16x8 q[RB][KS];
       int lim[RB];
       float m[RB], l[RB];
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         const int r = (rg * RB + rb) * 16 + col;
-        const bool real = r < nrows;
-        const int i = over_heads(p, r0 + (real ? r : 0)), h = r0 + (real ? r : 0) - i * p.heads;
-        lim[rb] = real ? max(0, base + i) : 0;
+        const int row = r0 + (r < nrows ? r : 0), i = over_heads(p, row);
+        lim[rb] = r < nrows ? max(0, base + i) : 0;
         m[rb] = -kInf;
         l[rb] = 0.0f;
-        const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)h * p.ql_hs + 8 * g;
-        const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)h * p.qp_hs + 8 * g;
+        if constexpr (!kByLds) {
+          const uint16_t* ql = p.ql + (int64_t)(s.t0 + i) * p.ql_ts + (int64_t)(row - i * p.heads) * p.ql_hs + 8 * g;
+          const uint16_t* qp = p.qp + (int64_t)(s.t0 + i) * p.qp_ts + (int64_t)(row - i * p.heads) * p.qp_hs + 8 * g;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          q[rb][ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
+          for (int ks = 0; ks < KS; ++ks)
+            q[rb][ks] = *(const bf16x8*)(ks < kL / 32 ? ql + 32 * ks : qp + 32 * (ks - kL / 32));
+        }
       }
       if (tid < 4) sm.moved[tid] = 0;
       f32x4 o[2][MB];
@@ -791,8 +814,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < MB; ++i) o[c][i] = f32x4{0, 0, 0, 0};
-      if (!PAGED) barrier();
-      wait_queries();
+      wait_all();
+      barrier();
+      if constexpr (kByLds) {
+        const int r = rg * 16 + col;
+        const uint32_t at = place + r * (2 * kL) + ((g ^ swz(col)) << 4);
+        const uint32_t pe_at = place + kRopeAt + r * (2 * kR) + ((g ^ swz_rope(col)) << 4);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          q[0][ks] = ks < kL / 32 ? lds_read<bf16x8>((at ^ ((ks & 3) << 6)) + (ks >> 2) * 256)
+                                  : lds_read<bf16x8>(pe_at ^ ((ks & 1) << 6));
+      }
       barrier();
       if (MX) barrier();
 
@@ -937,11 +969,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
           if (i < kAhead * kN) first[i] = address(tile0 * kN + i, e);
           else sm.ent[(tile0 + i / kN) % kEnts][i % kN] = e;
         }
-        wait_queries();  // (the entries)
+        wait_all();
+        barrier();
+      }
+      // (PAGED: the first tile, and the others behind the queries)
+      if (PAGED) {
+        issue(tile0, pg[0], first, false);
         barrier();
       }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i)
+      for (int i = PAGED; i < kAhead; ++i)
         if (tile0 + i < tend) issue(tile0 + i, pg[i], first + i * kN, false);
       int pg_next = pg[kAhead];  // the page of the tile that is requested next
       if (tile0 + kAhead < tend) resolve(tile0 + kAhead);
@@ -1007,69 +1044,70 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 }
 
 // ---------------------------------------------------------------- merge
-// Row tiles that were cut, their parts joined in order at their common maximum. The work of a
-// tile is M rows by 4 quarters of the latent values; kMergeWgs workgroups at each of its cuts
-// share it, so that a long sequence's many parts are read by many. Few parts: 32 lanes a row's
-// quarter; many: the workgroup's 8 groups of 32 lanes take every eighth part and add up in LDS.
+// Row tiles that were cut, their parts joined in order at their common maximum; kMergeWgs workgroups
+// at each of a tile's cuts share its items, so that a long sequence's many parts are read by many. Few
+// parts: an item is a row's 128 latent values, 32 lanes with up to kAtOnce parts' loads on their way;
+// many: 64 values, the workgroup's 16 groups of 16 lanes take every 16th part and add up in LDS.
 constexpr int kMergeWgs = 8;
-constexpr int kFewParts = 16;
+constexpr int kFewParts = 32;
+constexpr int kAtOnce = 8;
 
 template <int M>
 __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
-  __shared__ float s_w[kShares], s_red[8];
-  __shared__ f32x4 s_acc[8][32];
+  __shared__ float s_w[kShares], s_red[4];
+  __shared__ f32x4 s_acc[16][16];
   const Cut c = p.cut[blockIdx.x];
   if (c.parts == 0) return;
-  const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5;
+  const int tid = threadIdx.x;
   const int helper = (blockIdx.x - c.share) * kMergeWgs + blockIdx.y, helpers = (c.parts - 1) * kMergeWgs;
   auto at = [&](int i, int r) { return (int64_t)(2 * (c.share + i) + (i == 0 ? 1 : 0)) * M + r; };
-  auto store = [&](int r, int part, f32x4 acc, float top, float sum) {
+  auto store = [&](int r, int first, f32x4 acc, float top, float sum) {  // 4 values of row r
     const int qi = over_heads(p, c.r0 + r), h = (c.r0 + r) - qi * p.heads;
     const bool none = c.base + qi <= 0;
     acc *= none ? 0.0f : 1.0f / sum;
-    store4(p, (int64_t)(c.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + 128 * part + 4 * lane, acc);
-    if (p.lse && part == 0 && lane == 0)
-      p.lse[(int64_t)(c.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
+    store4(p, (int64_t)(c.t0 + qi) * p.o_ts + (int64_t)h * p.o_hs + first, acc);
+    if (p.lse && first == 0) p.lse[(int64_t)(c.t0 + qi) * p.heads + h] = none ? -kInf : (top + log2f(sum)) * (1.0f / kLog2e);
   };
-  if (c.parts < kFewParts) {
+  if (c.parts <= kFewParts) {
+    const int lane = tid & 31, grp = tid >> 5;
     for (int item = helper * 8 + grp; item < 4 * c.nrows; item += helpers * 8) {
-      const int r = item >> 2, part = item & 3;
+      const int r = item >> 2, first = 128 * (item & 3) + 4 * lane;
       float mi = -kInf, li = 0.0f;
       if (lane < c.parts) {
         mi = p.part_ml[at(lane, r) * 2];
         li = p.part_ml[at(lane, r) * 2 + 1];
       }
-      const float* src = p.part_o + 128 * part + 4 * lane;
-      f32x4 v[4];
+      const float* src = p.part_o + first;
+      f32x4 v[kAtOnce];
+      auto fetch = [&](int i0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = *(const f32x4*)(src + at(min(i, c.parts - 1), r) * kL);
+        for (int i = 0; i < kAtOnce; ++i)
+          if (i0 + i < c.parts) v[i] = *(const f32x4*)(src + at(i0 + i, r) * kL);
+      };
+      fetch(0);
       float top = mi;
 #pragma unroll
-      for (int d = 8; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
+      for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
       const float w = __builtin_amdgcn_exp2f(mi - (top == -kInf ? 0.0f : top));
       float sum = w * li;
 #pragma unroll
-      for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 32);
+      for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 32);
       f32x4 acc = {0, 0, 0, 0};
-      for (int i0 = 0; i0 < c.parts; i0 += 4) {
-        f32x4 next[4];
+      for (int i0 = 0; i0 < c.parts; i0 += kAtOnce) {
+        if (i0 > 0) fetch(i0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i0 + 4 < c.parts) next[i] = *(const f32x4*)(src + at(min(i0 + 4 + i, c.parts - 1), r) * kL);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kAtOnce; ++i)
           if (i0 + i < c.parts) acc += __shfl(w, i0 + i, 32) * v[i];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = next[i];
       }
       top = __shfl(top, 0, 32);
       sum = __shfl(sum, 0, 32);
-      store(r, part, acc, top, sum);
+      store(r, first, acc, top, sum);
     }
     return;
   }
-  for (int item = helper; item < 4 * c.nrows; item += helpers) {
-    const int r = item >> 2, part = item & 3;
+  const int lane = tid & 15, grp = tid >> 4;
+  for (int item = helper; item < 8 * c.nrows; item += helpers) {
+    const int r = item >> 3, first = 64 * (item & 7) + 4 * lane;
     float mi = -kInf, li = 0.0f;
     if (tid < c.parts) {
       mi = p.part_ml[at(tid, r) * 2];
@@ -1077,32 +1115,28 @@ __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
     }
     float top = mi;
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
-    if (lane == 0) s_red[grp] = top;
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if ((tid & 63) == 0) s_red[tid >> 6] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, s_red[i]);
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, s_red[i]);
     const float w = __builtin_amdgcn_exp2f(mi - (top == -kInf ? 0.0f : top));
     s_w[tid] = w;
     float sum = w * li;
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 32);
+    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
     __syncthreads();
-    if (lane == 0) s_red[grp] = sum;
-    const float* src = p.part_o + 128 * part + 4 * lane;
+    if ((tid & 63) == 0) s_red[tid >> 6] = sum;
+    const float* src = p.part_o + first;
     f32x4 acc = {0, 0, 0, 0};
 #pragma unroll 8
-    for (int i = grp; i < c.parts; i += 8) acc += s_w[i] * *(const f32x4*)(src + at(i, r) * kL);
+    for (int i = grp; i < c.parts; i += 16) acc += s_w[i] * *(const f32x4*)(src + at(i, r) * kL);
     s_acc[grp][lane] = acc;
     __syncthreads();
     if (grp == 0) {
-      sum = s_red[0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) {
-        acc += s_acc[i][lane];
-        sum += s_red[i];
-      }
-      store(r, part, acc, top, sum);
+      for (int i = 1; i < 16; ++i) acc += s_acc[i][lane];
+      store(r, first, acc, top, (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]));
     }
     __syncthreads();
   }
