@@ -266,6 +266,7 @@ constexpr int kRopeAt = kN * kL * 2;
 constexpr int kRing = 4;        // bf16 cache: tiles in LDS, one in use and three on their way
 constexpr int kMxRing = 3;      // MXFP8: raw tiles on their way
 constexpr int kSetup = 8;       // see setup()
+constexpr int kNarrow = 4096;   // see k_latent_attend
 constexpr int kEnts = 4;        // tiles whose page entries are in LDS
 // A row's maximum is moved only where a score passes it by more than 2^kSlack: numerators then stay
 // below 2^kSlack (bf16 and fp32 keep their relative precision there). After the first tiles almost
@@ -281,7 +282,8 @@ struct Cut {
                         // slots 2 (share + 1), 2 (share + 2) ..
   int32_t t0, r0, nrows;  // the sequence's first query token, the tile's rows of it
   int32_t base;         // tokens that its first query sees (may be negative)
-  int32_t unused[2];
+  int32_t m;            // rows a tile: 32 or 64
+  int32_t unused;
 };
 
 struct AttendParams {
@@ -348,6 +350,10 @@ __device__ __forceinline__ int row_tiles(const AttendParams& p, const Seq& s) {
 }
 __device__ __forceinline__ int kv_tiles(const Seq& s) { return max(1, (s.len + kN - 1) / kN); }
 __device__ __forceinline__ int setup(const Seq& s) { return s.len > 0 ? kSetup : 0; }
+template <int M>
+__device__ __forceinline__ int work_of(const AttendParams& p, const Seq& s) {
+  return row_tiles<M>(p, s) * (kv_tiles(s) + setup(s));
+}
 
 // 16-byte pieces c of LDS row r are stored at piece c ^ swz(r) (latent parts, rows of 64 pieces) or
 // c ^ swz_rope(r) (rope parts, rows of 8). The LDS has 64 banks, 16 pieces. A 16-byte read serves
@@ -448,7 +454,7 @@ struct __align__(256) AttendSmem {
 // PAGED: pages of kN tokens or more, so that a tile lies in one and its rows follow each other;
 // without it each token's page entry is looked up.
 template <int M, bool MX, bool PAGED>
-__global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
+__device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M, MX>& sm, const Seq& own) {
   static_assert(M == 32 || M == 64, "row blocks of 16 by two token groups on 4 or 8 waves");
   constexpr int MB = M / 16;             // row blocks
   constexpr int RB = MB / 2;             // row blocks of a scoring wave
@@ -459,7 +465,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   constexpr int kLoads = MX ? (kMxLoads + 3) / 4 : 9;  // of a wave, at most
   constexpr int kRowBytes = MX ? kMxRow : 2 * kRow;
   constexpr int kAhead = MX ? kMxRing : kRing - 1;    // tiles on their way
-  __shared__ AttendSmem<M, MX> sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
   const bool scores = wave < 4;
@@ -467,13 +472,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   const int lw = wave & 3;                        // of the others: their number
 
   // ---- the work list
-  int mine = 0;
-  Seq own = {0, 0, 0, false};
-  if (tid < p.seqs) {
-    const Seq s = own = seq_of(p, tid);
-    mine = row_tiles<M>(p, s) * (kv_tiles(s) + setup(s));
-    if (s.bad && blockIdx.x == 0) record(p.err, MKMOE_LATENT_ERR_LENGTH, tid);
-  }
+  const int mine = work_of<M>(p, own);
   int inc = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -946,7 +945,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
       }
       __syncthreads();
       if (tid == 0 && w >= w1) {
-        Cut c = {0, 0, s.t0, r0, nrows, base, 0, 0};
+        Cut c = {0, 0, s.t0, r0, nrows, base, M, 0};
         if (tile1 < kt) {
           c.share = (unit0 + pre) / share;
           c.parts = (unit0 + pre + kt - 1) / share - c.share + 1;
@@ -1043,6 +1042,35 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   }
 }
 
+// One share of the work, in row tiles of 32 or 64. WIDE: sequences bring more than 32 query rows on
+// average; 64 rows a tile read the cache half as often (48 sequences of 8192, 64 heads: 119 us against
+// 160), but start, store and join twice the rows in each share, so that less than kNarrow tiles are
+// taken as 32 rows (8 sequences of 1250 26 us against 33; at 4096 tiles both take 51 to 57)
+template <bool MX, bool PAGED, bool WIDE>
+__global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
+  __shared__ AttendSmem<WIDE ? 64 : 32, MX> sm;
+  const int tid = threadIdx.x;
+  Seq own = {0, 0, 0, false};
+  if (tid < p.seqs) {
+    own = seq_of(p, tid);
+    if (own.bad && blockIdx.x == 0) record(p.err, MKMOE_LATENT_ERR_LENGTH, tid);
+  }
+  if constexpr (WIDE) {
+    int total = work_of<64>(p, own);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d, 64);
+    if ((tid & 63) == 0) sm.scan[tid >> 6] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) total += sm.scan[i];
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(total) > kNarrow) return attend_share<64, MX, PAGED>(p, sm, own);
+  }
+  static_assert(sizeof(AttendSmem<32, MX>) <= sizeof(AttendSmem<64, MX>), "one allocation for both");
+  attend_share<32, MX, PAGED>(p, reinterpret_cast<AttendSmem<32, MX>&>(sm), own);
+}
+
 // ---------------------------------------------------------------- merge
 // Row tiles that were cut, their parts joined in order at their common maximum; kMergeWgs workgroups
 // at each of a tile's cuts share its items, so that a long sequence's many parts are read by many. Few
@@ -1052,7 +1080,6 @@ constexpr int kMergeWgs = 8;
 constexpr int kFewParts = 32;
 constexpr int kAtOnce = 8;
 
-template <int M>
 __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
   __shared__ float s_w[kShares], s_red[4];
   __shared__ f32x4 s_acc[16][16];
@@ -1060,7 +1087,7 @@ __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
   if (c.parts == 0) return;
   const int tid = threadIdx.x;
   const int helper = (blockIdx.x - c.share) * kMergeWgs + blockIdx.y, helpers = (c.parts - 1) * kMergeWgs;
-  auto at = [&](int i, int r) { return (int64_t)(2 * (c.share + i) + (i == 0 ? 1 : 0)) * M + r; };
+  auto at = [&](int i, int r) { return (int64_t)(2 * (c.share + i) + (i == 0 ? 1 : 0)) * c.m + r; };
   auto store = [&](int r, int first, f32x4 acc, float top, float sum) {  // 4 values of row r
     const int qi = over_heads(p, c.r0 + r), h = (c.r0 + r) - qi * p.heads;
     const bool none = c.base + qi <= 0;
@@ -1280,15 +1307,12 @@ inline int check_cache(const mkmoe_latent_cache& c) {
 }
 inline int launched() { return hipGetLastError() == hipSuccess ? MKMOE_OK : MKMOE_ERR_LAUNCH; }
 
-template <int M, bool MX>
-int attend(const AttendParams& p, hipStream_t st) {
-  if ((1 << p.page_shift) >= kN)
-    hipLaunchKernelGGL((k_latent_attend<M, MX, true>), dim3(kShares), dim3(kThreads), 0, st, p);
+template <bool MX, bool PAGED>
+void attend(const AttendParams& p, bool wide, hipStream_t st) {
+  if (wide)
+    hipLaunchKernelGGL((k_latent_attend<MX, PAGED, true>), dim3(kShares), dim3(kThreads), 0, st, p);
   else
-    hipLaunchKernelGGL((k_latent_attend<M, MX, false>), dim3(kShares), dim3(kThreads), 0, st, p);
-  if (int rc = launched()) return rc;
-  hipLaunchKernelGGL(k_latent_merge<M>, dim3(kShares, kMergeWgs), dim3(256), 0, st, p);
-  return launched();
+    hipLaunchKernelGGL((k_latent_attend<MX, PAGED, false>), dim3(kShares), dim3(kThreads), 0, st, p);
 }
 
 // the checks of each call and, where they pass, its kernel's parameters
@@ -1396,11 +1420,15 @@ inline int attend_params(const mkmoe_latent_attend_io* io, void* ws, size_t ws_b
 }
 inline int attend_launch(const mkmoe_latent_attend_io* io, const AttendParams& p, hipStream_t st) {
   if (io->tokens == 0) return MKMOE_OK;
-  const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8;
-  // 32 query rows a tile where a sequence has no more of them on average, else 64
-  const int64_t rows = ((int64_t)io->tokens * io->heads + io->seqs - 1) / io->seqs;
-  if (rows <= 32) return mx ? attend<32, true>(p, st) : attend<32, false>(p, st);
-  return mx ? attend<64, true>(p, st) : attend<64, false>(p, st);
+  const bool mx = io->cache.fmt == MKMOE_LATENT_MXFP8, paged = io->cache.page_size >= kN;
+  const bool wide = ((int64_t)io->tokens * io->heads + io->seqs - 1) / io->seqs > 32;
+  if (mx)
+    paged ? attend<true, true>(p, wide, st) : attend<true, false>(p, wide, st);
+  else
+    paged ? attend<false, true>(p, wide, st) : attend<false, false>(p, wide, st);
+  if (int rc = launched()) return rc;
+  hipLaunchKernelGGL(k_latent_merge, dim3(kShares, kMergeWgs), dim3(256), 0, st, p);
+  return launched();
 }
 inline int project_params(const mkmoe_latent_project_io* io, ProjectParams& p) {
   if (!io || !io->x || !io->w || !io->y) return MKMOE_ERR_NULL;

@@ -302,6 +302,56 @@ def test_attend_non_finite_tokens_reach_only_their_queries(fmt, heads, n):
     assert not bool(out[last].isfinite().all(-1).any())
 
 
+# Work of more than 4096 tiles of 64 query rows (a row tile counts its tiles of 32 cached tokens and 8)
+# is taken 64 rows at a time
+@pytest.mark.parametrize("fmt,page", [("bf16", 1), ("bf16", 64), ("mxfp8", 1), ("mxfp8", 64)])
+@pytest.mark.parametrize("heads,lens,n,starts", [
+    (128, [700, 641, 5, 0, 300, 64], 48, None),
+    (12, [451, 1000, 460, 9, 77], 0, [0, 451, 451, 902, 1353, 1360]),
+    (20, [2500, 1, 129], 0, [0, 600, 601, 605]),
+    (64, [32] * 101 + [0, 6000], 5, None),
+])  # fmt: skip
+def test_attend_tall(fmt, page, heads, lens, n, starts):
+    print(f"\nattend tall {fmt} page={page} heads={heads} n={n} {lens[:6]}", flush=True)
+    t = [n] * len(lens) if starts is None else [b - a for a, b in zip(starts, starts[1:])]
+    tiles = sum(-(-c * heads // 64) * (-(-m // 32) + 8) for c, m in zip(t, lens) if m)
+    assert tiles > 4096, tiles
+    _check_attend(_runner(heads), fmt, heads, page, lens, n, starts, seed=heads, stride=8 * (heads == 20))
+
+
+@pytest.mark.parametrize("fmt,page", [("bf16", 16), ("bf16", 64), ("mxfp8", 16), ("mxfp8", 64)])
+def test_attend_tall_sees_only_what_it_may(fmt, page):
+    """As the two tests above of garbage out of sight and of non-finite tokens, 64 rows at a time."""
+    heads, n, lens = 64, 64, [200, 300, 130, 1000]
+    run = _runner(heads)
+    cache, q_lat, q_pe, table, dl = _attend_case(fmt, heads, page, lens, n, seed=15)
+    want = run.attend(cache, q_lat, q_pe, table, dl).clone()
+    flat = cache.view(-1, cache.shape[-1])
+    used = torch.zeros(flat.shape[0], dtype=torch.bool, device="cuda")
+    t2 = table.clone()
+    for b, m in enumerate(lens):
+        at = torch.arange(m, device="cuda")
+        used[table[b].long()[at // page] * page + at % page] = True
+        t2[b, -(-m // page) :] = [-1, 1 << 30, -(1 << 31), 12345][b]
+    flat[~used] = NAN if fmt == "bf16" else 0xFF
+    assert torch.equal(run.attend(cache, q_lat, q_pe, t2, dl), want)
+    run.raise_on_device_error()
+    for b, m in enumerate(lens):  # the last token of each
+        at = int(table[b, (m - 1) // page]) * page + (m - 1) % page
+        flat[at, 100 + b] = [NAN, INF, -INF, NAN][b] if fmt == "bf16" else 0x7F
+    out = run.attend(cache, q_lat, q_pe, t2, dl)
+    last = torch.arange(n - 1, 4 * n, n, device="cuda")
+    first = torch.ones(4 * n, dtype=torch.bool, device="cuda")
+    first[last] = False
+    assert torch.equal(out[first], want[first])
+    assert not bool(out[last].isfinite().all(-1).any())
+    t2[2, 1] = cache.shape[0]
+    run.attend(cache, q_lat, q_pe, t2, dl)
+    with pytest.raises(RuntimeError, match="a page outside the cache, at sequence 2"):
+        run.raise_on_device_error()
+    run.clear_errors()
+
+
 def test_attend_non_finite_query_stays_in_its_row():
     run = _runner(16)
     cache, q_lat, q_pe, table, dl = _attend_case("bf16", 16, 16, [100, 30], seed=11)
