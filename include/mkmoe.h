@@ -298,7 +298,8 @@ const char* mkmoe_status_string(int status);
 #define MKMOE_LATENT_ERRW_WORDS 4
 #define MKMOE_LATENT_ERR_SLOT 1     /* slot >= pages page_size: the row is not written / read as 0 */
 #define MKMOE_LATENT_ERR_POSITION 2 /* position outside cos_sin: the token's rows are not written */
-#define MKMOE_LATENT_ERR_LENGTH 3   /* length or query starts outside their bounds: clamped */
+#define MKMOE_LATENT_ERR_LENGTH 3   /* length or query starts outside their bounds: clamped. Starts that
+                                     * run backwards: nothing is attended, out stays as it was */
 #define MKMOE_LATENT_ERR_PAGE 4     /* page outside the cache: its tokens read as rows of zeros */
 
 typedef struct mkmoe_latent_cache {
@@ -308,7 +309,8 @@ typedef struct mkmoe_latent_cache {
   int32_t fmt;       /* MKMOE_LATENT_BF16 / _MXFP8 */
 } mkmoe_latent_cache;
 
-/* strides in elements, multiples of 8 (0: broadcast); the last axis is contiguous */
+/* strides in elements, multiples of 8 (an input's may be 0: broadcast; no two rows of an output share
+ * a place, else MKMOE_ERR_ARG); the last axis is contiguous. Outputs overlap no input, but for q_out */
 typedef struct mkmoe_latent_append_io {
   mkmoe_latent_cache cache;
   int32_t tokens;       /* any number, 0 included */

@@ -323,11 +323,12 @@ __device__ __forceinline__ int over_heads(const AttendParams& p, int row) {
 // a sequence's query tokens and length, clamped to their bounds
 struct Seq {
   int t0, n, len;
-  bool bad;
+  bool bad, back;  // outside its bounds; its query starts run backwards
 };
 __device__ __forceinline__ Seq seq_of(const AttendParams& p, int b) {
   Seq s;
   const int len = p.lens[b];
+  s.back = false;
   s.len = min(max(len, 0), p.max_len);
   s.bad = s.len != len;
   if (p.starts) {
@@ -336,6 +337,7 @@ __device__ __forceinline__ Seq seq_of(const AttendParams& p, int b) {
     const int t1 = min(max(e, s.t0), p.tokens);
     s.n = t1 - s.t0;
     s.bad = s.bad || a != s.t0 || e != t1;
+    s.back = e < a;
   } else {
     s.t0 = b * p.n;
     s.n = p.n;
@@ -515,7 +517,7 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
 
   int b = __builtin_amdgcn_readfirstlane(sm.first[0]);
   Seq s = {__builtin_amdgcn_readfirstlane(sm.first[1]), __builtin_amdgcn_readfirstlane(sm.first[2]),
-           __builtin_amdgcn_readfirstlane(sm.first[3]), false};
+           __builtin_amdgcn_readfirstlane(sm.first[3]), false, false};
   for (int w = w0; w < w1;) {
     if (w > w0) {
       const int last = b;
@@ -1050,22 +1052,31 @@ template <bool MX, bool PAGED, bool WIDE>
 __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
   __shared__ AttendSmem<WIDE ? 64 : 32, MX> sm;
   const int tid = threadIdx.x;
-  Seq own = {0, 0, 0, false};
+  Seq own = {0, 0, 0, false, false};
   if (tid < p.seqs) {
     own = seq_of(p, tid);
     if (own.bad && blockIdx.x == 0) record(p.err, MKMOE_LATENT_ERR_LENGTH, tid);
+  }
+  // query starts that run backwards give rows to several sequences, and more work than was checked
+  auto over_waves = [&](int v) {  // the sum of the waves' values
+    if ((tid & 63) == 0) sm.scan[tid >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) v += sm.scan[i];
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  if (p.starts && over_waves(__any(own.back))) {
+    if (tid == 0) p.cut[blockIdx.x].parts = 0;
+    return;
   }
   if constexpr (WIDE) {
     int total = work_of<64>(p, own);
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d, 64);
-    if ((tid & 63) == 0) sm.scan[tid >> 6] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) total += sm.scan[i];
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(total) > kNarrow) return attend_share<64, MX, PAGED>(p, sm, own);
+    total = over_waves(total);
+    if (total > kNarrow) return attend_share<64, MX, PAGED>(p, sm, own);
   }
   static_assert(sizeof(AttendSmem<32, MX>) <= sizeof(AttendSmem<64, MX>), "one allocation for both");
   attend_share<32, MX, PAGED>(p, reinterpret_cast<AttendSmem<32, MX>&>(sm), own);
@@ -1291,6 +1302,14 @@ constexpr int64_t kMaxRows = (int64_t)1 << 24;  // query rows (tokens x heads) a
 
 inline bool aligned(const void* q, size_t a) { return ((uintptr_t)q % a) == 0; }
 inline bool strides8(int64_t a, int64_t b) { return a >= 0 && b >= 0 && a % 8 == 0 && b % 8 == 0; }
+// no two rows of an output share a place
+inline bool rows_apart(int64_t ts, int64_t tokens, int64_t hs, int64_t heads, int64_t width) {
+  const bool by_token = ts >= hs;
+  const int64_t big = by_token ? ts : hs, n_big = by_token ? tokens : heads;
+  const int64_t small = by_token ? hs : ts, n_small = by_token ? heads : tokens;
+  if (n_small <= 1) return n_big <= 1 || big >= width;
+  return small >= width && (n_big <= 1 || (big - width) / small >= n_small - 1);
+}
 
 inline int check_ws(const void* ws, size_t bytes) {
   if (!ws) return MKMOE_ERR_NULL;
@@ -1334,6 +1353,7 @@ inline int append_params(const mkmoe_latent_append_io* io, void* ws, size_t ws_b
                         !strides8(io->q_token_stride, io->q_head_stride) ||
                         !strides8(io->out_token_stride, io->out_head_stride)))
     return MKMOE_ERR_ALIGN;
+  if (io->heads > 0 && !rows_apart(io->out_token_stride, io->tokens, io->out_head_stride, io->heads, kR)) return MKMOE_ERR_ARG;
   p.kv = (const uint16_t*)io->kv;
   p.norm_w = (const uint16_t*)io->norm_w;
   p.cos_sin = (const float*)io->cos_sin;
@@ -1386,6 +1406,7 @@ inline int attend_params(const mkmoe_latent_attend_io* io, void* ws, size_t ws_b
   if (!strides8(io->ql_token_stride, io->ql_head_stride) || !strides8(io->qp_token_stride, io->qp_head_stride) ||
       !strides8(io->out_token_stride, io->out_head_stride))
     return MKMOE_ERR_ALIGN;
+  if (!rows_apart(io->out_token_stride, io->tokens, io->out_head_stride, io->heads, kL)) return MKMOE_ERR_ARG;
   p.ql = (const uint16_t*)io->q_lat;
   p.qp = (const uint16_t*)io->q_pe;
   p.cache = (const uint8_t*)io->cache.data;
@@ -1439,6 +1460,7 @@ inline int project_params(const mkmoe_latent_project_io* io, ProjectParams& p) {
   if (!aligned(io->x, 16) || !aligned(io->w, 16) || !aligned(io->y, 16) ||
       !strides8(io->x_token_stride, io->x_head_stride) || !strides8(io->y_token_stride, io->y_head_stride))
     return MKMOE_ERR_ALIGN;
+  if (!rows_apart(io->y_token_stride, io->tokens, io->y_head_stride, io->heads, io->expand ? kV : kL)) return MKMOE_ERR_ARG;
   p = ProjectParams{io->x, (const uint16_t*)io->w, (uint16_t*)io->y, io->x_token_stride, io->x_head_stride,
                     io->y_token_stride, io->y_head_stride, io->tokens, io->heads, io->x_f32};
   return MKMOE_OK;

@@ -387,6 +387,22 @@ def test_attend_records_bad_pages_lengths_and_starts():
         run.clear_errors()
 
 
+def test_attend_query_starts_that_run_backwards():
+    """They would give rows to several sequences: nothing is attended."""
+    run = _runner(64)
+    cache, q_lat, q_pe, table, dl = _attend_case("bf16", 64, 16, [40, 100, 60], starts=[0, 2, 4, 6], seed=17)
+    for starts in ([0, 6, 0, 6], [0, 4, 3, 6]):
+        out = torch.full((6, 64, 512), 7.0, dtype=BF, device="cuda")
+        run.attend(cache, q_lat, q_pe, table, dl, q_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"), out=out)
+        assert bool((out == 7).all())
+        with pytest.raises(RuntimeError, match="a length or query start"):
+            run.raise_on_device_error()
+        run.clear_errors()
+    run.attend(cache, q_lat, q_pe, table, dl, q_starts=torch.tensor([0, 2, 4, 6], dtype=torch.int32, device="cuda"), out=out)
+    assert torch.equal(out, run.attend(cache, q_lat, q_pe, table, dl))
+    run.raise_on_device_error()
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
 def test_attend_offsets_past_32_bits(fmt):
     """A cache of more than 2^32 bytes, its last pages in use."""
