@@ -129,8 +129,17 @@ __device__ __forceinline__ u32x4 rotate8(u32x4 v, const float* cs, int j, int ha
   return u32x4{o[0], o[1], o[2], o[3]};
 }
 
+// fp32 that a later rounding to fewer bits takes to the place where it would take x: cut off, the last
+// bit set where something was
+__device__ __forceinline__ float to_odd(double x) {
+  float f = __double2float_rz(x);
+  if ((double)f != x && fabsf(f) < INFINITY) f = u2f(f2u(f) | 1u);
+  return f;
+}
+
 // A wave a token of the first kv_blocks workgroups: lane l holds latent values 8 l .. 8 l + 7,
-// lanes 0 .. 7 the rope values too. The other workgroups rotate the query, 8 lanes a head's 64
+// lanes 0 .. 7 the rope values too. The norm's sum is formed in 64 bits, and so are MXFP8's products: a
+// code next to a border is the one that the definition has (fp32 missed one in some 10^5 of them). The other workgroups rotate the query, 8 lanes a head's 64
 // values. Bytes: each value is read and written once; a decode step's few rows are one trip to
 // memory and back.
 template <bool MX>
@@ -160,16 +169,21 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int block) {
     if (p.norm_w) {
       const u32x4 nv = *(const u32x4*)(p.norm_w + 8 * lane);
       const uint32_t nw[4] = {nv.x, nv.y, nv.z, nv.w};
-      float ss = 0.0f;
+      double ss = 0.0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+      for (int i = 0; i < 8; ++i) ss += (double)y[i] * (double)y[i];
 #pragma unroll
       for (int d = 32; d >= 1; d >>= 1) ss += __shfl_xor(ss, d, 64);
-      const float rstd = 1.0f / sqrtf(ss / (float)kL + p.eps);
+      const double rstd = 1.0 / sqrt(ss / kL + (double)p.eps);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        y[2 * i] = y[2 * i] * rstd * bf_lo(nw[i]);
-        y[2 * i + 1] = y[2 * i + 1] * rstd * bf_hi(nw[i]);
+        if constexpr (MX) {
+          y[2 * i] = to_odd((double)y[2 * i] * rstd * (double)bf_lo(nw[i]));
+          y[2 * i + 1] = to_odd((double)y[2 * i + 1] * rstd * (double)bf_hi(nw[i]));
+        } else {
+          y[2 * i] = y[2 * i] * (float)rstd * bf_lo(nw[i]);
+          y[2 * i + 1] = y[2 * i + 1] * (float)rstd * bf_hi(nw[i]);
+        }
       }
     }
     if constexpr (MX) {

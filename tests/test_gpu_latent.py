@@ -98,6 +98,23 @@ def test_append(fmt, rope, tokens, heads, page, index):
         assert float(((raw - kv[:, :512].double()).abs() / kv[:, :512].double().abs().clamp_min(0.05)).max()) <= 2.0**-4
 
 
+def test_append_codes_are_the_definitions():
+    """Each of half a million MXFP8 codes is the nearest one (ties to even) to the 64-bit norm, under
+    the least power of two that holds its 32 values: none next to a border falls to the other side."""
+    from sgl_amd_mono.moe.latent import cache_like
+
+    g, run, t = _gen(31), _runner(1), 1021
+    kv, w = _randn(g, t, 576), (1 + 0.1 * torch.randn(512, generator=g, device="cuda")).to(BF)
+    cache, rows = cache_like(t, 1, "mxfp8"), torch.arange(t, device="cuda")
+    run.append(cache, kv, w, _cos_sin(1), torch.zeros_like(rows), rows)
+    c = ref.norm(kv[:, :512], w, float(torch.tensor(1e-6))).view(t, 16, 32)
+    sc = torch.exp2(torch.ceil(torch.log2(c.abs().amax(-1, keepdim=True) / 448)))
+    a = (c / sc).abs()
+    step = torch.exp2(torch.floor(torch.log2(a.clamp_min(2.0**-6))) - 3)
+    want = (c.sign() * torch.round(a / step) * step * sc).view(t, 512)
+    assert torch.equal(ref.row_values(cache.view(t, -1))[:, :512], want)
+
+
 def test_append_skips_padding_and_records_bad_indices():
     from sgl_amd_mono.moe.latent import cache_like
 
@@ -136,7 +153,7 @@ def test_append_extremes():
     run = _runner(1)
     kv = torch.zeros(6, 576, dtype=BF, device="cuda")
     kv[1, :512] = 1e-30
-    kv[2, :512] = 3e38  # its squares pass fp32: the norm's root is infinite, the row 0
+    kv[2, :512] = 3e38  # its squares pass fp32
     kv[3, 5] = NAN
     kv[4, 5] = INF
     kv[5, 0] = 1.0  # one value among zeros
@@ -146,7 +163,7 @@ def test_append_extremes():
         cache = cache_like(6, 1, fmt)
         run.append(cache, kv, w, _cos_sin(1), pos, slots)
         got = run.rows(cache, slots).double().cpu()
-        assert bool((got[0] == 0).all()) and bool((got[2, :512] == 0).all())
+        assert bool((got[0] == 0).all()) and bool((got[2, :512] == 1).all())
         assert float((got[1, :512] - 1e-27).abs().max()) <= 1e-27 * 2.0**-3
         assert bool(got[3, :512].isnan().all())
         assert bool(got[4, 5].isnan())
