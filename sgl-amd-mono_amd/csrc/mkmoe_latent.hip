@@ -12,6 +12,10 @@
 //   k_latent_attend   the absorbed attention, its work cut into equal shares over the card
 //   k_latent_merge    joins the shares of a sequence that was cut
 //   k_latent_absorb / k_latent_expand   the two products of every head with its weights
+//   k_latent_front    a step's append and absorb in one launch
+//
+// Times below are of an MI355X, in graph replays. It copies 5.19 TB/s and multiplies bf16 matrices
+// at 1.25 PFLOP/s, which make the floors.
 
 #include <hip/hip_runtime.h>
 
@@ -138,7 +142,8 @@ __device__ __forceinline__ float to_odd(double x) {
 }
 
 // A wave a token of the first kv_blocks workgroups: lane l holds latent values 8 l .. 8 l + 7,
-// lanes 0 .. 7 the rope values too. The norm's sum is formed in 64 bits, and so are MXFP8's products: a
+// lanes 0 .. 7 the rope values too. Bound by memory on a prompt (8191 rows of 32 heads, 88 MB: 17.7 us
+// in graph replays, 5.0 TB/s) and by one trip to it on a decode step (7 rows 3.1 us). The norm's sum is formed in 64 bits, and so are MXFP8's products: a
 // code next to a border is the one that the definition has (fp32 missed one in some 10^5 of them). The other workgroups rotate the query, 8 lanes a head's 64
 // values. Bytes: each value is read and written once; a decode step's few rows are one trip to
 // memory and back.
@@ -359,7 +364,8 @@ __device__ __forceinline__ Seq seq_of(const AttendParams& p, int b) {
   return s;
 }
 // a sequence's work: its query row tiles, each as long as its tiles of cached tokens and kSetup
-// more, about what starting and storing a row tile takes (an empty sequence only stores its rows)
+// more, about what starting and storing a row tile takes (an empty sequence only stores its rows):
+// 3, 5, 7 and 9 gave 66.3, 66.3, 64.5, 63.3 us (verify, 12 sequences) and 45.4, 38.7, 38.3, 39.0 (24 short ones)
 template <int M>
 __device__ __forceinline__ int row_tiles(const AttendParams& p, const Seq& s) {
   return (int)(((int64_t)s.n * p.heads + M - 1) / M);
@@ -451,24 +457,36 @@ struct __align__(256) AttendSmem {
 
 // The absorbed attention. The work is a list of tiles: sequence by sequence, query row tile by
 // row tile (M rows: consecutive (token, head) pairs), kN cached tokens each. Every workgroup
-// computes the list's prefix sums itself and takes one equal contiguous share, so ragged
-// lengths load every CU alike. A row tile inside one share is finished there; one that was cut
-// leaves its running maximum, sum and fp32 outputs in the workspace for k_latent_merge.
+// computes the list's prefix sums itself and takes one equal contiguous share, one workgroup a CU, so
+// that ragged lengths load every CU alike. A row tile inside one share is finished there; one that was
+// cut leaves its running maximum, sum and fp32 outputs in the workspace for k_latent_merge.
 //
 // A tile: 32 rows of 576 bf16 in LDS, read once from memory for all M query rows and used twice.
 // Waves 0 .. 3 score, waves 4 .. 7 bring the tiles; both share the outputs' columns so that the
 // registers hold (a scoring wave has the queries there) and the MFMA has as much of either:
 //   S^T = K Q^T   scoring wave (rg, tg): the rows of half rg, tokens 16 tg ..: A = K (16-byte
-//                 reads of LDS, which bound this step: with 64 rows each serves two row blocks),
-//                 B = Q^T, which stays in registers
-//   P             exp2 of the scores less the rows' running maxima (moved for both token groups
-//                 at once), bf16, [row][token] in LDS; the sums stay fp32
+//                 reads of LDS; with 64 rows each serves two row blocks), B = Q^T in registers
+//   P             exp2 of the scores less the rows' running maxima, [row][token] in LDS, in bf16
+//                 because it is a matrix operand; the sums stay fp32
 //   O^T += V^T P^T   latent values 32 w .. of a scoring wave (32 of them), 16 of every 64 past 128 of the
 //                 others (96), for every row: A = V^T by transposing LDS reads of the same tile, B = P^T
-// bf16 rows go straight from memory to LDS, three tiles ahead; MXFP8 rows go there as they are,
-// and waves 4 .. 7 turn the next tile's into bf16 (exact) while waves 0 .. 3 score.
-// PAGED: pages of kN tokens or more, so that a tile lies in one and its rows follow each other;
-// without it each token's page entry is looked up.
+// One barrier a tile (bf16). bf16 rows go straight from memory to LDS, three tiles ahead; MXFP8 rows
+// go there as they are, and waves 4 .. 7 turn the next tile's into bf16 (exact) while waves 0 .. 3 score,
+// at the price of a second barrier. PAGED: pages of kN tokens or more, so that a tile lies in one, its
+// page is a scalar load and its rows follow each other; without it each token's page entry is looked up,
+// two tiles before its row is (pages of one token 103 us, of 64 100 us, at 48 sequences of 8192).
+//
+// What bounds it: 32 rows a tile in bf16, memory (48 sequences of 8192, 32 heads: 100 us with the merge,
+// 4.6 TB/s, of it about 20 us for the start, the outputs and the merge); 64 rows, LDS and the wave's
+// instruction issue (a tile takes 2300 cycles, of which its LDS reads and writes need 1800 and its MFMAs 1150:
+// 12 sequences of 8192, 64 heads, 4 queries each 64 us, 430 TFLOP/s); MXFP8, the conversion on 4 waves
+// (1550 of a tile's 2700 cycles: 64 sequences of up to 16384, 32 heads 93 us, 3.7 TB/s). Short work is bound
+// by the chain lengths -> pages and queries -> first tile -> outputs -> merge (1025 tokens: 13.4 us).
+//
+// Steps that brought it there: whole rows by ring and DMA (64 heads 380 -> 129 us), cut row tiles joined by
+// many (131071 tokens 189 -> 48), latent and rope parts apart in LDS without bank conflicts and maxima that
+// rarely move (verify 96 -> 73), half as many instructions a tile (MXFP8 167 -> 149), no spill beside the
+// tile loop (149 -> 138), queries by way of LDS (1025 tokens 16.1 -> 13.9).
 template <int M, bool MX, bool PAGED>
 __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M, MX>& sm, const Seq& own) {
   static_assert(M == 32 || M == 64, "row blocks of 16 by two token groups on 4 or 8 waves");
@@ -1097,10 +1115,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 }
 
 // ---------------------------------------------------------------- merge
-// Row tiles that were cut, their parts joined in order at their common maximum; kMergeWgs workgroups
-// at each of a tile's cuts share its items, so that a long sequence's many parts are read by many. Few
-// parts: an item is a row's 128 latent values, 32 lanes with up to kAtOnce parts' loads on their way;
-// many: 64 values, the workgroup's 16 groups of 16 lanes take every 16th part and add up in LDS.
+// Row tiles that were cut, their parts joined in order at their common maximum (so that the same call
+// gives the same bits). Bound by latency: the parts are 17 MB at 32 rows a tile, 33 MB at 64, and take
+// 7 to 10 us with the launch. kMergeWgs workgroups at each of a tile's cuts share its items, so that a
+// long sequence's many parts are read by many. Few parts: an item is a row's 128 latent values, 32 lanes
+// with up to kAtOnce parts' loads on their way; many: 64 values, the workgroup's 16 groups of 16 lanes
+// take every 16th part and add up in LDS (256 parts 8.5 us against 12.3 in items of 128; 8 sequences of
+// 16 to 32 parts took 38 us that way, 33 as few).
 constexpr int kMergeWgs = 8;
 constexpr int kFewParts = 32;
 constexpr int kAtOnce = 8;
