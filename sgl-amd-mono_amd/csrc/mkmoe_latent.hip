@@ -479,9 +479,10 @@ struct __align__(256) AttendSmem {
 // What bounds it: 32 rows a tile in bf16, memory (48 sequences of 8192, 32 heads: 100 us with the merge,
 // 4.6 TB/s, of it about 20 us for the start, the outputs and the merge); 64 rows, LDS and the wave's
 // instruction issue (a tile takes 2300 cycles, of which its LDS reads and writes need 1800 and its MFMAs 1150:
-// 12 sequences of 8192, 64 heads, 4 queries each 64 us, 430 TFLOP/s); MXFP8, the conversion on 4 waves
-// (1550 of a tile's 2700 cycles: 64 sequences of up to 16384, 32 heads 93 us, 3.7 TB/s). Short work is bound
-// by the chain lengths -> pages and queries -> first tile -> outputs -> merge (1025 tokens: 13.4 us).
+// 12 sequences of 8192, 64 heads, 4 queries each 64 us, 430 TFLOP/s); MXFP8, the codes' way through LDS
+// (64 sequences of up to 16384, 32 heads 93 us, 3.7 TB/s; 48 of 16384 134 us, of which it takes 19, while the
+// conversions themselves are free). Short work is bound by the chain of lengths, pages and queries, first
+// tile, outputs and merge (1025 tokens: 13.4 us).
 //
 // Steps that brought it there: whole rows by ring and DMA (64 heads 380 -> 129 us), cut row tiles joined by
 // many (131071 tokens 189 -> 48), latent and rope parts apart in LDS without bank conflicts and maxima that
@@ -1284,24 +1285,27 @@ __global__ __launch_bounds__(256) void k_latent_front(AppendParams a, ProjectPar
     append_block<MX>(a, blockIdx.x - absorb_blocks);
 }
 
-// y[t, h, j] = sum_l x[t, h, l] W_UV[h, j, l]: a workgroup a head, 16 columns and 64 tokens. The
+// y[t, h, j] = sum_l x[t, h, l] W_UV[h, j, l]: a workgroup a head, 16 NJ columns and 64 tokens. The
 // four waves split l, so that few tokens keep them all busy and no weight is read twice, and add up
 // in LDS; both operands are contiguous along l and come straight from memory. x in fp32 is taken as
-// the sum of two bf16 parts (2^-17 of it is left out) against the same weights
-template <bool F32>
+// the sum of two bf16 parts (2^-17 of it is left out) against the same weights. 48 tokens of 64 heads: 7.5 us
+// with 32 columns a workgroup, 9.7 with 16; 8 tokens of 32 heads 4.0 with 16
+template <bool F32, int NJ>
 __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
   constexpr int KS = kL / 32 / 4;  // MFMA steps of a wave
-  __shared__ f32x4 sums[4][4][64];
+  __shared__ f32x4 sums[4][NJ][4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int j0 = blockIdx.y * 16, h = blockIdx.x, t0 = blockIdx.z * 64, l0 = wave * (kL / 4) + 8 * g;
+  const int j0 = blockIdx.y * (16 * NJ), h = blockIdx.x, t0 = blockIdx.z * 64, l0 = wave * (kL / 4) + 8 * g;
   const uint16_t* w = p.w + ((int64_t)h * (kNope + kV) + kNope + j0 + col) * kL + l0;
   // every operand on its way before the first is used
   using X = std::conditional_t<F32, f32x4, u32x4>;
   constexpr int kX = F32 ? 2 : 1;
-  bf16x8 a[KS];
+  bf16x8 a[NJ][KS];
   X x[4][KS][kX];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) a[ks] = *(const bf16x8*)(w + 32 * ks);
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) a[j][ks] = *(const bf16x8*)(w + 16 * j * kL + 32 * ks);
 #pragma unroll
   for (int tb = 0; tb < 4; ++tb) {
     if (tb > 0 && t0 + 16 * tb >= p.tokens) continue;
@@ -1316,7 +1320,7 @@ __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
 #pragma unroll
   for (int tb = 0; tb < 4; ++tb) {
     if (tb > 0 && t0 + 16 * tb >= p.tokens) continue;
-    f32x4 acc = {0, 0, 0, 0};
+    f32x4 acc[NJ] = {};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if constexpr (F32) {
@@ -1327,19 +1331,29 @@ __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
           hi[i] = pack_bf(a0, a1);
           lo[i] = pack_bf(rest(a0, bf_lo(hi[i])), rest(a1, bf_hi(hi[i])));
         }
-        acc = mfma(a[ks], __builtin_bit_cast(bf16x8, lo), acc);
-        acc = mfma(a[ks], __builtin_bit_cast(bf16x8, hi), acc);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          acc[j] = mfma(a[j][ks], __builtin_bit_cast(bf16x8, lo), acc[j]);
+          acc[j] = mfma(a[j][ks], __builtin_bit_cast(bf16x8, hi), acc[j]);
+        }
       } else {
-        acc = mfma(a[ks], __builtin_bit_cast(bf16x8, x[tb][ks][0]), acc);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[j] = mfma(a[j][ks], __builtin_bit_cast(bf16x8, x[tb][ks][0]), acc[j]);
       }
     }
-    sums[tb][wave][lane] = acc;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) sums[tb][j][wave][lane] = acc[j];
   }
   __syncthreads();
   const int t = t0 + 16 * wave + col;
   if (t >= p.tokens) return;
-  const f32x4 v = (sums[wave][0][lane] + sums[wave][1][lane]) + (sums[wave][2][lane] + sums[wave][3][lane]);
-  *(u32x2*)(p.y + (int64_t)t * p.y_ts + (int64_t)h * p.y_hs + j0 + 4 * g) = u32x2{pack_bf(v[0], v[1]), pack_bf(v[2], v[3])};
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const f32x4* part = &sums[wave][j][0][lane];
+    const f32x4 v = (part[0] + part[64]) + (part[128] + part[192]);
+    *(u32x2*)(p.y + (int64_t)t * p.y_ts + (int64_t)h * p.y_hs + j0 + 16 * j + 4 * g) =
+        u32x2{pack_bf(v[0], v[1]), pack_bf(v[2], v[3])};
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -1519,11 +1533,17 @@ inline unsigned absorb_blocks(const ProjectParams& p) {
   return (unsigned)(kL / 64) * p.heads * ((p.tokens + 63) / 64);
 }
 inline int expand_launch(const ProjectParams& p, hipStream_t st) {
-  const dim3 grid(p.heads, kV / 16, (p.tokens + 63) / 64);
-  if (p.f32)
-    hipLaunchKernelGGL(k_latent_expand<true>, grid, dim3(256), 0, st, p);
+  // 32 columns a workgroup where that still gives every CU one
+  const bool wide = p.heads * (kV / 32) >= kShares;
+  const dim3 grid(p.heads, wide ? kV / 32 : kV / 16, (p.tokens + 63) / 64);
+  if (p.f32 && wide)
+    hipLaunchKernelGGL((k_latent_expand<true, 2>), grid, dim3(256), 0, st, p);
+  else if (p.f32)
+    hipLaunchKernelGGL((k_latent_expand<true, 1>), grid, dim3(256), 0, st, p);
+  else if (wide)
+    hipLaunchKernelGGL((k_latent_expand<false, 2>), grid, dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL(k_latent_expand<false>, grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_latent_expand<false, 1>), grid, dim3(256), 0, st, p);
   return launched();
 }
 
