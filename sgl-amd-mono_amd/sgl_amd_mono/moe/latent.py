@@ -115,30 +115,40 @@ class LatentRunner:
         """(pointer, token stride, head stride) of a [tokens, heads, width] tensor whose last axis is
         contiguous and whose rows start on 16 bytes."""
         h = self.heads
-        if t is not None and t.dtype == dtype and t.get_device() == self._index and t.shape == (tokens, h, width):
+        if t is not None and t.dtype is dtype and t.get_device() == self._index and t.shape == (tokens, h, width):
             ts, hs, last = t.stride()
-            ts, hs = ts if tokens > 1 else 0, hs if h > 1 else 0
             at = t.data_ptr()
-            ok = last == 1 and ts % 8 == 0 and hs % 8 == 0 and at % 16 == 0
-            if ok and written:  # no two rows of an output share a place
+            if tokens <= 1:
+                ts = 0
+            if h <= 1:
+                hs = 0
+            if last == 1 and not (ts | hs) & 7 and not at & 15:
+                if not written:
+                    return at, ts, hs
+                # no two rows of an output share a place
                 s0, n0, s1, n1 = (ts, tokens, hs, h) if ts >= hs else (hs, h, ts, tokens)
-                ok = (n1 == 1 or s1 >= width) and (n0 == 1 or s0 >= (n1 - 1) * s1 + width)
-            if ok:
-                return at, ts, hs
+                if (n1 <= 1 or s1 >= width) and (n0 <= 1 or s0 >= (n1 - 1) * s1 + width):
+                    return at, ts, hs
         raise self._bad(name, t, f"[{tokens}, {h}, {width}] {dtype}, rows of whole 16-byte pieces")
 
-    def _vec(self, name: str, t, n: int, *dtypes) -> int:
-        if (t is not None and t.dtype in dtypes and t.get_device() == self._index and t.shape == (n,)
-                and t.is_contiguous()):  # fmt: skip
+    def _vec(self, name: str, t, n: int, dtype) -> int:
+        if t is not None and t.dtype is dtype and t.get_device() == self._index and t.shape == (n,) and t.is_contiguous():
             return t.data_ptr()
-        raise self._bad(name, t, f"[{n}] {dtypes[0]} contiguous")
+        raise self._bad(name, t, f"[{n}] {dtype} contiguous")
+
+    def _index_type(self, name: str, t):
+        """int32 where ``t`` is, else int64 (which the check then asks for)."""
+        if t is None:
+            raise self._bad(name, t, "torch.int64 or torch.int32")
+        return torch.int32 if t.dtype is torch.int32 else torch.int64
 
     def _cache(self, t) -> tuple:
-        if t is not None and t.dim() == 3 and t.get_device() == self._index and t.is_contiguous():
-            pages, page, row = t.shape
-            if row == ROW and t.dtype == BF:
+        shape = () if t is None else t.shape
+        if len(shape) == 3 and t.get_device() == self._index and t.is_contiguous():
+            pages, page, row = shape
+            if row == ROW and t.dtype is BF:
                 return t.data_ptr(), pages, page, _lib.LATENT_BF16
-            if row == MX_ROW and t.dtype == torch.uint8:
+            if row == MX_ROW and t.dtype is torch.uint8:
                 return t.data_ptr(), pages, page, _lib.LATENT_MXFP8
         raise self._bad("cache", t, f"[pages, page_size, {ROW}] {BF} or [pages, page_size, {MX_ROW}] torch.uint8 contiguous")
 
@@ -149,7 +159,7 @@ class LatentRunner:
     def _call(self, fn, *args) -> None:
         """``fn`` on the current stream of this runner's GPU."""
         stream = torch._C._cuda_getCurrentRawStream(self._index)  # (current_stream()'s, without its object)
-        if torch.cuda.current_device() != self._index:
+        if torch._C._cuda_getDevice() != self._index:
             with torch.cuda.device(self.device):
                 rc = fn(*args, stream)
         else:
@@ -160,23 +170,25 @@ class LatentRunner:
     # ---- the calls' arguments, checked and written into their structures
     def _set_append(self, cache, kv, norm, cos_sin, positions, slots, heads: int, q: tuple, q_out: tuple) -> int:
         c = self._cache(cache)
-        if kv is None or kv.dim() != 2 or kv.shape[1] != ROW or kv.dtype != BF or kv.get_device() != self._index:
+        shape = () if kv is None else kv.shape
+        if len(shape) != 2 or shape[1] != ROW or kv.dtype is not BF or kv.get_device() != self._index:
             raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}")
-        tokens, at = kv.shape[0], kv.data_ptr()
+        tokens, at = shape[0], kv.data_ptr()
         stride, last = kv.stride()
         if tokens <= 1:
             stride = ROW
-        if last != 1 or stride % 8 or stride < ROW or at % 16:
+        if last != 1 or stride & 7 or stride < ROW or at & 15:
             raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}, rows of whole 16-byte pieces")
         w = 0 if norm is None else self._vec("norm", norm, LATENT, BF)
-        if (cos_sin is None or cos_sin.dim() != 2 or cos_sin.shape[1] != ROPE or cos_sin.dtype != torch.float32
+        turns = () if cos_sin is None else cos_sin.shape
+        if (len(turns) != 2 or turns[1] != ROPE or cos_sin.dtype is not torch.float32
                 or cos_sin.get_device() != self._index or not cos_sin.is_contiguous()):  # fmt: skip
             raise self._bad("cos_sin", cos_sin, f"[positions, {ROPE}] torch.float32 contiguous")
-        pos = self._vec("positions", positions, tokens, torch.int64, torch.int32)
-        slot = self._vec("slots", slots, tokens, positions.dtype)
+        index = self._index_type("positions", positions)
+        pos = self._vec("positions", positions, tokens, index)
+        slot = self._vec("slots", slots, tokens, index)
         _lib.LATENT_APPEND.pack_into(
-            self._append_io, 0, *c, tokens, heads, self.rope, 8 if positions.dtype == torch.int64 else 4,
-            cos_sin.shape[0], stride, q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot,
+            self._append_io, 0, *c, tokens, heads, self.rope, 8 if index is torch.int64 else 4, turns[0], stride, q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot,
             q[0], q_out[0], self.norm_eps, 0,
         )  # fmt: skip
         return tokens
@@ -184,11 +196,14 @@ class LatentRunner:
     def _set_attend(self, cache, tokens: int, q_lat: tuple, q_pe: tuple, table, lens, q_starts, out: tuple,
                     f32: int, lse: int) -> None:  # fmt: skip
         c = self._cache(cache)
-        if (table is None or table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != self._index
-                or table.stride(1) != 1 and table.shape[1] > 1):  # fmt: skip
+        shape = () if table is None else table.shape
+        if len(shape) != 2 or table.dtype is not torch.int32 or table.get_device() != self._index:
             raise self._bad("table", table, "[seqs, max_pages] torch.int32")
-        seqs, max_pages = table.shape
-        stride = table.stride(0) if seqs > 1 else max_pages
+        (seqs, max_pages), (stride, last) = shape, table.stride()
+        if last != 1 and max_pages > 1:
+            raise self._bad("table", table, "[seqs, max_pages] torch.int32, the pages of a sequence contiguous")
+        if seqs <= 1:
+            stride = max_pages
         at_lens = self._vec("lens", lens, seqs, torch.int32)
         at_starts = 0 if q_starts is None else self._vec("q_starts", q_starts, seqs + 1, torch.int32)
         if not 1 <= seqs <= _lib.LATENT_MAX_SEQS or (q_starts is None and tokens % seqs):
@@ -239,19 +254,17 @@ class LatentRunner:
         """-> bf16 [T, 576]: the values that the cache rows ``slots`` stand for (a negative slot's
         are 0), exactly."""
         c = _lib.LatentCache(*self._cache(cache))
-        if slots is None or slots.dim() != 1:
-            raise self._bad("slots", slots, "[tokens] torch.int64 contiguous")
-        tokens = slots.shape[0]
-        at = self._vec("slots", slots, tokens, torch.int64, torch.int32)
+        index = self._index_type("slots", slots)
+        tokens = slots.numel()
+        at = self._vec("slots", slots, tokens, index)
         if out is None:
             out = self._new("the rows", tokens, ROW)
-        if out.shape != (tokens, ROW) or out.dtype != BF or out.device != self.device or not out.is_contiguous():
+        elif out.shape != (tokens, ROW) or out.dtype is not BF or out.get_device() != self._index or not out.is_contiguous():
             raise self._bad("out", out, f"[{tokens}, {ROW}] {BF} contiguous")
         if tokens:
             self._call(
-                self.lib.mkmoe_latent_rows, c, at, 8 if slots.dtype == torch.int64 else 4, tokens, out.data_ptr(),
-                *self._ws,
-            )  # fmt: skip
+                self.lib.mkmoe_latent_rows, c, at, 8 if index is torch.int64 else 4, tokens, out.data_ptr(), *self._ws
+            )
         return out
 
     def _project(self, what: str, w, x, out, expand: int) -> torch.Tensor:
