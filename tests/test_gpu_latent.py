@@ -184,7 +184,7 @@ def _attend_case(fmt, heads, page, lens, n=1, starts=None, seed=0, stride=0):
     return cache, q_lat, q_pe, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
 
 
-def _check_attend(run, fmt, heads, page, lens, n=1, starts=None, seed=0, stride=0):
+def _check_attend(run, fmt, heads, page, lens, n=1, starts=None, seed=0, stride=0, scale=SCALE):
     cache, q_lat, q_pe, table, dl = _attend_case(fmt, heads, page, lens, n, starts, seed, stride)
     t = q_lat.shape[0]
     ds = None if starts is None else torch.tensor(starts, dtype=torch.int32, device="cuda")
@@ -192,7 +192,7 @@ def _check_attend(run, fmt, heads, page, lens, n=1, starts=None, seed=0, stride=
     out = run.attend(cache, q_lat, q_pe, table, dl, q_starts=ds, lse=lse)
     torch.cuda.synchronize()
     run.raise_on_device_error()
-    r, rl, bound, lbound = ref.attend(cache, q_lat, q_pe, table, lens, SCALE, starts)
+    r, rl, bound, lbound = ref.attend(cache, q_lat, q_pe, table, lens, scale, starts)
     ref.assert_within(out, r, bound, "out")
     ref.assert_within(lse, rl, lbound, "lse")
 
@@ -317,6 +317,35 @@ def test_attend_non_finite_tokens_reach_only_their_queries(fmt, heads, n):
     first[last] = False
     assert torch.equal(out[first], want[first])
     assert not bool(out[last].isfinite().all(-1).any())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("scale", [0.0, -0.09, 1.0])
+def test_attend_scales(fmt, scale):
+    """No scale at all (a plain mean), a negative one, and one that leaves a few tokens."""
+    from sgl_amd_mono.moe.latent import LatentRunner
+
+    print(f"\nattend {fmt} scale={scale}", flush=True)
+    _check_attend(LatentRunner(24, scale=scale), fmt, 24, 16, [130, 1, 700], 2, seed=18, scale=scale)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attend_at_random(seed):
+    """Heads, pages, lengths (some empty), query counts and strides at random."""
+    import random
+
+    r = random.Random(seed)
+    heads, page = r.choice([1, 3, 8, 12, 17, 32, 40, 64, 127, 128]), r.choice([1, 2, 4, 8, 16, 32, 64, 256])
+    seqs = r.choice([1, 2, 5, 13, 37])
+    lens = [0 if r.random() < 0.15 else int(10 ** r.uniform(0, 3.5)) for _ in range(seqs)]
+    fmt, n, starts = r.choice(["bf16", "mxfp8"]), r.choice([1, 1, 2, 3, 7]), None
+    if r.random() < 0.5:
+        starts = [0]
+        for _ in range(seqs):
+            starts.append(starts[-1] + r.choice([0, 1, 1, 2, 4, 9]))
+        starts[-1] += starts[-1] == 0
+    print(f"\nattend {fmt} heads={heads} page={page} n={n} starts={starts} lens={lens}", flush=True)
+    _check_attend(_runner(heads), fmt, heads, page, lens, n, starts, seed=seed, stride=8 * r.choice([0, 1, 5]))
 
 
 # Work of more than 4096 tiles of 64 query rows (a row tile counts its tiles of 32 cached tokens and 8)
