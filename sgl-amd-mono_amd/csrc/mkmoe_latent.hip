@@ -1118,14 +1118,15 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 // ---------------------------------------------------------------- merge
 // Row tiles that were cut, their parts joined in order at their common maximum (so that the same call
 // gives the same bits). Bound by latency: the parts are 17 MB at 32 rows a tile, 33 MB at 64, and take
-// 7 to 10 us with the launch. kMergeWgs workgroups at each of a tile's cuts share its items, so that a
-// long sequence's many parts are read by many. Few parts: an item is a row's 128 latent values, 32 lanes
-// with up to kAtOnce parts' loads on their way; many: 64 values, the workgroup's 16 groups of 16 lanes
-// take every 16th part and add up in LDS (256 parts 8.5 us against 12.3 in items of 128; 8 sequences of
-// 16 to 32 parts took 38 us that way, 33 as few).
+// 5 to 10 us with the launch. kMergeWgs workgroups at each of a tile's cuts share its items, so that a
+// long sequence's many parts are read by many, and every part's load is on its way before the first is
+// used: up to kFewParts, an item is a row's 128 latent values, 32 lanes; up to kMoreParts, 64 values, a
+// wave, whose 4 groups of 16 lanes take every fourth part; beyond, 64 values, a workgroup, 16 groups.
+// (A step of 8 sequences in 20 parts each 24.9 us so, 28.9 with 8 parts at a time by 32 lanes; 256 parts
+// 8.5 us by workgroups, 12.3 by 8 groups of 32 lanes; 16 to 32 parts by workgroups 5 us more than by lanes.)
 constexpr int kMergeWgs = 8;
-constexpr int kFewParts = 32;
-constexpr int kAtOnce = 8;
+constexpr int kFewParts = 8;
+constexpr int kMoreParts = 32;
 
 __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
   __shared__ float s_w[kShares], s_red[4];
@@ -1152,30 +1153,59 @@ __global__ __launch_bounds__(256) void k_latent_merge(AttendParams p) {
         li = p.part_ml[at(lane, r) * 2 + 1];
       }
       const float* src = p.part_o + first;
-      f32x4 v[kAtOnce];
-      auto fetch = [&](int i0) {
+      f32x4 v[kFewParts];
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-          if (i0 + i < c.parts) v[i] = *(const f32x4*)(src + at(i0 + i, r) * kL);
-      };
-      fetch(0);
+      for (int i = 0; i < kFewParts; ++i)
+        if (i < c.parts) v[i] = *(const f32x4*)(src + at(i, r) * kL);
       float top = mi;
 #pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
+      for (int d = kFewParts / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
       const float w = __builtin_amdgcn_exp2f(mi - (top == -kInf ? 0.0f : top));
       float sum = w * li;
 #pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 32);
+      for (int d = kFewParts / 2; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 32);
       f32x4 acc = {0, 0, 0, 0};
-      for (int i0 = 0; i0 < c.parts; i0 += kAtOnce) {
-        if (i0 > 0) fetch(i0);
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-          if (i0 + i < c.parts) acc += __shfl(w, i0 + i, 32) * v[i];
-      }
+      for (int i = 0; i < kFewParts; ++i)
+        if (i < c.parts) acc += __shfl(w, i, 32) * v[i];
       top = __shfl(top, 0, 32);
       sum = __shfl(sum, 0, 32);
       store(r, first, acc, top, sum);
+    }
+    return;
+  }
+  if (c.parts <= kMoreParts) {
+    constexpr int kEach = kMoreParts / 4;
+    const int lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+    for (int item = helper * 4 + wave; item < 8 * c.nrows; item += helpers * 4) {
+      const int r = item >> 3, first = 64 * (item & 7) + 4 * (lane & 15);
+      float mi = -kInf, li = 0.0f;
+      if (lane < c.parts) {
+        mi = p.part_ml[at(lane, r) * 2];
+        li = p.part_ml[at(lane, r) * 2 + 1];
+      }
+      const float* src = p.part_o + first;
+      f32x4 v[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (4 * i < c.parts) v[i] = *(const f32x4*)(src + at(min(4 * i + g, c.parts - 1), r) * kL);
+      float top = mi;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+      const float w = __builtin_amdgcn_exp2f(mi - (top == -kInf ? 0.0f : top));
+      float sum = w * li;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (4 * i < c.parts) {
+          const float wi = __shfl(w, 4 * i + g, 64);
+          if (4 * i + g < c.parts) acc += wi * v[i];
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = over_groups(acc[k], [](float a, float b) { return a + b; });
+      if (g == 0) store(r, first, acc, top, sum);
     }
     return;
   }
