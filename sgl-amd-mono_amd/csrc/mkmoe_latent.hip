@@ -143,7 +143,7 @@ __device__ __forceinline__ float to_odd(double x) {
 
 // A wave a token of the first kv_blocks workgroups: lane l holds latent values 8 l .. 8 l + 7,
 // lanes 0 .. 7 the rope values too. Bound by memory on a prompt (8191 rows of 32 heads, 88 MB: 17.7 us
-// in graph replays, 5.0 TB/s) and by one trip to it on a decode step (7 rows 3.1 us). The norm's sum is formed in 64 bits, and so are MXFP8's products: a
+// in graph replays, 5.0 TB/s) and by one trip to it on a decode step (7 rows 2.8 us). The norm's sum is formed in 64 bits, and so are MXFP8's products: a
 // code next to a border is the one that the definition has (fp32 missed one in some 10^5 of them). The other workgroups rotate the query, 8 lanes a head's 64
 // values. Bytes: each value is read and written once; a decode step's few rows are one trip to
 // memory and back.
@@ -1118,7 +1118,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
 // ---------------------------------------------------------------- merge
 // Row tiles that were cut, their parts joined in order at their common maximum (so that the same call
 // gives the same bits). Bound by latency: the parts are 17 MB at 32 rows a tile, 33 MB at 64, and take
-// 5 to 10 us with the launch. kMergeWgs workgroups at each of a tile's cuts share its items, so that a
+// 4 to 10 us with the launch. kMergeWgs workgroups at each of a tile's cuts share its items, so that a
 // long sequence's many parts are read by many, and every part's load is on its way before the first is
 // used: up to kFewParts, an item is a row's 128 latent values, 32 lanes; up to kMoreParts, 64 values, a
 // wave, whose 4 groups of 16 lanes take every fourth part; beyond, 64 values, a workgroup, 16 groups.
