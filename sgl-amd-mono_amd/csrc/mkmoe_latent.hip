@@ -667,26 +667,32 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
         }
       }
     };
-    // (waves 4 .. 7) the raw rows of tile t as bf16: 8 threads a row, the codes 8 j .. of every 64 each
+    // (waves 4 .. 7) the raw rows of tile t as bf16: 16 threads a row, the codes 8 c .. of every 128 each, so
+    // that the 16 lanes which a store serves at once meet every bank once
     auto unpack = [&](int t) {
       if constexpr (MX) {
-        const int ln = own_lane(), r = 8 * lw + (ln >> 3), j = ln & 7;
-        const uint32_t src = raws + (t - tile0) % kMxRing * (kN * kMxRow) + r * kMxRow;
-        const uint32_t tile = tiles + ((t - tile0) & 1) * kTileBytes;
-        const u32x4 scales = lds_read<u32x4>(src + kL);
-        u32x2 q[8];
+        const int ln = own_lane(), c = ln & 15;
+        const uint32_t raw = raws + (t - tile0) % kMxRing * (kN * kMxRow), tile = tiles + ((t - tile0) & 1) * kTileBytes;
+        const int r0 = 8 * lw + (ln >> 4), rp = 8 * lw + (ln >> 3), j = ln & 7;  // the rows r0, r0 + 4; rope parts
+        const uint32_t src = raw + r0 * kMxRow;
+        u32x4 scales[2];
+        u32x2 q[2][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = lds_read<u32x2>(src + 64 * i + 8 * j);
-        const u32x4 pe = lds_read<u32x4>(src + kL + kMxScales + 16 * j);
-        __builtin_amdgcn_sched_barrier(0);
-        const uint32_t at = ((j ^ swz(r)) << 4), dst = tile + r * (2 * kL);
+        for (int i = 0; i < 2; ++i) {
+          scales[i] = lds_read<u32x4>(src + 4 * i * kMxRow + kL);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // (the scale's byte, 2 i + j / 4, to the exponent's place)
-          const uint32_t two = scales[i >> 1] >> (8 * (j >> 2));
-          const uint32_t e = (i & 1 ? two << 7 : two << 23) & 0x7f800000u;
-          *(MKMOE_LDS u32x4*)(uintptr_t)((at ^ ((i & 1) << 7)) + dst + (i >> 1) * 256) = fp8x8(q[i].x, q[i].y, u2f(e));
+          for (int k = 0; k < 4; ++k) q[i][k] = lds_read<u32x2>(src + 4 * i * kMxRow + 128 * k + 8 * c);
         }
-        *(MKMOE_LDS u32x4*)(uintptr_t)(tile + kRopeAt + r * (2 * kR) + ((j ^ swz_rope(r)) << 4)) = pe;
+        const u32x4 pe = lds_read<u32x4>(raw + rp * kMxRow + kL + kMxScales + 16 * j);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t dst = tile + r0 * (2 * kL) + ((c ^ swz(r0)) << 4);  // (swz(r0 + 4) is swz(r0))
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // (the scale's byte, 4 k + c / 4)
+            *(MKMOE_LDS u32x4*)(uintptr_t)(dst + 4 * i * (2 * kL) + 256 * k) =
+                fp8x8(q[i][k].x, q[i][k].y, e8m0(scales[i][k] >> (8 * (c >> 2)) & 0xff));
+        *(MKMOE_LDS u32x4*)(uintptr_t)(tile + kRopeAt + rp * (2 * kR) + ((j ^ swz_rope(rp)) << 4)) = pe;
       }
     };
     // waits until the tile after which `newer` more were requested has landed
