@@ -142,11 +142,11 @@ __device__ __forceinline__ float to_odd(double x) {
 }
 
 // A wave a token of the first kv_blocks workgroups: lane l holds latent values 8 l .. 8 l + 7,
-// lanes 0 .. 7 the rope values too. Bound by memory on a prompt (8191 rows of 32 heads, 88 MB: 17.7 us
-// in graph replays, 5.0 TB/s) and by one trip to it on a decode step (7 rows 2.8 us). The norm's sum is formed in 64 bits, and so are MXFP8's products: a
-// code next to a border is the one that the definition has (fp32 missed one in some 10^5 of them). The other workgroups rotate the query, 8 lanes a head's 64
-// values. Bytes: each value is read and written once; a decode step's few rows are one trip to
-// memory and back.
+// lanes 0 .. 7 the rope values too. The other workgroups rotate the query, 8 lanes a head's 64 values.
+// Each value is read and written once: bound by memory on a prompt (8191 rows of 32 heads, 88 MB:
+// 17.7 us in graph replays, 5.0 TB/s) and by one trip to it on a decode step (7 rows 2.8 us). The
+// norm's sum is formed in 64 bits, and so are MXFP8's products: a code next to a border is the one that
+// the definition has (fp32 missed one in some 10^5 of them).
 template <bool MX>
 __device__ __forceinline__ void append_block(const AppendParams& p, int block) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -193,7 +193,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int block) {
     }
     if constexpr (MX) {
       // 32 values are 4 lanes; the scale is the least power of two that keeps them within 448
-      // (the "vllm" MXFP8 rule), so no code saturates; codes straight from the fp32 values
+      // (as the block's own MXFP8 activations have it), so no code saturates; codes straight from the values
       float top = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(y[i]));
@@ -662,7 +662,9 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
                                       (uint32_t)__builtin_amdgcn_readlane(lo, 8 * i));
             lds_dma16(from, at ^ (swz(i) << 4), to + i * (2 * kL));
           }
-          const uint8_t* from = !PAGED ? (const uint8_t*)row : in && r < left ? base + r * kRowBytes : (const uint8_t*)g_zero_row;
+          const uint8_t* from = !PAGED            ? (const uint8_t*)row
+                                : in && r < left ? base + r * kRowBytes
+                                                 : (const uint8_t*)g_zero_row;
           lds_dma16(from + rope_at, rope_to);
         }
       }
@@ -1453,7 +1455,8 @@ inline int append_params(const mkmoe_latent_append_io* io, void* ws, size_t ws_b
                         !strides8(io->q_token_stride, io->q_head_stride) ||
                         !strides8(io->out_token_stride, io->out_head_stride)))
     return MKMOE_ERR_ALIGN;
-  if (io->heads > 0 && !rows_apart(io->out_token_stride, io->tokens, io->out_head_stride, io->heads, kR)) return MKMOE_ERR_ARG;
+  if (io->heads > 0 && !rows_apart(io->out_token_stride, io->tokens, io->out_head_stride, io->heads, kR))
+    return MKMOE_ERR_ARG;
   p.kv = (const uint16_t*)io->kv;
   p.norm_w = (const uint16_t*)io->norm_w;
   p.cos_sin = (const float*)io->cos_sin;

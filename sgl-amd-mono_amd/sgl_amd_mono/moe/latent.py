@@ -188,8 +188,8 @@ class LatentRunner:
         pos = self._vec("positions", positions, tokens, index)
         slot = self._vec("slots", slots, tokens, index)
         _lib.LATENT_APPEND.pack_into(
-            self._append_io, 0, *c, tokens, heads, self.rope, 8 if index is torch.int64 else 4, turns[0], stride, q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot,
-            q[0], q_out[0], self.norm_eps, 0,
+            self._append_io, 0, *c, tokens, heads, self.rope, 8 if index is torch.int64 else 4, turns[0], stride,
+            q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot, q[0], q_out[0], self.norm_eps, 0,
         )  # fmt: skip
         return tokens
 
@@ -303,10 +303,11 @@ class LatentRunner:
         out: torch.Tensor | None = None,
         lse: torch.Tensor | None = None,  # [T, heads] fp32: receives log sum exp
     ) -> torch.Tensor:
-        """-> [T, heads, 512], bf16 or, where ``out`` is, fp32. A sequence's queries are its last tokens: of n, query i sees the
-        first ``len - n + 1 + i`` tokens; one that sees none gives 0 (``lse`` -inf). Rows of ``out``
-        behind the last sequence's queries stay as they were. Pages outside the cache and lengths
-        or starts outside their bounds are recorded (``raise_on_device_error``)."""
+        """-> [T, heads, 512], bf16 or, where ``out`` is, fp32. A sequence's queries are its last tokens:
+        of n, query i sees the first ``len - n + 1 + i`` tokens; one that sees none gives 0 (``lse``
+        -inf). Rows of ``out`` behind the last sequence's queries stay as they were; ``out`` overlaps no
+        input. Pages outside the cache and lengths or starts outside their bounds are recorded
+        (``raise_on_device_error``)."""
         if q_lat is None or q_lat.dim() != 3:
             raise self._bad("q_lat", q_lat, f"[tokens, {self.heads}, {LATENT}] {BF}")
         tokens = q_lat.shape[0]
@@ -354,7 +355,8 @@ class LatentRunner:
         y = self._rows3("out", out, tokens, V, written=True)
         if kv is None or kv.shape[0] != tokens:
             raise self._bad("kv", kv, f"[{tokens}, {ROW}] {BF}")
-        q_lat, q_pe, o_lat = ((t.data_ptr(), h * n, n) for t, n in ((self._q_lat, LATENT), (self._q_pe, ROPE), (self._o_lat, LATENT)))
+        parts = (self._q_lat, LATENT), (self._q_pe, ROPE), (self._o_lat, LATENT)
+        q_lat, q_pe, o_lat = ((t.data_ptr(), h * n, n) for t, n in parts)
         kv_b = w.kv_b.data_ptr()
         self._set_append(cache, kv, w.norm, cos_sin, positions, slots, h, (at + 2 * NOPE, ts, hs), q_pe)
         self._set_project(self._absorb_io, tokens, 0, 0, (at, ts, hs), kv_b, q_lat)
