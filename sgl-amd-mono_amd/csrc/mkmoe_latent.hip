@@ -488,6 +488,8 @@ struct __align__(256) AttendSmem {
 // many (131071 tokens 189 -> 48), latent and rope parts apart in LDS without bank conflicts and maxima that
 // rarely move (verify 96 -> 73), half as many instructions a tile (MXFP8 167 -> 149), no spill beside the
 // tile loop (149 -> 138), queries by way of LDS (1025 tokens 16.1 -> 13.9).
+// (64 rows spill 64 bytes a lane, at a row tile's start and end, none in the loop: a reload there would wait
+// for the tiles on their way.)
 template <int M, bool MX, bool PAGED>
 __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M, MX>& sm, const Seq& own) {
   static_assert(M == 32 || M == 64, "row blocks of 16 by two token groups on 4 or 8 waves");
