@@ -395,9 +395,11 @@ __device__ const u32x4 g_zero_row[kRow * 2 / 16] = {};
 __device__ __forceinline__ void lds_dma16(const void* g, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
 }
-// (lane l's from base + at)
+// (lane l's from base + at. A base that a VALU instruction wrote, v_readlane or the reload of a spilled one,
+// may be read 5 wait states later: the compiler does not see the load, so the statement holds them)
 __device__ __forceinline__ void lds_dma16(const void* base, uint32_t at, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(lds)
+               : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma4(const void* g, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
