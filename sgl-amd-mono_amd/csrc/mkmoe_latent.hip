@@ -391,9 +391,10 @@ __device__ const u32x4 g_zero_row[kRow * 2 / 16] = {};
 
 // Bytes from global memory straight into LDS: lane l's land at lds + 16 l (4 l). One asm
 // statement, so that the compiler does not wait for it before other reads of LDS; the caller
-// waits (wait_loads) before the bytes are read
+// waits (wait_loads) before the bytes are read. M0 may be read one wait state after it was written,
+// which the statement holds too
 __device__ __forceinline__ void lds_dma16(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
 }
 // (lane l's from base + at. A base that a VALU instruction wrote, v_readlane or the reload of a spilled one,
 // may be read 5 wait states later: the compiler does not see the load, so the statement holds them)
@@ -402,7 +403,7 @@ __device__ __forceinline__ void lds_dma16(const void* base, uint32_t at, uint32_
                : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma4(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
 }
 // waits until at most N of the wave's loads are on their way (they complete in order)
 template <int N>
