@@ -311,11 +311,12 @@ __device__ __forceinline__ i32x4 weight_rsrc_words(const void* w, uint32_t n) {
 // (lds wave-uniform). One asm statement, so that the compiler's wait insertion (which waits
 // for every LDS-direct load before any later access of LDS it cannot tell apart) leaves it
 // in flight while the wave computes; the caller waits (vmcnt) before it reads what it wrote.
-// M0 may be read one wait state after it was written, which the statement holds.
+// M0 may be read one wait state after it was written, and a resource word that a VALU instruction
+// wrote (v_readfirstlane, the reload of a spilled one) 5 after it: the statement holds both.
 __device__ __forceinline__ void lds_dma16(i32x4 rs, void* lds, uint32_t voff) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(uint8_t*)lds);
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen nt lds" ::"v"(voff), "s"(m0), "s"(rs)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %2, 0 offen nt lds" ::"v"(voff), "s"(m0), "s"(rs)
                : "memory", "m0");
 }
 // the same with the default cache policy, for data that neighbouring waves read again from the
@@ -323,7 +324,7 @@ __device__ __forceinline__ void lds_dma16(i32x4 rs, void* lds, uint32_t voff) {
 __device__ __forceinline__ void lds_dma16_cached(i32x4 rs, void* lds, uint32_t voff) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(uint8_t*)lds);
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(voff), "s"(m0), "s"(rs)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(voff), "s"(m0), "s"(rs)
                : "memory", "m0");
 }
 
