@@ -1568,7 +1568,8 @@ struct GateUpCol {
 template <int K>
 __device__ __forceinline__ void write_lane(float& v, float s) {
   const int u = __builtin_amdgcn_readfirstlane(__float_as_int(s));
-  asm volatile("v_writelane_b32 %0, %1, %2" : "+v"(v) : "s"(u), "i"(K));
+  // (the scalar may be read 2 wait states after v_readfirstlane wrote it: the compiler does not see that)
+  asm volatile("s_nop 1\n\tv_writelane_b32 %0, %1, %2" : "+v"(v) : "s"(u), "i"(K));
 }
 __device__ __forceinline__ float lane_pick(const float (&a)[kTokGroup]) {
   static_assert(kTokGroup == 8, "lanes written");

@@ -106,7 +106,7 @@ def test_the_reading_finds_what_it_should():
 
 # the hazards that each part of the library is read for
 CHECKED = [("mkmoe_latent", "vector memory"), ("mkmoe_latent", "M0"), ("others", "M0"),
-           ("others", "vector memory")]  # fmt: skip
+           ("others", "vector memory"), ("mkmoe_latent", "VALU read"), ("others", "VALU read")]  # fmt: skip
 
 
 @pytest.fixture(scope="module")
