@@ -370,12 +370,13 @@ int mkmoe_latent_append(const mkmoe_latent_append_io* io, void* ws, size_t ws_by
 int mkmoe_latent_rows(const mkmoe_latent_cache* cache, const void* slots, int32_t index_bytes, int32_t tokens, void* out,
                       void* ws, size_t ws_bytes, void* stream);
 /* The absorbed attention: query token i of a sequence's n sees its first len - n + 1 + i tokens.
- * Rows of out behind the last sequence's queries stay as they were. Two launches. */
+ * Rows of out that no sequence has by q_starts stay as they were. Two launches. */
 int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_bytes, void* stream);
 int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream);
 /* A layer's whole step: append and absorb (expand 0) in one launch, attend, expand (1), with the same
  * tokens in each. All four are checked before the first launch; each one's outputs are the next
- * one's inputs as the caller set them. */
+ * one's inputs as the caller set them. Rows of expand's y that no sequence has by q_starts stay as
+ * they were. */
 int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_project_io* absorb,
                       const mkmoe_latent_attend_io* attend, const mkmoe_latent_project_io* expand, void* ws,
                       size_t ws_bytes, void* stream);

@@ -315,6 +315,7 @@ struct AttendParams {
   void* out;  // bf16, or fp32 (f32)
   float* lse;
   int32_t* err;
+  int32_t* covered;  // [2]: receives the rows that the sequences have by starts, from and up to
   Cut* cut;        // [kShares]
   float* part_o;   // [2 kShares][M][512]
   float* part_ml;  // [2 kShares][M][2]
@@ -1113,9 +1114,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_latent_attend(AttendParams p) {
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(v);
   };
-  if (p.starts && over_waves(__any(own.back))) {
-    if (tid == 0) p.cut[blockIdx.x].parts = 0;
-    return;
+  if (p.starts) {
+    const bool back = over_waves(__any(own.back));
+    if (blockIdx.x == 0 && tid == 0) p.covered[0] = back ? 0 : own.t0;
+    if (blockIdx.x == 0 && tid == p.seqs - 1) p.covered[1] = back ? 0 : own.t0 + own.n;
+    if (back) {
+      if (tid == 0) p.cut[blockIdx.x].parts = 0;
+      return;
+    }
   }
   if constexpr (WIDE) {
     int total = work_of<64>(p, own);
@@ -1266,6 +1272,8 @@ struct ProjectParams {
   uint16_t* y;
   int64_t x_ts, x_hs, y_ts, y_hs;
   int tokens, heads, f32;
+  const int32_t* covered;  // expand in a step with query starts: the rows that attend wrote, NULL: all.
+                           // The others' x is an earlier call's, and their y stays as it was
 };
 
 // what bf16's rounding left of a value, nothing where that is not finite
@@ -1339,6 +1347,7 @@ __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
   __shared__ f32x4 sums[4][NJ][4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int j0 = blockIdx.y * (16 * NJ), h = blockIdx.x, t0 = blockIdx.z * 64, l0 = wave * (kL / 4) + 8 * g;
+  const int from = p.covered ? p.covered[0] : 0, upto = p.covered ? min(p.covered[1], p.tokens) : p.tokens;
   const uint16_t* w = p.w + ((int64_t)h * (kNope + kV) + kNope + j0 + col) * kL + l0;
   // every operand on its way before the first is used
   using X = std::conditional_t<F32, f32x4, u32x4>;
@@ -1389,7 +1398,7 @@ __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
   }
   __syncthreads();
   const int t = t0 + 16 * wave + col;
-  if (t >= p.tokens) return;
+  if (t < from || t >= upto) return;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const f32x4* part = &sums[wave][j][0][lane];
@@ -1400,7 +1409,7 @@ __global__ __launch_bounds__(256) void k_latent_expand(ProjectParams p) {
 }
 
 // ---------------------------------------------------------------- host
-constexpr size_t kCtlBytes = 256;
+constexpr size_t kCtlBytes = 256, kCoveredAt = 64;  // the error words, the covered rows
 constexpr size_t kCutBytes = kShares * sizeof(Cut);
 constexpr size_t kMlBytes = (size_t)2 * kShares * kRowsMax * 2 * 4;
 constexpr size_t kPartBytes = (size_t)2 * kShares * kRowsMax * kL * 4;
@@ -1526,6 +1535,7 @@ inline int attend_params(const mkmoe_latent_attend_io* io, void* ws, size_t ws_b
   p.lse = io->lse;
   uint8_t* at = (uint8_t*)ws;
   p.err = (int32_t*)at;
+  p.covered = (int32_t*)(at + kCoveredAt);
   p.cut = (Cut*)(at += kCtlBytes);
   p.part_ml = (float*)(at += kCutBytes);
   p.part_o = (float*)(at += kMlBytes);
@@ -1570,7 +1580,7 @@ inline int project_params(const mkmoe_latent_project_io* io, ProjectParams& p) {
     return MKMOE_ERR_ALIGN;
   if (!rows_apart(io->y_token_stride, io->tokens, io->y_head_stride, io->heads, io->expand ? kV : kL)) return MKMOE_ERR_ARG;
   p = ProjectParams{io->x, (const uint16_t*)io->w, (uint16_t*)io->y, io->x_token_stride, io->x_head_stride,
-                    io->y_token_stride, io->y_head_stride, io->tokens, io->heads, io->x_f32};
+                    io->y_token_stride, io->y_head_stride, io->tokens, io->heads, io->x_f32, nullptr};
   return MKMOE_OK;
 }
 inline unsigned absorb_blocks(const ProjectParams& p) {
@@ -1667,6 +1677,7 @@ int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_p
   if (append->tokens != attend->tokens || absorb->tokens != attend->tokens || expand->tokens != attend->tokens)
     return MKMOE_ERR_ROWS;
   if (s.tokens == 0) return MKMOE_OK;
+  if (s.starts) v.covered = s.covered;
   hipStream_t st = (hipStream_t)stream;
   const int first = (int)absorb_blocks(k);
   if (append->cache.fmt == MKMOE_LATENT_MXFP8)

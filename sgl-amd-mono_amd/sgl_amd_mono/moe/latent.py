@@ -305,8 +305,9 @@ class LatentRunner:
     ) -> torch.Tensor:
         """-> [T, heads, 512], bf16 or, where ``out`` is, fp32. A sequence's queries are its last tokens:
         of n, query i sees the first ``len - n + 1 + i`` tokens; one that sees none gives 0 (``lse``
-        -inf). Rows of ``out`` behind the last sequence's queries stay as they were; ``out`` overlaps no
-        input. Pages outside the cache and lengths or starts outside their bounds are recorded
+        -inf). Rows of ``out`` that no sequence has by ``q_starts`` (before the first one's queries, behind
+        the last one's, all of them where the starts run backwards) stay as they were; ``out`` overlaps
+        no input. Pages outside the cache and lengths or starts outside their bounds are recorded
         (``raise_on_device_error``)."""
         if q_lat is None or q_lat.dim() != 3:
             raise self._bad("q_lat", q_lat, f"[tokens, {self.heads}, {LATENT}] {BF}")
@@ -344,7 +345,8 @@ class LatentRunner:
     ) -> torch.Tensor:
         """A layer's whole step -> bf16 [T, heads, 128] (before the output projection): the rows
         appended, then every query's attention over the cache with them. The arguments are those
-        of ``append`` and ``attend``; ``lens`` counts the appended tokens."""
+        of ``append`` and ``attend``; ``lens`` counts the appended tokens. Rows of ``out`` that no
+        sequence has stay as they were, as in ``attend``."""
         if q is None or q.dim() != 3 or q.shape[0] > self.max_tokens:
             raise self._bad("q", q, f"[tokens <= {self.max_tokens}, {self.heads}, {NOPE + ROPE}] {BF}")
         tokens, h = q.shape[0], self.heads

@@ -658,3 +658,101 @@ def test_decode_steps_then_the_moe_block():
     x = out.reshape(seqs, heads * 128)
     assert bool(moe.moe(mw, x).isfinite().all())
     moe.raise_on_device_error()
+
+
+# ---------------------------------------------------------------- rows of no sequence, tokens that were not stored
+def _ragged_layer(fmt, heads, lens, starts, tokens, seed):
+    """A step of ``tokens`` rows of which the sequences have those from ``starts``, as in a step padded
+    to a captured size; the others are padded tokens (slot -1)."""
+    cnt = [b - a for a, b in zip(starts, starts[1:])]
+    d = _layer(fmt, heads, lens, 1, seed=seed)
+    g = _gen(seed + 1)
+    pos, slots = torch.zeros(tokens, dtype=torch.int64, device="cuda"), torch.full((tokens,), -1, device="cuda")
+    for b, (s, n) in enumerate(zip(starts, cnt)):
+        for i in range(n):
+            at = lens[b] - n + i
+            if at >= 0:
+                pos[s + i] = at
+                slots[s + i] = d["table"][b, at // 16].long() * 16 + at % 16
+    d.update(q=_randn(g, tokens, heads, 192), kv=_randn(g, tokens, 576), positions=pos, slots=slots,
+             q_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))  # fmt: skip
+    return d
+
+
+def _by_parts(run, d, rows):
+    """The step's output by its parts, of the rows that the sequences have."""
+    w, q, c2 = d["w"], d["q"], d["cache"].clone()
+    q_pe = run.append(c2, d["kv"], w.norm, d["cos_sin"], d["positions"], d["slots"], q_pe=q[..., 128:])
+    o = torch.zeros(q.shape[0], run.heads, 512, device="cuda")
+    run.attend(c2, run.absorb(w, q[..., :128]), q_pe, d["table"], d["lens"], q_starts=d["q_starts"], out=o)
+    return run.expand(w, o)[rows], c2
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads", [8, 64])
+@pytest.mark.parametrize("starts", [[0, 3, 3, 4, 24], [2, 3, 7, 8, 10], [5, 5, 5, 5, 5]])
+def test_attention_leaves_rows_of_no_sequence(fmt, heads, starts):
+    """q_starts that cover some of the step's rows: the others stay as they were, also on a runner whose
+    last call was another step, whose rows would otherwise come back."""
+    print(f"\nattention {fmt} heads={heads} starts={starts}", flush=True)
+    t, lens = 30, [70, 50, 129, 400]
+    run = _runner(heads)
+    first = _ragged_layer(fmt, heads, lens, [0, 10, 20, 29, 30], t, seed=51)
+    run.attention(**first)
+    d = _ragged_layer(fmt, heads, lens, starts, t, seed=61)
+    rows = slice(starts[0], starts[-1])
+    want, after = _by_parts(_runner(heads), d, rows)
+    out = torch.full((t, heads, 128), 7.0, dtype=BF, device="cuda")
+    assert run.attention(**d, out=out) is out
+    run.raise_on_device_error()
+    assert torch.equal(out[rows], want) and torch.equal(d["cache"], after)
+    out[rows] = 7.0
+    assert bool((out == 7).all())
+
+
+def test_attention_of_starts_that_run_backwards():
+    run, lens = _runner(32), [70, 50, 129]
+    run.attention(**_ragged_layer("bf16", 32, lens, [0, 1, 5, 6], 6, seed=51))
+    run.raise_on_device_error()
+    d = _ragged_layer("bf16", 32, lens, [0, 2, 4, 6], 6, seed=61)
+    for starts in ([0, 4, 3, 6], [0, 6, 0, 6], [4, 5, 6, 0]):
+        d["q_starts"].copy_(torch.tensor(starts, dtype=torch.int32))
+        out = torch.full((6, 32, 128), 7.0, dtype=BF, device="cuda")
+        run.attention(**d, out=out)
+        assert bool((out == 7).all())
+        with pytest.raises(RuntimeError, match="a length or query start"):
+            run.raise_on_device_error()
+        run.clear_errors()
+    d["q_starts"].copy_(torch.tensor([0, 2, 4, 6], dtype=torch.int32))
+    want, _ = _by_parts(_runner(32), d, slice(0, 6))
+    assert torch.equal(run.attention(**d), want)
+    run.raise_on_device_error()
+
+
+def test_attention_with_query_starts_in_a_graph():
+    """A captured step padded to 16 rows, replayed with other starts."""
+    t, heads, lens = 16, 32, [70, 50, 129, 400]
+    run, eager = _runner(heads), _runner(heads)
+    d = _ragged_layer("mxfp8", heads, lens, [0, 4, 8, 12, 16], t, seed=71)
+    out, base = torch.empty(t, heads, 128, dtype=BF, device="cuda"), d["cache"].clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        run.attention(**d, out=out)
+        with torch.cuda.graph(g, stream=s):
+            run.attention(**d, out=out)
+    torch.cuda.current_stream().wait_stream(s)
+    for rep, starts in enumerate([[0, 4, 8, 12, 16], [0, 1, 2, 3, 4], [3, 3, 8, 8, 9], [0, 0, 0, 0, 0], [0, 9, 10, 12, 16]]):
+        n = _ragged_layer("mxfp8", heads, lens, starts, t, seed=72 + rep)
+        for k in ("q", "kv", "positions", "slots", "q_starts"):
+            d[k].copy_(n[k])
+        d["cache"].copy_(base)
+        want, after = _by_parts(eager, d, slice(starts[0], starts[-1]))
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[starts[0] : starts[-1]], want) and torch.equal(d["cache"], after), rep
+        out[starts[0] : starts[-1]] = 7.0
+        assert bool((out == 7).all()), rep
+    run.raise_on_device_error()
