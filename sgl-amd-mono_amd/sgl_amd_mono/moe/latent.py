@@ -152,9 +152,10 @@ class LatentRunner:
                 return t.data_ptr(), pages, page, _lib.LATENT_MXFP8
         raise self._bad("cache", t, f"[pages, page_size, {ROW}] {BF} or [pages, page_size, {MX_ROW}] torch.uint8 contiguous")
 
-    def _new(self, what: str, *shape) -> torch.Tensor:
+    def _new(self, what: str, *shape, zeros: bool = False) -> torch.Tensor:
+        """An output of the call's own. ``zeros``: the call may leave rows of it unwritten."""
         no_capture(what)
-        return torch.empty(*shape, dtype=BF, device=self.device)
+        return (torch.zeros if zeros else torch.empty)(*shape, dtype=BF, device=self.device)
 
     def _call(self, fn, *args) -> None:
         """``fn`` on the current stream of this runner's GPU."""
@@ -306,8 +307,8 @@ class LatentRunner:
         """-> [T, heads, 512], bf16 or, where ``out`` is, fp32. A sequence's queries are its last tokens:
         of n, query i sees the first ``len - n + 1 + i`` tokens; one that sees none gives 0 (``lse``
         -inf). Rows of ``out`` that no sequence has by ``q_starts`` (before the first one's queries, behind
-        the last one's, all of them where the starts run backwards) stay as they were; ``out`` overlaps
-        no input. Pages outside the cache and lengths or starts outside their bounds are recorded
+        the last one's, all of them where the starts run backwards) stay as they were, 0 without ``out``;
+        ``out`` overlaps no input. Pages outside the cache and lengths or starts outside their bounds are recorded
         (``raise_on_device_error``)."""
         if q_lat is None or q_lat.dim() != 3:
             raise self._bad("q_lat", q_lat, f"[tokens, {self.heads}, {LATENT}] {BF}")
@@ -315,7 +316,7 @@ class LatentRunner:
         ql = self._rows3("q_lat", q_lat, tokens, LATENT)
         qp = self._rows3("q_pe", q_pe, tokens, ROPE)
         if out is None:
-            out = self._new("the attended rows", tokens, self.heads, LATENT)
+            out = self._new("the attended rows", tokens, self.heads, LATENT, zeros=q_starts is not None)
         f32 = out.dtype == torch.float32
         op = self._rows3("out", out, tokens, LATENT, written=True, dtype=torch.float32 if f32 else BF)
         at_lse = 0
@@ -353,7 +354,7 @@ class LatentRunner:
         at, ts, hs = self._rows3("q", q, tokens, NOPE + ROPE)
         w.check(h, self.device)
         if out is None:
-            out = self._new("the attention's output", tokens, h, V)
+            out = self._new("the attention's output", tokens, h, V, zeros=q_starts is not None)
         y = self._rows3("out", out, tokens, V, written=True)
         if kv is None or kv.shape[0] != tokens:
             raise self._bad("kv", kv, f"[{tokens}, {ROW}] {BF}")

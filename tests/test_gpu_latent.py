@@ -756,3 +756,24 @@ def test_attention_with_query_starts_in_a_graph():
         out[starts[0] : starts[-1]] = 7.0
         assert bool((out == 7).all()), rep
     run.raise_on_device_error()
+
+
+@pytest.mark.parametrize("heads", [8, 64])
+def test_rows_of_no_sequence_are_zeros_in_an_output_of_the_calls_own(heads):
+    """Without ``out``, rows that q_starts gives to nobody do not hold what the memory held before."""
+    t, lens = 30, [70, 50, 129, 400]
+    run = _runner(heads)
+    d = _ragged_layer("bf16", heads, lens, [2, 3, 7, 8, 10], t, seed=81)
+    q_lat, q_pe = _randn(_gen(82), t, heads, 512), _randn(_gen(83), t, heads, 64)
+    keep = torch.zeros(t, dtype=torch.bool, device="cuda")
+    keep[2:10] = True
+    for call in (lambda: run.attention(**d),
+                 lambda: run.attend(d["cache"], q_lat, q_pe, d["table"], d["lens"], q_starts=d["q_starts"])):  # fmt: skip
+        for _ in range(3):  # (memory that the allocator gives out again)
+            dirty = torch.full((t, heads, 512), NAN, dtype=BF, device="cuda")
+            small = torch.full((t, heads, 128), NAN, dtype=BF, device="cuda")
+            del dirty, small
+            out = call()
+            assert bool((out[~keep] == 0).all()) and bool(out[keep].isfinite().all()) and bool((out[keep] != 0).any())
+            del out
+    run.raise_on_device_error()
