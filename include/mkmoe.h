@@ -297,7 +297,7 @@ const char* mkmoe_status_string(int status);
 #define MKMOE_LATENT_ERRW_COUNT 2 /* how many were seen */
 #define MKMOE_LATENT_ERRW_WORDS 4
 #define MKMOE_LATENT_ERR_SLOT 1     /* slot >= pages page_size: the row is not written / read as 0 */
-#define MKMOE_LATENT_ERR_POSITION 2 /* position outside cos_sin: the token's rows are not written */
+#define MKMOE_LATENT_ERR_POSITION 2 /* position outside cos_sin: the token's rows are not written (q_out_nan) */
 #define MKMOE_LATENT_ERR_LENGTH 3   /* length or query starts outside their bounds: clamped. Starts that
                                      * run backwards: nothing is attended, out stays as it was */
 #define MKMOE_LATENT_ERR_PAGE 4     /* page outside the cache: its tokens read as rows of zeros */
@@ -328,7 +328,7 @@ typedef struct mkmoe_latent_append_io {
   const void* q_pe;      /* [tokens][heads][64] bf16 */
   void* q_out;           /* the same, rotated; may be q_pe itself */
   float norm_eps;
-  int32_t reserved;
+  int32_t q_out_nan;     /* q_out of a token whose position is outside cos_sin: 0 stays as it was, 1 NaN */
 } mkmoe_latent_append_io;
 
 typedef struct mkmoe_latent_attend_io {
@@ -375,7 +375,8 @@ int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_by
 int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream);
 /* A layer's whole step: append and absorb (expand 0) in one launch, attend, expand (1), with the same
  * tokens in each. All four are checked before the first launch; each one's outputs are the next
- * one's inputs as the caller set them. Rows of expand's y that no sequence has by q_starts stay as
+ * one's inputs as the caller set them. A token whose slot or position is outside its bounds gets a query
+ * of NaN, and so an output. Rows of expand's y that no sequence has by q_starts stay as
  * they were. */
 int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_project_io* absorb,
                       const mkmoe_latent_attend_io* attend, const mkmoe_latent_project_io* expand, void* ws,

@@ -92,7 +92,7 @@ struct AppendParams {
   int32_t* err;
   int64_t kv_stride, q_ts, q_hs, o_ts, o_hs;
   int64_t rows, table_rows;
-  int tokens, heads, half, wide, kv_blocks;
+  int tokens, heads, half, wide, kv_blocks, mark;
   float eps;
 };
 
@@ -147,7 +147,8 @@ __device__ __forceinline__ float to_odd(double x) {
 // 17.7 us in graph replays, 5.0 TB/s) and by one trip to it on a decode step (7 rows 2.8 us). The
 // norm's sum is formed in 64 bits, and so are MXFP8's products: a code next to a border is the one that
 // the definition has (fp32 missed one in some 10^5 of them).
-template <bool MX>
+// STEP: the query rows are attended with next, so that those of a token that cannot be stored become NaN
+template <bool MX, bool STEP>
 __device__ __forceinline__ void append_block(const AppendParams& p, int block) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (block < p.kv_blocks) {
@@ -226,17 +227,21 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int block) {
   if (r >= (int64_t)p.tokens * p.heads) return;
   const int t = (int)(r / p.heads), h = (int)(r - (int64_t)t * p.heads), j = lane & 7;
   const int64_t pos = index_at(p.positions, t, p.wide);
-  if (pos < 0 || pos >= p.table_rows) {
-    if (j == 0 && h == 0) record(p.err, MKMOE_LATENT_ERR_POSITION, t);
+  const bool lost = pos < 0 || pos >= p.table_rows, unstored = STEP && index_at(p.slots, t, p.wide) >= p.rows;
+  u32x4* to = (u32x4*)(p.q_out + t * p.o_ts + h * p.o_hs + 8 * j);
+  if (lost || unstored) {
+    if (lost && j == 0 && h == 0) record(p.err, MKMOE_LATENT_ERR_POSITION, t);
+    constexpr uint32_t kNan = 0x7fc07fc0u;
+    if (STEP || p.mark) *to = u32x4{kNan, kNan, kNan, kNan};
     return;
   }
   const u32x4 v = *(const u32x4*)(p.q + t * p.q_ts + h * p.q_hs + 8 * j);
-  *(u32x4*)(p.q_out + t * p.o_ts + h * p.o_hs + 8 * j) = rotate8(v, p.cos_sin + pos * kR, j, p.half);
+  *to = rotate8(v, p.cos_sin + pos * kR, j, p.half);
 }
 
 template <bool MX>
 __global__ __launch_bounds__(256) void k_latent_append(AppendParams p) {
-  append_block<MX>(p, blockIdx.x);
+  append_block<MX, false>(p, blockIdx.x);
 }
 
 // ---------------------------------------------------------------- rows as values
@@ -1333,7 +1338,7 @@ __global__ __launch_bounds__(256) void k_latent_front(AppendParams a, ProjectPar
   if ((int)blockIdx.x < absorb_blocks)
     absorb_block(p, blockIdx.x, wl);
   else
-    append_block<MX>(a, blockIdx.x - absorb_blocks);
+    append_block<MX, true>(a, blockIdx.x - absorb_blocks);
 }
 
 // y[t, h, j] = sum_l x[t, h, l] W_UV[h, j, l]: a workgroup a head, 16 NJ columns and 64 tokens. The
@@ -1458,7 +1463,7 @@ inline int append_params(const mkmoe_latent_append_io* io, void* ws, size_t ws_b
   if (!io->kv || !io->cos_sin || !io->positions || !io->slots) return MKMOE_ERR_NULL;
   if (io->tokens < 0 || io->tokens > kMaxRows) return MKMOE_ERR_ROWS;
   if (io->heads < 0 || io->heads > MKMOE_LATENT_MAX_HEADS || (io->rope & ~1) != 0 ||
-      (io->index_bytes != 4 && io->index_bytes != 8) || io->cos_sin_rows < 1 || !(io->norm_eps >= 0.0f) ||
+      (io->q_out_nan & ~1) != 0 || (io->index_bytes != 4 && io->index_bytes != 8) || io->cos_sin_rows < 1 || !(io->norm_eps >= 0.0f) ||
       !isfinite(io->norm_eps) || io->kv_stride < kRow)
     return MKMOE_ERR_ARG;
   if (io->heads > 0 && (!io->q_pe || !io->q_out)) return MKMOE_ERR_NULL;
@@ -1492,6 +1497,7 @@ inline int append_params(const mkmoe_latent_append_io* io, void* ws, size_t ws_b
   p.half = io->rope == MKMOE_ROPE_HALF;
   p.wide = io->index_bytes == 8;
   p.kv_blocks = (io->tokens + 3) / 4;
+  p.mark = io->q_out_nan;
   p.eps = io->norm_eps;
   return MKMOE_OK;
 }

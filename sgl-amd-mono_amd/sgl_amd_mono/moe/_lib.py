@@ -188,7 +188,7 @@ class LatentAppendIO(ctypes.Structure):
             )
         ]
         + [(n, ctypes.c_void_p) for n in ("kv", "norm_w", "cos_sin", "positions", "slots", "q_pe", "q_out")]
-        + [("norm_eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+        + [("norm_eps", ctypes.c_float), ("q_out_nan", ctypes.c_int32)]
     )  # fmt: skip
 
 

@@ -169,7 +169,8 @@ class LatentRunner:
             _lib.check(rc, fn.__name__)
 
     # ---- the calls' arguments, checked and written into their structures
-    def _set_append(self, cache, kv, norm, cos_sin, positions, slots, heads: int, q: tuple, q_out: tuple) -> int:
+    def _set_append(self, cache, kv, norm, cos_sin, positions, slots, heads: int, q: tuple, q_out: tuple,
+                    nan: int = 0) -> int:  # fmt: skip
         c = self._cache(cache)
         shape = () if kv is None else kv.shape
         if len(shape) != 2 or shape[1] != ROW or kv.dtype is not BF or kv.get_device() != self._index:
@@ -190,7 +191,7 @@ class LatentRunner:
         slot = self._vec("slots", slots, tokens, index)
         _lib.LATENT_APPEND.pack_into(
             self._append_io, 0, *c, tokens, heads, self.rope, 8 if index is torch.int64 else 4, turns[0], stride,
-            q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot, q[0], q_out[0], self.norm_eps, 0,
+            q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot, q[0], q_out[0], self.norm_eps, nan,
         )  # fmt: skip
         return tokens
 
@@ -234,9 +235,10 @@ class LatentRunner:
     ) -> torch.Tensor | None:
         """Store the step's rows; -> the query's rope part, rotated (``q_out``, which may be
         ``q_pe`` itself). A token with a negative slot is not stored. A slot outside the cache or
-        a position outside ``cos_sin`` leaves the token unwritten and is recorded
-        (``raise_on_device_error``)."""
+        a position outside ``cos_sin`` leaves the token unwritten (NaN in a query of the call's own)
+        and is recorded (``raise_on_device_error``)."""
         qp = op = (0, 0, 0)
+        own = q_out is None
         if q_pe is not None:
             if kv is None:
                 raise self._bad("kv", kv, f"[tokens, {ROW}] {BF}")
@@ -247,7 +249,8 @@ class LatentRunner:
             op = self._rows3("q_out", q_out, tokens, ROPE, written=True)
         elif q_out is not None:
             raise RuntimeError("mkmoe latent q_out: given without q_pe")
-        if self._set_append(cache, kv, norm, cos_sin, positions, slots, 0 if q_pe is None else self.heads, qp, op):
+        heads = 0 if q_pe is None else self.heads
+        if self._set_append(cache, kv, norm, cos_sin, positions, slots, heads, qp, op, int(own)):
             self._call(self.lib.mkmoe_latent_append, self._append_io, *self._ws)
         return q_out
 
@@ -347,7 +350,8 @@ class LatentRunner:
         """A layer's whole step -> bf16 [T, heads, 128] (before the output projection): the rows
         appended, then every query's attention over the cache with them. The arguments are those
         of ``append`` and ``attend``; ``lens`` counts the appended tokens. Rows of ``out`` that no
-        sequence has stay as they were, as in ``attend``."""
+        sequence has stay as they were, as in ``attend``; a token whose slot or position is outside
+        its bounds, which is recorded, gives NaN."""
         if q is None or q.dim() != 3 or q.shape[0] > self.max_tokens:
             raise self._bad("q", q, f"[tokens <= {self.max_tokens}, {self.heads}, {NOPE + ROPE}] {BF}")
         tokens, h = q.shape[0], self.heads

@@ -777,3 +777,49 @@ def test_rows_of_no_sequence_are_zeros_in_an_output_of_the_calls_own(heads):
             assert bool((out[~keep] == 0).all()) and bool(out[keep].isfinite().all()) and bool((out[keep] != 0).any())
             del out
     run.raise_on_device_error()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_attention_of_a_token_that_was_not_stored_is_nan(fmt):
+    """A position outside cos_sin or a slot outside the cache is recorded, and the token's output says so:
+    it is NaN, not what the runner's last step left of its query. The other tokens have theirs."""
+    heads, lens = 16, [70, 5, 400, 64, 33]
+    run = _runner(heads)
+    run.attention(**_layer(fmt, heads, lens, 1, seed=91))
+    d = _layer(fmt, heads, lens, 1, seed=92)
+    base = d["cache"].clone()
+    want = run.attention(**d).clone()
+    run.raise_on_device_error()
+    ok = torch.tensor([0, 2, 4], device="cuda")
+    for name, at, bad, why in (("positions", [1, 3], [d["cos_sin"].shape[0], -1], "a position outside cos_sin"),
+                               ("slots", [1, 3], [base.shape[0] * 16, 1 << 40], "a slot outside the cache")):  # fmt: skip
+        d["cache"].copy_(base)
+        good = d[name].clone()
+        d[name][at] = torch.tensor(bad, device="cuda")
+        out = run.attention(**d)
+        assert torch.equal(out[ok], want[ok])
+        assert bool(out[at].isnan().all())
+        with pytest.raises(RuntimeError, match=why):
+            run.raise_on_device_error()
+        run.clear_errors()
+        d[name].copy_(good)
+    d["cache"].copy_(base)
+    assert torch.equal(run.attention(**d), want)
+    run.raise_on_device_error()
+
+
+def test_append_of_a_bad_position_in_an_output_of_its_own():
+    """Without ``q_out``, the query rows of a position outside cos_sin are NaN, not what the memory held."""
+    from sgl_amd_mono.moe.latent import cache_like
+
+    g, run, t = _gen(97), _runner(4), 5
+    cache, kv, q = cache_like(4, 8), _randn(g, t, 576), _randn(g, t, 4, 64)
+    pos, slots = torch.tensor([1, 16, 3, -1, 5], device="cuda"), torch.arange(t, device="cuda")
+    for _ in range(3):
+        dirty = torch.full((t, 4, 64), 7.0, dtype=BF, device="cuda")
+        del dirty
+        out = run.append(cache, kv, None, _cos_sin(16), pos, slots, q_pe=q)
+        assert bool(out[[1, 3]].isnan().all()) and bool(out[[0, 2, 4]].isfinite().all())
+        del out
+    with pytest.raises(RuntimeError, match="a position outside cos_sin"):
+        run.raise_on_device_error()

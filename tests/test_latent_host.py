@@ -389,3 +389,18 @@ def test_calls_refuse_mismatched_tensors(host_runner):
     attend(), append(q_pe=qp, q_out=qp), r.expand(_weights(False), ql.float(), out=torch.empty(4, 8, 128, dtype=BF))
     assert [n for n, _ in r.calls] == ["mkmoe_latent_attend", "mkmoe_latent_append", "mkmoe_latent_project"]
     assert r._expand_io.x_f32 == 1
+
+
+def test_append_rejects_an_unknown_mark(lib):
+    L, n = lib
+    assert L.mkmoe_latent_append(ctypes.byref(_append(q_out_nan=2)), 0x200000, n, None) == -8
+    assert L.mkmoe_latent_append(ctypes.byref(_append(q_out_nan=1, tokens=0)), 0x200000, n, None) == 0
+
+
+def test_append_marks_an_output_of_its_own(host_runner, monkeypatch):
+    """A query that the caller provides keeps the rows of bad positions; one of the call's own has NaN there."""
+    r, d, q = host_runner, _step(), torch.zeros(4, 8, 64, dtype=BF)
+    monkeypatch.setattr(r, "_new", lambda what, *shape, **kw: torch.zeros(*shape, dtype=BF))
+    for q_out in (None, torch.zeros_like(q)):
+        r.append(d["cache"], d["kv"], None, d["cos_sin"], d["positions"], d["slots"], q_pe=q, q_out=q_out)
+        assert r._append_io.q_out_nan == (q_out is None)
