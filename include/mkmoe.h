@@ -324,7 +324,8 @@ typedef struct mkmoe_latent_append_io {
   const void* norm_w;    /* [512] bf16; NULL: the latent is stored as it is */
   const float* cos_sin;  /* [cos_sin_rows][64]: 32 cosines, 32 sines */
   const void* positions; /* [tokens] */
-  const void* slots;     /* [tokens] cache rows, distinct; negative: a padded token, not written */
+  const void* slots;     /* [tokens] cache rows, distinct; negative: a padded token, not written. Its position
+                          * may lie outside cos_sin: its query is 0 then */
   const void* q_pe;      /* [tokens][heads][64] bf16 */
   void* q_out;           /* the same, rotated; may be q_pe itself */
   float norm_eps;

@@ -230,9 +230,10 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int block) {
   const bool lost = pos < 0 || pos >= p.table_rows, unstored = STEP && index_at(p.slots, t, p.wide) >= p.rows;
   u32x4* to = (u32x4*)(p.q_out + t * p.o_ts + h * p.o_hs + 8 * j);
   if (lost || unstored) {
-    if (lost && j == 0 && h == 0) record(p.err, MKMOE_LATENT_ERR_POSITION, t);
-    constexpr uint32_t kNan = 0x7fc07fc0u;
-    if (STEP || p.mark) *to = u32x4{kNan, kNan, kNan, kNan};
+    const bool padded = index_at(p.slots, t, p.wide) < 0;  // it needs no position
+    if (lost && !padded && j == 0 && h == 0) record(p.err, MKMOE_LATENT_ERR_POSITION, t);
+    const uint32_t v = padded ? 0 : 0x7fc07fc0u;
+    if (padded || STEP || p.mark) *to = u32x4{v, v, v, v};
     return;
   }
   const u32x4 v = *(const u32x4*)(p.q + t * p.q_ts + h * p.q_hs + 8 * j);

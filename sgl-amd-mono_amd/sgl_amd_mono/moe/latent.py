@@ -234,7 +234,8 @@ class LatentRunner:
         q_out: torch.Tensor | None = None,
     ) -> torch.Tensor | None:
         """Store the step's rows; -> the query's rope part, rotated (``q_out``, which may be
-        ``q_pe`` itself). A token with a negative slot is not stored. A slot outside the cache or
+        ``q_pe`` itself). A token with a negative slot is a padded one and not stored (where its position
+        is outside ``cos_sin``, its query is 0). A slot outside the cache or
         a position outside ``cos_sin`` leaves the token unwritten (NaN in a query of the call's own)
         and is recorded (``raise_on_device_error``)."""
         qp = op = (0, 0, 0)

@@ -823,3 +823,32 @@ def test_append_of_a_bad_position_in_an_output_of_its_own():
         del out
     with pytest.raises(RuntimeError, match="a position outside cos_sin"):
         run.raise_on_device_error()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_padded_tokens_need_no_position(fmt):
+    """A token with a negative slot and a position outside cos_sin is a padded one: nothing is recorded, its
+    query rows are zeros. With a position inside, they are rotated as the others are."""
+    from sgl_amd_mono.moe.latent import cache_like
+
+    g, run = _gen(95), _runner(4)
+    cache, cs = cache_like(4, 8, fmt), _cos_sin(16)
+    kv, q = _randn(g, 6, 576), _randn(g, 6, 4, 64)
+    pos, slots = torch.tensor([1, -1, 3, 16, 5, 1 << 40], device="cuda"), torch.tensor([3, -1, 31, -7, -1, -1], device="cuda")
+    out = torch.full((6, 4, 64), 7.0, dtype=BF, device="cuda")
+    run.append(cache, kv, None, cs, pos, slots, q_pe=q, q_out=out)
+    run.raise_on_device_error()
+    assert (cache.view(32, -1) != 0).any(1).nonzero().flatten().tolist() == [3, 31]
+    assert bool((out[[1, 3, 5]] == 0).all())
+    real = torch.tensor([0, 2, 4], device="cuda")
+    want, size = ref.rotate(q[real].double(), cs[pos[real]][:, None], False)
+    ref.assert_within(out[real], want, want.abs() * ref.U16 + 3 * ref.U32 * size, "query")
+    # a padded step: the padded sequences are empty, their tokens have neither slot nor position
+    d = _layer(fmt, 16, [70, 400, 0, 0], 1, seed=96)
+    run = _runner(16)
+    base = d["cache"].clone()
+    want = run.attention(**d).clone()
+    d["cache"].copy_(base)
+    d["positions"][2:] = torch.tensor([-1, 1 << 30], device="cuda")
+    assert torch.equal(run.attention(**d), want) and bool((want[2:] == 0).all())
+    run.raise_on_device_error()
