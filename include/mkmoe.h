@@ -375,7 +375,8 @@ int mkmoe_latent_rows(const mkmoe_latent_cache* cache, const void* slots, int32_
 int mkmoe_latent_attend(const mkmoe_latent_attend_io* io, void* ws, size_t ws_bytes, void* stream);
 int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream);
 /* A layer's whole step: append and absorb (expand 0) in one launch, attend, expand (1), with the same
- * tokens in each. All four are checked before the first launch; each one's outputs are the next
+ * tokens, heads (append's may be 0: no query), cache and type of attended latents in each, else
+ * MKMOE_ERR_ROWS or _ARG. All four are checked before the first launch; each one's outputs are the next
  * one's inputs as the caller set them. A token whose slot or position is outside its bounds gets a query
  * of NaN, and so an output. Rows of expand's y that no sequence has by q_starts stay as
  * they were. */

@@ -1683,6 +1683,12 @@ int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_p
   if (absorb->expand || !expand->expand) return MKMOE_ERR_ARG;
   if (append->tokens != attend->tokens || absorb->tokens != attend->tokens || expand->tokens != attend->tokens)
     return MKMOE_ERR_ROWS;
+  // what one part writes is as large as what the next reads
+  const mkmoe_latent_cache &from = append->cache, &to = attend->cache;
+  if ((append->heads != 0 && append->heads != attend->heads) || absorb->heads != attend->heads ||
+      expand->heads != attend->heads || expand->x_f32 != attend->out_f32 || from.data != to.data ||
+      from.pages != to.pages || from.page_size != to.page_size || from.fmt != to.fmt)
+    return MKMOE_ERR_ARG;
   if (s.tokens == 0) return MKMOE_OK;
   if (s.starts) v.covered = s.covered;
   hipStream_t st = (hipStream_t)stream;

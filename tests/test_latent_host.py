@@ -404,3 +404,26 @@ def test_append_marks_an_output_of_its_own(host_runner, monkeypatch):
     for q_out in (None, torch.zeros_like(q)):
         r.append(d["cache"], d["kv"], None, d["cos_sin"], d["positions"], d["slots"], q_pe=q, q_out=q_out)
         assert r._append_io.q_out_nan == (q_out is None)
+
+
+@pytest.mark.parametrize("parts,code", [
+    (dict(append=dict(heads=4)), -8),
+    (dict(absorb=dict(heads=4)), -8),
+    (dict(attend=dict(heads=16, ql_token_stride=8192, qp_token_stride=1024, out_token_stride=8192)), -8),
+    (dict(expand=dict(heads=9, x_token_stride=9 * 512, y_token_stride=9 * 128)), -8),
+    (dict(expand=dict(x_f32=1)), -8),
+    (dict(attend=dict(out_f32=1)), -8),
+    (dict(append=dict(cache=dict(data=AT + 16))), -8),
+    (dict(append=dict(cache=dict(pages=11))), -8),
+    (dict(append=dict(cache=dict(page_size=8))), -8),
+    (dict(attend=dict(cache=dict(fmt=2))), -8),
+    (dict(append=dict(heads=0, tokens=0), absorb=dict(tokens=0), attend=dict(tokens=0), expand=dict(tokens=0)), 0),
+    (dict(append=dict(tokens=0), absorb=dict(tokens=0), attend=dict(tokens=0, out_f32=1), expand=dict(tokens=0, x_f32=1)), 0),
+])  # fmt: skip
+def test_step_wants_parts_that_fit(lib, parts, code):
+    """The same heads (append's may be none: no query), cache and type of the attended latents throughout:
+    a part with more heads than the one before wrote would read past its buffer. (Those that fit: no tokens.)"""
+    L, n = lib
+    get = lambda k: {a: _cache(**b) if a == "cache" else b for a, b in parts.get(k, {}).items()}  # noqa: E731
+    io = (_append(**get("append")), _project(0, **get("absorb")), _attend(**get("attend")), _project(1, **get("expand")))
+    assert L.mkmoe_latent_step(*map(ctypes.byref, io), 0x200000, n, None) == code
