@@ -181,14 +181,17 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int block) {
 #pragma unroll
       for (int d = 32; d >= 1; d >>= 1) ss += __shfl_xor(ss, d, 64);
       const double rstd = 1.0 / sqrt(ss / kL + (double)p.eps);
+      // (without eps, rows of bf16's subnormals: rstd reaches 2^138, past fp32. Its power of two goes to the values)
+      const bool far = rstd > 0x1p100;
+      const float up = far ? 0x1p64f : 1.0f, r32 = (float)(far ? rstd * 0x1p-64 : rstd);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (MX) {
           y[2 * i] = to_odd((double)y[2 * i] * rstd * (double)bf_lo(nw[i]));
           y[2 * i + 1] = to_odd((double)y[2 * i + 1] * rstd * (double)bf_hi(nw[i]));
         } else {
-          y[2 * i] = y[2 * i] * (float)rstd * bf_lo(nw[i]);
-          y[2 * i + 1] = y[2 * i + 1] * (float)rstd * bf_hi(nw[i]);
+          y[2 * i] = y[2 * i] * up * r32 * bf_lo(nw[i]);
+          y[2 * i + 1] = y[2 * i + 1] * up * r32 * bf_hi(nw[i]);
         }
       }
     }

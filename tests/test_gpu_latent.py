@@ -852,3 +852,29 @@ def test_padded_tokens_need_no_position(fmt):
     d["positions"][2:] = torch.tensor([-1, 1 << 30], device="cuda")
     assert torch.equal(run.attention(**d), want) and bool((want[2:] == 0).all())
     run.raise_on_device_error()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_append_without_eps(fmt):
+    """norm_eps 0 on rows whose root mean square's inverse passes fp32 (bf16's subnormals) or nearly so, and on
+    ordinary ones: each is the norm's within the bound of ``test_append``."""
+    from sgl_amd_mono.moe.latent import cache_like
+
+    sizes = [2.0**-133, 2.0**-130, 2.0**-127, 2.0**-126, 2.0**-110, 2.0**-100, 2.0**-99, 2.0**-66, 1.0, 2.0**100]
+    run, g, t = _runner(1, norm_eps=0.0), _gen(99), len(sizes)
+    kv = torch.zeros(t, 576, dtype=BF, device="cuda")
+    x = torch.randint(1, 4, (t, 512), generator=g, device="cuda") * (1 - 2 * torch.randint(0, 2, (t, 512), generator=g, device="cuda"))
+    kv[:, :512] = (x.double() * torch.tensor(sizes, dtype=torch.float64, device="cuda")[:, None]).to(BF)  # exact
+    assert torch.equal(kv[:, :512].double(), x.double() * torch.tensor(sizes, dtype=torch.float64, device="cuda")[:, None])
+    w = (1 + 0.1 * torch.randn(512, generator=g, device="cuda")).to(BF)
+    rows = torch.arange(t, device="cuda")
+    cache = cache_like(t, 1, fmt)
+    run.append(cache, kv, w, _cos_sin(1), torch.zeros_like(rows), rows)
+    got = ref.row_values(cache.view(t, -1))[:, :512]
+    c = ref.norm(kv[:, :512], w, 0.0)
+    if fmt == "bf16":
+        ref.assert_within(got, c, c.abs() * (ref.U16 + 2 * 540 * ref.U32), "latent")
+    else:
+        sc = torch.exp2(torch.ceil(torch.log2(c.view(t, 16, 32).abs().amax(-1) / 448))).repeat_interleave(32, 1)
+        ref.assert_within(got, c, torch.maximum(c.abs() * 2.0**-4, sc * 2.0**-10) * (1 + 1e-4), "latent")
+    run.raise_on_device_error()
