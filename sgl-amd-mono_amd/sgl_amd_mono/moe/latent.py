@@ -86,7 +86,8 @@ class LatentRunner:
         self.max_tokens = int(max_tokens)
         self.scale = (NOPE + ROPE) ** -0.5 if scale is None else float(scale)
         self.norm_eps = float(norm_eps)
-        if not math.isfinite(self.scale) or not (math.isfinite(self.norm_eps) and self.norm_eps >= 0):
+        f32 = lambda v: ctypes.c_float(v).value  # noqa: E731  (what the library is given)
+        if not math.isfinite(f32(self.scale)) or not (math.isfinite(f32(self.norm_eps)) and self.norm_eps >= 0):
             raise RuntimeError(f"mkmoe latent: scale {self.scale}, norm_eps {self.norm_eps}")
         self.rope = ROPES[rope]
         self.lib = _lib.lib()

@@ -427,3 +427,11 @@ def test_step_wants_parts_that_fit(lib, parts, code):
     get = lambda k: {a: _cache(**b) if a == "cache" else b for a, b in parts.get(k, {}).items()}  # noqa: E731
     io = (_append(**get("append")), _project(0, **get("absorb")), _attend(**get("attend")), _project(1, **get("expand")))
     assert L.mkmoe_latent_step(*map(ctypes.byref, io), 0x200000, n, None) == code
+
+
+def test_runner_rejects_options_that_fp32_does_not_hold():
+    from sgl_amd_mono.moe.latent import LatentRunner
+
+    for kw in (dict(scale=1e39), dict(scale=-1e300), dict(norm_eps=1e39)):
+        with pytest.raises(RuntimeError, match="scale .* norm_eps"):
+            LatentRunner(8, device="cuda", **kw)
