@@ -412,6 +412,20 @@ __device__ __forceinline__ void lds_dma16(const void* base, uint32_t at, uint32_
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(lds)
                : "memory", "m0");
 }
+// five of them in order, 4096 bytes apart in memory and in LDS: one wait for the base, M0's by the address's sum
+// (MXFP8, whose bringing waves are the ones that hold up a tile: with a wait each, 48 sequences of 16384 140 to
+// 143 us, so 133 to 135; the bf16 cache's eight rows gain nothing by it)
+__device__ __forceinline__ void lds_dma16_five(const void* base, uint32_t at, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+      "s_add_u32 m0, m0, 0x1000\n\tv_add_u32 %0, 0x1000, %0\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+      "s_add_u32 m0, m0, 0x1000\n\tv_add_u32 %0, 0x1000, %0\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+      "s_add_u32 m0, m0, 0x1000\n\tv_add_u32 %0, 0x1000, %0\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+      "s_add_u32 m0, m0, 0x1000\n\tv_add_u32 %0, 0x1000, %0\n\tglobal_load_lds_dwordx4 %0, %1"
+      : "+v"(at)
+      : "s"(base), "s"(lds)
+      : "memory", "m0", "scc");
+}
 __device__ __forceinline__ void lds_dma4(const void* g, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory", "m0");
 }
@@ -643,8 +657,8 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
         const bool ends = lw < kMxLoads % 4 && ln < kN * kPieces % 64;  // the last load, not a whole one
         if (PAGED && whole && in) {
           const uint32_t at = (lw * 64 + ln) << 4;
-#pragma unroll
-          for (int i = 0; i < kLoads - 1; ++i) lds_dma16(base, at + i * 4096, dst + i * 4096);
+          static_assert(kLoads == 6, "five loads, and one wave's sixth");
+          lds_dma16_five(base, at, dst);
           if (ends) lds_dma16(base, at + (kLoads - 1) * 4096, dst + (kLoads - 1) * 4096);
         } else {
 #pragma unroll

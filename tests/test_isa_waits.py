@@ -135,6 +135,9 @@ def test_m0_serves_the_loads_into_lds_alone(found):
     unnamed = re.compile(r"s_movrel|s_sendmsg|v_interp|s_set_gpr_idx|ds_\w*(addtid|gws)")  # (they read it unnamed)
     assert not [x for x in latent if unnamed.match(x[1])]
     uses = [(i, t) for i, (_, t) in enumerate(latent) if re.search(r"\bm0\b", t)]
-    for i, t in uses:  # written, waited for, read by a load
-        assert t.startswith("s_mov_b32 m0, s") and latent[i + 1][1].startswith("s_nop") and "_lds_" in latent[i + 2][1], latent[i : i + 3]
+    for i, t in uses:  # written, waited for or the address formed, read by a load
+        assert re.match(r"s_mov_b32 m0, s\d+$|s_add_u32 m0, m0, 0x[0-9a-f]+$", t), t
+        after = [u.split(" ")[0] for _, u in latent[i + 1 : i + 4]]
+        load = next(k for k, u in enumerate(after) if "_lds_" in u)
+        assert set(after[:load]) <= {"s_nop", "v_add_u32_e32"} and load > 0, (t, after)
     assert len(uses) == sum("_lds_" in t for _, t in latent)
