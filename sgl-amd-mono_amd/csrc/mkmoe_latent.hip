@@ -303,6 +303,14 @@ constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
 
+// bf16 parts that a numerator is taken as, a matrix operand: two leave out 2^-17 of it, one 2^-9. The second one's
+// products fit under the tile's loads at 32 rows of a bf16 cache (48 sequences of 8192 102 to 105 us either way, 36
+// ragged ones 46 and 45; error of the outputs 0.0021 -> 0.0017, which is their own rounding). At 64 rows the MFMAs
+// and LDS bound the tile, and in MXFP8 the waves that multiply unpack as well (64 sequences 105 us, with two parts
+// 115; 48 of 16384 141 and 156)
+template <int M, bool MX>
+constexpr int kPParts = M == 32 && !MX ? 2 : 1;
+
 // what the end of a share cut, for the merge: the row tile that goes on in the next share
 struct Cut {
   int32_t parts;        // 0: nothing was cut there
@@ -470,7 +478,7 @@ template <int M, bool MX>
 struct __align__(256) AttendSmem {
   uint8_t tile[MX ? 2 : kRing][kTileBytes];  // cached rows, bf16, swizzled pieces
   uint8_t raw[MX ? kMxRing : 1][MX ? kN * kMxRow : 16];
-  uint16_t p[MX ? 1 : 2][M * kPStride];  // softmax numerators of a tile [row][token]
+  uint16_t p[MX ? 1 : 2][kPParts<M, MX> * M * kPStride];  // softmax numerators of a tile [part][row][token]
   float mx[M * 2];             // [row][token group]: tile maxima
   float al[M];                 // the tile's rescaling of each row; at the end the maxima
   const uint8_t* addr[2][kN];  // the rows of the tile that is requested next
@@ -741,7 +749,8 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
 
     // ---- what both kinds of wave do with a tile
     auto tile_at = [&](int t) { return tiles + (MX ? (t - tile0) & 1 : (t - tile0) % kRing) * kTileBytes; };
-    auto p_of = [&](int t) { return p_at + (MX ? 0 : (t & 1) * (M * kPStride * 2)); };
+    constexpr int kPBytes = M * kPStride * 2;  // of a part
+    auto p_of = [&](int t) { return p_at + (MX ? 0 : (t & 1) * (kPParts<M, MX> * kPBytes)); };
     // tokens that only some of the rows see: their non-finite values must not reach the others
     // through 0 * V. They are cleared, and the rows that see them become NaN
     const bool edges = lim_lo < lim_hi;
@@ -780,11 +789,13 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
         va[c] = __builtin_bit_cast(bf16x8, both);
       }
     };
-    auto numerators_of = [&](int t, bf16x8(&pb)[MB]) {
+    auto numerators_of = [&](int t, bf16x8(&pb)[kPParts<M, MX>][MB]) {
       const int ln = own_lane();
       const uint32_t at = p_of(t) + (ln & 15) * (2 * kPStride) + ((ln >> 4) << 4);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) pb[i] = lds_read<bf16x8>(at + i * 16 * (2 * kPStride));
+      for (int k = 0; k < kPParts<M, MX>; ++k)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) pb[k][i] = lds_read<bf16x8>(at + k * kPBytes + i * 16 * (2 * kPStride));
     };
     auto rescale = [&](auto& o) {
       constexpr int C = sizeof(o) / sizeof(o[0]);
@@ -795,12 +806,14 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
         for (int c = 0; c < C; ++c) o[c][i] *= alpha;
       }
     };
-    auto add = [&](auto& o, auto& va, bf16x8(&pb)[MB]) {
+    auto add = [&](auto& o, auto& va, bf16x8(&pb)[kPParts<M, MX>][MB]) {
       constexpr int C = sizeof(o) / sizeof(o[0]);
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
+      for (int k = kPParts<M, MX> - 1; k >= 0; --k)
 #pragma unroll
-        for (int c = 0; c < C; ++c) o[c][i] = mfma(va[c], pb[i], o[c][i]);
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int c = 0; c < C; ++c) o[c][i] = mfma(va[c], pb[k][i], o[c][i]);
     };
     const bool whole = tile0 == 0 && tile1 == kt;
     const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
@@ -917,8 +930,12 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
 #pragma unroll
             for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(sc[rb][k] - mu);
             sum[rb] = (e[0] + e[1]) + (e[2] + e[3]);
-            *(MKMOE_LDS u32x2*)(uintptr_t)(p_of(t) + ((rg * RB + rb) * 16 + col) * (2 * kPStride) + 32 * tg + 8 * g) =
-                u32x2{pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
+            const uint32_t to = p_of(t) + ((rg * RB + rb) * 16 + col) * (2 * kPStride) + 32 * tg + 8 * g;
+            const u32x2 near = {pack_bf(e[0], e[1]), pack_bf(e[2], e[3])};
+            *(MKMOE_LDS u32x2*)(uintptr_t)to = near;
+            if constexpr (kPParts<M, MX> == 2)  // (infinite ones come before the maximum moves, and are not used)
+              *(MKMOE_LDS u32x2*)(uintptr_t)(to + kPBytes) =
+                  u32x2{pack_bf(e[0] - bf_lo(near.x), e[1] - bf_hi(near.x)), pack_bf(e[2] - bf_lo(near.y), e[3] - bf_hi(near.y))};
           }
         };
         // keys: this lane's row of the wave's 16, pieces 4 ks + g; read a few steps ahead, and no
@@ -950,7 +967,7 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
           __builtin_amdgcn_sched_barrier(0);
         }
         if (RB == 1) acc[0] += acc[1];
-        bf16x8 va[2], pb[MB];
+        bf16x8 va[2], pb[kPParts<M, MX>][MB];
         values(tile, 2 * wave, std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{}, va);
         bool move = false;
 #pragma unroll
@@ -1074,7 +1091,7 @@ __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M
       auto step = [&](int t, auto is_steady) __attribute__((always_inline)) {
         constexpr bool steady = decltype(is_steady)::value;
         if (!steady && edges && (t + 1) * kN > lim_lo) sanitize(t);
-        bf16x8 va[6], pb[MB];
+        bf16x8 va[6], pb[kPParts<M, MX>][MB];
         // MXFP8: the next tile takes the place of t - 1
         if (MX && (steady || t + 1 < tend)) unpack(t + 1);
         values(tile_at(t), lw, std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}, va);

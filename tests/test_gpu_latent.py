@@ -878,3 +878,30 @@ def test_append_without_eps(fmt):
         sc = torch.exp2(torch.ceil(torch.log2(c.view(t, 16, 32).abs().amax(-1) / 448))).repeat_interleave(32, 1)
         ref.assert_within(got, c, torch.maximum(c.abs() * 2.0**-4, sc * 2.0**-10) * (1 + 1e-4), "latent")
     run.raise_on_device_error()
+
+
+@pytest.mark.parametrize("page", [1, 64])
+@pytest.mark.parametrize("heads,lens,n", [(32, [1, 70, 0, 400, 3000], 1), (8, [129, 64, 5], 4), (64, [500, 33], 1)])
+def test_attend_numerators_of_a_bf16_cache(page, heads, lens, n):
+    """32 rows a tile over a bf16 cache take each numerator as two bf16 parts, which leave 2^-16 of it out
+    (one leaves up to 2^-8). In fp32 the output has no rounding beside the sums'. A score is a sum of
+    576 products in fp32, each addition off by 2^-24 of what is there, less than sum |q k|: in the mean
+    square sqrt(576) 2^-24 of that times the scale, and an output twice as much. Twice their sum is asked for."""
+    print(f"\nnumerators page={page} heads={heads} lens={lens} n={n}", flush=True)
+    run = _runner(heads)
+    cache, q_lat, q_pe, table, dl = _attend_case("bf16", heads, page, lens, n, seed=101)
+    out = torch.empty(q_lat.shape, device="cuda")
+    run.attend(cache, q_lat, q_pe, table, dl, out=out)
+    run.raise_on_device_error()
+    want, *_ = ref.attend(cache, q_lat, q_pe, table, lens, SCALE)
+    most = 0.0
+    for b, length in enumerate(lens):
+        kv = ref.row_values(ref.sequence_rows(cache, table, b, length)).abs()
+        q = torch.cat([q_lat, q_pe], 2)[b * n : b * n + n].double().abs()
+        if length:
+            most = max(most, float((q @ kv.T).max()) * SCALE)
+    asked = 2 * (2.0**-16 + 2 * 576**0.5 * ref.U32 * most + max(lens) ** 0.5 * ref.U32)
+    assert asked < 2.0**-11
+    err = float((out.double() - want).norm() / want.norm())
+    print(f"error {err:.2e}, asked {asked:.2e}", flush=True)
+    assert err <= asked
