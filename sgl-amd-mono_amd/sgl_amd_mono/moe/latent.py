@@ -69,7 +69,8 @@ class LatentRunner:
     """Latent attention of one rank's ``heads`` on one GPU: a workspace and the calls.
 
     ``max_tokens``: query tokens that ``attention`` takes at most (its intermediates' size; the
-    other calls have no such bound). ``scale``: of the scores (default 192^-0.5). ``rope``:
+    other calls have no such bound). ``scale``: of the scores (default 192^-0.5; a model whose rope
+    is scaled has another: DeepSeek-V3's is that times (0.1 ln 40 + 1)^2 = 1.874). ``rope``:
     "interleaved" (pairs (2 i, 2 i + 1)) or "half" ((i, i + 32)). One runner serves one stream at
     a time: calls that can overlap need runners of their own."""
 
