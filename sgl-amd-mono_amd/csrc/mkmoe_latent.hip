@@ -144,7 +144,7 @@ __device__ __forceinline__ float to_odd(double x) {
 // A wave a token of the first kv_blocks workgroups: lane l holds latent values 8 l .. 8 l + 7,
 // lanes 0 .. 7 the rope values too. The other workgroups rotate the query, 8 lanes a head's 64 values.
 // Each value is read and written once: bound by memory on a prompt (8191 rows of 32 heads, 88 MB:
-// 17.7 us in graph replays, 5.0 TB/s) and by one trip to it on a decode step (7 rows 2.8 us). The
+// 17.4 us in graph replays, 5.1 TB/s) and by one trip to it on a decode step (7 rows 2.8 us). The
 // norm's sum is formed in 64 bits, and so are MXFP8's products: a code next to a border is the one that
 // the definition has (fp32 missed one in some 10^5 of them).
 // STEP: the query rows are attended with next, so that those of a token that cannot be stored become NaN
@@ -502,28 +502,32 @@ struct __align__(256) AttendSmem {
 //   S^T = K Q^T   scoring wave (rg, tg): the rows of half rg, tokens 16 tg ..: A = K (16-byte
 //                 reads of LDS; with 64 rows each serves two row blocks), B = Q^T in registers
 //   P             exp2 of the scores less the rows' running maxima, [row][token] in LDS, in bf16
-//                 because it is a matrix operand; the sums stay fp32
+//                 because it is a matrix operand (kPParts); the sums stay fp32
 //   O^T += V^T P^T   latent values 32 w .. of a scoring wave (32 of them), 16 of every 64 past 128 of the
 //                 others (96), for every row: A = V^T by transposing LDS reads of the same tile, B = P^T
 // One barrier a tile (bf16). bf16 rows go straight from memory to LDS, three tiles ahead; MXFP8 rows
 // go there as they are, and waves 4 .. 7 turn the next tile's into bf16 (exact) while waves 0 .. 3 score,
 // at the price of a second barrier. PAGED: pages of kN tokens or more, so that a tile lies in one, its
 // page is a scalar load and its rows follow each other; without it each token's page entry is looked up,
-// two tiles before its row is (pages of one token 103 us, of 64 100 us, at 48 sequences of 8192).
+// two tiles before its row is (pages of one token 103 us, of 64 101 us, at 48 sequences of 8192).
 //
-// What bounds it: 32 rows a tile in bf16, memory (48 sequences of 8192, 32 heads: 100 us with the merge,
-// 4.6 TB/s, of it about 20 us for the start, the outputs and the merge); 64 rows, LDS and the wave's
-// instruction issue (a tile takes 2300 cycles, of which its LDS reads and writes need 1800 and its MFMAs 1150:
-// 12 sequences of 8192, 64 heads, 4 queries each 64 us, 430 TFLOP/s); MXFP8, the codes' way through LDS
-// (64 sequences of up to 16384, 32 heads 93 us, 3.7 TB/s; 48 of 16384 134 us, of which it takes 19, while the
-// conversions themselves are free). Short work is bound by the chain of lengths, pages and queries, first
-// tile, outputs and merge (1025 tokens: 13.4 us).
+// What bounds it, by counters at 2.3 GHz (a tile's time by the difference of two lengths). bf16: memory, 32 rows
+// (48 sequences of 8192, 32 heads: 101 us with the merge, 4.5 TB/s, of it about 20 us for the start, the outputs
+// and the merge; a further tile 1.7 to 2.1 us, where a copy's rate gives 1.8) and 64 rows, since every row tile
+// brings the sequence's rows past the L2 anew: 24 of 8192 with 128 heads read 479 MB, twice the cache, in 91 us
+// (97 with the merge), 5.3 TB/s; 48 with 64 heads as many, none of them twice, in 115 (122). A further tile of 64
+// rows takes 1.5 us while the cache fits the last-level cache and 1.8 beyond, 3400 to 4200 cycles, of which the
+// MFMAs need 1088 a SIMD and the LDS 714 (98 of them conflicts). 12 ragged sequences with 4 queries of 64 heads:
+// 245 MB in 56 us (66), 4.4 TB/s. MXFP8: the codes' way through LDS (a further tile of 32 rows 1.2 us, 2700 cycles, of
+// them 1059 of LDS and 544 of MFMA; 48 of 16384, 32 heads 133 to 144 us, 3.8 TB/s, of which it took 19, while
+// the conversions themselves are free; 64 of up to 16384 98). Short work is bound by the chain of lengths, pages
+// and queries, first tile, outputs and merge (1025 tokens: 14 us).
 //
 // Steps that brought it there: whole rows by ring and DMA (64 heads 380 -> 129 us), cut row tiles joined by
 // many (131071 tokens 189 -> 48), latent and rope parts apart in LDS without bank conflicts and maxima that
 // rarely move (verify 96 -> 73), half as many instructions a tile (MXFP8 167 -> 149), no spill beside the
 // tile loop (149 -> 138), queries by way of LDS (1025 tokens 16.1 -> 13.9).
-// (64 rows spill 64 bytes a lane, at a row tile's start and end, none in the loop: a reload there would wait
+// (64 rows spill 64 to 72 bytes a lane, at a row tile's start and end, none in the loop: a reload there would wait
 // for the tiles on their way.)
 template <int M, bool MX, bool PAGED>
 __device__ __forceinline__ void attend_share(const AttendParams& p, AttendSmem<M, MX>& sm, const Seq& own) {
