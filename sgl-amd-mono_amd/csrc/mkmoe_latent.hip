@@ -517,7 +517,7 @@ struct __align__(256) AttendSmem {
 // brings the sequence's rows past the L2 anew: 24 of 8192 with 128 heads read 479 MB, twice the cache, in 91 us
 // (97 with the merge), 5.3 TB/s; 48 with 64 heads as many, none of them twice, in 115 (122). A further tile of 64
 // rows takes 1.5 us while the cache fits the last-level cache and 1.8 beyond, 3400 to 4200 cycles, of which the
-// MFMAs need 1088 a SIMD and the LDS 714 (98 of them conflicts). 12 ragged sequences with 4 queries of 64 heads:
+// MFMAs need 1088 a SIMD and the LDS 714 (its 192 instructions a tile 1340 at the rate that 8 waves issue them). 12 ragged sequences with 4 queries of 64 heads:
 // 245 MB in 56 us (66), 4.4 TB/s. MXFP8: the codes' way through LDS (a further tile of 32 rows 1.2 us, 2700 cycles, of
 // them 1059 of LDS and 544 of MFMA; 48 of 16384, 32 heads 133 to 144 us, 3.8 TB/s, of which it took 19, while
 // the conversions themselves are free; 64 of up to 16384 98). Short work is bound by the chain of lengths, pages
