@@ -301,6 +301,7 @@ const char* mkmoe_status_string(int status);
 #define MKMOE_LATENT_ERR_LENGTH 3   /* length or query starts outside their bounds: clamped. Starts that
                                      * run backwards: nothing is attended, out stays as it was */
 #define MKMOE_LATENT_ERR_PAGE 4     /* page outside the cache: its tokens read as rows of zeros */
+#define MKMOE_LATENT_ERR_CONTEXT 5  /* (prompt) the cached tokens pass max_context: the sequence's output is NaN */
 
 typedef struct mkmoe_latent_cache {
   void* data;        /* [pages][page_size] rows, 16-byte aligned */
@@ -383,6 +384,46 @@ int mkmoe_latent_project(const mkmoe_latent_project_io* io, void* stream);
 int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_project_io* absorb,
                       const mkmoe_latent_attend_io* attend, const mkmoe_latent_project_io* expand, void* ws,
                       size_t ws_bytes, void* stream);
+
+/* ---- a prompt's tokens
+ * The same attention with a key and a value for each head and token, made from the cached rows by
+ * w: k = [W_UK c, k_pe], v = W_UV c, o = sum softmax(scale q . k) v: fewer operations than the absorbed form
+ * from about 171 query tokens a sequence. Keys, values and softmax's numerators are rounded to bf16, sums,
+ * scores and maxima are fp32. Query token i of a sequence's n sees its first len - n + 1 + i tokens. */
+typedef struct mkmoe_latent_prompt_io {
+  mkmoe_latent_cache cache;
+  int32_t seqs;        /* 1 .. MKMOE_LATENT_MAX_SEQS */
+  int32_t tokens;      /* query tokens, at most 2^20; without q_starts a multiple of seqs */
+  int32_t heads;       /* 1 .. MKMOE_LATENT_MAX_HEADS */
+  int32_t max_pages;   /* table entries a sequence: its length is at most max_pages page_size */
+  int32_t max_context; /* cached tokens that the workspace holds: those of the sequences with query tokens, each
+                        * one's rounded up to 64; at most 2^22 */
+  int32_t pad;
+  int64_t table_stride;
+  int64_t qn_token_stride, qn_head_stride, qp_token_stride, qp_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  const void* q_nope;      /* [tokens][heads][128] bf16 */
+  const void* q_pe;        /* [tokens][heads][64] bf16, rotated */
+  const void* w;           /* [heads][256][512] bf16 (kv_b): W_UK rows 0 .. 127, W_UV rows 128 .. 255 */
+  const int32_t* table;    /* [seqs][max_pages] pages */
+  const int32_t* lens;     /* [seqs] cached tokens, the queries' own among them; 0: none */
+  const int32_t* q_starts; /* [seqs + 1] first query token of each sequence, or NULL: equal counts */
+  void* out;               /* [tokens][heads][128] bf16; 0 for a query that sees nothing */
+  float* lse;              /* [tokens][heads] log of the sum of exp(s), or NULL; -inf there */
+  float scale;
+  int32_t pad2;
+} mkmoe_latent_prompt_io;
+
+/* Workspace bytes of the prompt calls, a latent workspace among them at its start (its error words zeroed
+ * once by the caller): 135 MB, and for each token of max_context 1152 bytes and 512 a head. */
+int mkmoe_latent_prompt_bytes(int32_t heads, int32_t max_context, size_t* bytes);
+/* Keys and values, then the attention over them. Rows of out that no sequence has by q_starts stay as they
+ * were. Four launches. */
+int mkmoe_latent_prompt(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_bytes, void* stream);
+/* The tokens' rows appended and their query rotated first, with the same tokens, heads (append's may be 0: no
+ * query) and cache, else MKMOE_ERR_ROWS or _ARG. Both are checked before the first launch. */
+int mkmoe_latent_prompt_step(const mkmoe_latent_append_io* append, const mkmoe_latent_prompt_io* io, void* ws,
+                             size_t ws_bytes, void* stream);
 /* Copy n error words to host memory (synchronises stream). */
 int mkmoe_latent_read_errors(const void* ws, int32_t* words, int32_t n, void* stream);
 

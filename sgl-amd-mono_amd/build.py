@@ -11,8 +11,8 @@ The library holds the kernels and the C ABI of ``include/mkmoe.h`` and
 file runs wherever the tree is copied. The MoE source compiles in parts, in
 parallel: one object per compiled MoE shape (``MKMOE_UNIT`` 0 .. 8) and one for
 the host code (``MKMOE_UNIT`` 9); the FFN seam's source (``csrc/mkmoe_seam.hip``)
-and the latent attention's (``csrc/mkmoe_latent.hip``) are one more object each; then
-one link. The test hooks of ``include/mkmoe_testing.h``
+and the latent attention's (``csrc/mkmoe_latent.hip``, ``mkmoe_prompt.hip``) are
+one more object each; then one link. The test hooks of ``include/mkmoe_testing.h``
 (``csrc/mkmoe_testing.hip``) build alongside, as ``libmkmoe_testing.so``.
 """
 
@@ -33,7 +33,7 @@ OUT_TIMELINE = ROOT / "sgl_amd_mono" / "moe" / "libmkmoe_tl.so"
 OUT_TESTING = ROOT / "sgl_amd_mono" / "moe" / "libmkmoe_testing.so"
 SOURCE = CSRC / "mkmoe_kernels.hip"
 SEAM_SOURCE = CSRC / "mkmoe_seam.hip"
-LATENT_SOURCE = CSRC / "mkmoe_latent.hip"
+LATENT_SOURCES = [CSRC / f"mkmoe_{n}.hip" for n in ("latent", "prompt")]
 TESTING_SOURCE = CSRC / "mkmoe_testing.hip"
 UNITS = (0, 1, 2, 3, 4, 5, 6, 7, 8, 9)  # the compiled shapes, then the host code
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -60,12 +60,13 @@ def build(check: bool = False, verbose: bool = False, timeline: bool = False) ->
     out = OUT_TIMELINE if timeline else OUT
     defs = ["-DMKMOE_TIMELINE"] if timeline else []
     with tempfile.TemporaryDirectory(prefix="mkmoe_build_") as tmpd:
-        objs = [Path(tmpd) / f"unit{u}.o" for u in UNITS] + [Path(tmpd) / "seam.o", Path(tmpd) / "latent.o"]
+        objs = [Path(tmpd) / f"unit{u}.o" for u in UNITS] + [Path(tmpd) / "seam.o"]
+        objs += [Path(tmpd) / f"{src.stem}.o" for src in LATENT_SOURCES]
         cmds = []
         for u, o in zip(UNITS, objs):
             cmds.append([HIPCC, *FLAGS, *defs, f"-DMKMOE_UNIT={u}", "-c", str(SOURCE), "-o", str(o)])
-        cmds.append([HIPCC, *FLAGS, "-c", str(SEAM_SOURCE), "-o", str(objs[-2])])
-        cmds.append([HIPCC, *FLAGS, "-c", str(LATENT_SOURCE), "-o", str(objs[-1])])
+        for src, o in zip([SEAM_SOURCE, *LATENT_SOURCES], objs[len(UNITS) :]):
+            cmds.append([HIPCC, *FLAGS, "-c", str(src), "-o", str(o)])
         testing_tmp = OUT_TESTING.with_suffix(".so.tmp")
         if not timeline:
             cmds.append([HIPCC, *FLAGS, "-shared", str(TESTING_SOURCE), "-o", str(testing_tmp)])

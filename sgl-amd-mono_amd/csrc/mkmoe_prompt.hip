@@ -1,0 +1,782 @@
+// Latent attention of a prompt's tokens on gfx950 (MI355X): HIP kernels and the C ABI of the prompt
+// section of include/mkmoe.h.
+//
+// A chunk of a sequence's new tokens attends over its cached rows, its own among them, with a key
+// and a value for every head and token, made from the row's latent part c by the head's weights:
+//   k = [W_UK c, k_pe] (128 + 64 values),  v = W_UV c (128),
+//   s = scale (q_nope . W_UK c + q_pe . k_pe),  o = sum softmax(s) v,
+// 640 operations a score where the absorbed form needs 2176, for 262144 a head and cached token once a
+// call: the fewer from about 171 new tokens a sequence.
+//
+//   k_prompt_rows     the cached rows as they are multiplied, one sequence after the other; the plan
+//   k_prompt_heads    every head's keys and values of them, a matrix product
+//   k_prompt_attend   the attention, its work cut into equal shares over the card
+//   k_prompt_merge    joins the shares of a query tile that was cut
+//
+// Operands are kept as the 32x32x16 matrix instruction takes them: a fragment is 1 KB, 16 bytes a
+// lane, so that every load is linear, in memory and in LDS, and no bank conflicts arise. Lane l of one
+// holds row l % 32 (a token, or an output value) and 8 of 16 values along the sum, those of half
+// l / 32. Sums run over values in any order that both operands share, and a product leaves lane l
+// with rows 8 i + 4 (l / 32) + j, i, j < 4, of column l % 32: the order kept here ("dealt": half
+// h holds values 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3 of 16), so that a product's output is
+// the next one's operand in place: keys and values are stored, and numerators used, without
+// any exchange between lanes.
+
+#include "mkmoe_latent.h"
+
+namespace mkmoe_latent {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kPromptShares = 256;  // equal shares of the attention's work at most, a workgroup each: one a CU
+constexpr int kLeastUnits = 6;      // units of work that a share has, where there is so much
+constexpr int kQRows = 256;         // query rows a tile of queries holds
+constexpr int kKeys = 64;           // cached tokens a tile of keys holds
+constexpr int kFrag = 1024;         // bytes of a fragment
+constexpr int kPromptSeqs = MKMOE_LATENT_MAX_SEQS;
+constexpr int kItemSetup = 4;       // what starting and storing a query tile takes, in tiles of keys
+constexpr float kMoveBy = 8.0f;     // a row's maximum moves where a score passes it by more than 2^kMoveBy
+constexpr float kLog2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
+
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// where each sequence's rows and work are; written by k_prompt_rows, read by the launches behind it
+struct Plan {
+  int32_t at[kPromptSeqs];    // first row of the packed tokens; -1: they do not fit
+  int32_t work[kPromptSeqs];  // first unit of the attention's work
+  int32_t rows;               // packed rows, a multiple of kKeys
+  int32_t total;              // units of work
+  int32_t shares;             // equal shares that it is cut into
+};
+
+struct PromptParams {
+  const uint16_t* qn;
+  const uint16_t* qp;
+  const uint16_t* w;
+  const uint8_t* cache;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* starts;  // NULL: n query tokens a sequence
+  uint16_t* out;
+  float* lse;
+  int32_t* err;
+  Plan* plan;
+  uint8_t* c;      // latent fragments [cap / 32][32][1 KB]
+  uint8_t* pe;     // rope fragments [cap / 32][4][1 KB]
+  uint8_t* k;      // key fragments [heads][cap / 32][8][1 KB]
+  uint8_t* v;      // value fragments [heads][cap / 32][2][4][1 KB]
+  int32_t* odd;    // [heads][cap / 64]: a tile's values are not all finite
+  float* part_o;   // [2 shares][8][4][4][64 lanes][4]
+  float* part_ml;  // [2 shares][256][2]
+  int64_t qn_ts, qn_hs, qp_ts, qp_hs, o_ts, o_hs, table_stride;
+  int64_t cap;     // packed rows that the workspace holds, a multiple of 128
+  int pages, seqs, tokens, heads, n, max_len, page_shift;
+  float scale2;    // |scale| log2(e)
+  uint32_t flip;   // 0x80008000 where scale is negative: the query's signs are turned
+};
+
+// a sequence's query tokens and length, clamped to their bounds
+struct PromptSeq {
+  int t0, n, len;
+  bool bad;  // outside its bounds
+};
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
+  PromptSeq s;
+  const int len = p.lens[b];
+  s.len = min(max(len, 0), p.max_len);
+  s.bad = s.len != len;
+  if (p.starts) {
+    const int a = p.starts[b], e = p.starts[b + 1];
+    s.t0 = min(max(a, 0), p.tokens);
+    const int t1 = min(max(e, s.t0), p.tokens);
+    s.n = t1 - s.t0;
+    s.bad = s.bad || a != s.t0 || e != t1;
+  } else {
+    s.t0 = b * p.n;
+    s.n = p.n;
+  }
+  return s;
+}
+
+// A head's query tiles in order, each of kItemSetup units and one for each tile of keys that its last
+// row sees. Tile i sees past + 256 (i + 1) keys (the last one past + n), past = len - n below 0 where there
+// are more queries than cached tokens: 4 (i + 1) + tiles(past) tiles.
+__device__ __forceinline__ int past_tiles(int past) { return (past + kKeys - 1) >> 6; }  // (rounded up, below 0 too)
+__device__ __forceinline__ int tiles_of(int past, int n, int i) {
+  return max(0, past + min(n, kQRows * (i + 1)) + kKeys - 1) >> 6;
+}
+// units before query tile i, none of those before it the last
+__device__ __forceinline__ int units_before(int past, int i) {
+  const int cp = past_tiles(past), first = cp < 0 ? (-cp) >> 2 : 0;  // the first tile that sees a key
+  int u = i * kItemSetup;
+  if (i > first) u += 2 * (i * (i + 1) - first * (first + 1)) + (i - first) * cp;
+  return u;
+}
+__device__ __forceinline__ int query_tiles(int n) { return (n + kQRows - 1) / kQRows; }
+__device__ __forceinline__ int head_units(int past, int n) {
+  const int last = query_tiles(n) - 1;
+  return units_before(past, last) + kItemSetup + tiles_of(past, n, last);
+}
+
+// ---------------------------------------------------------------- rows
+// the sum of v over the threads before this one of 256, and over all of them
+__device__ __forceinline__ int64_t scan256(int64_t v, int64_t* total, int64_t* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < wave) before += lds[i];
+    all += lds[i];
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// The packed rows, 32 tokens a workgroup and turn: a fragment a wave and turn, its lanes reading 16 bytes (MXFP8: 8
+// codes) of 32 rows each. Every workgroup forms the sequences' places itself; the first one leaves them
+// for the launches behind.
+template <bool MX>
+__global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
+  __shared__ int64_t sums[4];
+  __shared__ int at[kPromptSeqs];
+  __shared__ int upto;  // the end of the last rows that fit
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t rows = 0, work = 0;
+  if (tid == 0) upto = 0;  // (the scan's barriers come before it is used)
+  for (int b0 = 0; b0 < p.seqs; b0 += 256) {
+    const int b = b0 + tid;
+    int need = 0;
+    PromptSeq s{0, 0, 0, false};
+    if (b < p.seqs) {
+      s = prompt_seq(p, b);
+      if (s.bad && blockIdx.x == 0) record(p.err, MKMOE_LATENT_ERR_LENGTH, b);
+      if (s.n > 0) need = (s.len + kKeys - 1) & -kKeys;
+    }
+    int64_t all;
+    const int64_t from = rows + scan256(need, &all, sums);
+    rows += all;
+    const bool fits = need == 0 || from + need <= p.cap;
+    int64_t units = 0;
+    if (b < p.seqs && s.n > 0)
+      units = (int64_t)p.heads * (fits ? head_units(s.len - s.n, s.n) : query_tiles(s.n) * kItemSetup);
+    const int64_t first = work + scan256(units, &all, sums);
+    work += all;
+    if (b < p.seqs) {
+      at[b] = fits ? (int)min(from, p.cap) : (int)p.cap;  // (in order, to be searched)
+      if (fits) atomicMax(&upto, (int)min(from + need, p.cap));
+      if (blockIdx.x == 0) {
+        p.plan->at[b] = fits ? at[b] : -1;
+        p.plan->work[b] = (int)first;
+        if (!fits) record(p.err, MKMOE_LATENT_ERR_CONTEXT, b);
+      }
+    }
+  }
+  __syncthreads();
+  const int end = upto;
+  if (blockIdx.x == 0 && tid == 0) {
+    p.plan->rows = end;
+    p.plan->total = (int)work;
+    p.plan->shares = (int)max((int64_t)1, min((int64_t)kPromptShares, work / kLeastUnits));
+  }
+  const int r = lane & 31, half = lane >> 5;
+  for (int kb = blockIdx.x; kb < end >> 5; kb += gridDim.x) {
+    int lo = 0, hi = p.seqs - 1;  // the last sequence that starts at or before the block
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (at[mid] <= kb * 32) lo = mid; else hi = mid - 1;
+    }
+    const int b = lo, t = kb * 32 - at[b] + r;
+    const int len = min(max(p.lens[b], 0), p.max_len);
+    const uint8_t* src = nullptr;
+    if (t < len) {
+      const int page = p.table[(int64_t)b * p.table_stride + (t >> p.page_shift)];
+      if ((uint32_t)page < (uint32_t)p.pages) {
+        const int64_t row = ((int64_t)page << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+        src = p.cache + row * (MX ? kMxRow : 2 * kRow);
+      } else if (wave == 0 && half == 0) {
+        record(p.err, MKMOE_LATENT_ERR_PAGE, b);
+      }
+    }
+    uint8_t* c = p.c + (int64_t)kb * 32 * kFrag + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int ks = wave * 8 + i;
+      u32x4 v = {0, 0, 0, 0};
+      if (src) {
+        if constexpr (MX) {
+          const u32x2 q = *(const u32x2*)(src + 16 * ks + 8 * half);
+          v = fp8x8(q.x, q.y, e8m0(src[kL + (ks >> 1)]));
+        } else {
+          v = *(const u32x4*)(src + 32 * ks + 16 * half);
+        }
+      }
+      *(u32x4*)(c + ks * kFrag) = v;
+    }
+    u32x4 v = {0, 0, 0, 0};
+    if (src) v = *(const u32x4*)(src + (MX ? kL + kMxScales : 2 * kL) + 32 * wave + 16 * half);
+    *(u32x4*)(p.pe + ((int64_t)kb * 4 + wave) * kFrag + lane * 16) = v;
+  }
+}
+
+// ---------------------------------------------------------------- keys and values of every head
+constexpr int kMTok = 128;  // tokens a product tile, by one head's 256 rows of weights
+constexpr int kMK = 32;     // values along the sum a stage
+constexpr int kMStages = kL / kMK;
+constexpr int kMBytes = (kMTok + 256) * kMK * 2;
+constexpr int kMRing = 3;
+
+// Fragments of keys (A: the weights' rows, B: tokens) or values (A: tokens, B: the weights' rows)
+template <bool V>
+__device__ __forceinline__ void heads_stage(f32x16 (&acc)[2][4], uint32_t c_at, uint32_t w_at, int lane) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    bf16x8 c[2], w[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) c[t] = lds_read<bf16x8>(c_at + t * 2 * kFrag + s * kFrag);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = lane & 31, piece = 2 * s + (lane >> 5);
+      w[j] = lds_read<bf16x8>(w_at + j * 2 * kFrag + (r >> 2) * 256 + (r & 3) * 64 + ((piece ^ ((r >> 2) & 3)) << 4));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) acc[t][j] = V ? mfma32(c[t], w[j], acc[t][j]) : mfma32(w[j], c[t], acc[t][j]);
+  }
+}
+
+// The product of packed rows and kv_b: a tile is 128 tokens by a head's 128 + 128 rows of weights, 64 tokens by
+// 128 values a wave, K or V. Stages of 32 values along the sum through a ring of three in LDS, which runs on into the
+// next tile; two workgroups a CU, so that one's stores run under the other's products.
+template <bool V>  // the wave's part: values or keys
+__device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blocks = (p.plan->rows + kMTok - 1) / kMTok, tiles = blocks * p.heads;
+  const int first = blockIdx.x, step = gridDim.x;
+  const int mine = first < tiles ? (tiles - 1 - first) / step + 1 : 0, stages = mine * kMStages;
+  const int64_t kbs = p.cap / 32;
+
+  auto issue = [&](int g) {
+    if (g >= stages) return;
+    const int tile = first + (g / kMStages) * step, ks = g % kMStages;
+    const int head = tile / blocks, tok = tile - head * blocks;
+    const uint32_t to = lds + (g % kMRing) * kMBytes;
+    // wave w brings the tokens 32 w .. and the weights' rows 64 w ..
+    const uint8_t* c = p.c + ((int64_t)(tok * 4 + wave) * 32 + 2 * ks) * kFrag + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      lds_dma16(c + i * kFrag, __builtin_amdgcn_readfirstlane(to + (wave * 2 + i) * kFrag));
+    const uint16_t* w = p.w + ((int64_t)head * 256 + wave * 64 + (lane >> 2)) * kL + ks * kMK +
+                        8 * ((lane & 3) ^ ((lane >> 4) & 3));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      lds_dma16(w + (int64_t)i * 16 * kL, __builtin_amdgcn_readfirstlane(to + (8 + wave * 4 + i) * kFrag));
+  };
+
+  const int tg = wave & 1;
+  issue(0);
+  issue(1);
+  f32x16 acc[2][4];
+  for (int g = 0; g < stages; ++g) {
+    const int ks = g % kMStages;
+    if (ks == 0) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[t][j] = f32x16{};
+    }
+    if (g + 1 < stages)
+      wait_loads<6>();
+    else
+      wait_loads<0>();
+    barrier();
+    issue(g + 2);
+    const uint32_t at = lds + (g % kMRing) * kMBytes;
+    const uint32_t c_at = at + tg * 4 * kFrag + lane * 16, w_at = at + 8 * kFrag + (V ? 8 : 0) * kFrag;
+    heads_stage<V>(acc, c_at, w_at, lane);
+    if (ks == kMStages - 1) {
+      const int tile = first + (g / kMStages) * step;
+      const int head = tile / blocks, tok = tile - head * blocks;
+      const int64_t kb = (int64_t)head * kbs + tok * 4 + tg * 2;
+      uint32_t top = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[e] = pack_bf(acc[t][j][8 * u + 2 * e], acc[t][j][8 * u + 2 * e + 1]);
+              top = max(top, max(o[e] << 16 & 0x7fff0000u, o[e] & 0x7fff0000u));
+            }
+            uint8_t* to = (V ? p.v : p.k) + ((kb + t) * 8 + (V ? u * 4 + j : 2 * j + u)) * kFrag + lane * 16;
+            *(u32x4*)to = u32x4{o[0], o[1], o[2], o[3]};
+          }
+      if constexpr (V) {
+        const bool odd = __ballot(top >= 0x7f800000u) != 0;
+        if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + tok * 2 + tg] = odd;
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256, 2) void k_prompt_heads(PromptParams p) {
+  __shared__ __align__(1024) uint8_t ring[kMRing][kMBytes];
+  const uint32_t lds = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)&ring[0][0];
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= 2)
+    heads_loop<true>(p, lds);
+  else
+    heads_loop<false>(p, lds);
+}
+
+// ---------------------------------------------------------------- attend
+constexpr int kTileKB = 40;  // fragments of a tile of keys: 16 of keys, 8 of rope keys, 16 of values
+constexpr int kTileLds = kTileKB * kFrag;
+constexpr int kTileRing = 3;
+constexpr int kKeyAt = 0, kPeAt = 16 * kFrag, kValAt = 24 * kFrag;
+
+struct Item {
+  int b, head, qt;     // a sequence's head's query tile
+  int t0, n, past;     // the sequence's
+  int at;              // its packed rows; -1: none
+  int first, tiles;    // its first unit of work; tiles of keys
+};
+// the item that has unit u of the work
+__device__ __forceinline__ Item item_at(const PromptParams& p, int u) {
+  Item it;
+  int lo = 0, hi = p.seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.plan->work[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  it.b = lo;
+  const PromptSeq s = prompt_seq(p, lo);
+  it.t0 = s.t0;
+  it.n = s.n;
+  it.past = s.len - s.n;
+  it.at = p.plan->at[lo];
+  const int base = p.plan->work[lo];
+  int x = u - base;
+  if (it.at < 0) {  // it did not fit: no keys
+    it.tiles = 0;
+    const int qts = query_tiles(s.n), i = x / kItemSetup;
+    it.head = i / qts;
+    it.qt = i - it.head * qts;
+    it.first = base + i * kItemSetup;
+    return it;
+  }
+  const int per = head_units(it.past, it.n);
+  it.head = x / per;
+  x -= it.head * per;
+  int a = 0, z = query_tiles(it.n) - 1;
+  while (a < z) {
+    const int mid = (a + z + 1) >> 1;
+    if (units_before(it.past, mid) <= x) a = mid; else z = mid - 1;
+  }
+  it.qt = a;
+  it.first = base + it.head * per + units_before(it.past, a);
+  it.tiles = tiles_of(it.past, it.n, a);
+  return it;
+}
+__device__ __forceinline__ int share_start(int total, int shares, int s) { return (int)((int64_t)total * s / shares); }
+
+// a query row's values, its running maximum (of scores times log2 e) and sum
+__device__ __forceinline__ void store_row(const PromptParams& p, const Item& it, int row, f32x16 o, int vb, float inv,
+                                          int half) {
+  if (row >= it.n) return;
+  uint16_t* to = p.out + (int64_t)(it.t0 + row) * p.o_ts + (int64_t)it.head * p.o_hs + 32 * vb + 4 * half;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4)
+    *(u32x2*)(to + 2 * i) = u32x2{pack_bf(o[i] * inv, o[i + 1] * inv), pack_bf(o[i + 2] * inv, o[i + 3] * inv)};
+}
+
+__global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
+  __shared__ __align__(1024) uint8_t ring[kTileRing][kTileLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const uint32_t lds = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)&ring[0][0];
+  // an XCD's workgroups have shares that follow each other: heads whose keys its L2 keeps
+  const int total = p.plan->total, shares = p.plan->shares;
+  const int share = shares == kPromptShares ? (blockIdx.x & 7) * (kPromptShares / 8) + (blockIdx.x >> 3) : blockIdx.x;
+  if (share >= shares) return;
+  int u = share_start(total, shares, share);
+  const int end = share_start(total, shares, share + 1);
+  const int64_t kbs = p.cap / 32;
+
+  while (u < end) {
+    const Item it = item_at(p, __builtin_amdgcn_readfirstlane(u));
+    const int head = __builtin_amdgcn_readfirstlane(it.head), tiles = __builtin_amdgcn_readfirstlane(it.tiles);
+    const int item_end = it.first + kItemSetup + tiles;
+    const int from = __builtin_amdgcn_readfirstlane(max(0, u - it.first - kItemSetup));
+    const int upto = __builtin_amdgcn_readfirstlane(max(0, min(end, item_end) - it.first - kItemSetup));
+    const bool head_of_item = u == it.first;
+    u = item_end;
+    const int row0 = it.qt * kQRows + wave * 32, row = row0 + col;
+    if (tiles == 0) {
+      if (head_of_item && row < it.n) {
+        const float none = it.at < 0 ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+        for (int vb = 0; vb < 4; ++vb) store_row(p, it, row, f32x16{} + none, vb, 1.0f, half);
+        if (p.lse && half == 0) p.lse[(int64_t)(it.t0 + row) * p.heads + head] = it.at < 0 ? none : -__builtin_inff();
+      }
+      continue;
+    }
+    if (from == upto) continue;
+
+    const int64_t kb0 = it.at / 32;
+    const uint8_t* kbase = p.k + ((int64_t)head * kbs + kb0) * 8 * kFrag;
+    const uint8_t* vbase = p.v + ((int64_t)head * kbs + kb0) * 8 * kFrag;
+    const uint8_t* pbase = p.pe + kb0 * 4 * kFrag;
+    auto issue = [&](int kt) {
+      const uint32_t to = lds + (kt % kTileRing) * kTileLds;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int f = wave * 2 + i;
+        lds_dma16(kbase + (int64_t)kt * 16 * kFrag + f * kFrag + lane * 16, __builtin_amdgcn_readfirstlane(to + kKeyAt + f * kFrag));
+        lds_dma16(vbase + (int64_t)kt * 16 * kFrag + f * kFrag + lane * 16, __builtin_amdgcn_readfirstlane(to + kValAt + f * kFrag));
+      }
+      lds_dma16(pbase + (int64_t)kt * 8 * kFrag + wave * kFrag + lane * 16, __builtin_amdgcn_readfirstlane(to + kPeAt + wave * kFrag));
+    };
+
+    // the query: 8 fragments of its values without rotation, dealt, and 4 of the rotated ones
+    bf16x8 q[12];
+    {
+      const bool there = row < it.n;
+      const uint16_t* qn = p.qn + (int64_t)(it.t0 + row) * p.qn_ts + (int64_t)head * p.qn_hs;
+      const uint16_t* qp = p.qp + (int64_t)(it.t0 + row) * p.qp_ts + (int64_t)head * p.qp_hs;
+#pragma unroll
+      for (int ds = 0; ds < 8; ++ds) {
+        u32x2 a = {0, 0}, b = {0, 0};
+        if (there) {
+          a = *(const u32x2*)(qn + 16 * ds + 4 * half);
+          b = *(const u32x2*)(qn + 16 * ds + 4 * half + 8);
+        }
+        q[ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, b.x ^ p.flip, b.y ^ p.flip});
+      }
+#pragma unroll
+      for (int ds = 0; ds < 4; ++ds) {
+        u32x4 a = {0, 0, 0, 0};
+        if (there) a = *(const u32x4*)(qp + 16 * ds + 8 * half);
+        q[8 + ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, a.z ^ p.flip, a.w ^ p.flip});
+      }
+    }
+    wait_all();
+    barrier();  // every wave has read the tiles of the item before
+    issue(from);
+    if (from + 1 < upto) issue(from + 1);
+
+    f32x16 o[4] = {};
+    float m = -__builtin_inff(), mu = 0.0f, sum = 0.0f;  // mu: m, or 0 where no score was seen
+    const int sees = it.past + row;                      // the last key that the row sees
+    const int wave_sees = it.past + min(row0 + 31, it.n - 1);
+    for (int kt = from; kt < upto; ++kt) {
+      if (kt + 1 < upto)
+        wait_loads<5>();
+      else
+        wait_loads<0>();
+      barrier();
+      if (kt + 2 < upto) issue(kt + 2);
+      const int key0 = kt * kKeys;
+      if (row0 >= it.n || key0 > wave_sees) continue;
+      const uint32_t at = lds + (kt % kTileRing) * kTileLds + lane * 16;
+      f32x16 s[2] = {};
+#pragma unroll
+      for (int ds = 0; ds < 12; ++ds)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const uint32_t f = ds < 8 ? kKeyAt + (kb * 8 + ds) * kFrag : kPeAt + (kb * 4 + ds - 8) * kFrag;
+          s[kb] = mfma32(lds_read<bf16x8>(at + f), q[ds], s[kb]);
+        }
+      const bool masked = key0 + kKeys - 1 > it.past + row0;
+      if (masked) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3) > sees) s[kb][i] = -__builtin_inff();
+      }
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+      const auto sw = __builtin_amdgcn_permlane32_swap(f2u(top), f2u(top), false, false);
+      top = fmaxf(u2f(sw[0]), u2f(sw[1])) * p.scale2;
+      if (__ballot(top > m + kMoveBy)) {
+        const float to = fmaxf(m, top), by = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        mu = to == -__builtin_inff() ? 0.0f : to;
+        sum *= by;
+#pragma unroll
+        for (int vb = 0; vb < 4; ++vb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[vb][i] *= by;
+      }
+      bf16x8 num[2][2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = __builtin_amdgcn_exp2f(s[kb][8 * t + 2 * e] * p.scale2 - mu);
+            const float b = __builtin_amdgcn_exp2f(s[kb][8 * t + 2 * e + 1] * p.scale2 - mu);
+            sum += a + b;
+            w[e] = pack_bf(a, b);
+          }
+          num[kb][t] = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
+        }
+      if (masked && p.odd[(int64_t)head * (p.cap / kKeys) + it.at / kKeys + kt]) {
+        // values that are not finite, of tokens that some rows do not see: a key at a time, added where it is seen
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll 1
+          for (int x = 0; x < 16; ++x) {
+            const int h = x >> 3, e = x & 7;
+            const bool seen = key0 + 16 * g + 8 * (e >> 2) + 4 * h + (e & 3) <= sees;
+            const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+            const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
+            const bf16x8 one = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, num[g >> 1][g & 1]) & only);
+#pragma unroll
+            for (int vb = 0; vb < 4; ++vb) {
+              const u32x4 a = lds_read<u32x4>(at + kValAt + (g * 4 + vb) * kFrag);
+              const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[vb][i] += seen ? add[i] : 0.0f;
+            }
+          }
+        continue;
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int vb = 0; vb < 4; ++vb)
+            o[vb] = mfma32(lds_read<bf16x8>(at + kValAt + (kb * 8 + t * 4 + vb) * kFrag), num[kb][t], o[vb]);
+    }
+    const auto sw = __builtin_amdgcn_permlane32_swap(f2u(sum), f2u(sum), false, false);
+    sum = u2f(sw[0]) + u2f(sw[1]);
+    if (from == 0 && upto == tiles) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int vb = 0; vb < 4; ++vb) store_row(p, it, row, o[vb], vb, inv, half);
+      if (p.lse && half == 0 && row < it.n)
+        p.lse[(int64_t)(it.t0 + row) * p.heads + head] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * kLog2;
+    } else {
+      const int slot = 2 * share + (from == 0);
+      f32x4* to = (f32x4*)p.part_o + ((int64_t)slot * 8 + wave) * 16 * 64 + lane;
+#pragma unroll
+      for (int vb = 0; vb < 4; ++vb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          to[(vb * 4 + i) * 64] = f32x4{o[vb][4 * i], o[vb][4 * i + 1], o[vb][4 * i + 2], o[vb][4 * i + 3]};
+      if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * kQRows + wave * 32 + col) * 2) = f32x2{m, sum};
+    }
+  }
+}
+
+// The parts of a query tile whose first share ends inside it, joined in order: (share, 32 rows) a workgroup, 32 values a
+// wave. The lanes have the values that the attention's had.
+__global__ __launch_bounds__(256) void k_prompt_merge(PromptParams p) {
+  const int lane = threadIdx.x & 63, vb = threadIdx.x >> 6, share = blockIdx.x, group = blockIdx.y;
+  const int half = lane >> 5, col = lane & 31, total = p.plan->total,
+            shares = p.plan->shares;
+  if (share + 1 >= shares) return;
+  const int start = share_start(total, shares, share), end = share_start(total, shares, share + 1);
+  if (start == end) return;
+  const Item it = item_at(p, end);
+  const int keys = it.first + kItemSetup, item_end = keys + it.tiles;
+  // the tile's first keys are this share's, and not all of them
+  if (it.tiles == 0 || end <= keys || start > keys) return;
+  const int row = it.qt * kQRows + group * 32 + col;
+  if (it.qt * kQRows + group * 32 >= it.n) return;
+  float top = -__builtin_inff();
+  int last = share;
+  while (last + 1 < shares && share_start(total, shares, last + 1) < item_end) ++last;
+  for (int s = share; s <= last; ++s)
+    top = fmaxf(top, p.part_ml[((int64_t)(2 * s + (s == share)) * kQRows + group * 32 + col) * 2]);
+  f32x16 o = {};
+  float sum = 0.0f;
+  for (int s = share; s <= last; ++s) {
+    const int slot = 2 * s + (s == share);
+    const f32x2 ml = *(const f32x2*)(p.part_ml + ((int64_t)slot * kQRows + group * 32 + col) * 2);
+    const float by = ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - top);
+    sum += ml[1] * by;
+    const f32x4* from = (const f32x4*)p.part_o + ((int64_t)slot * 8 + group) * 16 * 64 + vb * 4 * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 x = from[i * 64];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[4 * i + j] += x[j] * by;
+    }
+  }
+  store_row(p, it, row, o, vb, sum == 0.0f ? 0.0f : 1.0f / sum, half);
+  if (p.lse && vb == 0 && half == 0 && row < it.n)
+    p.lse[(int64_t)(it.t0 + row) * p.heads + it.head] = sum == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLog2;
+}
+
+// ---------------------------------------------------------------- host
+// a workspace: the latent calls' own first (its error words serve both), then the prompt's
+struct PromptLayout {
+  size_t plan, part_ml, part_o, odd, pe, c, k, v, bytes;
+};
+inline PromptLayout prompt_layout(int heads, int64_t cap) {
+  PromptLayout l;
+  size_t at = 0;
+  (void)mkmoe_latent_workspace_bytes(&at);
+  auto take = [&](size_t n) {
+    const size_t from = at;
+    at += (n + 255) & ~(size_t)255;
+    return from;
+  };
+  l.plan = take(sizeof(Plan));
+  l.part_ml = take((size_t)2 * kPromptShares * kQRows * 2 * 4);
+  l.part_o = take((size_t)2 * kPromptShares * kQRows * kV * 4);
+  l.odd = take((size_t)heads * (cap / kKeys) * 4);
+  l.pe = take((size_t)cap * kR * 2);
+  l.c = take((size_t)cap * kL * 2);
+  l.k = take((size_t)heads * cap * kNope * 2);
+  l.v = take((size_t)heads * cap * kV * 2);
+  l.bytes = at;
+  return l;
+}
+constexpr int kMaxContext = 1 << 22, kMaxPromptTokens = 1 << 20;
+inline int64_t packed_rows(int32_t context) { return ((int64_t)context + kMTok - 1) & -(int64_t)kMTok; }
+
+inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_bytes, PromptParams& p) {
+  if (!io || !ws) return MKMOE_ERR_NULL;
+  if (!aligned(ws, 256)) return MKMOE_ERR_ALIGN;
+  if (int rc = check_cache(io->cache)) return rc;
+  if (!io->q_nope || !io->q_pe || !io->w || !io->table || !io->lens || !io->out) return MKMOE_ERR_NULL;
+  if (io->seqs < 1 || io->seqs > kPromptSeqs || io->tokens < 0 || io->tokens > kMaxPromptTokens) return MKMOE_ERR_ROWS;
+  if (!io->q_starts && io->tokens % io->seqs != 0) return MKMOE_ERR_ROWS;
+  if (io->heads < 1 || io->heads > MKMOE_LATENT_MAX_HEADS || io->max_context < 1 || io->max_context > kMaxContext)
+    return MKMOE_ERR_ARG;
+  const int64_t cap = packed_rows(io->max_context);
+  const PromptLayout l = prompt_layout(io->heads, cap);
+  if (ws_bytes < l.bytes) return MKMOE_ERR_WORKSPACE;
+  const float scale2 = fabsf(io->scale) * kLog2E;
+  if (!isfinite(scale2) || io->max_pages < 1 || io->table_stride < io->max_pages) return MKMOE_ERR_ARG;
+  const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
+  if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
+  // the work's units are counted in 32 bits
+  const int64_t keys = (max_len < cap ? max_len : cap) / kKeys + 1 + kItemSetup;
+  if (((int64_t)io->tokens / kQRows + io->seqs) * io->heads * keys > 0x3fffffff) return MKMOE_ERR_ARG;
+  const void* wide[] = {io->q_nope, io->q_pe, io->w, io->out};
+  for (const void* q : wide)
+    if (!aligned(q, 16)) return MKMOE_ERR_ALIGN;
+  const void* narrow[] = {io->table, io->lens, io->q_starts, io->lse};
+  for (const void* q : narrow)
+    if (!aligned(q, 4)) return MKMOE_ERR_ALIGN;
+  if (!strides8(io->qn_token_stride, io->qn_head_stride) || !strides8(io->qp_token_stride, io->qp_head_stride) ||
+      !strides8(io->out_token_stride, io->out_head_stride))
+    return MKMOE_ERR_ALIGN;
+  if (!rows_apart(io->out_token_stride, io->tokens, io->out_head_stride, io->heads, kV)) return MKMOE_ERR_ARG;
+  uint8_t* at = (uint8_t*)ws;
+  p.qn = (const uint16_t*)io->q_nope;
+  p.qp = (const uint16_t*)io->q_pe;
+  p.w = (const uint16_t*)io->w;
+  p.cache = (const uint8_t*)io->cache.data;
+  p.table = io->table;
+  p.lens = io->lens;
+  p.starts = io->q_starts;
+  p.out = (uint16_t*)io->out;
+  p.lse = io->lse;
+  p.err = (int32_t*)at;
+  p.plan = (Plan*)(at + l.plan);
+  p.part_ml = (float*)(at + l.part_ml);
+  p.part_o = (float*)(at + l.part_o);
+  p.odd = (int32_t*)(at + l.odd);
+  p.pe = at + l.pe;
+  p.c = at + l.c;
+  p.k = at + l.k;
+  p.v = at + l.v;
+  p.qn_ts = io->qn_token_stride;
+  p.qn_hs = io->qn_head_stride;
+  p.qp_ts = io->qp_token_stride;
+  p.qp_hs = io->qp_head_stride;
+  p.o_ts = io->out_token_stride;
+  p.o_hs = io->out_head_stride;
+  p.table_stride = io->table_stride;
+  p.cap = cap;
+  p.pages = (int)io->cache.pages;
+  p.seqs = io->seqs;
+  p.tokens = io->tokens;
+  p.heads = io->heads;
+  p.n = io->q_starts ? 0 : io->tokens / io->seqs;
+  p.max_len = (int)max_len;
+  p.page_shift = __builtin_ctz((unsigned)io->cache.page_size);
+  // (a scale of 0 weighs every visible token alike; the masked ones' infinities need a factor above 0)
+  p.scale2 = fmaxf(scale2, 0x1p-126f);
+  p.flip = io->scale < 0.0f ? 0x80008000u : 0u;
+  return MKMOE_OK;
+}
+
+inline int prompt_launch(const PromptParams& p, bool mx, hipStream_t st) {
+  const int64_t rows = p.cap < (int64_t)p.seqs * p.max_len ? p.cap : (int64_t)p.seqs * p.max_len;
+  const int64_t blocks = (rows + 31) / 32 + p.seqs;
+  const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024));
+  if (mx)
+    hipLaunchKernelGGL(k_prompt_rows<true>, grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL(k_prompt_rows<false>, grid, dim3(256), 0, st, p);
+  if (int rc = launched()) return rc;
+  hipLaunchKernelGGL(k_prompt_heads, dim3(2 * kPromptShares), dim3(256), 0, st, p);
+  if (int rc = launched()) return rc;
+  hipLaunchKernelGGL(k_prompt_attend, dim3(kPromptShares), dim3(512), 0, st, p);
+  if (int rc = launched()) return rc;
+  hipLaunchKernelGGL(k_prompt_merge, dim3(kPromptShares, kQRows / 32), dim3(256), 0, st, p);
+  return launched();
+}
+
+}  // namespace mkmoe_latent
+
+extern "C" {
+
+int mkmoe_latent_prompt_bytes(int32_t heads, int32_t max_context, size_t* bytes) {
+  using namespace mkmoe_latent;
+  if (!bytes) return MKMOE_ERR_NULL;
+  if (heads < 1 || heads > MKMOE_LATENT_MAX_HEADS || max_context < 1 || max_context > kMaxContext) return MKMOE_ERR_ARG;
+  *bytes = prompt_layout(heads, packed_rows(max_context)).bytes;
+  return MKMOE_OK;
+}
+
+int mkmoe_latent_prompt(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_bytes, void* stream) {
+  using namespace mkmoe_latent;
+  PromptParams p;
+  if (int rc = prompt_params(io, ws, ws_bytes, p)) return rc;
+  if (p.tokens == 0) return MKMOE_OK;
+  return prompt_launch(p, io->cache.fmt == MKMOE_LATENT_MXFP8, (hipStream_t)stream);
+}
+
+int mkmoe_latent_prompt_step(const mkmoe_latent_append_io* append, const mkmoe_latent_prompt_io* io, void* ws,
+                             size_t ws_bytes, void* stream) {
+  using namespace mkmoe_latent;
+  PromptParams p;
+  if (int rc = prompt_params(io, ws, ws_bytes, p)) return rc;
+  if (!append) return MKMOE_ERR_NULL;
+  if (append->tokens != io->tokens) return MKMOE_ERR_ROWS;
+  const mkmoe_latent_cache &from = append->cache, &to = io->cache;
+  if ((append->heads != 0 && append->heads != io->heads) || from.data != to.data || from.pages != to.pages ||
+      from.page_size != to.page_size || from.fmt != to.fmt)
+    return MKMOE_ERR_ARG;
+  // (it checks its own arguments before it launches)
+  if (int rc = append_for_step(append, ws, ws_bytes, (hipStream_t)stream)) return rc;
+  if (p.tokens == 0) return MKMOE_OK;
+  return prompt_launch(p, io->cache.fmt == MKMOE_LATENT_MXFP8, (hipStream_t)stream);
+}
+
+}  // extern "C"

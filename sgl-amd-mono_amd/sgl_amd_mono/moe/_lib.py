@@ -59,11 +59,13 @@ LATENT_DIM, LATENT_ROPE, LATENT_NOPE, LATENT_V, LATENT_MX_ROW = 512, 64, 128, 12
 LATENT_MAX_HEADS, LATENT_MAX_SEQS = 128, 512
 LATENT_BF16, LATENT_MXFP8 = 1, 2
 LATENT_ERRW_WORDS = 4
+LATENT_MAX_CONTEXT, LATENT_MAX_PROMPT = 1 << 22, 1 << 20
 LATENT_ERRORS = {
     1: "a slot outside the cache, at token",
     2: "a position outside cos_sin, at token",
     3: "a length or query start outside its bounds, at sequence",
     4: "a page outside the cache, at sequence",
+    5: "cached tokens past max_context, at sequence",
 }
 
 # every symbol include/mkmoe.h and include/mkmoe_seam.h declare
@@ -88,6 +90,9 @@ EXPORTS = (
     "mkmoe_latent_attend",
     "mkmoe_latent_project",
     "mkmoe_latent_step",
+    "mkmoe_latent_prompt_bytes",
+    "mkmoe_latent_prompt",
+    "mkmoe_latent_prompt_step",
     "mkmoe_latent_read_errors",
 )
 # every symbol include/mkmoe_testing.h declares (libmkmoe_testing.so)
@@ -220,6 +225,24 @@ class LatentProjectIO(ctypes.Structure):
     )
 
 
+class LatentPromptIO(ctypes.Structure):
+    """mkmoe_latent_prompt_io of include/mkmoe.h."""
+
+    _fields_ = (
+        [("cache", LatentCache)]
+        + [(n, ctypes.c_int32) for n in ("seqs", "tokens", "heads", "max_pages", "max_context", "pad")]
+        + [
+            (n, ctypes.c_int64)
+            for n in (
+                "table_stride", "qn_token_stride", "qn_head_stride", "qp_token_stride", "qp_head_stride",
+                "out_token_stride", "out_head_stride",
+            )
+        ]
+        + [(n, ctypes.c_void_p) for n in ("q_nope", "q_pe", "w", "table", "lens", "q_starts", "out", "lse")]
+        + [("scale", ctypes.c_float), ("pad2", ctypes.c_int32)]
+    )  # fmt: skip
+
+
 def packer(cls) -> struct.Struct:
     """Writes every field of a structure in one call (``pack_into(structure, 0, ...)``): a quarter
     of the time that the fields take one by one. A null pointer is 0."""
@@ -231,7 +254,9 @@ def packer(cls) -> struct.Struct:
     return s
 
 
-LATENT_APPEND, LATENT_ATTEND, LATENT_PROJECT = (packer(c) for c in (LatentAppendIO, LatentAttendIO, LatentProjectIO))
+LATENT_APPEND, LATENT_ATTEND, LATENT_PROJECT, LATENT_PROMPT = (
+    packer(c) for c in (LatentAppendIO, LatentAttendIO, LatentProjectIO, LatentPromptIO)
+)
 
 
 SEAM_HC = 4
@@ -288,6 +313,9 @@ def lib() -> ctypes.CDLL:
         L.mkmoe_latent_step.argtypes = [
             ctypes.POINTER(c) for c in (LatentAppendIO, LatentProjectIO, LatentAttendIO, LatentProjectIO)
         ] + [vp, sz, vp]
+        L.mkmoe_latent_prompt_bytes.argtypes = [i32, i32, ctypes.POINTER(sz)]
+        L.mkmoe_latent_prompt.argtypes = [ctypes.POINTER(LatentPromptIO), vp, sz, vp]
+        L.mkmoe_latent_prompt_step.argtypes = [ctypes.POINTER(c) for c in (LatentAppendIO, LatentPromptIO)] + [vp, sz, vp]
         L.mkmoe_latent_read_errors.argtypes = [vp, ctypes.POINTER(i32), i32, vp]
         if L.mkmoe_abi_version() != ABI_VERSION:
             raise RuntimeError(

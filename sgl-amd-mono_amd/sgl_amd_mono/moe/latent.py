@@ -65,17 +65,11 @@ class LatentWeights:
                 )
 
 
-class LatentRunner:
-    """Latent attention of one rank's ``heads`` on one GPU: a workspace and the calls.
+class _LatentCalls:
+    """What the latent runners share: one rank's heads on one GPU, a workspace whose first words record errors,
+    the checks of arguments, and the calls that store cache rows and give them back."""
 
-    ``max_tokens``: query tokens that ``attention`` takes at most (its intermediates' size; the
-    other calls have no such bound). ``scale``: of the scores (default 192^-0.5; a model whose rope
-    is scaled has another: DeepSeek-V3's is that times (0.1 ln 40 + 1)^2 = 1.874). ``rope``:
-    "interleaved" (pairs (2 i, 2 i + 1)) or "half" ((i, i + 32)). One runner serves one stream at
-    a time: calls that can overlap need runners of their own."""
-
-    def __init__(self, heads: int, device=None, max_tokens: int = 48, scale: float | None = None,
-                 norm_eps: float = 1e-6, rope: str = "interleaved"):  # fmt: skip
+    def __init__(self, heads: int, device, scale: float | None, norm_eps: float, rope: str):
         if not 1 <= heads <= _lib.LATENT_MAX_HEADS:
             raise RuntimeError(f"mkmoe latent: {heads} heads, want 1 .. {_lib.LATENT_MAX_HEADS}")
         if rope not in ROPES:
@@ -84,7 +78,6 @@ class LatentRunner:
         if dev.type != "cuda":
             raise RuntimeError(f"mkmoe latent: {dev} is not a GPU")
         self.heads = int(heads)
-        self.max_tokens = int(max_tokens)
         self.scale = (NOPE + ROPE) ** -0.5 if scale is None else float(scale)
         self.norm_eps = float(norm_eps)
         f32 = lambda v: ctypes.c_float(v).value  # noqa: E731  (what the library is given)
@@ -92,21 +85,21 @@ class LatentRunner:
             raise RuntimeError(f"mkmoe latent: scale {self.scale}, norm_eps {self.norm_eps}")
         self.rope = ROPES[rope]
         self.lib = _lib.lib()
-        n = ctypes.c_size_t()
-        _lib.check(self.lib.mkmoe_latent_workspace_bytes(ctypes.byref(n)), "latent workspace size")
-        self.device = torch.device("cuda", torch.cuda.current_device() if dev.index is None else dev.index)
+        self.device = dev
+        self._append_io = _lib.LatentAppendIO()
+
+    def _take_workspace(self, nbytes: int, *tensors: tuple) -> list:
+        """The workspace and further tensors, (dtype, shape) each, on this runner's GPU."""
+        self.device = torch.device("cuda", torch.cuda.current_device() if self.device.index is None else self.device.index)
         no_capture("the latent workspace")
         with torch.cuda.device(self.device):
-            self.ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+            self.ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             self.clear_errors()
-            mk = lambda w, t: torch.empty(self.max_tokens, self.heads, w, dtype=t, device=self.device)  # noqa: E731
-            # (the attended latents stay in fp32: one rounding less before the output's own)
-            self._q_lat, self._q_pe, self._o_lat = mk(LATENT, BF), mk(ROPE, BF), mk(LATENT, torch.float32)
+            out = [torch.empty(shape, dtype=t, device=self.device) for t, shape in tensors]
             torch.cuda.current_stream().synchronize()  # whichever stream comes first finds them cleared
         self._index = self.device.index
-        self._append_io, self._attend_io = _lib.LatentAppendIO(), _lib.LatentAttendIO()
-        self._absorb_io, self._expand_io = _lib.LatentProjectIO(), _lib.LatentProjectIO()
         self._ws = (self.ws.data_ptr(), self.ws.numel())
+        return out
 
     # ---- argument checks
     def _bad(self, name: str, t, want: str):
@@ -154,6 +147,32 @@ class LatentRunner:
                 return t.data_ptr(), pages, page, _lib.LATENT_MXFP8
         raise self._bad("cache", t, f"[pages, page_size, {ROW}] {BF} or [pages, page_size, {MX_ROW}] torch.uint8 contiguous")
 
+    def _batch(self, tokens: int, table, lens, q_starts) -> tuple:
+        """(sequences, table entries of one, table stride, pointers of the table, lengths and query starts)."""
+        shape = () if table is None else table.shape
+        if len(shape) != 2 or table.dtype is not torch.int32 or table.get_device() != self._index:
+            raise self._bad("table", table, "[seqs, max_pages] torch.int32")
+        (seqs, max_pages), (stride, last) = shape, table.stride()
+        if last != 1 and max_pages > 1:
+            raise self._bad("table", table, "[seqs, max_pages] torch.int32, the pages of a sequence contiguous")
+        if seqs <= 1:
+            stride = max_pages
+        at_lens = self._vec("lens", lens, seqs, torch.int32)
+        at_starts = 0 if q_starts is None else self._vec("q_starts", q_starts, seqs + 1, torch.int32)
+        if not 1 <= seqs <= _lib.LATENT_MAX_SEQS or (q_starts is None and tokens % seqs):
+            raise RuntimeError(
+                f"mkmoe latent: {seqs} sequences of {tokens} query tokens, want 1 .. {_lib.LATENT_MAX_SEQS} sequences "
+                "and, without q_starts, as many tokens in each"
+            )
+        return seqs, max_pages, stride, table.data_ptr(), at_lens, at_starts
+
+    def _lse(self, t, tokens: int) -> int:
+        if t is None:
+            return 0
+        if t.dtype != torch.float32 or t.shape != (tokens, self.heads) or t.device != self.device or not t.is_contiguous():
+            raise self._bad("lse", t, f"[{tokens}, {self.heads}] torch.float32 contiguous")
+        return t.data_ptr()
+
     def _new(self, what: str, *shape, zeros: bool = False) -> torch.Tensor:
         """An output of the call's own. ``zeros``: the call may leave rows of it unwritten."""
         no_capture(what)
@@ -196,32 +215,6 @@ class LatentRunner:
             q[1], q[2], q_out[1], q_out[2], at, w, cos_sin.data_ptr(), pos, slot, q[0], q_out[0], self.norm_eps, nan,
         )  # fmt: skip
         return tokens
-
-    def _set_attend(self, cache, tokens: int, q_lat: tuple, q_pe: tuple, table, lens, q_starts, out: tuple,
-                    f32: int, lse: int) -> None:  # fmt: skip
-        c = self._cache(cache)
-        shape = () if table is None else table.shape
-        if len(shape) != 2 or table.dtype is not torch.int32 or table.get_device() != self._index:
-            raise self._bad("table", table, "[seqs, max_pages] torch.int32")
-        (seqs, max_pages), (stride, last) = shape, table.stride()
-        if last != 1 and max_pages > 1:
-            raise self._bad("table", table, "[seqs, max_pages] torch.int32, the pages of a sequence contiguous")
-        if seqs <= 1:
-            stride = max_pages
-        at_lens = self._vec("lens", lens, seqs, torch.int32)
-        at_starts = 0 if q_starts is None else self._vec("q_starts", q_starts, seqs + 1, torch.int32)
-        if not 1 <= seqs <= _lib.LATENT_MAX_SEQS or (q_starts is None and tokens % seqs):
-            raise RuntimeError(
-                f"mkmoe latent: {seqs} sequences of {tokens} query tokens, want 1 .. {_lib.LATENT_MAX_SEQS} sequences "
-                "and, without q_starts, as many tokens in each"
-            )
-        _lib.LATENT_ATTEND.pack_into(
-            self._attend_io, 0, *c, seqs, tokens, self.heads, max_pages, stride, q_lat[1], q_lat[2], q_pe[1], q_pe[2],
-            out[1], out[2], q_lat[0], q_pe[0], table.data_ptr(), at_lens, at_starts, out[0], lse, self.scale, f32,
-        )  # fmt: skip
-
-    def _set_project(self, io, tokens: int, expand: int, f32: int, x: tuple, w: int, y: tuple) -> None:
-        _lib.LATENT_PROJECT.pack_into(io, 0, tokens, self.heads, expand, f32, x[1], x[2], y[1], y[2], x[0], w, y[0])
 
     # ---- the calls
     def append(
@@ -274,6 +267,61 @@ class LatentRunner:
             )
         return out
 
+    # ---- device errors
+    def read_errors(self) -> list[int]:
+        """The device error words (synchronises the stream)."""
+        words = (ctypes.c_int32 * _lib.LATENT_ERRW_WORDS)()
+        self._call(self.lib.mkmoe_latent_read_errors, self._ws[0], words, _lib.LATENT_ERRW_WORDS)
+        return list(words)
+
+    def raise_on_device_error(self) -> None:
+        """Raise if a call since the last ``clear_errors`` met a slot, position, length, query start
+        or page outside its bounds (synchronises the stream)."""
+        code, where, count, _ = self.read_errors()
+        if code:
+            raise RuntimeError(f"mkmoe latent: {_lib.LATENT_ERRORS.get(code, code)} {where} ({count} seen)")
+
+    def clear_errors(self) -> None:
+        """Forget recorded errors (on the current stream)."""
+        self.ws[: 4 * _lib.LATENT_ERRW_WORDS].zero_()
+
+
+class LatentRunner(_LatentCalls):
+    """Latent attention of one rank's ``heads`` on one GPU: a workspace and the calls.
+
+    ``max_tokens``: query tokens that ``attention`` takes at most (its intermediates' size; the
+    other calls have no such bound). ``scale``: of the scores (default 192^-0.5; a model whose rope
+    is scaled has another: DeepSeek-V3's is that times (0.1 ln 40 + 1)^2 = 1.874). ``rope``:
+    "interleaved" (pairs (2 i, 2 i + 1)) or "half" ((i, i + 32)). One runner serves one stream at
+    a time: calls that can overlap need runners of their own."""
+
+    def __init__(self, heads: int, device=None, max_tokens: int = 48, scale: float | None = None,
+                 norm_eps: float = 1e-6, rope: str = "interleaved"):  # fmt: skip
+        super().__init__(heads, device, scale, norm_eps, rope)
+        self.max_tokens = int(max_tokens)
+        n = ctypes.c_size_t()
+        _lib.check(self.lib.mkmoe_latent_workspace_bytes(ctypes.byref(n)), "latent workspace size")
+        of = lambda w, t: (t, (self.max_tokens, self.heads, w))  # noqa: E731
+        # (the attended latents stay in fp32: one rounding less before the output's own)
+        self._q_lat, self._q_pe, self._o_lat = self._take_workspace(
+            n.value, of(LATENT, BF), of(ROPE, BF), of(LATENT, torch.float32)
+        )
+        self._attend_io = _lib.LatentAttendIO()
+        self._absorb_io, self._expand_io = _lib.LatentProjectIO(), _lib.LatentProjectIO()
+
+    def _set_attend(self, cache, tokens: int, q_lat: tuple, q_pe: tuple, table, lens, q_starts, out: tuple,
+                    f32: int, lse: int) -> None:  # fmt: skip
+        c = self._cache(cache)
+        seqs, max_pages, stride, at_table, at_lens, at_starts = self._batch(tokens, table, lens, q_starts)
+        _lib.LATENT_ATTEND.pack_into(
+            self._attend_io, 0, *c, seqs, tokens, self.heads, max_pages, stride, q_lat[1], q_lat[2], q_pe[1], q_pe[2],
+            out[1], out[2], q_lat[0], q_pe[0], at_table, at_lens, at_starts, out[0], lse, self.scale, f32,
+        )  # fmt: skip
+
+    def _set_project(self, io, tokens: int, expand: int, f32: int, x: tuple, w: int, y: tuple) -> None:
+        _lib.LATENT_PROJECT.pack_into(io, 0, tokens, self.heads, expand, f32, x[1], x[2], y[1], y[2], x[0], w, y[0])
+
+    # ---- the calls
     def _project(self, what: str, w, x, out, expand: int) -> torch.Tensor:
         w.check(self.heads, self.device)
         width, wide = (LATENT, V) if expand else (NOPE, LATENT)
@@ -325,12 +373,7 @@ class LatentRunner:
             out = self._new("the attended rows", tokens, self.heads, LATENT, zeros=q_starts is not None)
         f32 = out.dtype == torch.float32
         op = self._rows3("out", out, tokens, LATENT, written=True, dtype=torch.float32 if f32 else BF)
-        at_lse = 0
-        if lse is not None:
-            if (lse.dtype != torch.float32 or lse.shape != (tokens, self.heads) or lse.device != self.device
-                    or not lse.is_contiguous()):  # fmt: skip
-                raise self._bad("lse", lse, f"[{tokens}, {self.heads}] torch.float32 contiguous")
-            at_lse = lse.data_ptr()
+        at_lse = self._lse(lse, tokens)
         self._set_attend(cache, tokens, ql, qp, table, lens, q_starts, op, int(f32), at_lse)
         if tokens:
             self._call(self.lib.mkmoe_latent_attend, self._attend_io, *self._ws)
@@ -378,21 +421,3 @@ class LatentRunner:
                 *self._ws,
             )  # fmt: skip
         return out
-
-    # ---- device errors
-    def read_errors(self) -> list[int]:
-        """The device error words (synchronises the stream)."""
-        words = (ctypes.c_int32 * _lib.LATENT_ERRW_WORDS)()
-        self._call(self.lib.mkmoe_latent_read_errors, self._ws[0], words, _lib.LATENT_ERRW_WORDS)
-        return list(words)
-
-    def raise_on_device_error(self) -> None:
-        """Raise if a call since the last ``clear_errors`` met a slot, position, length, query start
-        or page outside its bounds (synchronises the stream)."""
-        code, where, count, _ = self.read_errors()
-        if code:
-            raise RuntimeError(f"mkmoe latent: {_lib.LATENT_ERRORS.get(code, code)} {where} ({count} seen)")
-
-    def clear_errors(self) -> None:
-        """Forget recorded errors (on the current stream)."""
-        self.ws[: 4 * _lib.LATENT_ERRW_WORDS].zero_()
