@@ -427,6 +427,79 @@ int mkmoe_latent_prompt_step(const mkmoe_latent_append_io* append, const mkmoe_l
 /* Copy n error words to host memory (synchronises stream). */
 int mkmoe_latent_read_errors(const void* ws, int32_t* words, int32_t n, void* stream);
 
+/* ---------------------------------------------------------------- pages of a cache
+ * A pool of pages that one or several paged caches (a model's layers) are indexed by, and who holds them. A
+ * sequence of len tokens holds the pages that the first ceil(len / page_size) entries of its row of a table name.
+ * A full page may be held by several sequences, a partly filled one by one alone: its next token is written
+ * there. trim and fork keep to that by giving a sequence a page of its own with the other's bytes. Pages are
+ * taken lowest first, in the sequences' order: the same calls give the same tables. Pages that a call frees can be
+ * taken by the next one. No counterpart in the reference, whose caches are SGLang's.
+ *
+ * Every call runs on the caller's stream, allocates nothing, does not synchronise with the host and can be
+ * captured in a graph. Lengths, counts, parents and pages are read on the device and checked there: one outside its
+ * bounds is never used as an address, and is recorded. A workspace serves one stream at a time. */
+#define MKMOE_PAGES_MAX_SEQS 1024
+#define MKMOE_PAGES_REFS_AT 256 /* byte offset in a workspace of the pages' holders: int32 [pages] */
+
+/* error words at the head of a workspace (it is zeroed once by the caller, whole; adopt then makes it a pool) */
+#define MKMOE_PAGES_ERRW_CODE 0  /* 0, or the first error's code (MKMOE_PAGES_ERR_*) */
+#define MKMOE_PAGES_ERRW_WHERE 1 /* its sequence (copy: pair) */
+#define MKMOE_PAGES_ERRW_COUNT 2 /* how many were seen */
+#define MKMOE_PAGES_ERRW_WORDS 4
+#define MKMOE_PAGES_ERR_BOUNDS 1 /* a length, count or parent outside its bounds: clamped; no parent */
+#define MKMOE_PAGES_ERR_PAGE 2   /* a page outside the pool, or not held: left as it is */
+#define MKMOE_PAGES_ERR_FULL 3   /* too few free pages: grow and trim leave the sequence as it was, fork empty */
+#define MKMOE_PAGES_ERR_ROOM 4   /* grow: past the table or the call's tokens: the sequence stays as it was */
+#define MKMOE_PAGES_ERR_SHARED 5 /* adopt: a partly filled page of several sequences */
+
+typedef struct mkmoe_pages_cache {
+  void* data;         /* [pages][page_bytes], 16-byte aligned */
+  int64_t page_bytes; /* a multiple of 16 */
+} mkmoe_pages_cache;
+
+typedef struct mkmoe_pages_pool {
+  int32_t pages;      /* 1 .. 2^22; pages page_size < 2^31 */
+  int32_t page_size;  /* tokens a page: a power of two, 1 .. 1024 */
+  int32_t max_seqs;   /* rows of a table, 1 .. MKMOE_PAGES_MAX_SEQS */
+  int32_t max_pages;  /* its entries a row, 1 .. 2^22; max_pages page_size < 2^31 */
+  int32_t ncaches;    /* caches whose pages are copied, may be 0 */
+  int32_t pad;
+  const mkmoe_pages_cache* caches; /* [ncaches], in device memory */
+} mkmoe_pages_pool;
+
+typedef struct mkmoe_pages_table {
+  int32_t* table; /* [seqs][max_pages], stride entries a row */
+  int32_t* lens;  /* [seqs] tokens */
+  int64_t stride;
+  int32_t seqs, max_pages;
+} mkmoe_pages_table;
+
+int mkmoe_pages_workspace_bytes(int32_t pages, int32_t max_seqs, int32_t max_pages, size_t* bytes);
+/* The pool as the table says: each page held as often as it is named. NULL: all free. Three launches, or two. */
+int mkmoe_pages_adopt(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, void* ws, size_t ws_bytes, void* stream);
+/* add[b] tokens more for each sequence: lens grows, the table gets the pages taken. The call's tokens follow
+ * each other by sequence: starts [seqs + 1], positions [tokens], and slots [tokens], the cache rows (page page_size +
+ * offset) they go to; -1 (position 0) for those of a sequence that does not get them, and behind the last. One launch. */
+int mkmoe_pages_grow(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, const int32_t* add, int32_t tokens,
+                     int32_t* slots, int32_t* positions, int32_t* starts, void* ws, size_t ws_bytes, void* stream);
+/* Sequences cut to their first keep[b] tokens, pages behind them let go (0: freed; len or more: left as it is). Two launches. */
+int mkmoe_pages_trim(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, const int32_t* keep, void* ws,
+                     size_t ws_bytes, void* stream);
+/* Row b of the table goes on from row parents[b] as it was before the call (-1: empty). Full pages are shared;
+ * a last page that is not full stays with the lowest row, the others get copies. Rows that none goes on from let go of
+ * their pages. parents may hold b itself, and a row any number of times. Two launches. */
+int mkmoe_pages_fork(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, const int32_t* parents, void* ws,
+                     size_t ws_bytes, void* stream);
+/* The n pages held moved to pages 0 .. n - 1: those at n and behind to the free ones before, both in order. The table
+ * has every sequence that holds pages. Three launches. */
+int mkmoe_pages_compact(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, void* ws, size_t ws_bytes,
+                        void* stream);
+/* Pages src[i] copied to dst[i] in every cache; dst are distinct and none of them is among src. One launch. */
+int mkmoe_pages_copy(const mkmoe_pages_pool* pool, const int32_t* src, const int32_t* dst, int32_t count, void* ws,
+                     size_t ws_bytes, void* stream);
+/* Copy n error words to host memory (synchronises stream). */
+int mkmoe_pages_read_errors(const void* ws, int32_t* words, int32_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

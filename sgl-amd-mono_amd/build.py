@@ -11,8 +11,8 @@ The library holds the kernels and the C ABI of ``include/mkmoe.h`` and
 file runs wherever the tree is copied. The MoE source compiles in parts, in
 parallel: one object per compiled MoE shape (``MKMOE_UNIT`` 0 .. 8) and one for
 the host code (``MKMOE_UNIT`` 9); the FFN seam's source (``csrc/mkmoe_seam.hip``)
-and the latent attention's (``csrc/mkmoe_latent.hip``, ``mkmoe_prompt.hip``) are
-one more object each; then one link. The test hooks of ``include/mkmoe_testing.h``
+and the latent attention's (``csrc/mkmoe_latent.hip``, ``mkmoe_prompt.hip``) and the
+pages' (``csrc/mkmoe_pages.hip``) are one more object each; then one link. The test hooks of ``include/mkmoe_testing.h``
 (``csrc/mkmoe_testing.hip``) build alongside, as ``libmkmoe_testing.so``.
 """
 
@@ -33,7 +33,7 @@ OUT_TIMELINE = ROOT / "sgl_amd_mono" / "moe" / "libmkmoe_tl.so"
 OUT_TESTING = ROOT / "sgl_amd_mono" / "moe" / "libmkmoe_testing.so"
 SOURCE = CSRC / "mkmoe_kernels.hip"
 SEAM_SOURCE = CSRC / "mkmoe_seam.hip"
-LATENT_SOURCES = [CSRC / f"mkmoe_{n}.hip" for n in ("latent", "prompt")]
+LATENT_SOURCES = [CSRC / f"mkmoe_{n}.hip" for n in ("latent", "prompt", "pages")]
 TESTING_SOURCE = CSRC / "mkmoe_testing.hip"
 UNITS = (0, 1, 2, 3, 4, 5, 6, 7, 8, 9)  # the compiled shapes, then the host code
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

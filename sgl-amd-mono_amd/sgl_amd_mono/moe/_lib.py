@@ -68,6 +68,16 @@ LATENT_ERRORS = {
     5: "cached tokens past max_context, at sequence",
 }
 
+PAGES_MAX_SEQS, PAGES_MAX_PAGES, PAGES_REFS_AT = 1024, 1 << 22, 256
+PAGES_ERRW_WORDS = 4
+PAGES_ERRORS = {
+    1: "a length, count or parent outside its bounds, at sequence",
+    2: "a page outside the pool or not held, at sequence (copy: pair)",
+    3: "no free pages, at sequence",
+    4: "tokens past the table's entries or the call's outputs, at sequence",
+    5: "a partly filled page of several sequences, at sequence",
+}
+
 # every symbol include/mkmoe.h and include/mkmoe_seam.h declare
 EXPORTS = (
     "mkmoe_abi_version",
@@ -94,6 +104,14 @@ EXPORTS = (
     "mkmoe_latent_prompt",
     "mkmoe_latent_prompt_step",
     "mkmoe_latent_read_errors",
+    "mkmoe_pages_workspace_bytes",
+    "mkmoe_pages_adopt",
+    "mkmoe_pages_grow",
+    "mkmoe_pages_trim",
+    "mkmoe_pages_fork",
+    "mkmoe_pages_compact",
+    "mkmoe_pages_copy",
+    "mkmoe_pages_read_errors",
 )
 # every symbol include/mkmoe_testing.h declares (libmkmoe_testing.so)
 TESTING_EXPORTS = (
@@ -243,6 +261,22 @@ class LatentPromptIO(ctypes.Structure):
     )  # fmt: skip
 
 
+class PagesPool(ctypes.Structure):
+    """mkmoe_pages_pool of include/mkmoe.h."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("pages", "page_size", "max_seqs", "max_pages", "ncaches", "pad")] + [
+        ("caches", ctypes.c_void_p)
+    ]
+
+
+class PagesTable(ctypes.Structure):
+    """mkmoe_pages_table of include/mkmoe.h."""
+
+    _fields_ = [("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("stride", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("seqs", "max_pages")
+    ]
+
+
 def packer(cls) -> struct.Struct:
     """Writes every field of a structure in one call (``pack_into(structure, 0, ...)``): a quarter
     of the time that the fields take one by one. A null pointer is 0."""
@@ -254,8 +288,8 @@ def packer(cls) -> struct.Struct:
     return s
 
 
-LATENT_APPEND, LATENT_ATTEND, LATENT_PROJECT, LATENT_PROMPT = (
-    packer(c) for c in (LatentAppendIO, LatentAttendIO, LatentProjectIO, LatentPromptIO)
+LATENT_APPEND, LATENT_ATTEND, LATENT_PROJECT, LATENT_PROMPT, PAGES_TABLE = (
+    packer(c) for c in (LatentAppendIO, LatentAttendIO, LatentProjectIO, LatentPromptIO, PagesTable)
 )
 
 
@@ -317,6 +351,15 @@ def lib() -> ctypes.CDLL:
         L.mkmoe_latent_prompt.argtypes = [ctypes.POINTER(LatentPromptIO), vp, sz, vp]
         L.mkmoe_latent_prompt_step.argtypes = [ctypes.POINTER(c) for c in (LatentAppendIO, LatentPromptIO)] + [vp, sz, vp]
         L.mkmoe_latent_read_errors.argtypes = [vp, ctypes.POINTER(i32), i32, vp]
+        pool, table = ctypes.POINTER(PagesPool), ctypes.POINTER(PagesTable)
+        L.mkmoe_pages_workspace_bytes.argtypes = [i32, i32, i32, ctypes.POINTER(sz)]
+        L.mkmoe_pages_adopt.argtypes = [pool, table, vp, sz, vp]
+        L.mkmoe_pages_grow.argtypes = [pool, table, vp, i32, vp, vp, vp, vp, sz, vp]
+        L.mkmoe_pages_trim.argtypes = [pool, table, vp, vp, sz, vp]
+        L.mkmoe_pages_fork.argtypes = [pool, table, vp, vp, sz, vp]
+        L.mkmoe_pages_compact.argtypes = [pool, table, vp, sz, vp]
+        L.mkmoe_pages_copy.argtypes = [pool, vp, vp, i32, vp, sz, vp]
+        L.mkmoe_pages_read_errors.argtypes = [vp, ctypes.POINTER(i32), i32, vp]
         if L.mkmoe_abi_version() != ABI_VERSION:
             raise RuntimeError(
                 f"{LIB_PATH} has ABI {L.mkmoe_abi_version()}, this binding wants {ABI_VERSION}: rebuild it"
