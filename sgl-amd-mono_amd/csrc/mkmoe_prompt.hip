@@ -38,8 +38,28 @@ constexpr int kItemSetup = 4;       // what starting and storing a query tile ta
 constexpr float kMoveBy = 8.0f;     // a row's maximum moves where a score passes it by more than 2^kMoveBy
 constexpr float kLog2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// two fp32 as fp16 (nearest even), a in the low half
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const f16x2 v = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+// sums of numerators as they are multiplied: c + the two of w
+__device__ __forceinline__ float add_f16(uint32_t w, float c) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+}
+__device__ __forceinline__ float add_bf16(uint32_t w, float c) { return c + bf_lo(w) + bf_hi(w); }
+// the largest of scores; NaN where one is (their row's output is NaN either way)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 // where each sequence's rows and work are; written by k_prompt_rows, read by the launches behind it
@@ -67,7 +87,7 @@ struct PromptParams {
   uint8_t* pe;     // rope fragments [cap / 32][4][1 KB]
   uint8_t* k;      // key fragments [heads][cap / 32][8][1 KB]
   uint8_t* v;      // value fragments [heads][cap / 32][2][4][1 KB]
-  int32_t* odd;    // [heads][cap / 64]: a tile's values are not all finite
+  int32_t* odd;    // [heads][cap / 64]: a tile's values are bf16, not fp16
   float* part_o;   // [2 shares][8][4][4][64 lanes][4]
   float* part_ml;  // [2 shares][256][2]
   int64_t qn_ts, qn_hs, qp_ts, qp_hs, o_ts, o_hs, table_stride;
@@ -309,7 +329,20 @@ __device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) 
       const int tile = first + (g / kMStages) * step;
       const int head = tile / blocks, tok = tile - head * blocks;
       const int64_t kb = (int64_t)head * kbs + tok * 4 + tg * 2;
-      uint32_t top = 0;
+      bool half = false;
+      if constexpr (V) {
+        // fp16 where that loses nothing that counts: none above its range, the largest so far above its smallest
+        // normal value that what is below that is less than 2^-19 of it (or all 0)
+        uint32_t top = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max(top, f2u(acc[t][j][i]) & 0x7fffffffu);
+        half = __ballot(top >= f2u(65504.0f)) == 0 && (__ballot(top >= f2u(0x1p-6f)) != 0 || __ballot(top != 0) == 0);
+        if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + tok * 2 + tg] = !half;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -319,16 +352,12 @@ __device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) 
             uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              o[e] = pack_bf(acc[t][j][8 * u + 2 * e], acc[t][j][8 * u + 2 * e + 1]);
-              top = max(top, max(o[e] << 16 & 0x7fff0000u, o[e] & 0x7fff0000u));
+              const float x = acc[t][j][8 * u + 2 * e], y = acc[t][j][8 * u + 2 * e + 1];
+              o[e] = V && half ? pack_f16(x, y) : pack_bf(x, y);
             }
             uint8_t* to = (V ? p.v : p.k) + ((kb + t) * 8 + (V ? u * 4 + j : 2 * j + u)) * kFrag + lane * 16;
             *(u32x4*)to = u32x4{o[0], o[1], o[2], o[3]};
           }
-      if constexpr (V) {
-        const bool odd = __ballot(top >= 0x7f800000u) != 0;
-        if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + tok * 2 + tg] = odd;
-      }
     }
   }
 }
@@ -343,10 +372,11 @@ __global__ __launch_bounds__(256, 2) void k_prompt_heads(PromptParams p) {
 }
 
 // ---------------------------------------------------------------- attend
-constexpr int kTileKB = 40;  // fragments of a tile of keys: 16 of keys, 8 of rope keys, 16 of values
-constexpr int kTileLds = kTileKB * kFrag;
-constexpr int kTileRing = 3;
-constexpr int kKeyAt = 0, kPeAt = 16 * kFrag, kValAt = 24 * kFrag;
+constexpr int kKeyLds = 24 * kFrag;  // a tile's keys: 16 fragments, and 8 of rope keys from kPeAt
+constexpr int kPeAt = 16 * kFrag;
+constexpr int kValLds = 16 * kFrag;  // its values
+// tiles in LDS: of keys two in use (a block of 32 each), one there or on its way, one requested; of values one less
+constexpr int kKeyRing = 4, kValRing = 3;
 
 struct Item {
   int b, head, qt;     // a sequence's head's query tile
@@ -403,11 +433,60 @@ __device__ __forceinline__ void store_row(const PromptParams& p, const Item& it,
     *(u32x2*)(to + 2 * i) = u32x2{pack_bf(o[i] * inv, o[i + 1] * inv), pack_bf(o[i + 2] * inv, o[i + 3] * inv)};
 }
 
+// A wave's 32 query rows, a column of lanes each: what they hold while they go through the keys
+struct Rows {
+  bf16x8 q[12];   // 8 fragments of the values without rotation, dealt, and 4 of the rotated ones
+  f32x16 o[4];    // outputs, 32 values each
+  float m, mu;    // the maximum so far (times scale log2 e); what scores are taken less, kLift below it
+  float sum;      // of the lane's numerators
+  int sees;       // the last key that the row sees
+};
+// Numerators are up to 2^(kLift + kMoveBy), below fp16's largest, and what fp16 drops of them is below 2^-32 of the
+// largest one's
+constexpr float kLift = 7.0f;
+
+// a fragment along a block of 32 keys: 8 of them, then 4 of their rope values
+__device__ __forceinline__ uint32_t key_frag(int kb, int ds) {
+  return ds < 8 ? (kb * 8 + ds) * kFrag : kPeAt + (kb * 4 + ds - 8) * kFrag;
+}
+// scores of a block of 32 keys: A = keys, B = the queries
+__device__ __forceinline__ void score(const Rows& r, f32x16& s, uint32_t at, int kb) {
+#pragma unroll
+  for (int ds = 0; ds < 12; ++ds) s = mfma32(lds_read<bf16x8>(at + key_frag(kb, ds)), r.q[ds], ds == 0 ? f32x16{} : s);
+}
+__device__ __forceinline__ void mask_block(const Rows& r, f32x16& s, int key0, int half) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (key0 + 8 * (i >> 2) + 4 * half + (i & 3) > r.sees) s[i] = -__builtin_inff();
+}
+// the row's maximum moved to its new scores', where one of the wave's passes it by more than 2^kMoveBy
+__device__ __forceinline__ void move_max(const PromptParams& p, Rows& r, float top) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(f2u(top), f2u(top), false, false);
+  top = max3(u2f(sw[0]), u2f(sw[1]), u2f(sw[1])) * p.scale2;
+  if (__ballot(top > r.m + kMoveBy)) {
+    const float to = fmaxf(r.m, top), by = to == r.m ? 1.0f : __builtin_amdgcn_exp2f(r.m - to);
+    r.m = to;
+    r.mu = to == -__builtin_inff() ? 0.0f : to - kLift;
+    r.sum *= by;
+#pragma unroll
+    for (int vb = 0; vb < 4; ++vb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r.o[vb][i] *= by;
+  }
+}
+__device__ __forceinline__ float top_of(const f32x16& s) {
+  float top = s[0];
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) top = max3(top, s[i], s[i + 1]);
+  return top;
+}
+
 __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
-  __shared__ __align__(1024) uint8_t ring[kTileRing][kTileLds];
+  __shared__ __align__(1024) uint8_t ring[kKeyRing * kKeyLds + kValRing * kValLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const uint32_t lds = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)&ring[0][0];
+  const uint32_t lds = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)&ring[0];
+  const uint32_t k_ring = lds, v_ring = lds + kKeyRing * kKeyLds;
   // an XCD's workgroups have shares that follow each other: heads whose keys its L2 keeps
   const int total = p.plan->total, shares = p.plan->shares;
   const int share = shares == kPromptShares ? (blockIdx.x & 7) * (kPromptShares / 8) + (blockIdx.x >> 3) : blockIdx.x;
@@ -436,23 +515,26 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
     }
     if (from == upto) continue;
 
-    const int64_t kb0 = it.at / 32;
-    const uint8_t* kbase = p.k + ((int64_t)head * kbs + kb0) * 8 * kFrag;
-    const uint8_t* vbase = p.v + ((int64_t)head * kbs + kb0) * 8 * kFrag;
-    const uint8_t* pbase = p.pe + kb0 * 4 * kFrag;
-    auto issue = [&](int kt) {
-      const uint32_t to = lds + (kt % kTileRing) * kTileLds;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int f = wave * 2 + i;
-        lds_dma16(kbase + (int64_t)kt * 16 * kFrag + f * kFrag + lane * 16, __builtin_amdgcn_readfirstlane(to + kKeyAt + f * kFrag));
-        lds_dma16(vbase + (int64_t)kt * 16 * kFrag + f * kFrag + lane * 16, __builtin_amdgcn_readfirstlane(to + kValAt + f * kFrag));
-      }
-      lds_dma16(pbase + (int64_t)kt * 8 * kFrag + wave * kFrag + lane * 16, __builtin_amdgcn_readfirstlane(to + kPeAt + wave * kFrag));
+    const int64_t kb0 = __builtin_amdgcn_readfirstlane(it.at / 32);
+    // (a wave's fragments; scalar addresses, the lanes 16 bytes apart)
+    const uint8_t* kbase = p.k + ((int64_t)head * kbs + kb0) * 8 * kFrag + wave * 2 * kFrag;
+    const uint8_t* vbase = p.v + ((int64_t)head * kbs + kb0) * 8 * kFrag + wave * 2 * kFrag;
+    const uint8_t* pbase = p.pe + kb0 * 4 * kFrag + wave * kFrag;
+    auto issue_k = [&](int kt) {
+      const uint32_t to = k_ring + (kt % kKeyRing) * kKeyLds;
+      const uint8_t* from_k = kbase + (int64_t)kt * 16 * kFrag;
+      lds_dma16(from_k, lane * 16, to + wave * 2 * kFrag);
+      lds_dma16(from_k + kFrag, lane * 16, to + wave * 2 * kFrag + kFrag);
+      lds_dma16(pbase + (int64_t)kt * 8 * kFrag, lane * 16, to + kPeAt + wave * kFrag);
+    };
+    auto issue_v = [&](int kt) {
+      const uint32_t to = v_ring + (kt % kValRing) * kValLds + wave * 2 * kFrag;
+      const uint8_t* from_v = vbase + (int64_t)kt * 16 * kFrag;
+      lds_dma16(from_v, lane * 16, to);
+      lds_dma16(from_v + kFrag, lane * 16, to + kFrag);
     };
 
-    // the query: 8 fragments of its values without rotation, dealt, and 4 of the rotated ones
-    bf16x8 q[12];
+    Rows r;
     {
       const bool there = row < it.n;
       const uint16_t* qn = p.qn + (int64_t)(it.t0 + row) * p.qn_ts + (int64_t)head * p.qn_hs;
@@ -464,117 +546,171 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
           a = *(const u32x2*)(qn + 16 * ds + 4 * half);
           b = *(const u32x2*)(qn + 16 * ds + 4 * half + 8);
         }
-        q[ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, b.x ^ p.flip, b.y ^ p.flip});
+        r.q[ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, b.x ^ p.flip, b.y ^ p.flip});
       }
 #pragma unroll
       for (int ds = 0; ds < 4; ++ds) {
         u32x4 a = {0, 0, 0, 0};
         if (there) a = *(const u32x4*)(qp + 16 * ds + 8 * half);
-        q[8 + ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, a.z ^ p.flip, a.w ^ p.flip});
+        r.q[8 + ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, a.z ^ p.flip, a.w ^ p.flip});
       }
     }
+    // whether some of the tiles have values in bf16
+    const int32_t* odd = p.odd + (int64_t)head * (p.cap / kKeys) + it.at / kKeys;
+    bool mixed = false;
+    for (int kt = from + lane; kt < upto; kt += 64) mixed |= odd[kt] != 0;
+    mixed = __ballot(mixed) != 0;
     wait_all();
     barrier();  // every wave has read the tiles of the item before
-    issue(from);
-    if (from + 1 < upto) issue(from + 1);
 
-    f32x16 o[4] = {};
-    float m = -__builtin_inff(), mu = 0.0f, sum = 0.0f;  // mu: m, or 0 where no score was seen
-    const int sees = it.past + row;                      // the last key that the row sees
-    const int wave_sees = it.past + min(row0 + 31, it.n - 1);
-    for (int kt = from; kt < upto; ++kt) {
-      if (kt + 1 < upto)
+    r.m = -__builtin_inff();
+    r.mu = r.sum = 0.0f;
+    r.sees = it.past + row;  // the last key that the row sees
+#pragma unroll
+    for (int vb = 0; vb < 4; ++vb) r.o[vb] = f32x16{};
+    // the tiles that the wave's rows see, and those that all of them see whole
+    const int last_row = min(row0 + 31, it.n - 1);
+    const int seen = row0 < it.n ? min(upto, (it.past + last_row + kKeys) >> 6) : from;
+    const int whole = (it.past + row0 + 1) >> 6;
+
+    issue_k(from);
+    if (from + 1 < upto) issue_k(from + 1);
+    issue_v(from);
+    if (from + 2 < upto) issue_k(from + 2);
+    if (from + 1 < upto) issue_v(from + 1);
+    // at turn kt the keys of kt + 1 and the values of kt are there; the next turn's are on their way
+    auto turn = [&](int kt) {
+      if (kt + 2 < upto)
         wait_loads<5>();
       else
         wait_loads<0>();
       barrier();
-      if (kt + 2 < upto) issue(kt + 2);
-      const int key0 = kt * kKeys;
-      if (row0 >= it.n || key0 > wave_sees) continue;
-      const uint32_t at = lds + (kt % kTileRing) * kTileLds + lane * 16;
-      f32x16 s[2] = {};
-#pragma unroll
-      for (int ds = 0; ds < 12; ++ds)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const uint32_t f = ds < 8 ? kKeyAt + (kb * 8 + ds) * kFrag : kPeAt + (kb * 4 + ds - 8) * kFrag;
-          s[kb] = mfma32(lds_read<bf16x8>(at + f), q[ds], s[kb]);
-        }
-      const bool masked = key0 + kKeys - 1 > it.past + row0;
-      if (masked) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3) > sees) s[kb][i] = -__builtin_inff();
-      }
-      float top = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-      const auto sw = __builtin_amdgcn_permlane32_swap(f2u(top), f2u(top), false, false);
-      top = fmaxf(u2f(sw[0]), u2f(sw[1])) * p.scale2;
-      if (__ballot(top > m + kMoveBy)) {
-        const float to = fmaxf(m, top), by = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-        m = to;
-        mu = to == -__builtin_inff() ? 0.0f : to;
-        sum *= by;
-#pragma unroll
-        for (int vb = 0; vb < 4; ++vb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[vb][i] *= by;
-      }
-      bf16x8 num[2][2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = __builtin_amdgcn_exp2f(s[kb][8 * t + 2 * e] * p.scale2 - mu);
-            const float b = __builtin_amdgcn_exp2f(s[kb][8 * t + 2 * e + 1] * p.scale2 - mu);
-            sum += a + b;
-            w[e] = pack_bf(a, b);
-          }
-          num[kb][t] = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
-        }
-      if (masked && p.odd[(int64_t)head * (p.cap / kKeys) + it.at / kKeys + kt]) {
-        // values that are not finite, of tokens that some rows do not see: a key at a time, added where it is seen
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll 1
-          for (int x = 0; x < 16; ++x) {
-            const int h = x >> 3, e = x & 7;
-            const bool seen = key0 + 16 * g + 8 * (e >> 2) + 4 * h + (e & 3) <= sees;
-            const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
-            const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
-            const bf16x8 one = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, num[g >> 1][g & 1]) & only);
-#pragma unroll
-            for (int vb = 0; vb < 4; ++vb) {
-              const u32x4 a = lds_read<u32x4>(at + kValAt + (g * 4 + vb) * kFrag);
-              const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[vb][i] += seen ? add[i] : 0.0f;
-            }
-          }
-        continue;
-      }
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int vb = 0; vb < 4; ++vb)
-            o[vb] = mfma32(lds_read<bf16x8>(at + kValAt + (kb * 8 + t * 4 + vb) * kFrag), num[kb][t], o[vb]);
+      if (kt + 3 < upto) issue_k(kt + 3);
+      if (kt + 2 < upto) issue_v(kt + 2);
+    };
+    auto keys_at = [&](int kt) { return k_ring + (kt % kKeyRing) * kKeyLds + lane * 16; };
+    auto vals_at = [&](int kt) { return v_ring + (kt % kValRing) * kValLds + lane * 16; };
+    // a block of 32 keys' scores are formed one block ahead: its numerators then come under the next one's products
+    f32x16 s0, s1;
+    if (from + 2 < upto)
+      wait_loads<10>();
+    else
+      wait_loads<0>();
+    barrier();
+    int kt = from;
+    if (seen > from) {
+      score(r, s0, keys_at(from), 0);
+      if (from >= whole) mask_block(r, s0, from * kKeys, half);
+      move_max(p, r, top_of(s0));
     }
-    const auto sw = __builtin_amdgcn_permlane32_swap(f2u(sum), f2u(sum), false, false);
-    sum = u2f(sw[0]) + u2f(sw[1]);
+    if (!mixed) {
+      for (; kt + 1 < seen; ++kt) {
+        turn(kt);
+        const uint32_t k_at = keys_at(kt), next_at = keys_at(kt + 1), v_at = vals_at(kt);
+        // 40 fragments in turn: 12 of keys for the next block's scores, 8 of values for this one's outputs, twice; each is
+        // read two products before its own
+        auto frag = [&](int i) {
+          const int hh = i / 20, j = i % 20;
+          return lds_read<u32x4>(j >= 12 ? v_at + (hh * 8 + j - 12) * kFrag : hh == 0 ? k_at + key_frag(1, j) : next_at + key_frag(0, j));
+        };
+        u32x4 f[3];
+        f[0] = frag(0);
+        f[1] = frag(1);
+        u32x4 num[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          f32x16 &now = hh == 0 ? s0 : s1, &next = hh == 0 ? s1 : s0;
+#pragma unroll
+          for (int j = 0; j < 12; ++j) {
+            const int i = hh * 20 + j;
+            f[(i + 2) % 3] = frag(i + 2);
+            next = mfma32(__builtin_bit_cast(bf16x8, f[i % 3]), r.q[j], j == 0 ? f32x16{} : next);
+#pragma unroll
+            for (int x = j * 8 / 12; x < (j + 1) * 8 / 12; ++x) {
+              uint32_t w = pack_f16(__builtin_amdgcn_exp2f(now[2 * x] * p.scale2 - r.mu),
+                                    __builtin_amdgcn_exp2f(now[2 * x + 1] * p.scale2 - r.mu));
+              r.sum = add_f16(w, r.sum);
+              asm volatile("" : "+v"(w), "+v"(r.sum));  // (formed here, not where they are used)
+              num[x >> 2][x & 3] = w;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          const int key0 = kt * kKeys + (hh == 0 ? 32 : kKeys);
+          float top = -__builtin_inff();
+#pragma unroll
+          for (int j = 12; j < 20; ++j) {
+            const int i = hh * 20 + j, vb = j & 3;
+            if (i + 2 < 40) f[(i + 2) % 3] = frag(i + 2);
+            r.o[vb] = mfma32(__builtin_bit_cast(f16x8, f[i % 3]), __builtin_bit_cast(f16x8, num[(j - 12) >> 2]), r.o[vb]);
+            if (j == 14 && kt + hh >= whole) mask_block(r, next, key0, half);
+            if (j >= 14) {
+#pragma unroll
+              for (int x = (j - 14) * 8 / 6; x < (j - 13) * 8 / 6; ++x) top = max3(top, next[2 * x], next[2 * x + 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          move_max(p, r, top);
+        }
+      }
+    }
+    for (; kt < upto; ++kt) {
+      turn(kt);
+      if (kt >= seen) continue;
+      const bool in_bf = mixed && odd[kt] != 0;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
+        u32x4 num[2];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - r.mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - r.mu);
+          const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
+          r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
+          num[x >> 2][x & 3] = w;
+        }
+        if (in_bf && kt >= whole) {
+          // values that may not be finite, of tokens that some rows do not see: a key at a time, added where it is seen
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll 1
+            for (int x = 0; x < 16; ++x) {
+              const int h = x >> 3, e = x & 7;
+              const bool sees = kt * kKeys + 32 * hh + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= r.sees;
+              const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+              const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
+              const bf16x8 one = __builtin_bit_cast(bf16x8, num[t] & only);
+#pragma unroll
+              for (int vb = 0; vb < 4; ++vb) {
+                const u32x4 a = lds_read<u32x4>(v_at + (t * 4 + vb) * kFrag);
+                const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
+#pragma unroll
+                for (int i = 0; i < 16; ++i) r.o[vb][i] += sees ? add[i] : 0.0f;
+              }
+            }
+        } else if (in_bf) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            r.o[j & 3] = mfma32(lds_read<bf16x8>(v_at + j * kFrag), __builtin_bit_cast(bf16x8, num[j >> 2]), r.o[j & 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + j * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
+        }
+        if (kt + hh < seen) {
+          score(r, s0, hh == 0 ? keys_at(kt) : keys_at(kt + 1), 1 - hh);
+          if (kt + hh >= whole) mask_block(r, s0, kt * kKeys + (hh == 0 ? 32 : kKeys), half);
+          move_max(p, r, top_of(s0));
+        }
+      }
+    }
+    const auto sw = __builtin_amdgcn_permlane32_swap(f2u(r.sum), f2u(r.sum), false, false);
+    const float sum = u2f(sw[0]) + u2f(sw[1]);
     if (from == 0 && upto == tiles) {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-      for (int vb = 0; vb < 4; ++vb) store_row(p, it, row, o[vb], vb, inv, half);
+      for (int vb = 0; vb < 4; ++vb) store_row(p, it, row, r.o[vb], vb, inv, half);
       if (p.lse && half == 0 && row < it.n)
-        p.lse[(int64_t)(it.t0 + row) * p.heads + head] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * kLog2;
+        p.lse[(int64_t)(it.t0 + row) * p.heads + head] = sum == 0.0f ? -__builtin_inff() : (r.mu + __builtin_amdgcn_logf(sum)) * kLog2;
     } else {
       const int slot = 2 * share + (from == 0);
       f32x4* to = (f32x4*)p.part_o + ((int64_t)slot * 8 + wave) * 16 * 64 + lane;
@@ -582,8 +718,10 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
       for (int vb = 0; vb < 4; ++vb)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          to[(vb * 4 + i) * 64] = f32x4{o[vb][4 * i], o[vb][4 * i + 1], o[vb][4 * i + 2], o[vb][4 * i + 3]};
-      if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * kQRows + wave * 32 + col) * 2) = f32x2{m, sum};
+          to[(vb * 4 + i) * 64] = f32x4{r.o[vb][4 * i], r.o[vb][4 * i + 1], r.o[vb][4 * i + 2], r.o[vb][4 * i + 3]};
+      // (where the row saw no score yet its sum is 0, and the part counts for nothing)
+      const float mu = r.m == -__builtin_inff() ? r.m : r.mu;
+      if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * kQRows + wave * 32 + col) * 2) = f32x2{mu, sum};
     }
   }
 }
