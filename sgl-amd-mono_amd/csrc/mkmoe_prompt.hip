@@ -29,7 +29,7 @@ namespace mkmoe_latent {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kPromptShares = 256;  // equal shares of the attention's work at most, a workgroup each: one a CU
-constexpr int kLeastUnits = 6;      // units of work that a share has, where there is so much
+constexpr int kLeastUnits = 6;      // units of work that a share has
 constexpr int kQRows = 256;         // query rows a tile of queries holds
 constexpr int kKeys = 64;           // cached tokens a tile of keys holds
 constexpr int kFrag = 1024;         // bytes of a fragment
@@ -62,13 +62,32 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* q) {
+  const uint64_t v = (uint64_t)q;
+  return (const uint8_t*)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)(uint32_t)v));
+}
+
 // where each sequence's rows and work are; written by k_prompt_rows, read by the launches behind it
 struct Plan {
   int32_t at[kPromptSeqs];    // first row of the packed tokens; -1: they do not fit
   int32_t work[kPromptSeqs];  // first unit of the attention's work
+  int32_t item[kPromptSeqs];  // first item of it: a head's query tile each
+  int32_t first[kPromptShares];  // each share's first item
   int32_t rows;               // packed rows, a multiple of kKeys
   int32_t total;              // units of work
-  int32_t shares;             // equal shares that it is cut into
+  int32_t per;                // units a share
+  int32_t items;
+  int32_t odd;                // some tile's values are bf16
+};
+
+// what the end of a share cut, for the merge: a query tile that goes on in the shares behind it
+struct PromptCut {
+  int32_t parts;  // the shares behind it that have a part; 0: nothing was cut there
+  int32_t head, t0, n;  // the sequence's first query token, its query tokens
+  int32_t qt;
+  int32_t unused[3];
 };
 
 struct PromptParams {
@@ -88,13 +107,14 @@ struct PromptParams {
   uint8_t* k;      // key fragments [heads][cap / 32][8][1 KB]
   uint8_t* v;      // value fragments [heads][cap / 32][2][4][1 KB]
   int32_t* odd;    // [heads][cap / 64]: a tile's values are bf16, not fp16
+  PromptCut* cut;  // [shares]
   float* part_o;   // [2 shares][8][4][4][64 lanes][4]
   float* part_ml;  // [2 shares][256][2]
   int64_t qn_ts, qn_hs, qp_ts, qp_hs, o_ts, o_hs, table_stride;
   int64_t cap;     // packed rows that the workspace holds, a multiple of 128
   int pages, seqs, tokens, heads, n, max_len, page_shift;
   float scale2;    // |scale| log2(e)
-  uint32_t flip;   // 0x80008000 where scale is negative: the query's signs are turned
+  uint32_t flip;   // 0x80008000 where scale is negative: the keys' signs are turned
 };
 
 // a sequence's query tokens and length, clamped to their bounds
@@ -164,15 +184,16 @@ __device__ __forceinline__ int64_t scan256(int64_t v, int64_t* total, int64_t* l
 }
 
 // The packed rows, 32 tokens a workgroup and turn: a fragment a wave and turn, its lanes reading 16 bytes (MXFP8: 8
-// codes) of 32 rows each. Every workgroup forms the sequences' places itself; the first one leaves them
-// for the launches behind.
+// codes) of 32 rows each. Every workgroup forms the sequences' places itself; one more
+// plans the attention.
 template <bool MX>
 __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
   __shared__ int64_t sums[4];
-  __shared__ int at[kPromptSeqs];
+  __shared__ int at[kPromptSeqs], unit[kPromptSeqs], item[kPromptSeqs];
   __shared__ int upto;  // the end of the last rows that fit
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int64_t rows = 0, work = 0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = gridDim.x - 1;
+  const bool planner = (int)blockIdx.x == groups;
+  int64_t rows = 0, work = 0, items = 0;
   if (tid == 0) upto = 0;  // (the scan's barriers come before it is used)
   for (int b0 = 0; b0 < p.seqs; b0 += 256) {
     const int b = b0 + tid;
@@ -180,37 +201,73 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
     PromptSeq s{0, 0, 0, false};
     if (b < p.seqs) {
       s = prompt_seq(p, b);
-      if (s.bad && blockIdx.x == 0) record(p.err, MKMOE_LATENT_ERR_LENGTH, b);
+      if (s.bad && planner) record(p.err, MKMOE_LATENT_ERR_LENGTH, b);
       if (s.n > 0) need = (s.len + kKeys - 1) & -kKeys;
     }
     int64_t all;
     const int64_t from = rows + scan256(need, &all, sums);
     rows += all;
     const bool fits = need == 0 || from + need <= p.cap;
-    int64_t units = 0;
-    if (b < p.seqs && s.n > 0)
+    if (b < p.seqs) {
+      at[b] = (int)(fits ? min(from, p.cap) : p.cap);  // (in order, to be searched)
+      if (fits) atomicMax(&upto, (int)min(from + need, p.cap));
+    }
+    if (!planner) continue;
+    int64_t units = 0, mine = 0;
+    if (b < p.seqs && s.n > 0) {
       units = (int64_t)p.heads * (fits ? head_units(s.len - s.n, s.n) : query_tiles(s.n) * kItemSetup);
+      mine = (int64_t)p.heads * query_tiles(s.n);
+    }
     const int64_t first = work + scan256(units, &all, sums);
     work += all;
+    const int64_t first_item = items + scan256(mine, &all, sums);
+    items += all;
     if (b < p.seqs) {
-      at[b] = fits ? (int)min(from, p.cap) : (int)p.cap;  // (in order, to be searched)
-      if (fits) atomicMax(&upto, (int)min(from + need, p.cap));
-      if (blockIdx.x == 0) {
-        p.plan->at[b] = fits ? at[b] : -1;
-        p.plan->work[b] = (int)first;
-        if (!fits) record(p.err, MKMOE_LATENT_ERR_CONTEXT, b);
-      }
+      unit[b] = p.plan->work[b] = (int)first;
+      item[b] = p.plan->item[b] = (int)first_item;
+      p.plan->at[b] = fits ? at[b] : -1;
+      if (!fits) record(p.err, MKMOE_LATENT_ERR_CONTEXT, b);
     }
   }
   __syncthreads();
   const int end = upto;
-  if (blockIdx.x == 0 && tid == 0) {
-    p.plan->rows = end;
-    p.plan->total = (int)work;
-    p.plan->shares = (int)max((int64_t)1, min((int64_t)kPromptShares, work / kLeastUnits));
+  if (planner) {
+    const int per = (int)max((int64_t)kLeastUnits, (work + kPromptShares - 1) / kPromptShares);
+    if (tid == 0) {
+      p.plan->rows = end;
+      p.plan->total = (int)work;
+      p.plan->items = (int)items;
+      p.plan->per = per;
+      p.plan->odd = 0;
+    }
+    const int64_t u = (int64_t)tid * per;
+    if (tid >= kPromptShares || u >= work) return;
+    // the share's first item: the one that has its first unit
+    int lo = 0, hi = p.seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (unit[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    const PromptSeq s = prompt_seq(p, lo);
+    const int qts = query_tiles(s.n), past = s.len - s.n;
+    int x = (int)u - unit[lo], i = 0;
+    if (at[lo] == p.cap && s.len > 0) {  // it does not fit: no keys
+      i = x / kItemSetup;
+    } else {
+      const int head = x / head_units(past, s.n);
+      x -= head * head_units(past, s.n);
+      int a = 0, z = qts - 1;
+      while (a < z) {
+        const int mid = (a + z + 1) >> 1;
+        if (units_before(past, mid) <= x) a = mid; else z = mid - 1;
+      }
+      i = head * qts + a;
+    }
+    p.plan->first[tid] = item[lo] + i;
+    return;
   }
   const int r = lane & 31, half = lane >> 5;
-  for (int kb = blockIdx.x; kb < end >> 5; kb += gridDim.x) {
+  for (int kb = blockIdx.x; kb < end >> 5; kb += groups) {
     int lo = 0, hi = p.seqs - 1;  // the last sequence that starts at or before the block
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -245,7 +302,7 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
     }
     u32x4 v = {0, 0, 0, 0};
     if (src) v = *(const u32x4*)(src + (MX ? kL + kMxScales : 2 * kL) + 32 * wave + 16 * half);
-    *(u32x4*)(p.pe + ((int64_t)kb * 4 + wave) * kFrag + lane * 16) = v;
+    *(u32x4*)(p.pe + ((int64_t)kb * 4 + wave) * kFrag + lane * 16) = u32x4{v.x ^ p.flip, v.y ^ p.flip, v.z ^ p.flip, v.w ^ p.flip};
   }
 }
 
@@ -255,6 +312,7 @@ constexpr int kMK = 32;     // values along the sum a stage
 constexpr int kMStages = kL / kMK;
 constexpr int kMBytes = (kMTok + 256) * kMK * 2;
 constexpr int kMRing = 3;
+constexpr int kMGroup = 8;
 
 // Fragments of keys (A: the weights' rows, B: tokens) or values (A: tokens, B: the weights' rows)
 template <bool V>
@@ -281,27 +339,41 @@ __device__ __forceinline__ void heads_stage(f32x16 (&acc)[2][4], uint32_t c_at, 
 // next tile; two workgroups a CU, so that one's stores run under the other's products.
 template <bool V>  // the wave's part: values or keys
 __device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int blocks = (p.plan->rows + kMTok - 1) / kMTok, tiles = blocks * p.heads;
-  const int first = blockIdx.x, step = gridDim.x;
-  const int mine = first < tiles ? (tiles - 1 - first) / step + 1 : 0, stages = mine * kMStages;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  // Product tiles in groups of 8 blocks of tokens, a group head by head: an XCD's workgroups, which have tiles that follow
+  // each other, read a few MB of rows and weights between them, which its L2 keeps
+  const int blocks = uniform((p.plan->rows + kMTok - 1) / kMTok), tiles = blocks * p.heads;
+  const int xcd = blockIdx.x & 7, first = xcd * (tiles / 8) + min(xcd, tiles % 8);
+  const int end = (xcd + 1) * (tiles / 8) + min(xcd + 1, tiles % 8), step = gridDim.x >> 3;
+  const int begin = first + (int)(blockIdx.x >> 3);
+  const int stages = begin < end ? ((end - 1 - begin) / step + 1) * kMStages : 0;
   const int64_t kbs = p.cap / 32;
+  auto place = [&](int g, int& head, int& tok) {  // of stage g's tile
+    const int tile = begin + (g / kMStages) * step, group = tile / (kMGroup * p.heads);
+    const int in = tile - group * kMGroup * p.heads, wide = min(kMGroup, blocks - kMGroup * group);
+    head = uniform(in / wide);
+    tok = uniform(kMGroup * group + in % wide);
+  };
 
+  // wave w brings the tokens 32 w .. and the weights' rows 64 w ..
+  const uint8_t* c = nullptr;
+  const uint8_t* w = nullptr;
+  const uint32_t w_lane = (uint32_t)((lane >> 2) * kL + 8 * ((lane & 3) ^ ((lane >> 4) & 3))) * 2;
   auto issue = [&](int g) {
     if (g >= stages) return;
-    const int tile = first + (g / kMStages) * step, ks = g % kMStages;
-    const int head = tile / blocks, tok = tile - head * blocks;
+    if (g % kMStages == 0) {
+      int head, tok;
+      place(g, head, tok);
+      c = p.c + (int64_t)(tok * 4 + wave) * 32 * kFrag;
+      w = (const uint8_t*)(p.w + ((int64_t)head * 256 + wave * 64) * kL);
+    }
     const uint32_t to = lds + (g % kMRing) * kMBytes;
-    // wave w brings the tokens 32 w .. and the weights' rows 64 w ..
-    const uint8_t* c = p.c + ((int64_t)(tok * 4 + wave) * 32 + 2 * ks) * kFrag + lane * 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      lds_dma16(c + i * kFrag, __builtin_amdgcn_readfirstlane(to + (wave * 2 + i) * kFrag));
-    const uint16_t* w = p.w + ((int64_t)head * 256 + wave * 64 + (lane >> 2)) * kL + ks * kMK +
-                        8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    for (int i = 0; i < 2; ++i) lds_dma16(c + i * kFrag, lane * 16, to + (wave * 2 + i) * kFrag);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      lds_dma16(w + (int64_t)i * 16 * kL, __builtin_amdgcn_readfirstlane(to + (8 + wave * 4 + i) * kFrag));
+    for (int i = 0; i < 4; ++i) lds_dma16(w + i * 16 * kL * 2, w_lane, to + (8 + wave * 4 + i) * kFrag);
+    c += 2 * kFrag;
+    w += kMK * 2;
   };
 
   const int tg = wave & 1;
@@ -326,8 +398,8 @@ __device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) 
     const uint32_t c_at = at + tg * 4 * kFrag + lane * 16, w_at = at + 8 * kFrag + (V ? 8 : 0) * kFrag;
     heads_stage<V>(acc, c_at, w_at, lane);
     if (ks == kMStages - 1) {
-      const int tile = first + (g / kMStages) * step;
-      const int head = tile / blocks, tok = tile - head * blocks;
+      int head, tok;
+      place(g, head, tok);
       const int64_t kb = (int64_t)head * kbs + tok * 4 + tg * 2;
       bool half = false;
       if constexpr (V) {
@@ -342,6 +414,7 @@ __device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) 
             for (int i = 0; i < 16; ++i) top = max(top, f2u(acc[t][j][i]) & 0x7fffffffu);
         half = __ballot(top >= f2u(65504.0f)) == 0 && (__ballot(top >= f2u(0x1p-6f)) != 0 || __ballot(top != 0) == 0);
         if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + tok * 2 + tg] = !half;
+        if (lane == 0 && !half) atomicOr(&p.plan->odd, 1);
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -353,7 +426,7 @@ __device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float x = acc[t][j][8 * u + 2 * e], y = acc[t][j][8 * u + 2 * e + 1];
-              o[e] = V && half ? pack_f16(x, y) : pack_bf(x, y);
+              o[e] = V ? (half ? pack_f16(x, y) : pack_bf(x, y)) : pack_bf(x, y) ^ p.flip;
             }
             uint8_t* to = (V ? p.v : p.k) + ((kb + t) * 8 + (V ? u * 4 + j : 2 * j + u)) * kFrag + lane * 16;
             *(u32x4*)to = u32x4{o[0], o[1], o[2], o[3]};
@@ -378,59 +451,62 @@ constexpr int kValLds = 16 * kFrag;  // its values
 // tiles in LDS: of keys two in use (a block of 32 each), one there or on its way, one requested; of values one less
 constexpr int kKeyRing = 4, kValRing = 3;
 
+// a sequence's head's query tile, and the share's part of its keys
 struct Item {
-  int b, head, qt;     // a sequence's head's query tile
-  int t0, n, past;     // the sequence's
-  int at;              // its packed rows; -1: none
-  int first, tiles;    // its first unit of work; tiles of keys
+  int head, qt;       // qt: of 256 query rows
+  int t0, n, past;    // the sequence's
+  int tile;           // its first tile of packed rows; -1: they do not fit, -2: the end of the share
+  int tiles;          // of keys that the query tile sees
+  int from, upto;     // the share's of them
+  int parts;          // the shares behind this one that have some, where this one has the first and not all
 };
-// the item that has unit u of the work
-__device__ __forceinline__ Item item_at(const PromptParams& p, int u) {
-  Item it;
+constexpr int kItemWords = sizeof(Item) / 4, kItems = 64;
+// item o of the work, for the units begin .. end - 1 of share
+__device__ __forceinline__ Item item_of(const PromptParams& p, int o, int share, int begin, int end, int per) {
+  Item it{};
+  it.tile = -2;
+  if (o >= p.plan->items) return it;
   int lo = 0, hi = p.seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.plan->work[mid] <= u) lo = mid; else hi = mid - 1;
+    if (p.plan->item[mid] <= o) lo = mid; else hi = mid - 1;
   }
-  it.b = lo;
   const PromptSeq s = prompt_seq(p, lo);
+  const int at = p.plan->at[lo], qts = query_tiles(s.n), i = o - p.plan->item[lo];
   it.t0 = s.t0;
   it.n = s.n;
   it.past = s.len - s.n;
-  it.at = p.plan->at[lo];
-  const int base = p.plan->work[lo];
-  int x = u - base;
-  if (it.at < 0) {  // it did not fit: no keys
-    it.tiles = 0;
-    const int qts = query_tiles(s.n), i = x / kItemSetup;
-    it.head = i / qts;
-    it.qt = i - it.head * qts;
-    it.first = base + i * kItemSetup;
-    return it;
+  it.head = i / qts;
+  it.qt = i - it.head * qts;
+  int first = p.plan->work[lo];
+  if (at < 0) {
+    first += i * kItemSetup;
+  } else {
+    first += it.head * head_units(it.past, it.n) + units_before(it.past, it.qt);
+    it.tiles = tiles_of(it.past, it.n, it.qt);
   }
-  const int per = head_units(it.past, it.n);
-  it.head = x / per;
-  x -= it.head * per;
-  int a = 0, z = query_tiles(it.n) - 1;
-  while (a < z) {
-    const int mid = (a + z + 1) >> 1;
-    if (units_before(it.past, mid) <= x) a = mid; else z = mid - 1;
-  }
-  it.qt = a;
-  it.first = base + it.head * per + units_before(it.past, a);
-  it.tiles = tiles_of(it.past, it.n, a);
+  if (first >= end) return it;
+  it.tile = at < 0 ? -1 : at >> 6;
+  const int keys = first + kItemSetup;
+  it.from = max(0, begin - keys);
+  it.upto = min(it.tiles, max(0, end - keys));
+  if (it.tiles == 0 && first < begin) it.from = 1;  // (stored by the share that has its first unit)
+  it.parts = it.from == 0 && it.upto > 0 && it.upto < it.tiles ? (keys + it.tiles - 1) / per - share : 0;
   return it;
 }
-__device__ __forceinline__ int share_start(int total, int shares, int s) { return (int)((int64_t)total * s / shares); }
 
-// a query row's values, its running maximum (of scores times log2 e) and sum
-__device__ __forceinline__ void store_row(const PromptParams& p, const Item& it, int row, f32x16 o, int vb, float inv,
+// A query row's 32 output values of block vb. The row's two lanes have 4 values of 8 each: they exchange, so that each
+// stores 8 that follow each other
+__device__ __forceinline__ void store_row(const PromptParams& p, int t0, int n, int head, int row, f32x16 o, int vb, float inv,
                                           int half) {
-  if (row >= it.n) return;
-  uint16_t* to = p.out + (int64_t)(it.t0 + row) * p.o_ts + (int64_t)it.head * p.o_hs + 32 * vb + 4 * half;
+  uint16_t* to = p.out + (int64_t)(t0 + row) * p.o_ts + (int64_t)head * p.o_hs + 32 * vb + 8 * half;
 #pragma unroll
-  for (int i = 0; i < 16; i += 4)
-    *(u32x2*)(to + 2 * i) = u32x2{pack_bf(o[i] * inv, o[i + 1] * inv), pack_bf(o[i + 2] * inv, o[i + 3] * inv)};
+  for (int i = 0; i < 16; i += 8) {
+    // the first 8 values' words of this lane, the next 8's; then those of half 0's lane are the first 8 values, half 1's the next
+    const auto x = __builtin_amdgcn_permlane32_swap(pack_bf(o[i] * inv, o[i + 1] * inv), pack_bf(o[i + 4] * inv, o[i + 5] * inv), false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(pack_bf(o[i + 2] * inv, o[i + 3] * inv), pack_bf(o[i + 6] * inv, o[i + 7] * inv), false, false);
+    if (row < n) *(u32x4*)(to + 2 * i) = u32x4{x[0], y[0], x[1], y[1]};
+  }
 }
 
 // A wave's 32 query rows, a column of lanes each: what they hold while they go through the keys
@@ -483,85 +559,141 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
 
 __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
   __shared__ __align__(1024) uint8_t ring[kKeyRing * kKeyLds + kValRing * kValLds];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const uint32_t lds = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)&ring[0];
   const uint32_t k_ring = lds, v_ring = lds + kKeyRing * kKeyLds;
   // an XCD's workgroups have shares that follow each other: heads whose keys its L2 keeps
-  const int total = p.plan->total, shares = p.plan->shares;
-  const int share = shares == kPromptShares ? (blockIdx.x & 7) * (kPromptShares / 8) + (blockIdx.x >> 3) : blockIdx.x;
-  if (share >= shares) return;
-  int u = share_start(total, shares, share);
-  const int end = share_start(total, shares, share + 1);
+  const int total = uniform(p.plan->total), per = uniform(p.plan->per), shares = (total + per - 1) / per;
+  const int by_xcd = (shares + 7) >> 3, share = (blockIdx.x & 7) * by_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= by_xcd || share >= shares) return;
+  const int begin = share * per, end = min(total, begin + per);
+  const bool any_odd = uniform(p.plan->odd) != 0;
+  PromptCut cut{};
+  __shared__ int list[kItems][kItemWords];
+  int listed = uniform(p.plan->first[share]) - kItems, in_list = kItems;
+  // the share's next item (every wave at once: it may fill the list anew)
+  auto next_item = [&]() {
+    if (in_list == kItems) {
+      listed += kItems;
+      in_list = 0;
+      __syncthreads();
+      if (threadIdx.x < kItems) {
+        const Item x = item_of(p, listed + threadIdx.x, share, begin, end, per);
+        int* to = list[threadIdx.x];
+        to[0] = x.head, to[1] = x.qt, to[2] = x.t0, to[3] = x.n, to[4] = x.past, to[5] = x.tile, to[6] = x.tiles, to[7] = x.from,
+        to[8] = x.upto, to[9] = x.parts;
+      }
+      __syncthreads();
+    }
+    const int* x = list[in_list++];
+    return Item{uniform(x[0]), uniform(x[1]), uniform(x[2]), uniform(x[3]), uniform(x[4]),
+                uniform(x[5]), uniform(x[6]), uniform(x[7]), uniform(x[8]), uniform(x[9])};
+  };
   const int64_t kbs = p.cap / 32;
 
-  while (u < end) {
-    const Item it = item_at(p, __builtin_amdgcn_readfirstlane(u));
-    const int head = __builtin_amdgcn_readfirstlane(it.head), tiles = __builtin_amdgcn_readfirstlane(it.tiles);
-    const int item_end = it.first + kItemSetup + tiles;
-    const int from = __builtin_amdgcn_readfirstlane(max(0, u - it.first - kItemSetup));
-    const int upto = __builtin_amdgcn_readfirstlane(max(0, min(end, item_end) - it.first - kItemSetup));
-    const bool head_of_item = u == it.first;
-    u = item_end;
-    const int row0 = it.qt * kQRows + wave * 32, row = row0 + col;
-    if (tiles == 0) {
-      if (head_of_item && row < it.n) {
-        const float none = it.at < 0 ? __builtin_nanf("") : 0.0f;
-#pragma unroll
-        for (int vb = 0; vb < 4; ++vb) store_row(p, it, row, f32x16{} + none, vb, 1.0f, half);
-        if (p.lse && half == 0) p.lse[(int64_t)(it.t0 + row) * p.heads + head] = it.at < 0 ? none : -__builtin_inff();
-      }
-      continue;
-    }
-    if (from == upto) continue;
-
-    const int64_t kb0 = __builtin_amdgcn_readfirstlane(it.at / 32);
-    // (a wave's fragments; scalar addresses, the lanes 16 bytes apart)
-    const uint8_t* kbase = p.k + ((int64_t)head * kbs + kb0) * 8 * kFrag + wave * 2 * kFrag;
-    const uint8_t* vbase = p.v + ((int64_t)head * kbs + kb0) * 8 * kFrag + wave * 2 * kFrag;
-    const uint8_t* pbase = p.pe + kb0 * 4 * kFrag + wave * kFrag;
-    auto issue_k = [&](int kt) {
-      const uint32_t to = k_ring + (kt % kKeyRing) * kKeyLds;
-      const uint8_t* from_k = kbase + (int64_t)kt * 16 * kFrag;
-      lds_dma16(from_k, lane * 16, to + wave * 2 * kFrag);
-      lds_dma16(from_k + kFrag, lane * 16, to + wave * 2 * kFrag + kFrag);
-      lds_dma16(pbase + (int64_t)kt * 8 * kFrag, lane * 16, to + kPeAt + wave * kFrag);
-    };
-    auto issue_v = [&](int kt) {
-      const uint32_t to = v_ring + (kt % kValRing) * kValLds + wave * 2 * kFrag;
-      const uint8_t* from_v = vbase + (int64_t)kt * 16 * kFrag;
-      lds_dma16(from_v, lane * 16, to);
-      lds_dma16(from_v + kFrag, lane * 16, to + kFrag);
-    };
-
-    Rows r;
-    {
-      const bool there = row < it.n;
-      const uint16_t* qn = p.qn + (int64_t)(it.t0 + row) * p.qn_ts + (int64_t)head * p.qn_hs;
-      const uint16_t* qp = p.qp + (int64_t)(it.t0 + row) * p.qp_ts + (int64_t)head * p.qp_hs;
+  // The tiles of the share's items follow each other in LDS: tile i of the share in slot i of the rings. Where an item's
+  // are, a wave's fragments of the share's tile 0 had it come before it (scalar addresses, the lanes 16 bytes apart)
+  struct Source {
+    const uint8_t *k, *v, *pe;
+  };
+  auto source_of = [&](const Item& it, int pos) {
+    const int64_t tile = it.tile + it.from - pos, block = (int64_t)it.head * kbs + 2 * tile;
+    return Source{p.k + block * 8 * kFrag + wave * 2 * kFrag, p.v + block * 8 * kFrag + wave * 2 * kFrag,
+                  p.pe + (tile * 8 + wave) * kFrag};
+  };
+  Source here{}, there{};
+  int own = 0;  // the share's tiles up to the item's end
+  auto issue_k = [&](int i) {
+    const uint32_t to = uniform(k_ring + (i % kKeyRing) * kKeyLds + wave * 2 * kFrag);
+    const uint8_t* k = uniform((i < own ? here.k : there.k) + (int64_t)i * 16 * kFrag);
+    const uint8_t* pe = uniform((i < own ? here.pe : there.pe) + (int64_t)i * 8 * kFrag);
+    lds_dma16(k, lane * 16, to);
+    lds_dma16(k + kFrag, lane * 16, to + kFrag);
+    lds_dma16(pe, lane * 16, to + kPeAt - wave * kFrag);
+  };
+  auto issue_v = [&](int i) {
+    const uint32_t to = uniform(v_ring + (i % kValRing) * kValLds + wave * 2 * kFrag);
+    const uint8_t* v = uniform((i < own ? here.v : there.v) + (int64_t)i * 16 * kFrag);
+    lds_dma16(v, lane * 16, to);
+    lds_dma16(v + kFrag, lane * 16, to + kFrag);
+  };
+  Rows r;
+  auto load_q = [&](const Item& it) {
+    const int row = it.qt * kQRows + wave * 32 + col;
+    const uint16_t* qn = p.qn + (int64_t)(it.t0 + row) * p.qn_ts + (int64_t)it.head * p.qn_hs + 4 * half;
+    const uint16_t* qp = p.qp + (int64_t)(it.t0 + row) * p.qp_ts + (int64_t)it.head * p.qp_hs + 8 * half;
+    if (row < it.n) {  // (the other lanes' columns reach nothing)
 #pragma unroll
       for (int ds = 0; ds < 8; ++ds) {
-        u32x2 a = {0, 0}, b = {0, 0};
-        if (there) {
-          a = *(const u32x2*)(qn + 16 * ds + 4 * half);
-          b = *(const u32x2*)(qn + 16 * ds + 4 * half + 8);
-        }
-        r.q[ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, b.x ^ p.flip, b.y ^ p.flip});
+        const u32x2 a = *(const u32x2*)(qn + 16 * ds), b = *(const u32x2*)(qn + 16 * ds + 8);
+        r.q[ds] = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
       }
 #pragma unroll
-      for (int ds = 0; ds < 4; ++ds) {
-        u32x4 a = {0, 0, 0, 0};
-        if (there) a = *(const u32x4*)(qp + 16 * ds + 8 * half);
-        r.q[8 + ds] = __builtin_bit_cast(bf16x8, u32x4{a.x ^ p.flip, a.y ^ p.flip, a.z ^ p.flip, a.w ^ p.flip});
-      }
+      for (int ds = 0; ds < 4; ++ds) r.q[8 + ds] = *(const bf16x8*)(qp + 16 * ds);
+    } else {
+#pragma unroll
+      for (int ds = 0; ds < 12; ++ds) r.q[ds] = bf16x8{};
     }
+  };
+  Item it{}, next = next_item();
+  load_q(next);
+  int pos = 0;           // the share's tiles before the item's
+  int k_to = 0, v_to = 0;  // its tiles whose keys, values are requested
+  int k_there = 0;       // its tiles whose keys are there
+  bool steady = false;   // the last loads are the keys and values of one tile each, requested in turn
+  while (next.tile != -2) {
+    it = next;
+    next = next_item();
+    const int row0 = it.qt * kQRows + wave * 32, row = row0 + col;
+    const int from = it.from, upto = it.upto;
+    if (from >= upto) {
+      if (it.tiles == 0 && from == 0) {
+        const float none = it.tile < 0 ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+        for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, it.head, row, f32x16{} + none, vb, 1.0f, half);
+        if (p.lse && half == 0 && row < it.n) p.lse[(int64_t)(it.t0 + row) * p.heads + it.head] = it.tile < 0 ? none : -__builtin_inff();
+      }
+      load_q(next);
+      continue;
+    }
+    const int next_tiles = next.tile >= 0 ? max(0, next.upto - next.from) : 0;
+    here = source_of(it, pos);
+    own = pos + upto - from;
+    if (next_tiles > 0) there = source_of(next, own);
+    const int known = own + next_tiles;
+    auto request = [&](int k_end, int v_end) {
+      for (k_end = min(k_end, known); k_to < k_end; ++k_to) issue_k(k_to);
+      for (v_end = min(v_end, known); v_to < v_end; ++v_to) issue_v(v_to);
+    };
+    // at a tile's turn its own and the next one's keys are there, and its values; the ones behind are on their way
+    auto turn = [&](int i) {
+      if (steady) {
+        wait_loads<5>();
+        k_there = i + 2;
+      } else {
+        wait_loads<0>();
+        k_there = k_to;
+      }
+      barrier();
+      steady = k_to == i + 3 && v_to == i + 2 && i + 3 < known;
+      if (steady) {
+        issue_k(k_to++);
+        issue_v(v_to++);
+      } else {
+        request(i + 4, i + 3);
+      }
+    };
+
     // whether some of the tiles have values in bf16
-    const int32_t* odd = p.odd + (int64_t)head * (p.cap / kKeys) + it.at / kKeys;
+    const int32_t* odd = p.odd + (int64_t)it.head * (p.cap / kKeys) + it.tile;
     bool mixed = false;
-    for (int kt = from + lane; kt < upto; kt += 64) mixed |= odd[kt] != 0;
-    mixed = __ballot(mixed) != 0;
-    wait_all();
-    barrier();  // every wave has read the tiles of the item before
+    if (any_odd) {
+      for (int kt = from + lane; kt < upto; kt += 64) mixed |= odd[kt] != 0;
+      mixed = __ballot(mixed) != 0;
+    }
+    request(pos + 3, pos + 2);
+    steady = false;  // (other loads and stores are on their way)
 
     r.m = -__builtin_inff();
     r.mu = r.sum = 0.0f;
@@ -572,40 +704,47 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
     const int last_row = min(row0 + 31, it.n - 1);
     const int seen = row0 < it.n ? min(upto, (it.past + last_row + kKeys) >> 6) : from;
     const int whole = (it.past + row0 + 1) >> 6;
-
-    issue_k(from);
-    if (from + 1 < upto) issue_k(from + 1);
-    issue_v(from);
-    if (from + 2 < upto) issue_k(from + 2);
-    if (from + 1 < upto) issue_v(from + 1);
-    // at turn kt the keys of kt + 1 and the values of kt are there; the next turn's are on their way
-    auto turn = [&](int kt) {
-      if (kt + 2 < upto)
-        wait_loads<5>();
-      else
-        wait_loads<0>();
-      barrier();
-      if (kt + 3 < upto) issue_k(kt + 3);
-      if (kt + 2 < upto) issue_v(kt + 2);
-    };
-    auto keys_at = [&](int kt) { return k_ring + (kt % kKeyRing) * kKeyLds + lane * 16; };
-    auto vals_at = [&](int kt) { return v_ring + (kt % kValRing) * kValLds + lane * 16; };
+    auto keys_at = [&](int kt) { return k_ring + ((pos + kt - from) % kKeyRing) * kKeyLds + lane * 16; };
+    auto vals_at = [&](int kt) { return v_ring + ((pos + kt - from) % kValRing) * kValLds + lane * 16; };
     // a block of 32 keys' scores are formed one block ahead: its numerators then come under the next one's products
+    auto finish = [&]() {
+      const auto sw = __builtin_amdgcn_permlane32_swap(f2u(r.sum), f2u(r.sum), false, false);
+      const float sum = u2f(sw[0]) + u2f(sw[1]);
+      if (from == 0 && upto == it.tiles) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, it.head, row, r.o[vb], vb, inv, half);
+        if (p.lse && half == 0 && row < it.n)
+          p.lse[(int64_t)(it.t0 + row) * p.heads + it.head] = sum == 0.0f ? -__builtin_inff() : (r.mu + __builtin_amdgcn_logf(sum)) * kLog2;
+      } else if (row0 < it.n) {
+        const int slot = 2 * share + (from == 0);
+        f32x4* to = (f32x4*)p.part_o + ((int64_t)slot * 8 + wave) * 16 * 64 + lane;
+#pragma unroll
+        for (int vb = 0; vb < 4; ++vb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            to[(vb * 4 + i) * 64] = f32x4{r.o[vb][4 * i], r.o[vb][4 * i + 1], r.o[vb][4 * i + 2], r.o[vb][4 * i + 3]};
+        // (where the row saw no score yet its sum is 0, and the part counts for nothing)
+        const float mu = r.m == -__builtin_inff() ? r.m : r.mu;
+        if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * kQRows + wave * 32 + col) * 2) = f32x2{mu, sum};
+      }
+    };
     f32x16 s0, s1;
-    if (from + 2 < upto)
-      wait_loads<10>();
-    else
+    if (k_there <= pos) {
       wait_loads<0>();
-    barrier();
+      barrier();
+      k_there = k_to;
+    }
     int kt = from;
     if (seen > from) {
       score(r, s0, keys_at(from), 0);
       if (from >= whole) mask_block(r, s0, from * kKeys, half);
       move_max(p, r, top_of(s0));
     }
-    if (!mixed) {
-      for (; kt + 1 < seen; ++kt) {
-        turn(kt);
+    if (!mixed && seen > from) {
+      for (;; ++kt) {
+        turn(pos + kt - from);
+        const bool more = kt + 1 < seen;
         const uint32_t k_at = keys_at(kt), next_at = keys_at(kt + 1), v_at = vals_at(kt);
         // 40 fragments in turn: 12 of keys for the next block's scores, 8 of values for this one's outputs, twice; each is
         // read two products before its own
@@ -613,26 +752,26 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
           const int hh = i / 20, j = i % 20;
           return lds_read<u32x4>(j >= 12 ? v_at + (hh * 8 + j - 12) * kFrag : hh == 0 ? k_at + key_frag(1, j) : next_at + key_frag(0, j));
         };
-        u32x4 f[3];
+        u32x4 f[3], num[2];
+        auto pair = [&](const f32x16& now, int x) {
+          uint32_t w = pack_f16(__builtin_amdgcn_exp2f(now[2 * x] * p.scale2 - r.mu), __builtin_amdgcn_exp2f(now[2 * x + 1] * p.scale2 - r.mu));
+          r.sum = add_f16(w, r.sum);
+          asm volatile("" : "+v"(w), "+v"(r.sum));  // (formed here, not where they are used)
+          num[x >> 2][x & 3] = w;
+        };
         f[0] = frag(0);
         f[1] = frag(1);
-        u32x4 num[2];
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          f32x16 &now = hh == 0 ? s0 : s1, &next = hh == 0 ? s1 : s0;
+          f32x16 &now = hh == 0 ? s0 : s1, &next_s = hh == 0 ? s1 : s0;
+          if (hh == 1 && !more) break;
 #pragma unroll
           for (int j = 0; j < 12; ++j) {
             const int i = hh * 20 + j;
             f[(i + 2) % 3] = frag(i + 2);
-            next = mfma32(__builtin_bit_cast(bf16x8, f[i % 3]), r.q[j], j == 0 ? f32x16{} : next);
+            next_s = mfma32(__builtin_bit_cast(bf16x8, f[i % 3]), r.q[j], j == 0 ? f32x16{} : next_s);
 #pragma unroll
-            for (int x = j * 8 / 12; x < (j + 1) * 8 / 12; ++x) {
-              uint32_t w = pack_f16(__builtin_amdgcn_exp2f(now[2 * x] * p.scale2 - r.mu),
-                                    __builtin_amdgcn_exp2f(now[2 * x + 1] * p.scale2 - r.mu));
-              r.sum = add_f16(w, r.sum);
-              asm volatile("" : "+v"(w), "+v"(r.sum));  // (formed here, not where they are used)
-              num[x >> 2][x & 3] = w;
-            }
+            for (int x = j * 8 / 12; x < (j + 1) * 8 / 12; ++x) pair(now, x);
             __builtin_amdgcn_sched_barrier(0);
           }
           const int key0 = kt * kKeys + (hh == 0 ? 32 : kKeys);
@@ -642,134 +781,123 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
             const int i = hh * 20 + j, vb = j & 3;
             if (i + 2 < 40) f[(i + 2) % 3] = frag(i + 2);
             r.o[vb] = mfma32(__builtin_bit_cast(f16x8, f[i % 3]), __builtin_bit_cast(f16x8, num[(j - 12) >> 2]), r.o[vb]);
-            if (j == 14 && kt + hh >= whole) mask_block(r, next, key0, half);
+            if (j == 14 && kt + hh >= whole) mask_block(r, next_s, key0, half);
             if (j >= 14) {
 #pragma unroll
-              for (int x = (j - 14) * 8 / 6; x < (j - 13) * 8 / 6; ++x) top = max3(top, next[2 * x], next[2 * x + 1]);
+              for (int x = (j - 14) * 8 / 6; x < (j - 13) * 8 / 6; ++x) top = max3(top, next_s[2 * x], next_s[2 * x + 1]);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
           move_max(p, r, top);
         }
+        if (more) continue;
+        // the last block: the queries have been used, the next item's arrive meanwhile
+        load_q(next);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) pair(s1, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + (8 + j) * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
+        ++kt;
+        break;
       }
-    }
-    for (; kt < upto; ++kt) {
-      turn(kt);
-      if (kt >= seen) continue;
-      const bool in_bf = mixed && odd[kt] != 0;
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
-        u32x4 num[2];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - r.mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - r.mu);
-          const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
-          r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
-          num[x >> 2][x & 3] = w;
-        }
-        if (in_bf && kt >= whole) {
-          // values that may not be finite, of tokens that some rows do not see: a key at a time, added where it is seen
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll 1
-            for (int x = 0; x < 16; ++x) {
-              const int h = x >> 3, e = x & 7;
-              const bool sees = kt * kKeys + 32 * hh + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= r.sees;
-              const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
-              const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
-              const bf16x8 one = __builtin_bit_cast(bf16x8, num[t] & only);
-#pragma unroll
-              for (int vb = 0; vb < 4; ++vb) {
-                const u32x4 a = lds_read<u32x4>(v_at + (t * 4 + vb) * kFrag);
-                const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
-#pragma unroll
-                for (int i = 0; i < 16; ++i) r.o[vb][i] += sees ? add[i] : 0.0f;
-              }
-            }
-        } else if (in_bf) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            r.o[j & 3] = mfma32(lds_read<bf16x8>(v_at + j * kFrag), __builtin_bit_cast(bf16x8, num[j >> 2]), r.o[j & 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + j * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
-        }
-        if (kt + hh < seen) {
-          score(r, s0, hh == 0 ? keys_at(kt) : keys_at(kt + 1), 1 - hh);
-          if (kt + hh >= whole) mask_block(r, s0, kt * kKeys + (hh == 0 ? 32 : kKeys), half);
-          move_max(p, r, top_of(s0));
-        }
-      }
-    }
-    const auto sw = __builtin_amdgcn_permlane32_swap(f2u(r.sum), f2u(r.sum), false, false);
-    const float sum = u2f(sw[0]) + u2f(sw[1]);
-    if (from == 0 && upto == tiles) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-      for (int vb = 0; vb < 4; ++vb) store_row(p, it, row, r.o[vb], vb, inv, half);
-      if (p.lse && half == 0 && row < it.n)
-        p.lse[(int64_t)(it.t0 + row) * p.heads + head] = sum == 0.0f ? -__builtin_inff() : (r.mu + __builtin_amdgcn_logf(sum)) * kLog2;
+      finish();
+      for (; kt < upto; ++kt) turn(pos + kt - from);
     } else {
-      const int slot = 2 * share + (from == 0);
-      f32x4* to = (f32x4*)p.part_o + ((int64_t)slot * 8 + wave) * 16 * 64 + lane;
+      for (; kt < upto; ++kt) {
+        turn(pos + kt - from);
+        if (kt >= seen) continue;
+        const bool in_bf = mixed && odd[kt] != 0;
 #pragma unroll
-      for (int vb = 0; vb < 4; ++vb)
+        for (int hh = 0; hh < 2; ++hh) {
+          const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
+          u32x4 num[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          to[(vb * 4 + i) * 64] = f32x4{r.o[vb][4 * i], r.o[vb][4 * i + 1], r.o[vb][4 * i + 2], r.o[vb][4 * i + 3]};
-      // (where the row saw no score yet its sum is 0, and the part counts for nothing)
-      const float mu = r.m == -__builtin_inff() ? r.m : r.mu;
-      if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * kQRows + wave * 32 + col) * 2) = f32x2{mu, sum};
+          for (int x = 0; x < 8; ++x) {
+            const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - r.mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - r.mu);
+            const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
+            r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
+            num[x >> 2][x & 3] = w;
+          }
+          if (in_bf && kt >= whole) {
+            // values that may not be finite, of tokens that some rows do not see: a key at a time, added where it is seen
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll 1
+              for (int x = 0; x < 16; ++x) {
+                const int h = x >> 3, e = x & 7;
+                const bool sees = kt * kKeys + 32 * hh + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= r.sees;
+                const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+                const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
+                const bf16x8 one = __builtin_bit_cast(bf16x8, num[t] & only);
+#pragma unroll
+                for (int vb = 0; vb < 4; ++vb) {
+                  const u32x4 a = lds_read<u32x4>(v_at + (t * 4 + vb) * kFrag);
+                  const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) r.o[vb][i] += sees ? add[i] : 0.0f;
+                }
+              }
+          } else if (in_bf) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              r.o[j & 3] = mfma32(lds_read<bf16x8>(v_at + j * kFrag), __builtin_bit_cast(bf16x8, num[j >> 2]), r.o[j & 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + j * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
+          }
+          if (kt + hh < seen) {
+            score(r, s0, hh == 0 ? keys_at(kt) : keys_at(kt + 1), 1 - hh);
+            if (kt + hh >= whole) mask_block(r, s0, kt * kKeys + (hh == 0 ? 32 : kKeys), half);
+            move_max(p, r, top_of(s0));
+          }
+        }
+      }
+      load_q(next);
+      finish();
     }
+    if (it.parts > 0) cut = PromptCut{it.parts, it.head, it.t0, it.n, it.qt, {}};
+    pos += upto - from;
   }
+  if (threadIdx.x == 0) p.cut[share] = cut;
 }
 
-// The parts of a query tile whose first share ends inside it, joined in order: (share, 32 rows) a workgroup, 32 values a
+// The parts of a query tile that the end of a share cut, joined in order: (share, 32 rows) a workgroup, 32 values a
 // wave. The lanes have the values that the attention's had.
 __global__ __launch_bounds__(256) void k_prompt_merge(PromptParams p) {
   const int lane = threadIdx.x & 63, vb = threadIdx.x >> 6, share = blockIdx.x, group = blockIdx.y;
-  const int half = lane >> 5, col = lane & 31, total = p.plan->total,
-            shares = p.plan->shares;
-  if (share + 1 >= shares) return;
-  const int start = share_start(total, shares, share), end = share_start(total, shares, share + 1);
-  if (start == end) return;
-  const Item it = item_at(p, end);
-  const int keys = it.first + kItemSetup, item_end = keys + it.tiles;
-  // the tile's first keys are this share's, and not all of them
-  if (it.tiles == 0 || end <= keys || start > keys) return;
-  const int row = it.qt * kQRows + group * 32 + col;
-  if (it.qt * kQRows + group * 32 >= it.n) return;
+  const int half = lane >> 5, col = lane & 31;
+  if (share * p.plan->per >= p.plan->total) return;  // (no such share)
+  const PromptCut c = p.cut[share];
+  const int row0 = c.qt * kQRows + group * 32, row = row0 + col;
+  if (c.parts == 0 || row0 >= c.n) return;
+  auto slot = [&](int i) { return 2 * (share + i) + (i == 0); };
   float top = -__builtin_inff();
-  int last = share;
-  while (last + 1 < shares && share_start(total, shares, last + 1) < item_end) ++last;
-  for (int s = share; s <= last; ++s)
-    top = fmaxf(top, p.part_ml[((int64_t)(2 * s + (s == share)) * kQRows + group * 32 + col) * 2]);
+  for (int i = 0; i <= c.parts; ++i) top = fmaxf(top, p.part_ml[((int64_t)slot(i) * kQRows + group * 32 + col) * 2]);
   f32x16 o = {};
   float sum = 0.0f;
-  for (int s = share; s <= last; ++s) {
-    const int slot = 2 * s + (s == share);
-    const f32x2 ml = *(const f32x2*)(p.part_ml + ((int64_t)slot * kQRows + group * 32 + col) * 2);
+  for (int i = 0; i <= c.parts; ++i) {
+    const f32x2 ml = *(const f32x2*)(p.part_ml + ((int64_t)slot(i) * kQRows + group * 32 + col) * 2);
     const float by = ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - top);
     sum += ml[1] * by;
-    const f32x4* from = (const f32x4*)p.part_o + ((int64_t)slot * 8 + group) * 16 * 64 + vb * 4 * 64 + lane;
+    const f32x4* from = (const f32x4*)p.part_o + ((int64_t)slot(i) * 8 + group) * 16 * 64 + vb * 4 * 64 + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 x = from[i * 64];
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 x = from[j * 64];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[4 * i + j] += x[j] * by;
+      for (int e = 0; e < 4; ++e) o[4 * j + e] += x[e] * by;
     }
   }
-  store_row(p, it, row, o, vb, sum == 0.0f ? 0.0f : 1.0f / sum, half);
-  if (p.lse && vb == 0 && half == 0 && row < it.n)
-    p.lse[(int64_t)(it.t0 + row) * p.heads + it.head] = sum == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLog2;
+  store_row(p, c.t0, c.n, c.head, row, o, vb, sum == 0.0f ? 0.0f : 1.0f / sum, half);
+  if (p.lse && vb == 0 && half == 0 && row < c.n)
+    p.lse[(int64_t)(c.t0 + row) * p.heads + c.head] = sum == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * kLog2;
 }
 
 // ---------------------------------------------------------------- host
 // a workspace: the latent calls' own first (its error words serve both), then the prompt's
 struct PromptLayout {
-  size_t plan, part_ml, part_o, odd, pe, c, k, v, bytes;
+  size_t plan, cut, part_ml, part_o, odd, pe, c, k, v, bytes;
 };
 inline PromptLayout prompt_layout(int heads, int64_t cap) {
   PromptLayout l;
@@ -781,6 +909,7 @@ inline PromptLayout prompt_layout(int heads, int64_t cap) {
     return from;
   };
   l.plan = take(sizeof(Plan));
+  l.cut = take(kPromptShares * sizeof(PromptCut));
   l.part_ml = take((size_t)2 * kPromptShares * kQRows * 2 * 4);
   l.part_o = take((size_t)2 * kPromptShares * kQRows * kV * 4);
   l.odd = take((size_t)heads * (cap / kKeys) * 4);
@@ -835,6 +964,7 @@ inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_b
   p.lse = io->lse;
   p.err = (int32_t*)at;
   p.plan = (Plan*)(at + l.plan);
+  p.cut = (PromptCut*)(at + l.cut);
   p.part_ml = (float*)(at + l.part_ml);
   p.part_o = (float*)(at + l.part_o);
   p.odd = (int32_t*)(at + l.odd);
@@ -866,7 +996,7 @@ inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_b
 inline int prompt_launch(const PromptParams& p, bool mx, hipStream_t st) {
   const int64_t rows = p.cap < (int64_t)p.seqs * p.max_len ? p.cap : (int64_t)p.seqs * p.max_len;
   const int64_t blocks = (rows + 31) / 32 + p.seqs;
-  const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024));
+  const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024) + 1);  // (and the planner)
   if (mx)
     hipLaunchKernelGGL(k_prompt_rows<true>, grid, dim3(256), 0, st, p);
   else
