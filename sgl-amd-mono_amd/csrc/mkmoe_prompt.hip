@@ -22,16 +22,21 @@
 // the next one's operand in place: keys and values are stored, and numerators used, without
 // any exchange between lanes.
 
+#include <stdlib.h>
 #include "mkmoe_latent.h"
 
 namespace mkmoe_latent {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kPromptShares = 256;  // equal shares of the attention's work at most, a workgroup each: one a CU
+// The attention's cuts, by the waves of a workgroup, W = 4 or 8: 32 W query rows a query tile, 8 W cached tokens a
+// turn, and as many equal shares of the work as two or one workgroups a CU
+constexpr int kMaxShares = 512;
+constexpr __host__ __device__ int shares_of(int waves) { return 2048 / waves; }
+constexpr __host__ __device__ int rows_of(int waves) { return 32 * waves; }
+constexpr __host__ __device__ int key_shift(int waves) { return waves == 8 ? 6 : 5; }
+constexpr int kKeys = 64;           // a sequence's packed rows are a multiple of so many
 constexpr int kLeastUnits = 6;      // units of work that a share has
-constexpr int kQRows = 256;         // query rows a tile of queries holds
-constexpr int kKeys = 64;           // cached tokens a tile of keys holds
 constexpr int kFrag = 1024;         // bytes of a fragment
 constexpr int kPromptSeqs = MKMOE_LATENT_MAX_SEQS;
 constexpr int kItemSetup = 4;       // what starting and storing a query tile takes, in tiles of keys
@@ -74,7 +79,7 @@ struct Plan {
   int32_t at[kPromptSeqs];    // first row of the packed tokens; -1: they do not fit
   int32_t work[kPromptSeqs];  // first unit of the attention's work
   int32_t item[kPromptSeqs];  // first item of it: a head's query tile each
-  int32_t first[kPromptShares];  // each share's first item
+  int32_t first[kMaxShares];  // each share's first item
   int32_t rows;               // packed rows, a multiple of kKeys
   int32_t total;              // units of work
   int32_t per;                // units a share
@@ -108,11 +113,12 @@ struct PromptParams {
   uint8_t* v;      // value fragments [heads][cap / 32][2][4][1 KB]
   int32_t* odd;    // [heads][cap / 64]: a tile's values are bf16, not fp16
   PromptCut* cut;  // [shares]
-  float* part_o;   // [2 shares][8][4][4][64 lanes][4]
-  float* part_ml;  // [2 shares][256][2]
+  float* part_o;   // [2 shares][W][4][4][64 lanes][4]
+  float* part_ml;  // [2 shares][32 W][2]
   int64_t qn_ts, qn_hs, qp_ts, qp_hs, o_ts, o_hs, table_stride;
   int64_t cap;     // packed rows that the workspace holds, a multiple of 128
   int pages, seqs, tokens, heads, n, max_len, page_shift;
+  int waves;       // of the attention's workgroups
   float scale2;    // |scale| log2(e)
   uint32_t flip;   // 0x80008000 where scale is negative: the keys' signs are turned
 };
@@ -140,24 +146,24 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
   return s;
 }
 
-// A head's query tiles in order, each of kItemSetup units and one for each tile of keys that its last
-// row sees. Tile i sees past + 256 (i + 1) keys (the last one past + n), past = len - n below 0 where there
-// are more queries than cached tokens: 4 (i + 1) + tiles(past) tiles.
-__device__ __forceinline__ int past_tiles(int past) { return (past + kKeys - 1) >> 6; }  // (rounded up, below 0 too)
-__device__ __forceinline__ int tiles_of(int past, int n, int i) {
-  return max(0, past + min(n, kQRows * (i + 1)) + kKeys - 1) >> 6;
+// A head's query tiles in order, each of kItemSetup units and one for each turn of keys that its last
+// row sees. Tile i sees past + rows (i + 1) keys (the last one past + n), past = len - n below 0 where there
+// are more queries than cached tokens: 4 (i + 1) + turns(past) turns, for 4 turns are a query tile's rows.
+__device__ __forceinline__ int turns_of(int past, int n, int i, int w) {
+  return max(0, past + min(n, rows_of(w) * (i + 1)) + (1 << key_shift(w)) - 1) >> key_shift(w);
 }
 // units before query tile i, none of those before it the last
-__device__ __forceinline__ int units_before(int past, int i) {
-  const int cp = past_tiles(past), first = cp < 0 ? (-cp) >> 2 : 0;  // the first tile that sees a key
+__device__ __forceinline__ int units_before(int past, int i, int w) {
+  const int cp = (past + (1 << key_shift(w)) - 1) >> key_shift(w);  // (rounded up, below 0 too)
+  const int first = cp < 0 ? (-cp) >> 2 : 0;                        // the first tile that sees a key
   int u = i * kItemSetup;
   if (i > first) u += 2 * (i * (i + 1) - first * (first + 1)) + (i - first) * cp;
   return u;
 }
-__device__ __forceinline__ int query_tiles(int n) { return (n + kQRows - 1) / kQRows; }
-__device__ __forceinline__ int head_units(int past, int n) {
-  const int last = query_tiles(n) - 1;
-  return units_before(past, last) + kItemSetup + tiles_of(past, n, last);
+__device__ __forceinline__ int query_tiles(int n, int w) { return (n + rows_of(w) - 1) / rows_of(w); }
+__device__ __forceinline__ int head_units(int past, int n, int w) {
+  const int last = query_tiles(n, w) - 1;
+  return units_before(past, last, w) + kItemSetup + turns_of(past, n, last, w);
 }
 
 // ---------------------------------------------------------------- rows
@@ -215,8 +221,8 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
     if (!planner) continue;
     int64_t units = 0, mine = 0;
     if (b < p.seqs && s.n > 0) {
-      units = (int64_t)p.heads * (fits ? head_units(s.len - s.n, s.n) : query_tiles(s.n) * kItemSetup);
-      mine = (int64_t)p.heads * query_tiles(s.n);
+      units = (int64_t)p.heads * (fits ? head_units(s.len - s.n, s.n, p.waves) : query_tiles(s.n, p.waves) * kItemSetup);
+      mine = (int64_t)p.heads * query_tiles(s.n, p.waves);
     }
     const int64_t first = work + scan256(units, &all, sums);
     work += all;
@@ -232,7 +238,7 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
   __syncthreads();
   const int end = upto;
   if (planner) {
-    const int per = (int)max((int64_t)kLeastUnits, (work + kPromptShares - 1) / kPromptShares);
+    const int shares = shares_of(p.waves), per = (int)max((int64_t)kLeastUnits, (work + shares - 1) / shares);
     if (tid == 0) {
       p.plan->rows = end;
       p.plan->total = (int)work;
@@ -240,30 +246,32 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
       p.plan->per = per;
       p.plan->odd = 0;
     }
-    const int64_t u = (int64_t)tid * per;
-    if (tid >= kPromptShares || u >= work) return;
-    // the share's first item: the one that has its first unit
-    int lo = 0, hi = p.seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (unit[mid] <= u) lo = mid; else hi = mid - 1;
-    }
-    const PromptSeq s = prompt_seq(p, lo);
-    const int qts = query_tiles(s.n), past = s.len - s.n;
-    int x = (int)u - unit[lo], i = 0;
-    if (at[lo] == p.cap && s.len > 0) {  // it does not fit: no keys
-      i = x / kItemSetup;
-    } else {
-      const int head = x / head_units(past, s.n);
-      x -= head * head_units(past, s.n);
-      int a = 0, z = qts - 1;
-      while (a < z) {
-        const int mid = (a + z + 1) >> 1;
-        if (units_before(past, mid) <= x) a = mid; else z = mid - 1;
+    for (int share = tid; share < shares; share += 256) {
+      const int64_t u = (int64_t)share * per;
+      if (u >= work) break;
+      // the share's first item: the one that has its first unit
+      int lo = 0, hi = p.seqs - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (unit[mid] <= u) lo = mid; else hi = mid - 1;
       }
-      i = head * qts + a;
+      const PromptSeq s = prompt_seq(p, lo);
+      const int qts = query_tiles(s.n, p.waves), past = s.len - s.n;
+      int x = (int)u - unit[lo], i = 0;
+      if (at[lo] == p.cap && s.len > 0) {  // it does not fit: no keys
+        i = x / kItemSetup;
+      } else {
+        const int head = x / head_units(past, s.n, p.waves);
+        x -= head * head_units(past, s.n, p.waves);
+        int a = 0, z = qts - 1;
+        while (a < z) {
+          const int mid = (a + z + 1) >> 1;
+          if (units_before(past, mid, p.waves) <= x) a = mid; else z = mid - 1;
+        }
+        i = head * qts + a;
+      }
+      p.plan->first[share] = item[lo] + i;
     }
-    p.plan->first[tid] = item[lo] + i;
     return;
   }
   const int r = lane & 31, half = lane >> 5;
@@ -445,24 +453,26 @@ __global__ __launch_bounds__(256, 2) void k_prompt_heads(PromptParams p) {
 }
 
 // ---------------------------------------------------------------- attend
-constexpr int kKeyLds = 24 * kFrag;  // a tile's keys: 16 fragments, and 8 of rope keys from kPeAt
-constexpr int kPeAt = 16 * kFrag;
-constexpr int kValLds = 16 * kFrag;  // its values
-// tiles in LDS: of keys two in use (a block of 32 each), one there or on its way, one requested; of values one less
+// A turn's blocks of 32 keys, W / 4, in LDS: 8 fragments of keys each, then 4 of rope keys each; 8 of values each
+constexpr __device__ int blocks_of(int waves) { return waves / 4; }
+constexpr __device__ int pe_at(int waves) { return blocks_of(waves) * 8 * kFrag; }
+constexpr __device__ int key_lds(int waves) { return blocks_of(waves) * 12 * kFrag; }
+constexpr __device__ int val_lds(int waves) { return blocks_of(waves) * 8 * kFrag; }
+// turns in LDS: of keys two in use (a block of 32 each), one there or on its way, one requested; of values one less
 constexpr int kKeyRing = 4, kValRing = 3;
 
 // a sequence's head's query tile, and the share's part of its keys
 struct Item {
-  int head, qt;       // qt: of 256 query rows
+  int head, qt;       // qt: of 32 W query rows
   int t0, n, past;    // the sequence's
   int tile;           // its first tile of packed rows; -1: they do not fit, -2: the end of the share
-  int tiles;          // of keys that the query tile sees
+  int tiles;          // turns of keys that the query tile sees
   int from, upto;     // the share's of them
   int parts;          // the shares behind this one that have some, where this one has the first and not all
 };
 constexpr int kItemWords = sizeof(Item) / 4, kItems = 64;
 // item o of the work, for the units begin .. end - 1 of share
-__device__ __forceinline__ Item item_of(const PromptParams& p, int o, int share, int begin, int end, int per) {
+__device__ __forceinline__ Item item_of(const PromptParams& p, int o, int share, int begin, int end, int per, int w) {
   Item it{};
   it.tile = -2;
   if (o >= p.plan->items) return it;
@@ -472,7 +482,7 @@ __device__ __forceinline__ Item item_of(const PromptParams& p, int o, int share,
     if (p.plan->item[mid] <= o) lo = mid; else hi = mid - 1;
   }
   const PromptSeq s = prompt_seq(p, lo);
-  const int at = p.plan->at[lo], qts = query_tiles(s.n), i = o - p.plan->item[lo];
+  const int at = p.plan->at[lo], qts = query_tiles(s.n, w), i = o - p.plan->item[lo];
   it.t0 = s.t0;
   it.n = s.n;
   it.past = s.len - s.n;
@@ -482,8 +492,8 @@ __device__ __forceinline__ Item item_of(const PromptParams& p, int o, int share,
   if (at < 0) {
     first += i * kItemSetup;
   } else {
-    first += it.head * head_units(it.past, it.n) + units_before(it.past, it.qt);
-    it.tiles = tiles_of(it.past, it.n, it.qt);
+    first += it.head * head_units(it.past, it.n, w) + units_before(it.past, it.qt, w);
+    it.tiles = turns_of(it.past, it.n, it.qt, w);
   }
   if (first >= end) return it;
   it.tile = at < 0 ? -1 : at >> 6;
@@ -522,13 +532,15 @@ struct Rows {
 constexpr float kLift = 7.0f;
 
 // a fragment along a block of 32 keys: 8 of them, then 4 of their rope values
+template <int W>
 __device__ __forceinline__ uint32_t key_frag(int kb, int ds) {
-  return ds < 8 ? (kb * 8 + ds) * kFrag : kPeAt + (kb * 4 + ds - 8) * kFrag;
+  return ds < 8 ? (kb * 8 + ds) * kFrag : pe_at(W) + (kb * 4 + ds - 8) * kFrag;
 }
 // scores of a block of 32 keys: A = keys, B = the queries
+template <int W>
 __device__ __forceinline__ void score(const Rows& r, f32x16& s, uint32_t at, int kb) {
 #pragma unroll
-  for (int ds = 0; ds < 12; ++ds) s = mfma32(lds_read<bf16x8>(at + key_frag(kb, ds)), r.q[ds], ds == 0 ? f32x16{} : s);
+  for (int ds = 0; ds < 12; ++ds) s = mfma32(lds_read<bf16x8>(at + key_frag<W>(kb, ds)), r.q[ds], ds == 0 ? f32x16{} : s);
 }
 __device__ __forceinline__ void mask_block(const Rows& r, f32x16& s, int key0, int half) {
 #pragma unroll
@@ -557,7 +569,9 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
   return top;
 }
 
-__global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
+template <int W>
+__global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
+  constexpr int NB = blocks_of(W), TK = 32 * NB, kKeyLds = key_lds(W), kValLds = val_lds(W);
   __shared__ __align__(1024) uint8_t ring[kKeyRing * kKeyLds + kValRing * kValLds];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
@@ -579,7 +593,7 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
       in_list = 0;
       __syncthreads();
       if (threadIdx.x < kItems) {
-        const Item x = item_of(p, listed + threadIdx.x, share, begin, end, per);
+        const Item x = item_of(p, listed + threadIdx.x, share, begin, end, per, W);
         int* to = list[threadIdx.x];
         to[0] = x.head, to[1] = x.qt, to[2] = x.t0, to[3] = x.n, to[4] = x.past, to[5] = x.tile, to[6] = x.tiles, to[7] = x.from,
         to[8] = x.upto, to[9] = x.parts;
@@ -592,108 +606,64 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
   };
   const int64_t kbs = p.cap / 32;
 
-  // The tiles of the share's items follow each other in LDS: tile i of the share in slot i of the rings. Where an item's
-  // are, a wave's fragments of the share's tile 0 had it come before it (scalar addresses, the lanes 16 bytes apart)
-  struct Source {
-    const uint8_t *k, *v, *pe;
-  };
-  auto source_of = [&](const Item& it, int pos) {
-    const int64_t tile = it.tile + it.from - pos, block = (int64_t)it.head * kbs + 2 * tile;
-    return Source{p.k + block * 8 * kFrag + wave * 2 * kFrag, p.v + block * 8 * kFrag + wave * 2 * kFrag,
-                  p.pe + (tile * 8 + wave) * kFrag};
-  };
-  Source here{}, there{};
-  int own = 0;  // the share's tiles up to the item's end
-  auto issue_k = [&](int i) {
-    const uint32_t to = uniform(k_ring + (i % kKeyRing) * kKeyLds + wave * 2 * kFrag);
-    const uint8_t* k = uniform((i < own ? here.k : there.k) + (int64_t)i * 16 * kFrag);
-    const uint8_t* pe = uniform((i < own ? here.pe : there.pe) + (int64_t)i * 8 * kFrag);
-    lds_dma16(k, lane * 16, to);
-    lds_dma16(k + kFrag, lane * 16, to + kFrag);
-    lds_dma16(pe, lane * 16, to + kPeAt - wave * kFrag);
-  };
-  auto issue_v = [&](int i) {
-    const uint32_t to = uniform(v_ring + (i % kValRing) * kValLds + wave * 2 * kFrag);
-    const uint8_t* v = uniform((i < own ? here.v : there.v) + (int64_t)i * 16 * kFrag);
-    lds_dma16(v, lane * 16, to);
-    lds_dma16(v + kFrag, lane * 16, to + kFrag);
-  };
-  Rows r;
-  auto load_q = [&](const Item& it) {
-    const int row = it.qt * kQRows + wave * 32 + col;
-    const uint16_t* qn = p.qn + (int64_t)(it.t0 + row) * p.qn_ts + (int64_t)it.head * p.qn_hs + 4 * half;
-    const uint16_t* qp = p.qp + (int64_t)(it.t0 + row) * p.qp_ts + (int64_t)it.head * p.qp_hs + 8 * half;
-    if (row < it.n) {  // (the other lanes' columns reach nothing)
-#pragma unroll
-      for (int ds = 0; ds < 8; ++ds) {
-        const u32x2 a = *(const u32x2*)(qn + 16 * ds), b = *(const u32x2*)(qn + 16 * ds + 8);
-        r.q[ds] = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
-      }
-#pragma unroll
-      for (int ds = 0; ds < 4; ++ds) r.q[8 + ds] = *(const bf16x8*)(qp + 16 * ds);
-    } else {
-#pragma unroll
-      for (int ds = 0; ds < 12; ++ds) r.q[ds] = bf16x8{};
-    }
-  };
-  Item it{}, next = next_item();
-  load_q(next);
-  int pos = 0;           // the share's tiles before the item's
-  int k_to = 0, v_to = 0;  // its tiles whose keys, values are requested
-  int k_there = 0;       // its tiles whose keys are there
-  bool steady = false;   // the last loads are the keys and values of one tile each, requested in turn
-  while (next.tile != -2) {
-    it = next;
-    next = next_item();
-    const int row0 = it.qt * kQRows + wave * 32, row = row0 + col;
-    const int from = it.from, upto = it.upto;
+  for (;;) {
+    const Item it = next_item();
+    if (it.tile == -2) break;
+    const int head = it.head, from = it.from, upto = it.upto;
+    const int row0 = it.qt * rows_of(W) + wave * 32, row = row0 + col;
     if (from >= upto) {
       if (it.tiles == 0 && from == 0) {
         const float none = it.tile < 0 ? __builtin_nanf("") : 0.0f;
 #pragma unroll
-        for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, it.head, row, f32x16{} + none, vb, 1.0f, half);
-        if (p.lse && half == 0 && row < it.n) p.lse[(int64_t)(it.t0 + row) * p.heads + it.head] = it.tile < 0 ? none : -__builtin_inff();
+        for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, head, row, f32x16{} + none, vb, 1.0f, half);
+        if (p.lse && half == 0 && row < it.n) p.lse[(int64_t)(it.t0 + row) * p.heads + head] = it.tile < 0 ? none : -__builtin_inff();
       }
-      load_q(next);
       continue;
     }
-    const int next_tiles = next.tile >= 0 ? max(0, next.upto - next.from) : 0;
-    here = source_of(it, pos);
-    own = pos + upto - from;
-    if (next_tiles > 0) there = source_of(next, own);
-    const int known = own + next_tiles;
-    auto request = [&](int k_end, int v_end) {
-      for (k_end = min(k_end, known); k_to < k_end; ++k_to) issue_k(k_to);
-      for (v_end = min(v_end, known); v_to < v_end; ++v_to) issue_v(v_to);
+
+    const int64_t kb0 = 2 * (int64_t)it.tile;
+    // (a wave's fragments; scalar addresses, the lanes 16 bytes apart)
+    const uint8_t* kbase = p.k + ((int64_t)head * kbs + kb0) * 8 * kFrag + wave * 2 * kFrag;
+    const uint8_t* vbase = p.v + ((int64_t)head * kbs + kb0) * 8 * kFrag + wave * 2 * kFrag;
+    const uint8_t* pbase = p.pe + kb0 * 4 * kFrag + wave * kFrag;
+    auto issue_k = [&](int kt) {
+      const uint32_t to = k_ring + (kt % kKeyRing) * kKeyLds;
+      const uint8_t* from_k = kbase + (int64_t)kt * NB * 8 * kFrag;
+      lds_dma16(from_k, lane * 16, to + wave * 2 * kFrag);
+      lds_dma16(from_k + kFrag, lane * 16, to + wave * 2 * kFrag + kFrag);
+      lds_dma16(pbase + (int64_t)kt * NB * 4 * kFrag, lane * 16, to + pe_at(W) + wave * kFrag);
     };
-    // at a tile's turn its own and the next one's keys are there, and its values; the ones behind are on their way
-    auto turn = [&](int i) {
-      if (steady) {
-        wait_loads<5>();
-        k_there = i + 2;
-      } else {
-        wait_loads<0>();
-        k_there = k_to;
-      }
-      barrier();
-      steady = k_to == i + 3 && v_to == i + 2 && i + 3 < known;
-      if (steady) {
-        issue_k(k_to++);
-        issue_v(v_to++);
-      } else {
-        request(i + 4, i + 3);
-      }
+    auto issue_v = [&](int kt) {
+      const uint32_t to = v_ring + (kt % kValRing) * kValLds + wave * 2 * kFrag;
+      const uint8_t* from_v = vbase + (int64_t)kt * NB * 8 * kFrag;
+      lds_dma16(from_v, lane * 16, to);
+      lds_dma16(from_v + kFrag, lane * 16, to + kFrag);
     };
 
+    Rows r;
+    {
+      const uint16_t* qn = p.qn + (int64_t)(it.t0 + row) * p.qn_ts + (int64_t)head * p.qn_hs + 4 * half;
+      const uint16_t* qp = p.qp + (int64_t)(it.t0 + row) * p.qp_ts + (int64_t)head * p.qp_hs + 8 * half;
+#pragma unroll
+      for (int ds = 0; ds < 12; ++ds) r.q[ds] = bf16x8{};
+      if (row < it.n) {  // (the other columns reach nothing)
+#pragma unroll
+        for (int ds = 0; ds < 8; ++ds) {
+          const u32x2 a = *(const u32x2*)(qn + 16 * ds), b = *(const u32x2*)(qn + 16 * ds + 8);
+          r.q[ds] = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+        }
+#pragma unroll
+        for (int ds = 0; ds < 4; ++ds) r.q[8 + ds] = *(const bf16x8*)(qp + 16 * ds);
+      }
+    }
     // whether some of the tiles have values in bf16
-    const int32_t* odd = p.odd + (int64_t)it.head * (p.cap / kKeys) + it.tile;
+    const int32_t* odd = p.odd + (int64_t)head * (p.cap / kKeys) + it.tile;
     bool mixed = false;
     if (any_odd) {
-      for (int kt = from + lane; kt < upto; kt += 64) mixed |= odd[kt] != 0;
+      for (int kt = from + lane; kt < upto; kt += 64) mixed |= odd[kt * TK / kKeys] != 0;
       mixed = __ballot(mixed) != 0;
     }
-    request(pos + 3, pos + 2);
-    steady = false;  // (other loads and stores are on their way)
+    barrier();  // every wave has read the turns of the item before
 
     r.m = -__builtin_inff();
     r.mu = r.sum = 0.0f;
@@ -702,186 +672,194 @@ __global__ __launch_bounds__(512, 2) void k_prompt_attend(PromptParams p) {
     for (int vb = 0; vb < 4; ++vb) r.o[vb] = f32x16{};
     // the tiles that the wave's rows see, and those that all of them see whole
     const int last_row = min(row0 + 31, it.n - 1);
-    const int seen = row0 < it.n ? min(upto, (it.past + last_row + kKeys) >> 6) : from;
-    const int whole = (it.past + row0 + 1) >> 6;
-    auto keys_at = [&](int kt) { return k_ring + ((pos + kt - from) % kKeyRing) * kKeyLds + lane * 16; };
-    auto vals_at = [&](int kt) { return v_ring + ((pos + kt - from) % kValRing) * kValLds + lane * 16; };
-    // a block of 32 keys' scores are formed one block ahead: its numerators then come under the next one's products
-    auto finish = [&]() {
-      const auto sw = __builtin_amdgcn_permlane32_swap(f2u(r.sum), f2u(r.sum), false, false);
-      const float sum = u2f(sw[0]) + u2f(sw[1]);
-      if (from == 0 && upto == it.tiles) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, it.head, row, r.o[vb], vb, inv, half);
-        if (p.lse && half == 0 && row < it.n)
-          p.lse[(int64_t)(it.t0 + row) * p.heads + it.head] = sum == 0.0f ? -__builtin_inff() : (r.mu + __builtin_amdgcn_logf(sum)) * kLog2;
-      } else if (row0 < it.n) {
-        const int slot = 2 * share + (from == 0);
-        f32x4* to = (f32x4*)p.part_o + ((int64_t)slot * 8 + wave) * 16 * 64 + lane;
-#pragma unroll
-        for (int vb = 0; vb < 4; ++vb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            to[(vb * 4 + i) * 64] = f32x4{r.o[vb][4 * i], r.o[vb][4 * i + 1], r.o[vb][4 * i + 2], r.o[vb][4 * i + 3]};
-        // (where the row saw no score yet its sum is 0, and the part counts for nothing)
-        const float mu = r.m == -__builtin_inff() ? r.m : r.mu;
-        if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * kQRows + wave * 32 + col) * 2) = f32x2{mu, sum};
-      }
-    };
-    f32x16 s0, s1;
-    if (k_there <= pos) {
-      wait_loads<0>();
+    const int seen = row0 < it.n ? min(upto, (it.past + last_row + TK) >> key_shift(W)) : from;
+    const int whole = (it.past + row0 + 1) >> key_shift(W);
+
+    issue_k(from);
+    if (from + 1 < upto) issue_k(from + 1);
+    issue_v(from);
+    if (from + 2 < upto) issue_k(from + 2);
+    if (from + 1 < upto) issue_v(from + 1);
+    // at turn kt the keys of kt + 1 and the values of kt are there; the next turn's are on their way
+    auto turn = [&](int kt) {
+      if (kt + 2 < upto)
+        wait_loads<5>();
+      else
+        wait_loads<0>();
       barrier();
-      k_there = k_to;
-    }
+      if (kt + 3 < upto) issue_k(kt + 3);
+      if (kt + 2 < upto) issue_v(kt + 2);
+    };
+    auto keys_at = [&](int kt) { return k_ring + (kt % kKeyRing) * kKeyLds + lane * 16; };
+    auto vals_at = [&](int kt) { return v_ring + (kt % kValRing) * kValLds + lane * 16; };
+    // a block of 32 keys' scores are formed one block ahead: its numerators then come under the next one's products
+    f32x16 s0, s1;
+    if (from + 2 < upto)
+      wait_loads<10>();
+    else
+      wait_loads<0>();
+    barrier();
     int kt = from;
     if (seen > from) {
-      score(r, s0, keys_at(from), 0);
-      if (from >= whole) mask_block(r, s0, from * kKeys, half);
+      score<W>(r, s0, keys_at(from), 0);
+      if (from >= whole) mask_block(r, s0, from * TK, half);
       move_max(p, r, top_of(s0));
     }
-    if (!mixed && seen > from) {
-      for (;; ++kt) {
-        turn(pos + kt - from);
-        const bool more = kt + 1 < seen;
-        const uint32_t k_at = keys_at(kt), next_at = keys_at(kt + 1), v_at = vals_at(kt);
-        // 40 fragments in turn: 12 of keys for the next block's scores, 8 of values for this one's outputs, twice; each is
-        // read two products before its own
-        auto frag = [&](int i) {
-          const int hh = i / 20, j = i % 20;
-          return lds_read<u32x4>(j >= 12 ? v_at + (hh * 8 + j - 12) * kFrag : hh == 0 ? k_at + key_frag(1, j) : next_at + key_frag(0, j));
-        };
-        u32x4 f[3], num[2];
-        auto pair = [&](const f32x16& now, int x) {
-          uint32_t w = pack_f16(__builtin_amdgcn_exp2f(now[2 * x] * p.scale2 - r.mu), __builtin_amdgcn_exp2f(now[2 * x + 1] * p.scale2 - r.mu));
-          r.sum = add_f16(w, r.sum);
-          asm volatile("" : "+v"(w), "+v"(r.sum));  // (formed here, not where they are used)
-          num[x >> 2][x & 3] = w;
+    bool swapped = false;
+    while (!mixed && kt + 1 < seen) {  // two blocks a time, of one turn or of two
+      turn(kt);
+      uint32_t k_at = keys_at(NB == 2 ? kt : kt + 1), v_at = vals_at(kt), next_at = keys_at(kt + 1);
+      // 20 fragments a block in turn: 12 of keys for the next block's scores, 8 of values for this one's outputs; each
+      // is read two products before its own
+      u32x4 f[3], num[2];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        if (NB == 1 && hh == 1) {
+          ++kt;
+          swapped = kt + 1 >= seen;
+          if (swapped) break;
+          turn(kt);
+          next_at = keys_at(kt + 1);
+          v_at = vals_at(kt);
+        }
+        f32x16 &now = hh == 0 ? s0 : s1, &then = hh == 0 ? s1 : s0;
+        auto frag = [&](int j) {
+          return lds_read<u32x4>(j >= 12  ? v_at + ((NB == 2 ? hh * 8 : 0) + j - 12) * kFrag
+                                 : hh == 0 ? k_at + key_frag<W>(NB - 1, j)
+                                           : next_at + key_frag<W>(0, j));
         };
         f[0] = frag(0);
         f[1] = frag(1);
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          f32x16 &now = hh == 0 ? s0 : s1, &next_s = hh == 0 ? s1 : s0;
-          if (hh == 1 && !more) break;
+        for (int j = 0; j < 12; ++j) {
+          f[(j + 2) % 3] = frag(j + 2);
+          then = mfma32(__builtin_bit_cast(bf16x8, f[j % 3]), r.q[j], j == 0 ? f32x16{} : then);
 #pragma unroll
-          for (int j = 0; j < 12; ++j) {
-            const int i = hh * 20 + j;
-            f[(i + 2) % 3] = frag(i + 2);
-            next_s = mfma32(__builtin_bit_cast(bf16x8, f[i % 3]), r.q[j], j == 0 ? f32x16{} : next_s);
-#pragma unroll
-            for (int x = j * 8 / 12; x < (j + 1) * 8 / 12; ++x) pair(now, x);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          const int key0 = kt * kKeys + (hh == 0 ? 32 : kKeys);
-          float top = -__builtin_inff();
-#pragma unroll
-          for (int j = 12; j < 20; ++j) {
-            const int i = hh * 20 + j, vb = j & 3;
-            if (i + 2 < 40) f[(i + 2) % 3] = frag(i + 2);
-            r.o[vb] = mfma32(__builtin_bit_cast(f16x8, f[i % 3]), __builtin_bit_cast(f16x8, num[(j - 12) >> 2]), r.o[vb]);
-            if (j == 14 && kt + hh >= whole) mask_block(r, next_s, key0, half);
-            if (j >= 14) {
-#pragma unroll
-              for (int x = (j - 14) * 8 / 6; x < (j - 13) * 8 / 6; ++x) top = max3(top, next_s[2 * x], next_s[2 * x + 1]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          move_max(p, r, top);
-        }
-        if (more) continue;
-        // the last block: the queries have been used, the next item's arrive meanwhile
-        load_q(next);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) pair(s1, x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + (8 + j) * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
-        ++kt;
-        break;
-      }
-      finish();
-      for (; kt < upto; ++kt) turn(pos + kt - from);
-    } else {
-      for (; kt < upto; ++kt) {
-        turn(pos + kt - from);
-        if (kt >= seen) continue;
-        const bool in_bf = mixed && odd[kt] != 0;
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
-          u32x4 num[2];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - r.mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - r.mu);
-            const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
-            r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
+          for (int x = j * 8 / 12; x < (j + 1) * 8 / 12; ++x) {
+            uint32_t w = pack_f16(__builtin_amdgcn_exp2f(now[2 * x] * p.scale2 - r.mu),
+                                  __builtin_amdgcn_exp2f(now[2 * x + 1] * p.scale2 - r.mu));
+            r.sum = add_f16(w, r.sum);
+            asm volatile("" : "+v"(w), "+v"(r.sum));  // (formed here, not where they are used)
             num[x >> 2][x & 3] = w;
           }
-          if (in_bf && kt >= whole) {
-            // values that may not be finite, of tokens that some rows do not see: a key at a time, added where it is seen
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // the next block's turn and first key
+        const int next_kt = NB == 2 ? kt + hh : kt + 1, key0 = NB == 2 ? kt * TK + (hh + 1) * 32 : (kt + 1) * TK;
+        float top = -__builtin_inff();
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+        for (int j = 12; j < 20; ++j) {
+          const int vb = j & 3;
+          if (j + 2 < 20) f[(j + 2) % 3] = frag(j + 2);
+          r.o[vb] = mfma32(__builtin_bit_cast(f16x8, f[j % 3]), __builtin_bit_cast(f16x8, num[(j - 12) >> 2]), r.o[vb]);
+          if (j == 14 && next_kt >= whole) mask_block(r, then, key0, half);
+          if (j >= 14) {
+#pragma unroll
+            for (int x = (j - 14) * 8 / 6; x < (j - 13) * 8 / 6; ++x) top = max3(top, then[2 * x], then[2 * x + 1]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        move_max(p, r, top);
+      }
+      if (!swapped) ++kt;
+    }
+    if (swapped) s0 = s1;
+    for (; kt < upto; ++kt) {
+      turn(kt);
+      if (kt >= seen) continue;
+      const bool in_bf = mixed && odd[kt * TK / kKeys] != 0;
+#pragma unroll
+      for (int hh = 0; hh < NB; ++hh) {
+        const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
+        u32x4 num[2];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - r.mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - r.mu);
+          const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
+          r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
+          num[x >> 2][x & 3] = w;
+        }
+        if (in_bf && kt >= whole) {
+          // values that may not be finite, of tokens that some rows do not see: a key at a time, added where it is seen
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
 #pragma unroll 1
-              for (int x = 0; x < 16; ++x) {
-                const int h = x >> 3, e = x & 7;
-                const bool sees = kt * kKeys + 32 * hh + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= r.sees;
-                const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
-                const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
-                const bf16x8 one = __builtin_bit_cast(bf16x8, num[t] & only);
+            for (int x = 0; x < 16; ++x) {
+              const int h = x >> 3, e = x & 7;
+              const bool sees = kt * TK + 32 * hh + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= r.sees;
+              const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+              const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
+              const bf16x8 one = __builtin_bit_cast(bf16x8, num[t] & only);
 #pragma unroll
-                for (int vb = 0; vb < 4; ++vb) {
-                  const u32x4 a = lds_read<u32x4>(v_at + (t * 4 + vb) * kFrag);
-                  const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
+              for (int vb = 0; vb < 4; ++vb) {
+                const u32x4 a = lds_read<u32x4>(v_at + (t * 4 + vb) * kFrag);
+                const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) r.o[vb][i] += sees ? add[i] : 0.0f;
-                }
+                for (int i = 0; i < 16; ++i) r.o[vb][i] += sees ? add[i] : 0.0f;
               }
-          } else if (in_bf) {
+            }
+        } else if (in_bf) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              r.o[j & 3] = mfma32(lds_read<bf16x8>(v_at + j * kFrag), __builtin_bit_cast(bf16x8, num[j >> 2]), r.o[j & 3]);
-          } else {
+          for (int j = 0; j < 8; ++j)
+            r.o[j & 3] = mfma32(lds_read<bf16x8>(v_at + j * kFrag), __builtin_bit_cast(bf16x8, num[j >> 2]), r.o[j & 3]);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + j * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
-          }
-          if (kt + hh < seen) {
-            score(r, s0, hh == 0 ? keys_at(kt) : keys_at(kt + 1), 1 - hh);
-            if (kt + hh >= whole) mask_block(r, s0, kt * kKeys + (hh == 0 ? 32 : kKeys), half);
-            move_max(p, r, top_of(s0));
-          }
+          for (int j = 0; j < 8; ++j)
+            r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + j * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
+        }
+        const int then = kt + (hh + 1) / NB;  // the next block's turn
+        if (then < seen) {
+          score<W>(r, s0, keys_at(then), (hh + 1) % NB);
+          if (then >= whole) mask_block(r, s0, kt * TK + (hh + 1) * 32, half);
+          move_max(p, r, top_of(s0));
         }
       }
-      load_q(next);
-      finish();
+    }
+    const auto sw = __builtin_amdgcn_permlane32_swap(f2u(r.sum), f2u(r.sum), false, false);
+    const float sum = u2f(sw[0]) + u2f(sw[1]);
+    if (from == 0 && upto == it.tiles) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, head, row, r.o[vb], vb, inv, half);
+      if (p.lse && half == 0 && row < it.n)
+        p.lse[(int64_t)(it.t0 + row) * p.heads + head] = sum == 0.0f ? -__builtin_inff() : (r.mu + __builtin_amdgcn_logf(sum)) * kLog2;
+    } else if (row0 < it.n) {
+      const int slot = 2 * share + (from == 0);
+      f32x4* to = (f32x4*)p.part_o + ((int64_t)slot * W + wave) * 16 * 64 + lane;
+#pragma unroll
+      for (int vb = 0; vb < 4; ++vb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          to[(vb * 4 + i) * 64] = f32x4{r.o[vb][4 * i], r.o[vb][4 * i + 1], r.o[vb][4 * i + 2], r.o[vb][4 * i + 3]};
+      // (where the row saw no score yet its sum is 0, and the part counts for nothing)
+      const float mu = r.m == -__builtin_inff() ? r.m : r.mu;
+      if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * rows_of(W) + wave * 32 + col) * 2) = f32x2{mu, sum};
     }
     if (it.parts > 0) cut = PromptCut{it.parts, it.head, it.t0, it.n, it.qt, {}};
-    pos += upto - from;
   }
   if (threadIdx.x == 0) p.cut[share] = cut;
 }
 
 // The parts of a query tile that the end of a share cut, joined in order: (share, 32 rows) a workgroup, 32 values a
 // wave. The lanes have the values that the attention's had.
+template <int W>
 __global__ __launch_bounds__(256) void k_prompt_merge(PromptParams p) {
   const int lane = threadIdx.x & 63, vb = threadIdx.x >> 6, share = blockIdx.x, group = blockIdx.y;
   const int half = lane >> 5, col = lane & 31;
   if (share * p.plan->per >= p.plan->total) return;  // (no such share)
   const PromptCut c = p.cut[share];
-  const int row0 = c.qt * kQRows + group * 32, row = row0 + col;
+  const int row0 = c.qt * rows_of(W) + group * 32, row = row0 + col;
   if (c.parts == 0 || row0 >= c.n) return;
   auto slot = [&](int i) { return 2 * (share + i) + (i == 0); };
   float top = -__builtin_inff();
-  for (int i = 0; i <= c.parts; ++i) top = fmaxf(top, p.part_ml[((int64_t)slot(i) * kQRows + group * 32 + col) * 2]);
+  for (int i = 0; i <= c.parts; ++i) top = fmaxf(top, p.part_ml[((int64_t)slot(i) * rows_of(W) + group * 32 + col) * 2]);
   f32x16 o = {};
   float sum = 0.0f;
   for (int i = 0; i <= c.parts; ++i) {
-    const f32x2 ml = *(const f32x2*)(p.part_ml + ((int64_t)slot(i) * kQRows + group * 32 + col) * 2);
+    const f32x2 ml = *(const f32x2*)(p.part_ml + ((int64_t)slot(i) * rows_of(W) + group * 32 + col) * 2);
     const float by = ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - top);
     sum += ml[1] * by;
-    const f32x4* from = (const f32x4*)p.part_o + ((int64_t)slot(i) * 8 + group) * 16 * 64 + vb * 4 * 64 + lane;
+    const f32x4* from = (const f32x4*)p.part_o + ((int64_t)slot(i) * W + group) * 16 * 64 + vb * 4 * 64 + lane;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const f32x4 x = from[j * 64];
@@ -909,9 +887,9 @@ inline PromptLayout prompt_layout(int heads, int64_t cap) {
     return from;
   };
   l.plan = take(sizeof(Plan));
-  l.cut = take(kPromptShares * sizeof(PromptCut));
-  l.part_ml = take((size_t)2 * kPromptShares * kQRows * 2 * 4);
-  l.part_o = take((size_t)2 * kPromptShares * kQRows * kV * 4);
+  l.cut = take(kMaxShares * sizeof(PromptCut));
+  l.part_ml = take((size_t)2 * 2048 * 32 * 2 * 4);
+  l.part_o = take((size_t)2 * 2048 * 32 * kV * 4);
   l.odd = take((size_t)heads * (cap / kKeys) * 4);
   l.pe = take((size_t)cap * kR * 2);
   l.c = take((size_t)cap * kL * 2);
@@ -923,6 +901,10 @@ inline PromptLayout prompt_layout(int heads, int64_t cap) {
 constexpr int kMaxContext = 1 << 22, kMaxPromptTokens = 1 << 20;
 inline int64_t packed_rows(int32_t context) { return ((int64_t)context + kMTok - 1) & -(int64_t)kMTok; }
 
+inline int waves_for(const mkmoe_latent_prompt_io* io) {
+  const char* e = getenv("MKW");
+  return e ? atoi(e) : 8;
+}
 inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_bytes, PromptParams& p) {
   if (!io || !ws) return MKMOE_ERR_NULL;
   if (!aligned(ws, 256)) return MKMOE_ERR_ALIGN;
@@ -940,8 +922,9 @@ inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_b
   const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
   if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
   // the work's units are counted in 32 bits
-  const int64_t keys = (max_len < cap ? max_len : cap) / kKeys + 1 + kItemSetup;
-  if (((int64_t)io->tokens / kQRows + io->seqs) * io->heads * keys > 0x3fffffff) return MKMOE_ERR_ARG;
+  p.waves = waves_for(io);
+  const int64_t units = ((max_len < cap ? max_len : cap) >> key_shift(p.waves)) + 1 + kItemSetup;
+  if (((int64_t)io->tokens / rows_of(p.waves) + io->seqs) * io->heads * units > 0x3fffffff) return MKMOE_ERR_ARG;
   const void* wide[] = {io->q_nope, io->q_pe, io->w, io->out};
   for (const void* q : wide)
     if (!aligned(q, 16)) return MKMOE_ERR_ALIGN;
@@ -993,6 +976,13 @@ inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_b
   return MKMOE_OK;
 }
 
+template <int W>
+int attend_and_merge(const PromptParams& p, hipStream_t st) {
+  hipLaunchKernelGGL(k_prompt_attend<W>, dim3(shares_of(W)), dim3(64 * W), 0, st, p);
+  if (int rc = launched()) return rc;
+  hipLaunchKernelGGL(k_prompt_merge<W>, dim3(shares_of(W), W), dim3(256), 0, st, p);
+  return launched();
+}
 inline int prompt_launch(const PromptParams& p, bool mx, hipStream_t st) {
   const int64_t rows = p.cap < (int64_t)p.seqs * p.max_len ? p.cap : (int64_t)p.seqs * p.max_len;
   const int64_t blocks = (rows + 31) / 32 + p.seqs;
@@ -1002,12 +992,9 @@ inline int prompt_launch(const PromptParams& p, bool mx, hipStream_t st) {
   else
     hipLaunchKernelGGL(k_prompt_rows<false>, grid, dim3(256), 0, st, p);
   if (int rc = launched()) return rc;
-  hipLaunchKernelGGL(k_prompt_heads, dim3(2 * kPromptShares), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(k_prompt_heads, dim3(512), dim3(256), 0, st, p);
   if (int rc = launched()) return rc;
-  hipLaunchKernelGGL(k_prompt_attend, dim3(kPromptShares), dim3(512), 0, st, p);
-  if (int rc = launched()) return rc;
-  hipLaunchKernelGGL(k_prompt_merge, dim3(kPromptShares, kQRows / 32), dim3(256), 0, st, p);
-  return launched();
+  return p.waves == 8 ? attend_and_merge<8>(p, st) : attend_and_merge<4>(p, st);
 }
 
 }  // namespace mkmoe_latent
