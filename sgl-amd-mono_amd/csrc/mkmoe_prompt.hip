@@ -22,7 +22,6 @@
 // the next one's operand in place: keys and values are stored, and numerators used, without
 // any exchange between lanes.
 
-#include <stdlib.h>
 #include "mkmoe_latent.h"
 
 namespace mkmoe_latent {
@@ -39,7 +38,7 @@ constexpr int kKeys = 64;           // a sequence's packed rows are a multiple o
 constexpr int kLeastUnits = 6;      // units of work that a share has
 constexpr int kFrag = 1024;         // bytes of a fragment
 constexpr int kPromptSeqs = MKMOE_LATENT_MAX_SEQS;
-constexpr int kItemSetup = 4;       // what starting and storing a query tile takes, in tiles of keys
+constexpr int kItemSetup = 8;       // what starting and storing a query tile takes, in tiles of keys
 constexpr float kMoveBy = 8.0f;     // a row's maximum moves where a score passes it by more than 2^kMoveBy
 constexpr float kLog2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 
@@ -852,14 +851,17 @@ __global__ __launch_bounds__(256) void k_prompt_merge(PromptParams p) {
   if (c.parts == 0 || row0 >= c.n) return;
   auto slot = [&](int i) { return 2 * (share + i) + (i == 0); };
   float top = -__builtin_inff();
+#pragma unroll 8
   for (int i = 0; i <= c.parts; ++i) top = fmaxf(top, p.part_ml[((int64_t)slot(i) * rows_of(W) + group * 32 + col) * 2]);
   f32x16 o = {};
   float sum = 0.0f;
+  const f32x4* parts = (const f32x4*)p.part_o + (int64_t)group * 16 * 64 + vb * 4 * 64 + lane;
+#pragma unroll 4  // (so many parts' loads on their way)
   for (int i = 0; i <= c.parts; ++i) {
     const f32x2 ml = *(const f32x2*)(p.part_ml + ((int64_t)slot(i) * rows_of(W) + group * 32 + col) * 2);
     const float by = ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - top);
+    const f32x4* from = parts + (int64_t)slot(i) * W * 16 * 64;
     sum += ml[1] * by;
-    const f32x4* from = (const f32x4*)p.part_o + ((int64_t)slot(i) * W + group) * 16 * 64 + vb * 4 * 64 + lane;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const f32x4 x = from[j * 64];
@@ -901,9 +903,13 @@ inline PromptLayout prompt_layout(int heads, int64_t cap) {
 constexpr int kMaxContext = 1 << 22, kMaxPromptTokens = 1 << 20;
 inline int64_t packed_rows(int32_t context) { return ((int64_t)context + kMTok - 1) & -(int64_t)kMTok; }
 
+// 8 waves a workgroup read the keys and values half as often, 4 (two workgroups a CU) run one's start and end under the
+// other's turns: 4 where there are few query tiles, unless the cached tokens may be many more than the new ones (4 and 8
+// waves, us: 193 tokens over 893, 16 heads 42 and 50; 512 and 2048 tokens alone, 32 heads 47 and 53, 102 and 106;
+// 4096 alone 246 and 242, 8 times 1024 over 2048, 16 heads 254 and 238; 300 over 65300, 16 heads 723 and 672)
 inline int waves_for(const mkmoe_latent_prompt_io* io) {
-  const char* e = getenv("MKW");
-  return e ? atoi(e) : 8;
+  const int64_t tiles = ((int64_t)io->tokens / rows_of(8) + io->seqs) * io->heads;
+  return tiles <= 320 && io->max_context / 128 < io->tokens ? 4 : 8;
 }
 inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_bytes, PromptParams& p) {
   if (!io || !ws) return MKMOE_ERR_NULL;
