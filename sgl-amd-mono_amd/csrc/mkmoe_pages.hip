@@ -75,18 +75,26 @@ __device__ __forceinline__ int pages_for(const Params& p, int len) { return (int
 __device__ __forceinline__ int clamped(const Params& p, int len) {
   return (int)min((int64_t)max(len, 0), (int64_t)p.max_pages << p.shift);
 }
-// a page's sequence lets go of it
-__device__ __forceinline__ void release(const Params& p, int page, int where) {
-  if ((uint32_t)page >= (uint32_t)p.pages) {
+// Pages' sequences let go of them, a page a lane (where there is one). The blocks' free pages are counted a wave at a
+// time: an atomic addition for each page took 310 us where 98000 that follow each other were freed, so 7
+__device__ __forceinline__ void release(const Params& p, bool there, int page, int where) {
+  bool freed = false;
+  if (there && (uint32_t)page >= (uint32_t)p.pages) {
     record(p.head, MKMOE_PAGES_ERR_PAGE, where);
-    return;
+  } else if (there) {
+    const int was = atomicSub(p.refs + page, 1);
+    freed = was == 1;
+    if (was < 1) {  // nobody held it
+      atomicAdd(p.refs + page, 1);
+      record(p.head, MKMOE_PAGES_ERR_PAGE, where);
+    }
   }
-  const int was = atomicSub(p.refs + page, 1);
-  if (was == 1) {
-    atomicAdd(p.free_in + page / kBlock, 1);
-  } else if (was < 1) {  // nobody held it
-    atomicAdd(p.refs + page, 1);
-    record(p.head, MKMOE_PAGES_ERR_PAGE, where);
+  const int block = page / kBlock;
+  for (uint64_t left = __ballot(freed); left != 0;) {
+    const int first = __builtin_ctzll(left);
+    const uint64_t same = __ballot(freed && block == __builtin_amdgcn_readlane(block, first));
+    if ((int)(threadIdx.x & 63) == first) atomicAdd(p.free_in + block, __builtin_popcountll(same));
+    left &= ~same;
   }
 }
 
@@ -175,6 +183,8 @@ template <int OP>
 __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
   __shared__ TakeSmem sm;
   const int tid = threadIdx.x;
+  // (the first sequences' values, on their way meanwhile)
+  const int len0 = tid < p.seqs ? p.lens[tid] : 0, arg0 = tid < p.seqs ? p.arg[tid] : 0;
   // free pages before each block
   int free_pages = 0;
   for (int j0 = 0; j0 < p.blocks; j0 += kThreads) {
@@ -189,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
     for (int b = tid; b < p.seqs; b += kThreads) sm.lead[b] = p.seqs;
     __syncthreads();
     for (int b = tid; b < p.seqs; b += kThreads) {
-      const int r = p.arg[b];
+      const int r = b < kThreads ? arg0 : p.arg[b];
       if ((uint32_t)r < (uint32_t)p.seqs) atomicMin(&sm.lead[r], b);
     }
   }
@@ -202,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
     int len = 0, to = 0, need = 0, add = 0;
     bool room = true;
     if (there) {
-      const int raw = p.lens[b], arg = p.arg[b];
+      const int raw = b0 == 0 ? len0 : p.lens[b], arg = b0 == 0 ? arg0 : p.arg[b];
       len = to = clamped(p, raw);
       if (len != raw && blockIdx.x == 0) record(p.head, MKMOE_PAGES_ERR_BOUNDS, b);
       if constexpr (OP == kGrow) {
@@ -255,6 +265,7 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
   for (int j = blockIdx.x; j < p.blocks; j += gridDim.x) {
     const int before = sm.before[j];
     if (before >= taken) break;  // (in order)
+    if ((j + 1 < p.blocks ? sm.before[j + 1] : free_pages) == before) continue;
     i32x4 refs = {1, 1, 1, 1};
     const int page0 = j * kBlock + 4 * tid;
     if (page0 + 4 <= p.pages)
@@ -286,9 +297,7 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
         sm.at[mine - before] = entry << p.shift;
         sm.seq[mine - before] = lo;
       } else {
-        const int row = OP == kTrim ? lo : p.arg[lo];
         p.new_page[lo] = page;
-        p.src[mine] = p.table[row * p.table_stride + (sm.to[lo] >> p.shift)];
         p.dst[mine] = page;
       }
     }
@@ -327,14 +336,19 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
       p.slots[t] = slot;
       p.positions[t] = at;
     }
-    if (blockIdx.x == 0)
+    if (blockIdx.x == gridDim.x - 1)
       for (int b = tid; b <= p.seqs; b += kThreads) p.starts[b] = sm.from[b];
-  } else if (blockIdx.x == 0) {
+  } else if (blockIdx.x == gridDim.x - 1) {
     for (int b = tid; b < p.seqs; b += kThreads) {
       p.old_len[b] = sm.len[b];
       p.new_len[b] = sm.to[b];
       // (no page was taken for it where the next one's first rank is its own)
-      if ((b + 1 < p.seqs ? sm.first[b + 1] : taken) <= sm.first[b] || sm.first[b] >= taken) p.new_page[b] = -1;
+      if ((b + 1 < p.seqs ? sm.first[b + 1] : taken) <= sm.first[b] || sm.first[b] >= taken) {
+        p.new_page[b] = -1;
+      } else {
+        const int row = OP == kTrim ? b : p.arg[b];
+        p.src[sm.first[b]] = p.table[row * p.table_stride + (sm.to[b] >> p.shift)];
+      }
     }
     if (tid == 0) p.head->moves = taken;
   }
@@ -344,7 +358,7 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
       const int n = pages_for(p, sm.len[b]);
       for (int i = tid; i < n; i += kThreads) p.held[(int64_t)b * p.max_pages + i] = p.table[b * p.table_stride + i];
     }
-    if (blockIdx.x == 0) {
+    if (blockIdx.x == gridDim.x / 2) {
       for (int b = tid; b < p.seqs; b += kThreads) sm.lead[b] = 0;
       __syncthreads();
       for (int b = tid; b < p.seqs; b += kThreads) {
@@ -358,14 +372,16 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
 
   // the last one to be done: nobody reads what it writes any more
   __syncthreads();
-  if (tid == 0) {
+  if (gridDim.x > 1) {
+    if (tid == 0) {
+      __threadfence();
+      sm.last = atomicAdd(&p.head->arrived, 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!sm.last) return;
     __threadfence();
-    sm.last = atomicAdd(&p.head->arrived, 1) == (int)gridDim.x - 1;
+    if (tid == 0) p.head->arrived = 0;
   }
-  __syncthreads();
-  if (!sm.last) return;
-  __threadfence();
-  if (tid == 0) p.head->arrived = 0;
   for (int j = tid; j < p.blocks; j += kThreads) {
     const int before = sm.before[j];
     if (before >= taken) break;
@@ -376,39 +392,60 @@ __global__ __launch_bounds__(kThreads) void k_pages_take(Params p) {
 }
 
 // ---------------------------------------------------------------- pages copied
-// Pages src[i] to dst[i] of every cache, 16 KB a workgroup and turn; pages outside the pool are left out
+// Pages src[i] to dst[i] of every cache, 16 KB a workgroup and turn; pages outside the pool are left out. The caches'
+// chunks follow each other, so that few pages keep every workgroup at work, and the caches' places are in LDS: read one
+// after the other, 24 of them took 25 us where there was nothing to copy
+constexpr int kCaches = 128;  // places in LDS
 __device__ __forceinline__ void copy_pages(const Params& p, const int32_t* src, const int32_t* dst, int n, bool check) {
-  const int tid = threadIdx.x, groups = gridDim.x * gridDim.y, me = blockIdx.y * gridDim.x + blockIdx.x;
-  for (int c = 0; c < p.ncaches; ++c) {
-    const mkmoe_pages_cache cache = p.caches[c];
-    const uint32_t q = (uint32_t)(cache.page_bytes / 16);
-    const int64_t pieces = (int64_t)n * q, chunks = (pieces + kChunk - 1) / kChunk;
-    // (each cache starts where the one before ended, so that few pages keep every workgroup at work)
-    int64_t k = me - (c * chunks) % groups;
-    if (k < 0) k += groups;
-    for (; k < chunks; k += groups) {
-      const int64_t base = k * kChunk, i0 = base / q;
+  __shared__ mkmoe_pages_cache place[kCaches];
+  __shared__ int64_t before[kCaches + 1], sums[kThreads / 64];
+  if (n == 0) return;
+  const int tid = threadIdx.x;
+  const int64_t groups = gridDim.x * gridDim.y, me = blockIdx.y * gridDim.x + blockIdx.x;
+  for (int c0 = 0; c0 < p.ncaches; c0 += kCaches) {
+    const int some = min(kCaches, p.ncaches - c0);
+    __syncthreads();
+    int64_t mine = 0, all;
+    if (tid < some) {
+      place[tid] = p.caches[c0 + tid];
+      mine = (n * (place[tid].page_bytes / 16) + kChunk - 1) / kChunk;
+    }
+    const int64_t first = scan(mine, &all, sums);
+    if (tid < some) before[tid] = first;
+    if (tid == 0) before[some] = all;
+    __syncthreads();
+    int c = 0;
+    for (int64_t k = me; k < all; k += groups) {
+      while (before[c + 1] <= k) ++c;
+      const mkmoe_pages_cache cache = place[c];
+      const uint32_t q = (uint32_t)(cache.page_bytes / 16);
+      const int64_t base = (k - before[c]) * kChunk, i0 = base / q;
       const uint32_t rest = (uint32_t)(base - i0 * q);
-      u32x4 v[4];
-      u32x4* to[4];
+      // (the places first, then the bytes: loads complete in order, and one behind a place's would wait for it)
+      uint32_t part[4];
+      int a[4], b[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t x = rest + i * kThreads + tid;
         const int64_t at = i0 + x / q;
-        to[i] = nullptr;
-        if (at >= n) continue;
-        const uint32_t part = x % q;
-        const int a = src[at], b = dst[at];
-        if (check && ((uint32_t)a >= (uint32_t)p.pages || (uint32_t)b >= (uint32_t)p.pages)) {
-          if (part == 0 && c == 0) record(p.head, MKMOE_PAGES_ERR_PAGE, (int)at);
-          continue;
-        }
-        v[i] = *(const u32x4*)((const uint8_t*)cache.data + a * cache.page_bytes + part * 16);
-        to[i] = (u32x4*)((uint8_t*)cache.data + b * cache.page_bytes + part * 16);
+        part[i] = x % q;
+        a[i] = b[i] = -1;
+        if (at < n) a[i] = src[at], b[i] = dst[at];
       }
 #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool out = (uint32_t)a[i] >= (uint32_t)p.pages || (uint32_t)b[i] >= (uint32_t)p.pages;
+        const int64_t at = i0 + (rest + i * kThreads + tid) / q;
+        if (check && out && at < n && part[i] == 0 && c0 + c == 0) record(p.head, MKMOE_PAGES_ERR_PAGE, (int)at);
+        if (out) a[i] = -1;
+      }
+      u32x4 v[4];
+#pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (to[i]) *to[i] = v[i];
+        if (a[i] >= 0) v[i] = *(const u32x4*)((const uint8_t*)cache.data + a[i] * cache.page_bytes + part[i] * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (a[i] >= 0) *(u32x4*)((uint8_t*)cache.data + b[i] * cache.page_bytes + part[i] * 16) = v[i];
     }
   }
 }
@@ -418,43 +455,41 @@ __global__ __launch_bounds__(kThreads) void k_pages_copy(Params p, const int32_t
 
 // ---------------------------------------------------------------- second halves
 __global__ __launch_bounds__(kThreads) void k_pages_trim(Params p) {
-  for (int b = blockIdx.x; b < p.seqs; b += gridDim.x) {
-    const int len = p.old_len[b], to = p.new_len[b], page = p.new_page[b];
-    // entries from the first one that is not kept, or that gets a page of its own
-    const int first = pages_for(p, to) - (page >= 0), end = pages_for(p, len);
-    for (int i = first + blockIdx.y * kThreads + threadIdx.x; i < end; i += gridDim.y * kThreads) {
-      int32_t* at = p.table + b * p.table_stride + i;
-      release(p, *at, b);
-      if (page >= 0 && i == first) *at = page;
-    }
-    if (threadIdx.x == 0 && blockIdx.y == 0) p.lens[b] = to;
+  const int b = blockIdx.x, len = p.old_len[b], to = p.new_len[b], page = p.new_page[b];
+  // entries from the first one that is not kept, or that gets a page of its own
+  const int first = pages_for(p, to) - (page >= 0), end = pages_for(p, len);
+  for (int i0 = first + blockIdx.y * kThreads; i0 < end; i0 += gridDim.y * kThreads) {
+    const int i = i0 + threadIdx.x;
+    int32_t* at = p.table + b * p.table_stride + i;
+    release(p, i < end, i < end ? *at : 0, b);
+    if (page >= 0 && i == first) *at = page;
   }
+  if (threadIdx.x == 0 && blockIdx.y == 0) p.lens[b] = to;
   copy_pages(p, p.src, p.dst, p.head->moves, true);
 }
 
 __global__ __launch_bounds__(kThreads) void k_pages_fork(Params p) {
-  for (int b = blockIdx.x; b < p.seqs; b += gridDim.x) {
-    // as a parent: its full pages are held by each row that goes on, a last one that is not full by the first
-    const int len = p.old_len[b], full = len >> p.shift, end = pages_for(p, len), kids = p.kids[b];
-    const int32_t* held = p.held + (int64_t)b * p.max_pages;
-    for (int i = blockIdx.y * kThreads + threadIdx.x; i < end; i += gridDim.y * kThreads) {
-      const int page = held[i];
-      if (kids == 0)
-        release(p, page, b);
-      else if (kids > 1 && i < full && (uint32_t)page < (uint32_t)p.pages)
-        atomicAdd(p.refs + page, kids - 1);
-    }
-    // as a row that goes on
-    const int to = max(p.new_len[b], 0), own = p.new_page[b], parent = p.arg[b];
-    if (parent != b && to > 0) {
-      const int32_t* from = p.held + (int64_t)parent * p.max_pages;
-      const int n = pages_for(p, to);
-      for (int i = blockIdx.y * kThreads + threadIdx.x; i < n; i += gridDim.y * kThreads)
-        p.table[b * p.table_stride + i] = own >= 0 && i == n - 1 ? own : from[i];
-    }
-    if (own >= 0 && parent == b && threadIdx.x == 0 && blockIdx.y == 0) p.table[b * p.table_stride + (to >> p.shift)] = own;
-    if (threadIdx.x == 0 && blockIdx.y == 0) p.lens[b] = to;
+  const int b = blockIdx.x;
+  // as a parent: its full pages are held by each row that goes on, a last one that is not full by the first
+  const int len = p.old_len[b], full = len >> p.shift, end = pages_for(p, len), kids = p.kids[b];
+  const int32_t* held = p.held + (int64_t)b * p.max_pages;
+  for (int i0 = blockIdx.y * kThreads; i0 < end && kids != 1; i0 += gridDim.y * kThreads) {
+    const int i = i0 + threadIdx.x, page = i < end ? held[i] : 0;
+    if (kids == 0)
+      release(p, i < end, page, b);
+    else if (i < full && (uint32_t)page < (uint32_t)p.pages)
+      atomicAdd(p.refs + page, kids - 1);
   }
+  // as a row that goes on
+  const int to = max(p.new_len[b], 0), own = p.new_page[b], parent = p.arg[b];
+  if (parent != b && to > 0) {
+    const int32_t* from = p.held + (int64_t)parent * p.max_pages;
+    const int n = pages_for(p, to);
+    for (int i = blockIdx.y * kThreads + threadIdx.x; i < n; i += gridDim.y * kThreads)
+      p.table[b * p.table_stride + i] = own >= 0 && i == n - 1 ? own : from[i];
+  }
+  if (own >= 0 && parent == b && threadIdx.x == 0 && blockIdx.y == 0) p.table[b * p.table_stride + (to >> p.shift)] = own;
+  if (threadIdx.x == 0 && blockIdx.y == 0) p.lens[b] = to;
   copy_pages(p, p.src, p.dst, p.head->moves, true);
 }
 
@@ -620,17 +655,17 @@ inline unsigned rows_y(const Params& p) {  // workgroups a row of the table
 }
 // a grid for a table's rows, with enough workgroups for the caches' pages
 inline dim3 rows_grid(const Params& p) {
-  const unsigned y = p.ncaches > 0 ? 16 : rows_y(p);
-  return dim3(p.ncaches > 0 ? 128 : (unsigned)p.seqs, y);
+  unsigned y = rows_y(p);
+  if (p.ncaches > 0 && y * p.seqs < 2048) y = (2047 + p.seqs) / p.seqs;
+  return dim3((unsigned)p.seqs, y);
 }
 template <int OP>
 int take(const Params& p, hipStream_t st) {
-  const int64_t by_tokens = OP == kGrow ? (p.tokens + 4 * kThreads - 1) / (4 * kThreads) : 0;
-  const int64_t by_rows = OP == kFork ? p.seqs : 0;
-  int64_t n = (p.blocks + 3) / 4;
+  const int64_t by_tokens = OP == kGrow ? p.tokens / (3 * kThreads) : 0, by_rows = OP == kFork ? p.seqs / 8 : 0;
+  int64_t n = p.blocks / 16;
   n = n < by_tokens ? by_tokens : n;
   n = n < by_rows ? by_rows : n;
-  hipLaunchKernelGGL(k_pages_take<OP>, dim3((unsigned)(n < 1 ? 1 : n > 256 ? 256 : n)), dim3(kThreads), 0, st, p);
+  hipLaunchKernelGGL(k_pages_take<OP>, dim3((unsigned)(n < 1 ? 1 : n > 128 ? 128 : n)), dim3(kThreads), 0, st, p);
   return launched();
 }
 
