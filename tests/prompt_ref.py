@@ -57,10 +57,11 @@ def attend(cache, kv_b, q_nope, q_pe, table, lens, starts, scale):
     return out, lse, bound, lbound
 
 
-def close(got, want, bound, lens, what="out"):
-    """Every value within its bound, and the whole within what independent roundings make: of the output, its
-    numerators, its values and, through the scores (of a standard deviation up to about 1), its keys: each
-    2^-8 / sqrt 3 of the whole at most, so 2 2^-8 / sqrt 3 together."""
+def close(got, want, bound, what="out", sigma=1.0):
+    """Every value within its bound, and the whole within what independent roundings make: u = 2^-8 / sqrt 3 of it
+    each for the output's, its numerators' and its values', and for the keys', which move a score by u times the
+    scores' own standard deviation sigma and the output by as much of it: u sqrt(3 + sigma^2) together (2 u at
+    sigma 1: queries and keys of values near 1 have sigma = |scale| sqrt 192)."""
     ref.assert_within(got, want, bound, what)
     rel = ((got.double() - want).norm() / want.norm().clamp_min(1e-300)).item()
-    assert rel <= 2 * U16 / 3**0.5, (what, rel)
+    assert rel <= U16 / 3**0.5 * (3 + sigma**2) ** 0.5, (what, rel)
