@@ -35,8 +35,9 @@ class PagePool:
 
     ``caches``: tensors whose first axis is the pages (``latent.cache_like``'s, a layer each), whose bytes
     ``fork``, ``trim``, ``compact`` and ``copy`` move; they are used in place and kept alive. ``max_seqs``,
-    ``max_pages``: the largest table that a call takes ([B, max_pages], a sequence a row). One pool
-    serves one stream at a time."""
+    ``max_pages``: the largest table that a call takes ([B, max_pages], a sequence a row; by default sequences
+    of 131072 tokens, or the pool's): the pool keeps a copy of so many entries (4 bytes each), and 16 bytes a
+    page. One pool serves one stream at a time."""
 
     def __init__(self, pages: int, page_size: int, caches=(), max_seqs: int = 512, max_pages: int | None = None, device=None):
         if not 1 <= page_size <= 1024 or page_size & (page_size - 1):
@@ -45,7 +46,7 @@ class PagePool:
             raise RuntimeError(
                 f"mkmoe pages: {pages} pages of {page_size}, want 1 .. {_lib.PAGES_MAX_PAGES} and below 2^31 tokens"
             )
-        max_pages = pages if max_pages is None else max_pages
+        max_pages = min(pages, max(1, 131072 // page_size)) if max_pages is None else max_pages
         if not 1 <= max_pages <= _lib.PAGES_MAX_PAGES or max_pages * page_size >= 1 << 31:
             raise RuntimeError(
                 f"mkmoe pages: max_pages {max_pages} of {page_size}, want 1 .. {_lib.PAGES_MAX_PAGES} and below 2^31 tokens"

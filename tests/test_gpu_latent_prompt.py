@@ -180,13 +180,10 @@ def test_rows_of_no_sequence_stay():
     assert not own[:7].any() and not own[117:].any() and torch.equal(own[7:117], out[7:117])
 
 
-@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
-@pytest.mark.parametrize("bad", [NAN, INF, -INF, 3e38])
+@pytest.mark.parametrize("fmt,bad", [("bf16", NAN), ("bf16", INF), ("bf16", -INF), ("bf16", 3e38), ("mxfp8", NAN)])
 @pytest.mark.parametrize("at", [0, 63, 100, 199])
 def test_values_that_are_not_finite_reach_only_what_sees_them(fmt, bad, at):
     """A token's latents at their worst, among the new tokens: the queries before it are as without it."""
-    if fmt == "mxfp8" and bad not in (NAN,):
-        pytest.skip("e4m3 holds NaN alone")
     heads, n, length = 3, 180, 200
     b = Batch(11, heads, fmt, 16, [n], [length])
     where = b.table[0, at // 16].item(), at % 16
