@@ -246,8 +246,9 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
       p.plan->odd = 0;
     }
     for (int share = tid; share < shares; share += 256) {
+      p.cut[share].parts = 0;  // (the attention's share says otherwise)
       const int64_t u = (int64_t)share * per;
-      if (u >= work) break;
+      if (u >= work) continue;
       // the share's first item: the one that has its first unit
       int lo = 0, hi = p.seqs - 1;
       while (lo < hi) {
@@ -836,16 +837,16 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
     }
     if (it.parts > 0) cut = PromptCut{it.parts, it.head, it.t0, it.n, it.qt, {}};
   }
-  if (threadIdx.x == 0) p.cut[share] = cut;
+  if (threadIdx.x == 0 && cut.parts > 0) p.cut[share] = cut;
 }
 
-// The parts of a query tile that the end of a share cut, joined in order: (share, 32 rows) a workgroup, 32 values a
-// wave. The lanes have the values that the attention's had.
+// The parts of a query tile that the end of a share cut, joined in order: 128 of its rows a workgroup, 32 rows by 32
+// values a wave. The lanes have the values that the attention's had.
 template <int W>
-__global__ __launch_bounds__(256) void k_prompt_merge(PromptParams p) {
-  const int lane = threadIdx.x & 63, vb = threadIdx.x >> 6, share = blockIdx.x, group = blockIdx.y;
+__global__ __launch_bounds__(1024) void k_prompt_merge(PromptParams p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, vb = wave & 3, share = blockIdx.x;
+  const int group = blockIdx.y * 4 + (wave >> 2);
   const int half = lane >> 5, col = lane & 31;
-  if (share * p.plan->per >= p.plan->total) return;  // (no such share)
   const PromptCut c = p.cut[share];
   const int row0 = c.qt * rows_of(W) + group * 32, row = row0 + col;
   if (c.parts == 0 || row0 >= c.n) return;
@@ -986,7 +987,7 @@ template <int W>
 int attend_and_merge(const PromptParams& p, hipStream_t st) {
   hipLaunchKernelGGL(k_prompt_attend<W>, dim3(shares_of(W)), dim3(64 * W), 0, st, p);
   if (int rc = launched()) return rc;
-  hipLaunchKernelGGL(k_prompt_merge<W>, dim3(shares_of(W), W), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(k_prompt_merge<W>, dim3(shares_of(W), W / 4), dim3(1024), 0, st, p);
   return launched();
 }
 inline int prompt_launch(const PromptParams& p, bool mx, hipStream_t st) {
