@@ -21,6 +21,14 @@
 // h holds values 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3 of 16), so that a product's output is
 // the next one's operand in place: keys and values are stored, and numerators used, without
 // any exchange between lanes.
+//
+// Rounded to fewer bits than fp32 are the operands of the matrix instructions: keys to bf16, whose range
+// queries need, numerators and values to fp16 (3 more bits), a tile's values to bf16 where fp16 would lose some
+// (k_prompt_heads). Against 64 bits, in the 2-norm, where the output's own rounding is 0.0017: 0.0021 where rows see few
+// keys (bf16 numerators and values 0.0028), 0.0017 over long ones. Sums, maxima, outputs and parts are fp32.
+//
+// Times below are of an MI355X, of passes among others. It copies 4.9 TB/s and multiplies bf16 matrices at 1.39
+// PFLOP/s, which make the floors.
 
 #include "mkmoe_latent.h"
 
@@ -35,10 +43,12 @@ constexpr __host__ __device__ int shares_of(int waves) { return 2048 / waves; }
 constexpr __host__ __device__ int rows_of(int waves) { return 32 * waves; }
 constexpr __host__ __device__ int key_shift(int waves) { return waves == 8 ? 6 : 5; }
 constexpr int kKeys = 64;           // a sequence's packed rows are a multiple of so many
-constexpr int kLeastUnits = 6;      // units of work that a share has
+// units of work that a share has at least (6, 10, 16: 193 tokens over 893 42, 44, 47 us)
+constexpr int kLeastUnits = 6;
 constexpr int kFrag = 1024;         // bytes of a fragment
 constexpr int kPromptSeqs = MKMOE_LATENT_MAX_SEQS;
-constexpr int kItemSetup = 8;       // what starting and storing a query tile takes, in tiles of keys
+// What starting and storing a query tile takes, in turns of keys (2, 4, 8: ragged prompts' step 209, 197, 192 us)
+constexpr int kItemSetup = 8;
 constexpr float kMoveBy = 8.0f;     // a row's maximum moves where a score passes it by more than 2^kMoveBy
 constexpr float kLog2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 
@@ -189,8 +199,10 @@ __device__ __forceinline__ int64_t scan256(int64_t v, int64_t* total, int64_t* l
 }
 
 // The packed rows, 32 tokens a workgroup and turn: a fragment a wave and turn, its lanes reading 16 bytes (MXFP8: 8
-// codes) of 32 rows each. Every workgroup forms the sequences' places itself; one more
-// plans the attention.
+// codes) of 32 rows each; a row's lines are read once and hit the cache then. Rows behind a sequence's end are zeros, so
+// that nothing there reaches its keys. Every workgroup forms the sequences' places itself; one more plans the attention: its
+// work list's prefix sums and each share's first item, so that nothing is planned on the host and a captured graph replays
+// with other lengths. Memory bounds it (65300 rows in bf16, 150 MB: 36 us, 4.2 TB/s), on few rows latency (893 rows 6 us).
 template <bool MX>
 __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
   __shared__ int64_t sums[4];
@@ -274,6 +286,7 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
     }
     return;
   }
+  // (a fragment's row and half)
   const int r = lane & 31, half = lane >> 5;
   for (int kb = blockIdx.x; kb < end >> 5; kb += groups) {
     int lo = 0, hi = p.seqs - 1;  // the last sequence that starts at or before the block
@@ -344,7 +357,11 @@ __device__ __forceinline__ void heads_stage(f32x16 (&acc)[2][4], uint32_t c_at, 
 
 // The product of packed rows and kv_b: a tile is 128 tokens by a head's 128 + 128 rows of weights, 64 tokens by
 // 128 values a wave, K or V. Stages of 32 values along the sum through a ring of three in LDS, which runs on into the
-// next tile; two workgroups a CU, so that one's stores run under the other's products.
+// next tile; two workgroups a CU, so that one's stores run under the other's products. The weights' rows are read as the
+// checkpoint has them: their 16-byte pieces are swizzled in LDS, without bank conflicts (0 measured).
+// 10752 tokens of 64 heads take 121 us (1.49 PFLOP/s; a library's product of 16384 x 8192 x 512 reaches 0.77), 16383 of 32
+// heads 165 us before and after an attention of 2 ms, which leaves the card at 1.7 GHz of 2.4: power bounds it there.
+// On few tokens it is the chain of 16 stages' loads (893 tokens, 16 heads, 112 tiles: 15 us).
 template <bool V>  // the wave's part: values or keys
 __device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -569,6 +586,23 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
   return top;
 }
 
+// The attention. The work is a list of items (a sequence's head's query tile) of units: kItemSetup for an item's start and
+// end, and its turns of keys. Every workgroup takes one equal share of the units, whatever the lengths and the causal border
+// make of the items; an item that a share's end cuts leaves each wave's fp32 outputs, maxima and sums for
+// k_prompt_merge. A wave has 32 query rows, a column of lanes each, and all keys:
+//   S^T = K Q^T   A = keys from LDS, B = queries in registers: a lane has 16 scores of its row, so that the row's
+//                 maximum takes one exchange with the other half's lane
+//   P^T           exp2 of the scores less the maximum, which moves where one passes it by 2^8: fp16, in place
+//   O^T += V^T P^T   A = values from LDS, B = P^T as it lies: a row's rescaling is a lane's own factor
+// Scores are formed a block of 32 keys ahead, and the code alternates their products with the numerators of the block
+// before, then the products of the outputs with the next maximum: a wave's matrix and vector instructions run under
+// each other (chunk_large below: 2.63 -> 2.03 ms). Keys and values come straight from memory to LDS two turns ahead,
+// one barrier a turn.
+//
+// What bounds it: power. 8191 tokens over 16383 with 32 heads, 2.06 PFLOP, take 1.95 ms, 1.06 PFLOP/s (the floor's
+// rate is 1.39): the matrix units are busy for 61 % of the cycles and the clock falls to 1.7 GHz; counters: 3.3 vector
+// instructions to a matrix instruction, LDS busy for 31 %, without conflicts. Ahead of that, short prompts: an item's
+// start and end (its queries, first keys, outputs) of 6 to 9 us beside turns of 1.5 to 2 us of 64 keys.
 template <int W>
 __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
   constexpr int NB = blocks_of(W), TK = 32 * NB, kKeyLds = key_lds(W), kValLds = val_lds(W);

@@ -233,9 +233,11 @@ def test_values_outside_what_fp16_holds(size):
         prompt_ref.close(out[150:, h], o[150:, h], bound[150:, h], f"head {h}")
 
 
-def test_long_tails_of_small_numerators():
-    """One key that weighs e^17 times any other of 6000: the others' numerators still count."""
-    heads, length = 2, 6000
+@pytest.mark.parametrize("far,length", [(17.0, 6000), (15.25, 60000)])
+def test_long_tails_of_small_numerators(far, length):
+    """One key that weighs e^far times any other: the others' numerators still count, and in their sum (60000 of
+    2^-22 are 1.4 % of it, more than the bound)."""
+    heads = 2
     b = Batch(14, heads, "bf16", 64, [130], [length])
     b.cache[..., :] = 0
     b.cache[..., 0] = 1.0  # every token's latents: e_0; the first one's: 32 e_1
@@ -247,10 +249,10 @@ def test_long_tails_of_small_numerators():
     w[:, 1, :, 0] = 1.0  # v: 1 for the others, 0 for the first one
     b.q_nope, b.q_pe = torch.zeros(130, heads, 128, dtype=BF, device="cuda"), torch.zeros(130, heads, 64, dtype=BF, device="cuda")
     b.q_nope[..., 0] = 1.0
-    out = _runner(heads, scale=17.0 / 32, max_context=6144).attend(*b.args())
+    out = _runner(heads, scale=far / 32, max_context=length + 100).attend(*b.args())
     see = torch.arange(length - 130, length, device="cuda").double()
-    want = (see / (see + torch.e**17))[:, None, None].expand(130, heads, 128)
-    assert ((out.double() - want).abs() <= want * (2 * ref.U16 + 6000 * ref.U32)).all()
+    want = (see / (see + torch.e**far))[:, None, None].expand(130, heads, 128)
+    assert ((out.double() - want).abs() <= want * (2 * ref.U16 + length * ref.U32)).all()
 
 
 def test_lengths_starts_and_pages_outside_their_bounds():
