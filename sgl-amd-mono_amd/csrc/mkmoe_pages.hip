@@ -14,7 +14,9 @@
 //   k_pages_plan     which pages move where (compact)
 //   k_pages_copy     pages that the caller names
 //
-// Every call is bound by its launches (2 to 4 us each) but for the pages' bytes, read and written once.
+// A call with few pages is bound by its launches (3 to 7 us each of dependent reads: lengths, counts, pages, tables),
+// others by the pages' bytes, read and written once: 301 pages of 24 caches copied in 127 us, 4.8 TB/s, where
+// a copy of 2 GiB reaches 4.9 on this card.
 
 #include <hip/hip_runtime.h>
 
