@@ -299,7 +299,8 @@ const char* mkmoe_status_string(int status);
 #define MKMOE_LATENT_ERR_SLOT 1     /* slot >= pages page_size: the row is not written / read as 0 */
 #define MKMOE_LATENT_ERR_POSITION 2 /* position outside cos_sin: the token's rows are not written (q_out_nan) */
 #define MKMOE_LATENT_ERR_LENGTH 3   /* length or query starts outside their bounds: clamped. Starts that
-                                     * run backwards: nothing is attended, out stays as it was */
+                                     * run backwards: nothing is attended, out stays as it was; (prompt) a
+                                     * sequence begins where those before it end */
 #define MKMOE_LATENT_ERR_PAGE 4     /* page outside the cache: its tokens read as rows of zeros */
 #define MKMOE_LATENT_ERR_CONTEXT 5  /* (prompt) the cached tokens pass max_context: the sequence's output is NaN */
 
@@ -388,8 +389,8 @@ int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_p
 /* ---- a prompt's tokens
  * The same attention with a key and a value for each head and token, made from the cached rows by
  * w: k = [W_UK c, k_pe], v = W_UV c, o = sum softmax(scale q . k) v: fewer operations than the absorbed form
- * from about 171 query tokens a sequence. Keys, values and softmax's numerators are rounded to bf16, sums,
- * scores and maxima are fp32. Query token i of a sequence's n sees its first len - n + 1 + i tokens. */
+ * from about 171 query tokens a sequence. Keys are rounded to bf16, values and softmax's numerators to fp16 (values
+ * that it does not hold to bf16), sums, scores and maxima are fp32. Query token i of a sequence's n sees its first len - n + 1 + i tokens. */
 typedef struct mkmoe_latent_prompt_io {
   mkmoe_latent_cache cache;
   int32_t seqs;        /* 1 .. MKMOE_LATENT_MAX_SEQS */

@@ -94,6 +94,7 @@ struct Plan {
   int32_t per;                // units a share
   int32_t items;
   int32_t odd;                // some tile's values are bf16
+  int32_t back;               // query starts run backwards
 };
 
 // what the end of a share cut, for the merge: a query tile that goes on in the shares behind it
@@ -132,19 +133,22 @@ struct PromptParams {
   uint32_t flip;   // 0x80008000 where scale is negative: the keys' signs are turned
 };
 
-// a sequence's query tokens and length, clamped to their bounds
+// a sequence's query tokens and length, clamped to their bounds. Where query starts run backwards (back), it begins
+// where those before it end: no row is two sequences', and there is no more work than was checked
 struct PromptSeq {
   int t0, n, len;
   bool bad;  // outside its bounds
 };
-__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b, bool back) {
   PromptSeq s;
   const int len = p.lens[b];
   s.len = min(max(len, 0), p.max_len);
   s.bad = s.len != len;
   if (p.starts) {
     const int a = p.starts[b], e = p.starts[b + 1];
-    s.t0 = min(max(a, 0), p.tokens);
+    s.t0 = a;
+    for (int i = 0; back && i < b; ++i) s.t0 = max(s.t0, p.starts[i]);
+    s.t0 = min(max(s.t0, 0), p.tokens);
     const int t1 = min(max(e, s.t0), p.tokens);
     s.n = t1 - s.t0;
     s.bad = s.bad || a != s.t0 || e != t1;
@@ -212,12 +216,15 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
   const bool planner = (int)blockIdx.x == groups;
   int64_t rows = 0, work = 0, items = 0;
   if (tid == 0) upto = 0;  // (the scan's barriers come before it is used)
+  int behind = 0;
+  for (int b = tid; p.starts && b < p.seqs; b += 256) behind |= p.starts[b + 1] < p.starts[b];
+  const bool back = __syncthreads_or(behind) != 0;
   for (int b0 = 0; b0 < p.seqs; b0 += 256) {
     const int b = b0 + tid;
     int need = 0;
     PromptSeq s{0, 0, 0, false};
     if (b < p.seqs) {
-      s = prompt_seq(p, b);
+      s = prompt_seq(p, b, back);
       if (s.bad && planner) record(p.err, MKMOE_LATENT_ERR_LENGTH, b);
       if (s.n > 0) need = (s.len + kKeys - 1) & -kKeys;
     }
@@ -256,6 +263,7 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
       p.plan->items = (int)items;
       p.plan->per = per;
       p.plan->odd = 0;
+      p.plan->back = back;
     }
     for (int share = tid; share < shares; share += 256) {
       p.cut[share].parts = 0;  // (the attention's share says otherwise)
@@ -267,7 +275,7 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
         const int mid = (lo + hi + 1) >> 1;
         if (unit[mid] <= u) lo = mid; else hi = mid - 1;
       }
-      const PromptSeq s = prompt_seq(p, lo);
+      const PromptSeq s = prompt_seq(p, lo, back);
       const int qts = query_tiles(s.n, p.waves), past = s.len - s.n;
       int x = (int)u - unit[lo], i = 0;
       if (at[lo] == p.cap && s.len > 0) {  // it does not fit: no keys
@@ -498,7 +506,7 @@ __device__ __forceinline__ Item item_of(const PromptParams& p, int o, int share,
     const int mid = (lo + hi + 1) >> 1;
     if (p.plan->item[mid] <= o) lo = mid; else hi = mid - 1;
   }
-  const PromptSeq s = prompt_seq(p, lo);
+  const PromptSeq s = prompt_seq(p, lo, p.plan->back != 0);
   const int at = p.plan->at[lo], qts = query_tiles(s.n, w), i = o - p.plan->item[lo];
   it.t0 = s.t0;
   it.n = s.n;

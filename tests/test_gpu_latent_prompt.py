@@ -292,6 +292,25 @@ def test_lengths_starts_and_pages_outside_their_bounds():
         run.raise_on_device_error()
 
 
+@pytest.mark.parametrize("starts", [[0, 40, 10, 70, 60, 90], [30, 0, 90, 0, 90, 0], [0, 90] * 2 + [0, 90]])
+def test_starts_that_run_backwards(starts):
+    """A sequence begins where those before it end: every row is one sequence's, and rows of none stay as they were."""
+    b = Batch(16, 4, "bf16", 16, [18] * 5, [200, 70, 65, 130, 90])
+    run = _runner(4)
+    dev = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    out = torch.full((90, 4, 128), 7.0, dtype=BF, device="cuda")
+    lse = torch.full((90, 4), 7.0, device="cuda")
+    run.attend(*b.args(), q_starts=dev, out=out, lse=lse)
+    torch.cuda.synchronize()
+    assert run.read_errors()[0] == 3
+    b.starts = torch.cummax(torch.tensor(starts), 0).values.tolist()
+    first = b.starts[0]
+    assert (out[:first] == 7).all() and (lse[:first] == 7).all()
+    o, l, bound, lbound = b.want()
+    prompt_ref.close(out[first:], o[first:], bound[first:])
+    ref.assert_within(lse[first:].double(), l[first:], lbound[first:], "lse")
+
+
 def test_context_that_the_workspace_does_not_hold():
     new, lens = [20, 30, 40, 10], [200, 300, 100, 0]
     b = Batch(16, 3, "bf16", 16, new, lens)
