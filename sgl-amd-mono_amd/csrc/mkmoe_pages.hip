@@ -100,6 +100,17 @@ __device__ __forceinline__ void release(const Params& p, bool there, int page, i
   }
 }
 
+// A held page gets more holders. One that nobody holds stays free: a table may name what it does not hold
+__device__ __forceinline__ void hold(const Params& p, int page, int more, int where) {
+  int was = __hip_atomic_load(p.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  while (was > 0) {
+    const int seen = atomicCAS(p.refs + page, was, was + more);
+    if (seen == was) return;
+    was = seen;
+  }
+  record(p.head, MKMOE_PAGES_ERR_PAGE, where);
+}
+
 // the sum of v over the threads before this one, and over all of them
 template <class T>
 __device__ __forceinline__ T scan(T v, T* total, T* lds) {
@@ -480,7 +491,7 @@ __global__ __launch_bounds__(kThreads) void k_pages_fork(Params p) {
     if (kids == 0)
       release(p, i < end, page, b);
     else if (i < full && (uint32_t)page < (uint32_t)p.pages)
-      atomicAdd(p.refs + page, kids - 1);
+      hold(p, page, kids - 1, b);
   }
   // as a row that goes on
   const int to = max(p.new_len[b], 0), own = p.new_page[b], parent = p.arg[b];

@@ -241,6 +241,23 @@ def test_bad_tables_touch_nothing():
     assert b.pool.read_errors()[2] > 0 and int(b.pool.refs.min()) >= 0
 
 
+def test_pages_that_nobody_holds_stay_free():
+    """Rows forked that name free pages: these get no holders, so that what is free stays counted."""
+    b = Both(10, 4, 4, 3)
+    b.set([[1, 2], [5, 6, 7]], [8, 12, 0, 0])
+    b.pool.adopt(b.table[:1], b.lens[:1])  # the second row holds nothing
+    for _ in range(3):
+        b.pool.fork(b.table, b.lens, _i32([0, 1, 1, 0]))
+        assert b.pool.refs.tolist() == [0, 2, 2, 0, 0, 0, 0, 0, 0, 0]
+        b.pool.trim(b.table, b.lens, _i32([8, 0, 0, 0]))
+        assert b.pool.refs.tolist() == [0, 1, 1, 0, 0, 0, 0, 0, 0, 0]
+        b.lens[1] = 12
+    assert b.pool.read_errors()[2] == 3 * (3 + 6)
+    b.lens[1] = 0
+    slots = b.pool.grow(b.table, b.lens, _i32([0, 12, 12, 12]), 36)[0]
+    assert sorted(set((slots // 4).tolist())) == [-1, 0, 3, 4, 5, 6, 7]  # (of 8 free pages two rows take 6)
+
+
 def test_adopt_finds_shared_partial_pages():
     b = Both(10, 4, 2, 2)
     b.set([[1, 2], [1, 2]], [8, 7])
