@@ -452,6 +452,8 @@ int mkmoe_latent_read_errors(const void* ws, int32_t* words, int32_t n, void* st
 #define MKMOE_PAGES_ERR_FULL 3   /* too few free pages: grow and trim leave the sequence as it was, fork empty */
 #define MKMOE_PAGES_ERR_ROOM 4   /* grow: past the table or the call's tokens: the sequence stays as it was */
 #define MKMOE_PAGES_ERR_SHARED 5 /* adopt: a partly filled page of several sequences */
+#define MKMOE_PAGES_ERR_TABLE 6  /* compact: the table's rows are not all that hold pages: nothing is moved. In place of a
+                                  * sequence: how many holders it has not (below 0: too many) */
 
 typedef struct mkmoe_pages_cache {
   void* data;         /* [pages][page_bytes], 16-byte aligned */
@@ -492,7 +494,7 @@ int mkmoe_pages_trim(const mkmoe_pages_pool* pool, const mkmoe_pages_table* tabl
 int mkmoe_pages_fork(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, const int32_t* parents, void* ws,
                      size_t ws_bytes, void* stream);
 /* The n pages held moved to pages 0 .. n - 1: those at n and behind to the free ones before, both in order. The table
- * has every sequence that holds pages. Three launches. */
+ * has every sequence that holds pages, or nothing is moved. Three launches. */
 int mkmoe_pages_compact(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, void* ws, size_t ws_bytes,
                         void* stream);
 /* Pages src[i] copied to dst[i] in every cache; dst are distinct and none of them is among src. One launch. */

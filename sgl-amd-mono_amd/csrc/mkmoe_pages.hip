@@ -41,6 +41,8 @@ struct Head {
   int32_t arrived;  // workgroups of k_pages_take that are done; 0 between launches
   int32_t moves;    // pages that the launch behind copies: src[i] to dst[i]
   int32_t live;     // compact: pages held
+  int32_t missing;  // compact: holders that the table does not have; 0 between calls
+  int32_t refused;  // compact: that many, and nothing is moved
 };
 static_assert(sizeof(Head) <= MKMOE_PAGES_REFS_AT, "the counts follow the head");
 
@@ -507,7 +509,8 @@ __global__ __launch_bounds__(kThreads) void k_pages_fork(Params p) {
 }
 
 // Compact: of n pages held, those at n and behind go to the free ones before n, both in order. A workgroup
-// finds its blocks' pages and their ranks.
+// finds its blocks' pages and their ranks. The pages' holders are counted against the table's entries: a row that the
+// table does not have would be left with pages that are others' afterwards, so then nothing is moved.
 __global__ __launch_bounds__(kThreads) void k_pages_plan(Params p) {
   __shared__ int before[kMaxBlocks];
   __shared__ int sums[kThreads / 64];
@@ -523,13 +526,20 @@ __global__ __launch_bounds__(kThreads) void k_pages_plan(Params p) {
   __syncthreads();
   const int live = p.pages - free_pages;
   if (blockIdx.x == 0 && tid == 0) p.head->live = live;
+  // the pages' holders, less those that the table has
+  int missing = 0;
+  for (int b = blockIdx.x; b < p.seqs; b += gridDim.x) {
+    const int n = pages_for(p, clamped(p, p.lens[b]));
+    for (int i = tid; i < n; i += kThreads) missing -= (uint32_t)p.table[b * p.table_stride + i] < (uint32_t)p.pages;
+  }
   for (int j = blockIdx.x; j < p.blocks; j += gridDim.x) {
     int n = 0, used[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int page = j * kBlock + 4 * tid + i;
-      used[i] = page < p.pages ? p.refs[page] != 0 : 2;
+      const int page = j * kBlock + 4 * tid + i, refs = page < p.pages ? p.refs[page] : 0;
+      used[i] = page < p.pages ? refs != 0 : 2;
       n += used[i] == 0;
+      missing += refs;
     }
     int all;
     int frees = before[j] + scan(n, &all, sums);  // free pages before this one
@@ -551,10 +561,18 @@ __global__ __launch_bounds__(kThreads) void k_pages_plan(Params p) {
     }
   }
   if (live == p.pages && blockIdx.x == 0 && tid == 0) p.head->moves = 0;
+  int all;
+  (void)scan(missing, &all, sums);
+  if (tid == 0 && all != 0) atomicAdd(&p.head->missing, all);
 }
 __global__ __launch_bounds__(kThreads) void k_pages_compact(Params p) {
-  const int live = p.head->live, moves = p.head->moves;
+  const int live = p.head->live, moves = p.head->moves, missing = p.head->missing;
   const int groups = gridDim.x * gridDim.y, me = blockIdx.y * gridDim.x + blockIdx.x;
+  if (me == 0 && threadIdx.x == 0) p.head->refused = missing;
+  if (missing != 0) {
+    if (me == 0 && threadIdx.x == 0) record(p.head, MKMOE_PAGES_ERR_TABLE, missing);
+    return;
+  }
   // (rank + moves: the place among the pages that move)
   for (int page = live + me * kThreads + threadIdx.x; page < p.pages; page += groups * kThreads)
     if (p.refs[page] != 0) p.src[p.rank[page] + moves] = page;
@@ -576,6 +594,8 @@ __global__ __launch_bounds__(kThreads) void k_pages_compact(Params p) {
 __global__ __launch_bounds__(kThreads) void k_pages_move(Params p) {
   const int live = p.head->live, moves = p.head->moves;
   const int groups = gridDim.x * gridDim.y, me = blockIdx.y * gridDim.x + blockIdx.x;
+  if (me == 0 && threadIdx.x == 0) p.head->missing = 0;
+  if (p.head->refused != 0) return;
   for (int i = me * kThreads + threadIdx.x; i < moves; i += groups * kThreads) {
     p.refs[p.dst[i]] = p.refs[p.src[i]];
     p.refs[p.src[i]] = 0;
@@ -764,7 +784,8 @@ int mkmoe_pages_compact(const mkmoe_pages_pool* pool, const mkmoe_pages_table* t
   if (int rc = params(pool, ws, ws_bytes, p)) return rc;
   if (int rc = table_params(pool, table, p)) return rc;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(k_pages_plan, dim3((unsigned)(p.blocks < 256 ? p.blocks : 256)), dim3(kThreads), 0, st, p);
+  const int plan = p.blocks < p.seqs ? p.seqs : p.blocks;
+  hipLaunchKernelGGL(k_pages_plan, dim3((unsigned)(plan < 256 ? plan : 256)), dim3(kThreads), 0, st, p);
   if (int rc = launched()) return rc;
   hipLaunchKernelGGL(k_pages_compact, dim3((unsigned)p.seqs, rows_y(p)), dim3(kThreads), 0, st, p);
   if (int rc = launched()) return rc;

@@ -76,6 +76,7 @@ PAGES_ERRORS = {
     3: "no free pages, at sequence",
     4: "tokens past the table's entries or the call's outputs, at sequence",
     5: "a partly filled page of several sequences, at sequence",
+    6: "a table to compact by without all rows that hold pages (nothing moved), holders missing:",
 }
 
 # every symbol include/mkmoe.h and include/mkmoe_seam.h declare

@@ -177,7 +177,8 @@ class PagePool:
 
     def compact(self, table, lens) -> None:
         """The n pages held moved to the pool's first n, the table's entries with them: those behind to the free
-        ones before, both in order. ``table`` has every sequence that holds pages."""
+        ones before, both in order. ``table`` has every sequence that holds pages; where their number shows that
+        it does not, nothing is moved and it is recorded."""
         self._set_table(table, lens)
         self._call(self.lib.mkmoe_pages_compact, self._pool, self._table)
 

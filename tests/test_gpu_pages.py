@@ -195,6 +195,35 @@ def test_compact_a_full_pool():
     b.same()
 
 
+def test_compact_needs_every_row():
+    b = Both(3000, 2, 3, 900)
+    b.grow([600, 40, 1500])
+    b.trim([600, 0, 1500])
+    b.pool.compact(b.table[:2], b.lens[:2])
+    b.ref.errors.append((6, 750))  # the third row's holders
+    b.same()
+    with pytest.raises(RuntimeError, match="holders missing: 750 "):
+        b.pool.raise_on_device_error()
+    b.compact()
+    b.same()
+    b.pool.clear_errors()
+    b.ref.errors.clear()
+    graph = torch.cuda.CUDAGraph()
+    some, lens = b.table[:1], b.lens[:1]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        b.pool.compact(some, lens)
+        b.pool.compact(b.table, b.lens)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        b.ref.errors.append((6, 750))
+        b.ref.compact(b.rows, b.n)
+        b.same()
+        keep = [n - 9 for n in b.n[:1]] + b.n[1:]
+        b.trim(keep)
+
+
 @pytest.mark.parametrize("n", [0, 1, 7, 300])
 def test_copy(n):
     from sgl_amd_mono.moe.pages import PagePool
