@@ -126,7 +126,7 @@ struct PromptParams {
   float* part_o;   // [2 shares][W][4][4][64 lanes][4]
   float* part_ml;  // [2 shares][32 W][2]
   int64_t qn_ts, qn_hs, qp_ts, qp_hs, o_ts, o_hs, table_stride;
-  int64_t cap;     // packed rows that the workspace holds, a multiple of 128
+  int64_t cap;     // packed rows that the workspace holds, a multiple of kKeys
   int pages, seqs, tokens, heads, n, max_len, page_shift;
   int waves;       // of the attention's workgroups
   float scale2;    // |scale| log2(e)
@@ -336,145 +336,121 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
 }
 
 // ---------------------------------------------------------------- keys and values of every head
-constexpr int kMTok = 128;  // tokens a product tile, by one head's 256 rows of weights
-constexpr int kMK = 32;     // values along the sum a stage
-constexpr int kMStages = kL / kMK;
-constexpr int kMBytes = (kMTok + 256) * kMK * 2;
-constexpr int kMRing = 3;
-constexpr int kMGroup = 8;
-
-// Fragments of keys (A: the weights' rows, B: tokens) or values (A: tokens, B: the weights' rows)
+// The product of packed rows and kv_b. A workgroup, one a CU, keeps 128 of the weights' rows, a head's W_UK or W_UV, in
+// LDS as fragments, and its waves go through the tokens on their own, 64 a turn by the 128 rows, the tokens' fragments
+// coming from memory four ahead. The weights are read from LDS by every wave for 64 tokens: half of what LDS can deliver.
+constexpr int kHalfHead = 128 * kL * 2;  // bytes
+constexpr int kAhead = 4;
 template <bool V>
-__device__ __forceinline__ void heads_stage(f32x16 (&acc)[2][4], uint32_t c_at, uint32_t w_at, int lane) {
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    bf16x8 c[2], w[4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) c[t] = lds_read<bf16x8>(c_at + t * 2 * kFrag + s * kFrag);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = lane & 31, piece = 2 * s + (lane >> 5);
-      w[j] = lds_read<bf16x8>(w_at + j * 2 * kFrag + (r >> 2) * 256 + (r & 3) * 64 + ((piece ^ ((r >> 2) & 3)) << 4));
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) acc[t][j] = V ? mfma32(c[t], w[j], acc[t][j]) : mfma32(w[j], c[t], acc[t][j]);
-  }
-}
-
-// The product of packed rows and kv_b: a tile is 128 tokens by a head's 128 + 128 rows of weights, 64 tokens by
-// 128 values a wave, K or V. Stages of 32 values along the sum through a ring of three in LDS, which runs on into the
-// next tile; two workgroups a CU, so that one's stores run under the other's products. The weights' rows are read as the
-// checkpoint has them: their 16-byte pieces are swizzled in LDS, without bank conflicts (0 measured).
-// 10752 tokens of 64 heads take 121 us (1.49 PFLOP/s; a library's product of 16384 x 8192 x 512 reaches 0.77), 16383 of 32
-// heads 165 us before and after an attention of 2 ms, which leaves the card at 1.7 GHz of 2.4: power bounds it there.
-// On few tokens it is the chain of 16 stages' loads (893 tokens, 16 heads, 112 tiles: 15 us).
-template <bool V>  // the wave's part: values or keys
-__device__ __forceinline__ void heads_loop(const PromptParams& p, uint32_t lds) {
+__device__ __forceinline__ void heads_blocks(const PromptParams& p, uint32_t w_at, int head, int from, int upto) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  // Product tiles in groups of 8 blocks of tokens, a group head by head: an XCD's workgroups, which have tiles that follow
-  // each other, read a few MB of rows and weights between them, which its L2 keeps
-  const int blocks = uniform((p.plan->rows + kMTok - 1) / kMTok), tiles = blocks * p.heads;
-  const int xcd = blockIdx.x & 7, first = xcd * (tiles / 8) + min(xcd, tiles % 8);
-  const int end = (xcd + 1) * (tiles / 8) + min(xcd + 1, tiles % 8), step = gridDim.x >> 3;
-  const int begin = first + (int)(blockIdx.x >> 3);
-  const int stages = begin < end ? ((end - 1 - begin) / step + 1) * kMStages : 0;
-  const int64_t kbs = p.cap / 32;
-  auto place = [&](int g, int& head, int& tok) {  // of stage g's tile
-    const int tile = begin + (g / kMStages) * step, group = tile / (kMGroup * p.heads);
-    const int in = tile - group * kMGroup * p.heads, wide = min(kMGroup, blocks - kMGroup * group);
-    head = uniform(in / wide);
-    tok = uniform(kMGroup * group + in % wide);
-  };
-
-  // wave w brings the tokens 32 w .. and the weights' rows 64 w ..
-  const uint8_t* c = nullptr;
-  const uint8_t* w = nullptr;
-  const uint32_t w_lane = (uint32_t)((lane >> 2) * kL + 8 * ((lane & 3) ^ ((lane >> 4) & 3))) * 2;
-  auto issue = [&](int g) {
-    if (g >= stages) return;
-    if (g % kMStages == 0) {
-      int head, tok;
-      place(g, head, tok);
-      c = p.c + (int64_t)(tok * 4 + wave) * 32 * kFrag;
-      w = (const uint8_t*)(p.w + ((int64_t)head * 256 + wave * 64) * kL);
-    }
-    const uint32_t to = lds + (g % kMRing) * kMBytes;
+  int blk = from + wave;
+  if (blk >= upto) return;
+  constexpr int64_t kBlockBytes = 64 * kL * 2;
+  const uint8_t* at = p.c + blk * kBlockBytes;
+  bf16x8 c[kAhead][2], w[2][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) lds_dma16(c + i * kFrag, lane * 16, to + (wave * 2 + i) * kFrag);
+  for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds_dma16(w + i * 16 * kL * 2, w_lane, to + (8 + wave * 4 + i) * kFrag);
-    c += 2 * kFrag;
-    w += kMK * 2;
-  };
-
-  const int tg = wave & 1;
-  issue(0);
-  issue(1);
-  f32x16 acc[2][4];
-  for (int g = 0; g < stages; ++g) {
-    const int ks = g % kMStages;
-    if (ks == 0) {
+    for (int t = 0; t < 2; ++t) c[u][t] = *(const bf16x8*)(at + t * kBlockBytes / 2 + u * kFrag + lane * 16);
+  for (;; blk += 8) {
+    const bool more = blk + 8 < upto;
+    const uint8_t* next = more ? at + 8 * kBlockBytes : at;
+    f32x16 acc[2][4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[t][j] = f32x16{};
-    }
-    if (g + 1 < stages)
-      wait_loads<6>();
-    else
-      wait_loads<0>();
-    barrier();
-    issue(g + 2);
-    const uint32_t at = lds + (g % kMRing) * kMBytes;
-    const uint32_t c_at = at + tg * 4 * kFrag + lane * 16, w_at = at + 8 * kFrag + (V ? 8 : 0) * kFrag;
-    heads_stage<V>(acc, c_at, w_at, lane);
-    if (ks == kMStages - 1) {
-      int head, tok;
-      place(g, head, tok);
-      const int64_t kb = (int64_t)head * kbs + tok * 4 + tg * 2;
-      bool half = false;
-      if constexpr (V) {
-        // fp16 where that loses nothing that counts: none above its range, the largest so far above its smallest
-        // normal value that what is below that is less than 2^-19 of it (or all 0)
-        uint32_t top = 0;
+      for (int j = 0; j < 4; ++j) acc[t][j] = f32x16{};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+    for (int j = 0; j < 4; ++j) w[0][j] = lds_read<bf16x8>(w_at + j * (kL / 16) * kFrag);
+#pragma unroll 1
+    for (int k = 0; k < kL / 16; k += kAhead) {
+      const uint8_t* ahead = k + kAhead < kL / 16 ? at + (k + kAhead) * kFrag : next;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+      for (int u = 0; u < kAhead; ++u) {
+        const int after = (k + u + 1) % (kL / 16);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = max(top, f2u(acc[t][j][i]) & 0x7fffffffu);
-        half = __ballot(top >= f2u(65504.0f)) == 0 && (__ballot(top >= f2u(0x1p-6f)) != 0 || __ballot(top != 0) == 0);
-        if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + tok * 2 + tg] = !half;
-        if (lane == 0 && !half) atomicOr(&p.plan->odd, 1);
+        for (int j = 0; j < 4; ++j) w[(u + 1) & 1][j] = lds_read<bf16x8>(w_at + (j * (kL / 16) + after) * kFrag);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            acc[t][j] = V ? mfma32(c[u][t], w[u & 1][j], acc[t][j]) : mfma32(w[u & 1][j], c[u][t], acc[t][j]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) c[u][t] = *(const bf16x8*)(ahead + t * kBlockBytes / 2 + u * kFrag + lane * 16);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    const int64_t kb = (int64_t)head * (p.cap / 32) + 2 * blk;
+    auto store = [&](auto pack) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = acc[t][j][8 * u + 2 * e], y = acc[t][j][8 * u + 2 * e + 1];
-              o[e] = V ? (half ? pack_f16(x, y) : pack_bf(x, y)) : pack_bf(x, y) ^ p.flip;
-            }
-            uint8_t* to = (V ? p.v : p.k) + ((kb + t) * 8 + (V ? u * 4 + j : 2 * j + u)) * kFrag + lane * 16;
-            *(u32x4*)to = u32x4{o[0], o[1], o[2], o[3]};
+            const f32x16& a = acc[t][j];
+            const u32x4 o = {pack(a[8 * u], a[8 * u + 1]), pack(a[8 * u + 2], a[8 * u + 3]), pack(a[8 * u + 4], a[8 * u + 5]),
+                             pack(a[8 * u + 6], a[8 * u + 7])};
+            *(u32x4*)((V ? p.v : p.k) + ((kb + t) * 8 + (V ? u * 4 + j : 2 * j + u)) * kFrag + lane * 16) = o;
           }
+    };
+    if constexpr (V) {
+      // fp16 where that loses nothing that counts: none above its range, the largest so far above its smallest
+      // normal value that what is below that is less than 2^-19 of it (or all 0)
+      uint32_t top = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = max(top, f2u(acc[t][j][i]) & 0x7fffffffu);
+      const bool half = __ballot(top >= f2u(65504.0f)) == 0 && (__ballot(top >= f2u(0x1p-6f)) != 0 || __ballot(top != 0) == 0);
+      if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + blk] = !half;
+      if (half) {
+        store([](float x, float y) { return pack_f16(x, y); });
+      } else {
+        if (lane == 0) atomicOr(&p.plan->odd, 1);
+        store([](float x, float y) { return pack_bf(x, y); });
+      }
+    } else {
+      store([&](float x, float y) { return pack_bf(x, y) ^ p.flip; });
     }
+    if (!more) return;
+    at = next;
   }
 }
 
-__global__ __launch_bounds__(256, 2) void k_prompt_heads(PromptParams p) {
-  __shared__ __align__(1024) uint8_t ring[kMRing][kMBytes];
-  const uint32_t lds = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)&ring[0][0];
-  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= 2)
-    heads_loop<true>(p, lds);
-  else
-    heads_loop<false>(p, lds);
+__global__ __launch_bounds__(512, 2) void k_prompt_heads(PromptParams p) {
+  __shared__ __align__(1024) uint8_t weights[kHalfHead];
+  const uint32_t lds = (uint32_t)(uintptr_t)(MKMOE_LDS uint8_t*)&weights[0];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int blocks = uniform(p.plan->rows) / kKeys, halves = 2 * p.heads;
+  // The tokens in as many parts as one or eight, and a part's blocks of 64, half head by half head, in equal shares for its
+  // workgroups. Eight: an XCD's workgroups go through its part together, and its L2 keeps the tokens between them
+  const int parts = blocks >= 512 ? 8 : 1, groups = gridDim.x / parts;
+  const int part = parts == 8 ? blockIdx.x & 7 : 0, me = parts == 8 ? blockIdx.x >> 3 : (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
+  const int first = (int)((int64_t)blocks * part / parts), wide = (int)((int64_t)blocks * (part + 1) / parts) - first;
+  const int64_t units = (int64_t)wide * halves;
+  const int end = (int)(units * (me + 1) / groups);
+  for (int unit = (int)(units * me / groups); unit < end;) {
+    const int hh = uniform(unit / wide), from = uniform(unit - hh * wide), upto = uniform(min(wide, end - hh * wide));
+    __syncthreads();  // (every wave is done with the weights before)
+    const uint8_t* w = (const uint8_t*)(p.w + (int64_t)hh * 128 * kL);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int f = wave * 16 + i;  // its rows, and values along the sum
+      lds_dma16(w + (f >> 5) * 32 * kL * 2 + (f & 31) * 32, (lane & 31) * kL * 2 + (lane >> 5) * 16, lds + f * kFrag);
+    }
+    wait_all();
+    __syncthreads();
+    if (hh & 1)
+      heads_blocks<true>(p, lds + lane * 16, hh >> 1, first + from, first + upto);
+    else
+      heads_blocks<false>(p, lds + lane * 16, hh >> 1, first + from, first + upto);
+    unit = hh * wide + upto;
+  }
 }
 
 // ---------------------------------------------------------------- attend
@@ -944,7 +920,7 @@ inline PromptLayout prompt_layout(int heads, int64_t cap) {
   return l;
 }
 constexpr int kMaxContext = 1 << 22, kMaxPromptTokens = 1 << 20;
-inline int64_t packed_rows(int32_t context) { return ((int64_t)context + kMTok - 1) & -(int64_t)kMTok; }
+inline int64_t packed_rows(int32_t context) { return ((int64_t)context + kKeys - 1) & -(int64_t)kKeys; }
 
 // 8 waves a workgroup read the keys and values half as often, 4 (two workgroups a CU) run one's start and end under the
 // other's turns: 4 where there are few query tiles, unless the cached tokens may be many more than the new ones (4 and 8
@@ -1041,7 +1017,7 @@ inline int prompt_launch(const PromptParams& p, bool mx, hipStream_t st) {
   else
     hipLaunchKernelGGL(k_prompt_rows<false>, grid, dim3(256), 0, st, p);
   if (int rc = launched()) return rc;
-  hipLaunchKernelGGL(k_prompt_heads, dim3(512), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(k_prompt_heads, dim3(256), dim3(512), 0, st, p);
   if (int rc = launched()) return rc;
   return p.waves == 8 ? attend_and_merge<8>(p, st) : attend_and_merge<4>(p, st);
 }
