@@ -342,17 +342,32 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
 constexpr int kHalfHead = 128 * kL * 2;  // bytes
 constexpr int kAhead = 4;
 template <bool V>
-__device__ __forceinline__ void heads_blocks(const PromptParams& p, uint32_t w_at, int head, int from, int upto) {
+__device__ __forceinline__ void heads_blocks(const PromptParams& p, uint32_t lds, int head, int from, int upto) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   int blk = from + wave;
-  if (blk >= upto) return;
   constexpr int64_t kBlockBytes = 64 * kL * 2;
   const uint8_t* at = p.c + blk * kBlockBytes;
   bf16x8 c[kAhead][2], w[2][4];
+  if (blk < upto) {
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u)
+    for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) c[u][t] = *(const bf16x8*)(at + t * kBlockBytes / 2 + u * kFrag + lane * 16);
+      for (int t = 0; t < 2; ++t) c[u][t] = *(const bf16x8*)(at + t * kBlockBytes / 2 + u * kFrag + lane * 16);
+  }
+  // the weights, a row a load, so that its lines are read whole. A row's 16-byte pieces are in the order of their number
+  // exclusive or the row's, so that reads of a fragment, a piece of 32 rows each, have no bank conflicts
+  const uint8_t* rows = (const uint8_t*)(p.w + (int64_t)(2 * head + V) * 128 * kL);
+  __syncthreads();  // (every wave is done with the weights before)
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = wave * 16 + i;
+    lds_dma16(rows + r * kL * 2, (lane ^ (r & 31)) * 16, lds + r * kL * 2);
+  }
+  wait_all();
+  __syncthreads();
+  if (blk >= upto) return;
+  const uint32_t w_at = lds + (lane & 31) * kL * 2 + ((lane & 31) ^ (lane >> 5)) * 16;
+  auto weight = [&](int j, int ks) { return lds_read<bf16x8>((w_at ^ (ks << 5)) + j * 32 * kL * 2); };
   for (;; blk += 8) {
     const bool more = blk + 8 < upto;
     const uint8_t* next = more ? at + 8 * kBlockBytes : at;
@@ -362,7 +377,7 @@ __device__ __forceinline__ void heads_blocks(const PromptParams& p, uint32_t w_a
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[t][j] = f32x16{};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[0][j] = lds_read<bf16x8>(w_at + j * (kL / 16) * kFrag);
+    for (int j = 0; j < 4; ++j) w[0][j] = weight(j, 0);
 #pragma unroll 1
     for (int k = 0; k < kL / 16; k += kAhead) {
       const uint8_t* ahead = k + kAhead < kL / 16 ? at + (k + kAhead) * kFrag : next;
@@ -370,7 +385,7 @@ __device__ __forceinline__ void heads_blocks(const PromptParams& p, uint32_t w_a
       for (int u = 0; u < kAhead; ++u) {
         const int after = (k + u + 1) % (kL / 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[(u + 1) & 1][j] = lds_read<bf16x8>(w_at + (j * (kL / 16) + after) * kFrag);
+        for (int j = 0; j < 4; ++j) w[(u + 1) & 1][j] = weight(j, after);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -451,19 +466,10 @@ __global__ __launch_bounds__(512, 2) void k_prompt_heads(PromptParams p) {
   const int end = (int)(units * (me + 1) / groups);
   for (int unit = (int)(units * me / groups); unit < end;) {
     const int hh = uniform(unit / wide), from = uniform(unit - hh * wide), upto = uniform(min(wide, end - hh * wide));
-    __syncthreads();  // (every wave is done with the weights before)
-    const uint8_t* w = (const uint8_t*)(p.w + (int64_t)hh * 128 * kL);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int f = wave * 16 + i;  // its rows, and values along the sum
-      lds_dma16(w + (f >> 5) * 32 * kL * 2 + (f & 31) * 32, (lane & 31) * kL * 2 + (lane >> 5) * 16, lds + f * kFrag);
-    }
-    wait_all();
-    __syncthreads();
     if (hh & 1)
-      heads_blocks<true>(p, lds + lane * 16, hh >> 1, first + from, first + upto);
+      heads_blocks<true>(p, lds, hh >> 1, first + from, first + upto);
     else
-      heads_blocks<false>(p, lds + lane * 16, hh >> 1, first + from, first + upto);
+      heads_blocks<false>(p, lds, hh >> 1, first + from, first + upto);
     unit = hh * wide + upto;
   }
 }
@@ -881,11 +887,12 @@ template <int W>
 __global__ __launch_bounds__(1024, 8) void k_prompt_merge(PromptParams p) {
   __shared__ f32x4 sums[3][4][4][64];
   __shared__ f32x2 tops[3][4][64];
-  __shared__ int list[kMaxShares], counts[kMaxShares / 64];
+  __shared__ int list[kMaxShares][6], counts[kMaxShares / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, vb = wave & 3, slice = wave >> 2;
   const int half = lane >> 5, col = lane & 31;
-  const bool is_cut = tid < shares_of(W) && p.cut[tid].parts > 0;
-  const uint64_t those = __ballot(is_cut);
+  PromptCut mine{};
+  if (tid < shares_of(W)) mine = p.cut[tid];
+  const uint64_t those = __ballot(mine.parts > 0);
   if (lane == 0 && wave < kMaxShares / 64) counts[wave] = __builtin_popcountll(those);
   __syncthreads();
   int before = 0, cuts = 0;
@@ -894,32 +901,44 @@ __global__ __launch_bounds__(1024, 8) void k_prompt_merge(PromptParams p) {
     if (i < wave) before += counts[i];
     cuts += counts[i];
   }
-  if (is_cut) list[before + __builtin_popcountll(those & ((1ull << lane) - 1))] = tid;
+  if (mine.parts > 0) {
+    int* to = list[before + __builtin_popcountll(those & ((1ull << lane) - 1))];
+    to[0] = mine.parts, to[1] = mine.head, to[2] = mine.t0, to[3] = mine.n, to[4] = mine.qt, to[5] = tid;
+  }
   for (int job = blockIdx.x; job < cuts * W; job += gridDim.x) {
     __syncthreads();  // (the list is there; the sums before have been read)
-    const int share = uniform(list[job / W]), group = job % W;
-    const PromptCut c = p.cut[share];
+    const int* from = list[job / W];
+    const PromptCut c = {uniform(from[0]), uniform(from[1]), uniform(from[2]), uniform(from[3]), uniform(from[4]), {}};
+    const int share = uniform(from[5]), group = job % W;
     const int row0 = c.qt * rows_of(W) + group * 32, row = row0 + col;
     if (row0 >= c.n) continue;
     auto slot = [&](int i) { return 2 * (share + i) + (i == 0); };
     auto ml_of = [&](int i) { return *(const f32x2*)(p.part_ml + ((int64_t)slot(i) * rows_of(W) + group * 32 + col) * 2); };
-    float top = -__builtin_inff();
-#pragma unroll 8
-    for (int i = slice; i <= c.parts; i += 4) top = fmaxf(top, ml_of(i)[0]);
+    auto part_of = [&](int i, f32x4 (&x)[4]) {
+      const f32x4* from = (const f32x4*)p.part_o + (((int64_t)slot(i) * W + group) * 16 + vb * 4) * 64 + lane;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = from[j * 64];
+    };
     f32x16 o = {};
-    float sum = 0.0f;
-    const f32x4* parts = (const f32x4*)p.part_o + (int64_t)group * 16 * 64 + vb * 4 * 64 + lane;
-#pragma unroll 2
-    for (int i = slice; i <= c.parts; i += 4) {
-      const f32x2 ml = ml_of(i);
+    float sum = 0.0f, top = -__builtin_inff();
+    auto add = [&](f32x2 ml, const f32x4 (&x)[4]) {
       const float by = ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - top);
-      const f32x4* from = parts + (int64_t)slot(i) * W * 16 * 64;
       sum += ml[1] * by;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 x = from[j * 64];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[4 * j + e] += x[e] * by;
+      for (int i = 0; i < 16; ++i) o[i] += x[i >> 2][i & 3] * by;
+    };
+    if (slice <= c.parts) {
+      f32x4 x[4];
+      const f32x2 ml = ml_of(slice);
+      part_of(slice, x);  // (on its way while the maximum is found)
+      top = ml[0];
+#pragma unroll 8
+      for (int i = slice + 4; i <= c.parts; i += 4) top = fmaxf(top, ml_of(i)[0]);
+      add(ml, x);
+#pragma unroll 2
+      for (int i = slice + 4; i <= c.parts; i += 4) {
+        part_of(i, x);
+        add(ml_of(i), x);
       }
     }
     if (slice > 0 && slice <= c.parts) {
