@@ -1002,12 +1002,14 @@ constexpr int kMaxContext = 1 << 22, kMaxPromptTokens = 1 << 20;
 inline int64_t packed_rows(int32_t context) { return ((int64_t)context + kKeys - 1) & -(int64_t)kKeys; }
 
 // 8 waves a workgroup read the keys and values half as often, 4 (two workgroups a CU) run one's start and end under the
-// other's turns: 4 where there are few query tiles, unless the cached tokens may be many more than the new ones (4 and 8
-// waves, us: 193 tokens over 893, 16 heads 42 and 50; 512 and 2048 tokens alone, 32 heads 47 and 53, 102 and 106;
-// 4096 alone 246 and 242, 8 times 1024 over 2048, 16 heads 254 and 238; 300 over 65300, 16 heads 723 and 672)
+// other's turns. So 4 for short prompts and chunks, unless the cached tokens may be many: by the mean query tokens of a
+// sequence and what bounds its length (4 and 8 waves, us a call, 16 to 64 heads: 193 tokens over 700 38 and 44; 512 and
+// 2048 tokens alone 43 and 47, 100 and 100; 16 ragged prompts of up to 500 70 and 78, of up to 1000 209 and 224; 8 of up to 300
+// over 3000 144 and 157; 4 of up to 1024 over 4096 293 and 294; 512 over 16384 185 and 179; 300 over 65000 615 and 592; 8191 alone
+// 769 and 742)
 inline int waves_for(const mkmoe_latent_prompt_io* io) {
-  const int64_t tiles = ((int64_t)io->tokens / rows_of(8) + io->seqs) * io->heads;
-  return tiles <= 320 && io->max_context / 128 < io->tokens ? 4 : 8;
+  const int64_t table = (int64_t)io->max_pages * io->cache.page_size, context = io->max_context / io->seqs;
+  return io->tokens / io->seqs <= 2048 && (context < table ? context : table) <= 32768 ? 4 : 8;
 }
 inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_bytes, PromptParams& p) {
   if (!io || !ws) return MKMOE_ERR_NULL;

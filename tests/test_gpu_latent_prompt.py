@@ -102,6 +102,18 @@ def test_attend(case, fmt):
     b.check(out, lse)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("new,lens,heads", [([1], [1], 3), ([33, 0, 2], [97, 50, 1500], 16), ([255, 256, 257], [300, 256, 2000], 2),
+                                            ([300, 70], [1300, 700], 2), ([513], [1600], 4), ([777], [777], 16)])  # fmt: skip
+def test_tables_of_long_sequences(new, lens, heads, fmt):
+    """Where a sequence may be long by its table and by max_context, a call is cut otherwise."""
+    print(f"\nlong tables {fmt} {new} {lens} {heads}", flush=True)
+    b = Batch(sum(new) + 1, heads, fmt, 64, new, lens, width=520)
+    lse = torch.empty(sum(new), heads, device="cuda")
+    out = _runner(heads, max_context=33280 * len(new)).attend(*b.args(), q_starts=b.dev_starts, lse=lse)
+    b.check(out, lse)
+
+
 @pytest.mark.parametrize("context", [2048, 65536])  # the call's cut: few query tiles, or cached tokens that may be many
 @pytest.mark.parametrize("new,lens,heads", [([130], [130], 3), ([300, 70], [1300, 700], 2), ([513], [1600], 4)])
 def test_both_cuts(new, lens, heads, context):
