@@ -337,8 +337,13 @@ __global__ __launch_bounds__(256) void k_prompt_rows(PromptParams p) {
 
 // ---------------------------------------------------------------- keys and values of every head
 // The product of packed rows and kv_b. A workgroup, one a CU, keeps 128 of the weights' rows, a head's W_UK or W_UV, in
-// LDS as fragments, and its waves go through the tokens on their own, 64 a turn by the 128 rows, the tokens' fragments
-// coming from memory four ahead. The weights are read from LDS by every wave for 64 tokens: half of what LDS can deliver.
+// LDS, and its 8 waves go through the tokens on their own, without barriers: 64 tokens a turn by the 128 rows (8 matrix
+// instructions to 4 reads of LDS, half of what it can deliver, and 2 of memory), the tokens' fragments coming from memory
+// four steps ahead, on into the next turn. Stages of tokens and weights through LDS with a barrier each took a quarter longer (300
+// over 65300 677 -> 613 us a call, 8191 over 16383 178 -> 143 of it).
+// Power bounds it: 16384 tokens of 32 heads, 137 GFLOP, take 135 to 143 us (0.96 to 1.02 PFLOP/s), the matrix units busy for 61 % of
+// the cycles at 1.75 GHz; 65300 of 16 heads, 535 MB written, 246 to 306. 893 of 16 heads take 12: the weights' and tokens'
+// first loads and one turn (32 rows a wave, four waves a turn, instead: 13).
 constexpr int kHalfHead = 128 * kL * 2;  // bytes
 constexpr int kAhead = 4;
 template <bool V>
@@ -1027,10 +1032,13 @@ inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_b
   if (!isfinite(scale2) || io->max_pages < 1 || io->table_stride < io->max_pages) return MKMOE_ERR_ARG;
   const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
   if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
-  // the work's units are counted in 32 bits
-  p.waves = waves_for(io);
-  const int64_t units = ((max_len < cap ? max_len : cap) >> key_shift(p.waves)) + 1 + kItemSetup;
-  if (((int64_t)io->tokens / rows_of(p.waves) + io->seqs) * io->heads * units > 0x3fffffff) return MKMOE_ERR_ARG;
+  // the work's units are counted in 32 bits (a quarter as many with 8 waves)
+  auto countable = [&](int waves) {
+    const int64_t units = ((max_len < cap ? max_len : cap) >> key_shift(waves)) + 1 + kItemSetup;
+    return ((int64_t)io->tokens / rows_of(waves) + io->seqs) * io->heads * units <= 0x3fffffff;
+  };
+  if (!countable(8)) return MKMOE_ERR_ARG;
+  p.waves = countable(4) ? waves_for(io) : 8;
   const void* wide[] = {io->q_nope, io->q_pe, io->w, io->out};
   for (const void* q : wide)
     if (!aligned(q, 16)) return MKMOE_ERR_ALIGN;

@@ -98,6 +98,10 @@ def test_more_work_than_32_bits_count(lib):
     io = _prompt(tokens=1 << 20, seqs=1, heads=128, max_pages=1 << 18, table_stride=1 << 18, max_context=1 << 22,
                  out_token_stride=16384, qn_token_stride=24576, qp_token_stride=8192)  # fmt: skip
     assert L.mkmoe_latent_prompt(ctypes.byref(io), WS, 1 << 40, None) == -8
+    # (counted: 64 sequences of 1024 that may have 2^20 cached tokens, in one of its two cuts; the next check refuses)
+    io = _prompt(tokens=1 << 16, seqs=64, heads=128, max_pages=1 << 14, table_stride=1 << 14, max_context=1 << 20,
+                 out_token_stride=16384, qn_token_stride=24576, qp_token_stride=8192, w=AT + 2)  # fmt: skip
+    assert L.mkmoe_latent_prompt(ctypes.byref(io), WS, 1 << 40, None) == -4
 
 
 @pytest.mark.parametrize("ws,size,code", [(None, 0, -1), (WS + 128, 0, -4), (WS, -1, -5)])
