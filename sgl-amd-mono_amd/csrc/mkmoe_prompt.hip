@@ -43,11 +43,11 @@ constexpr __host__ __device__ int shares_of(int waves) { return 2048 / waves; }
 constexpr __host__ __device__ int rows_of(int waves) { return 32 * waves; }
 constexpr __host__ __device__ int key_shift(int waves) { return waves == 8 ? 6 : 5; }
 constexpr int kKeys = 64;           // a sequence's packed rows are a multiple of so many
-// units of work that a share has at least (6, 10, 16: 193 tokens over 893 42, 44, 47 us)
+// units of work that a share has at least (4, 6, 9: 193 tokens over 893 37.5, 36.1, 37.6 us)
 constexpr int kLeastUnits = 6;
 constexpr int kFrag = 1024;         // bytes of a fragment
 constexpr int kPromptSeqs = MKMOE_LATENT_MAX_SEQS;
-// What starting and storing a query tile takes, in turns of keys (2, 4, 8: ragged prompts' step 209, 197, 192 us)
+// What starting and storing a query tile takes, in turns of keys (5, 8, 12: ragged prompts' step 183, 179, 179 us)
 constexpr int kItemSetup = 8;
 constexpr float kMoveBy = 8.0f;     // a row's maximum moves where a score passes it by more than 2^kMoveBy
 constexpr float kLog2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
@@ -463,7 +463,8 @@ __global__ __launch_bounds__(512, 2) void k_prompt_heads(PromptParams p) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int blocks = uniform(p.plan->rows) / kKeys, halves = 2 * p.heads;
   // The tokens in as many parts as one or eight, and a part's blocks of 64, half head by half head, in equal shares for its
-  // workgroups. Eight: an XCD's workgroups go through its part together, and its L2 keeps the tokens between them
+  // workgroups. Eight: an XCD's workgroups go through its part together, and its L2 keeps the tokens between them; one: the
+  // shares are evener turns of 8 waves (300 over 65300: 610 and 626 us; ragged prompts' step of 6000 tokens: 205 and 193)
   const int parts = blocks >= 512 ? 8 : 1, groups = gridDim.x / parts;
   const int part = parts == 8 ? blockIdx.x & 7 : 0, me = parts == 8 ? blockIdx.x >> 3 : (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
   const int first = (int)((int64_t)blocks * part / parts), wide = (int)((int64_t)blocks * (part + 1) / parts) - first;
