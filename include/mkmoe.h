@@ -389,8 +389,9 @@ int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_p
 /* ---- a prompt's tokens
  * The same attention with a key and a value for each head and token, made from the cached rows by
  * w: k = [W_UK c, k_pe], v = W_UV c, o = sum softmax(scale q . k) v: fewer operations than the absorbed form
- * from about 171 query tokens a sequence. Keys are rounded to bf16, values and softmax's numerators to fp16 (values
- * that it does not hold to bf16), sums, scores and maxima are fp32. Query token i of a sequence's n sees its first len - n + 1 + i tokens. */
+ * from about 171 query tokens a sequence. Keys are rounded to bf16, values and softmax's numerators to fp16 (to
+ * bf16 in tiles of 64 tokens with a value, not 0, outside 2^-26 .. 128), sums, scores and maxima are fp32. Values whose size
+ * passes 2^100 may give infinities. Query token i of a sequence's n sees its first len - n + 1 + i tokens. */
 typedef struct mkmoe_latent_prompt_io {
   mkmoe_latent_cache cache;
   int32_t seqs;        /* 1 .. MKMOE_LATENT_MAX_SEQS */

@@ -23,8 +23,8 @@
 // any exchange between lanes.
 //
 // Rounded to fewer bits than fp32 are the operands of the matrix instructions: keys to bf16, whose range
-// queries need, numerators and values to fp16 (3 more bits), a tile's values to bf16 where fp16 would lose some
-// (k_prompt_heads). Against 64 bits, in the 2-norm, where the output's own rounding is 0.0017: 0.0021 where rows see few
+// queries need, numerators and values to fp16 (3 more bits), a tile's values to bf16 where fp16 would be coarser
+// for one of them (k_prompt_heads). Against 64 bits, in the 2-norm, where the output's own rounding is 0.0017: 0.0021 where rows see few
 // keys (bf16 numerators and values 0.0028), 0.0017 over long ones. Sums, maxima, outputs and parts are fp32.
 //
 // Times below are of an MI355X, of passes among others. It copies 4.9 TB/s and multiplies bf16 matrices at 1.39
@@ -51,6 +51,10 @@ constexpr int kPromptSeqs = MKMOE_LATENT_MAX_SEQS;
 constexpr int kItemSetup = 8;
 constexpr float kMoveBy = 8.0f;     // a row's maximum moves where a score passes it by more than 2^kMoveBy
 constexpr float kLog2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
+// Values in fp16 are held 2^kValueLift above themselves, so that fp16 is no coarser than bf16 for any from 2^-26, where its
+// spacing of 2^-24 is bf16's 2^-7 of them, up to kValueMost. Outputs are 2^kValueLift above themselves until they are stored
+constexpr int kValueLift = 9;
+constexpr float kValueUnit = 0x1p-9f, kValueLeast = 0x1p-17f * kValueUnit, kValueMost = 65504.0f * kValueUnit;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -70,8 +74,9 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 __device__ __forceinline__ float add_f16(uint32_t w, float c) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
 }
-__device__ __forceinline__ float add_bf16(uint32_t w, float c) { return c + bf_lo(w) + bf_hi(w); }
-// the largest of scores; NaN where one is (their row's output is NaN either way)
+// (bf16 ones are 2^kValueLift above fp16's, whose values are)
+__device__ __forceinline__ float add_bf16(uint32_t w, float c) { return fmaf(bf_lo(w) + bf_hi(w), kValueUnit, c); }
+// the largest, of scores say; NaN where one is (their row's output is NaN either way)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
@@ -432,19 +437,27 @@ __device__ __forceinline__ void heads_blocks(const PromptParams& p, uint32_t lds
         store_as(pack, [] { return false; });
     };
     if constexpr (V) {
-      // fp16 where that loses nothing that counts: none above its range, the largest so far above its smallest
-      // normal value that what is below that is less than 2^-19 of it (or all 0)
-      uint32_t top = 0;
+      // fp16 where it is no coarser than bf16 for any of the values that is not 0: a query may see one token alone, and
+      // outputs are never mixed, so what a value loses is not measured by another one
+      float top = 0.0f;
+      uint32_t low = ~0u;  // of a size's bits, less one: 0, which is held exactly, comes last
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top = max(top, f2u(acc[t][j][i]) & 0x7fffffffu);
-      const bool half = __ballot(top >= f2u(65504.0f)) == 0 && (__ballot(top >= f2u(0x1p-6f)) != 0 || __ballot(top != 0) == 0);
+          for (int i = 0; i < 16; i += 2) {
+            const float x = acc[t][j][i], y = acc[t][j][i + 1];
+            top = max3(top, fabsf(x), fabsf(y));
+            low = min(min(low, (f2u(x) << 1) - 1), (f2u(y) << 1) - 1);
+          }
+      const bool half = __ballot(!(top < kValueMost) || low < (f2u(kValueLeast) << 1) - 1) == 0;
       if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + blk] = !half;
       if (half) {
-        store([](float x, float y) { return pack_f16(x, y); });
+        store([](float x, float y) {
+          // (a fused product and sum is rounded to fp16 by the same instruction)
+          return pack_f16(fmaf(x, 1.0f / kValueUnit, 0.0f), fmaf(y, 1.0f / kValueUnit, 0.0f));
+        });
       } else {
         if (lane == 0) atomicOr(&p.plan->odd, 1);
         store([](float x, float y) { return pack_bf(x, y); });
@@ -816,10 +829,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
 #pragma unroll
       for (int hh = 0; hh < NB; ++hh) {
         const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
+        const float mu = in_bf ? r.mu - kValueLift : r.mu;
         u32x4 num[2];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - r.mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - r.mu);
+          const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - mu);
           const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
           r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
           num[x >> 2][x & 3] = w;
@@ -863,7 +877,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
     const auto sw = __builtin_amdgcn_permlane32_swap(f2u(r.sum), f2u(r.sum), false, false);
     const float sum = u2f(sw[0]) + u2f(sw[1]);
     if (from == 0 && upto == it.tiles) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float inv = sum == 0.0f ? 0.0f : kValueUnit / sum;
 #pragma unroll
       for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, head, row, r.o[vb], vb, inv, half);
       if (p.lse && half == 0 && row < it.n)
@@ -972,7 +986,7 @@ __global__ __launch_bounds__(1024, 8) void k_prompt_merge(PromptParams p) {
         for (int e = 0; e < 4; ++e) o[4 * j + e] += x[e] * by;
       }
     }
-    store_row(p, c.t0, c.n, c.head, row, o, vb, sum == 0.0f ? 0.0f : 1.0f / sum, half);
+    store_row(p, c.t0, c.n, c.head, row, o, vb, sum == 0.0f ? 0.0f : kValueUnit / sum, half);
     if (p.lse && vb == 0 && half == 0 && row < c.n)
       p.lse[(int64_t)(c.t0 + row) * p.heads + c.head] = sum == 0.0f ? -__builtin_inff() : (all + __builtin_amdgcn_logf(sum)) * kLog2;
   }
