@@ -564,7 +564,7 @@ __device__ __forceinline__ void store_row(const PromptParams& p, int t0, int n, 
 struct Rows {
   bf16x8 q[12];   // 8 fragments of the values without rotation, dealt, and 4 of the rotated ones
   f32x16 o[4];    // outputs, 32 values each
-  float m, mu;    // the maximum so far (times scale log2 e); what scores are taken less, kLift below it
+  float top, mu;  // the largest score so far; what scores times scale log2 e are taken less, kLift below its
   float sum;      // of the lane's numerators
   int sees;       // the last key that the row sees
 };
@@ -588,20 +588,28 @@ __device__ __forceinline__ void mask_block(const Rows& r, f32x16& s, int key0, i
   for (int i = 0; i < 16; ++i)
     if (key0 + 8 * (i >> 2) + 4 * half + (i & 3) > r.sees) s[i] = -__builtin_inff();
 }
+// Scores times scale log2 e are rounded together with what they are taken less, which differs from the largest one's own
+// exponent by its rounding: no more than 2^-13 for exponents up to kFar. Past it (far) scores are taken less the largest one first
+constexpr float kFar = 0x1p10f;
 // the row's maximum moved to its new scores', where one of the wave's passes it by more than 2^kMoveBy
-__device__ __forceinline__ void move_max(const PromptParams& p, Rows& r, float top) {
+__device__ __forceinline__ void move_max(const PromptParams& p, Rows& r, bool& far, float top) {
   const auto sw = __builtin_amdgcn_permlane32_swap(f2u(top), f2u(top), false, false);
-  top = max3(u2f(sw[0]), u2f(sw[1]), u2f(sw[1])) * p.scale2;
-  if (__ballot(top > r.m + kMoveBy)) {
-    const float to = fmaxf(r.m, top), by = to == r.m ? 1.0f : __builtin_amdgcn_exp2f(r.m - to);
-    r.m = to;
-    r.mu = to == -__builtin_inff() ? 0.0f : to - kLift;
+  top = max3(u2f(sw[0]), u2f(sw[1]), u2f(sw[1]));
+  if (__ballot((top - r.top) * p.scale2 > kMoveBy)) {
+    const float to = fmaxf(r.top, top), by = to == r.top ? 1.0f : __builtin_amdgcn_exp2f((r.top - to) * p.scale2);
+    r.top = to;
+    r.mu = to == -__builtin_inff() ? 0.0f : fmaf(to, p.scale2, -kLift);
+    far = __ballot(fabsf(r.mu) > kFar) != 0;
     r.sum *= by;
 #pragma unroll
     for (int vb = 0; vb < 4; ++vb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) r.o[vb][i] *= by;
   }
+}
+// log sum exp of a row whose largest score is top
+__device__ __forceinline__ float lse_of(const PromptParams& p, float top, float sum) {
+  return sum == 0.0f ? -__builtin_inff() : (fmaf(top, p.scale2, -kLift) + __builtin_amdgcn_logf(sum)) * kLog2;
 }
 __device__ __forceinline__ float top_of(const f32x16& s) {
   float top = s[0];
@@ -723,7 +731,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
     }
     barrier();  // every wave has read the turns of the item before
 
-    r.m = -__builtin_inff();
+    r.top = -__builtin_inff();
     r.mu = r.sum = 0.0f;
     r.sees = it.past + row;  // the last key that the row sees
 #pragma unroll
@@ -758,13 +766,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
       wait_loads<0>();
     barrier();
     int kt = from;
+    bool far = false;  // some row's scores are
     if (seen > from) {
       score<W>(r, s0, keys_at(from), 0);
       if (from >= whole) mask_block(r, s0, from * TK, half);
-      move_max(p, r, top_of(s0));
+      move_max(p, r, far, top_of(s0));
     }
     bool swapped = false;
-    while (!mixed && kt + 1 < seen) {  // two blocks a time, of one turn or of two
+    while (!mixed && !far && kt + 1 < seen) {  // two blocks a time, of one turn or of two
       turn(kt);
       uint32_t k_at = keys_at(NB == 2 ? kt : kt + 1), v_at = vals_at(kt), next_at = keys_at(kt + 1);
       // 20 fragments a block in turn: 12 of keys for the next block's scores, 8 of values for this one's outputs; each
@@ -772,13 +781,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
       u32x4 f[3], num[2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        if (NB == 1 && hh == 1) {
-          ++kt;
-          swapped = kt + 1 >= seen;
+        if (hh == 1) {
+          if (NB == 1) ++kt;
+          swapped = far || (NB == 1 && kt + 1 >= seen);
           if (swapped) break;
-          turn(kt);
-          next_at = keys_at(kt + 1);
-          v_at = vals_at(kt);
+          if (NB == 1) {
+            turn(kt);
+            next_at = keys_at(kt + 1);
+            v_at = vals_at(kt);
+          }
         }
         f32x16 &now = hh == 0 ? s0 : s1, &then = hh == 0 ? s1 : s0;
         auto frag = [&](int j) {
@@ -817,23 +828,30 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        move_max(p, r, top);
+        move_max(p, r, far, top);
       }
       if (!swapped) ++kt;
+      if (swapped) break;
     }
-    if (swapped) s0 = s1;
-    for (; kt < upto; ++kt) {
-      turn(kt);
+    int done = 0;  // blocks of turn kt that are
+    if (swapped) {
+      s0 = s1;
+      done = NB - 1;
+    }
+    for (; kt < upto; ++kt, done = 0) {
+      if (done == 0) turn(kt);
       if (kt >= seen) continue;
       const bool in_bf = mixed && odd[kt * TK / kKeys] != 0;
 #pragma unroll
       for (int hh = 0; hh < NB; ++hh) {
+        if (hh < done) continue;
         const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
-        const float mu = in_bf ? r.mu - kValueLift : r.mu;
+        const float top = r.top == -__builtin_inff() ? 0.0f : r.top, lift = in_bf ? kLift + kValueLift : kLift;
         u32x4 num[2];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          const float y = __builtin_amdgcn_exp2f(s0[2 * x] * p.scale2 - mu), z = __builtin_amdgcn_exp2f(s0[2 * x + 1] * p.scale2 - mu);
+          const float y = __builtin_amdgcn_exp2f(fmaf(s0[2 * x] - top, p.scale2, lift));
+          const float z = __builtin_amdgcn_exp2f(fmaf(s0[2 * x + 1] - top, p.scale2, lift));
           const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
           r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
           num[x >> 2][x & 3] = w;
@@ -870,7 +888,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
         if (then < seen) {
           score<W>(r, s0, keys_at(then), (hh + 1) % NB);
           if (then >= whole) mask_block(r, s0, kt * TK + (hh + 1) * 32, half);
-          move_max(p, r, top_of(s0));
+          move_max(p, r, far, top_of(s0));
         }
       }
     }
@@ -881,7 +899,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
 #pragma unroll
       for (int vb = 0; vb < 4; ++vb) store_row(p, it.t0, it.n, head, row, r.o[vb], vb, inv, half);
       if (p.lse && half == 0 && row < it.n)
-        p.lse[(int64_t)(it.t0 + row) * p.heads + head] = sum == 0.0f ? -__builtin_inff() : (r.mu + __builtin_amdgcn_logf(sum)) * kLog2;
+        p.lse[(int64_t)(it.t0 + row) * p.heads + head] = lse_of(p, r.top, sum);
     } else if (row0 < it.n) {
       const int slot = 2 * share + (from == 0);
       f32x4* to = (f32x4*)p.part_o + ((int64_t)slot * W + wave) * 16 * 64 + lane;
@@ -890,9 +908,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           to[(vb * 4 + i) * 64] = f32x4{r.o[vb][4 * i], r.o[vb][4 * i + 1], r.o[vb][4 * i + 2], r.o[vb][4 * i + 3]};
-      // (where the row saw no score yet its sum is 0, and the part counts for nothing)
-      const float mu = r.m == -__builtin_inff() ? r.m : r.mu;
-      if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * rows_of(W) + wave * 32 + col) * 2) = f32x2{mu, sum};
+      // (where the row saw no score yet its largest is -inf, its sum 0, and the part counts for nothing)
+      if (half == 0) *(f32x2*)(p.part_ml + ((int64_t)slot * rows_of(W) + wave * 32 + col) * 2) = f32x2{r.top, sum};
     }
     if (it.parts > 0) cut = PromptCut{it.parts, it.head, it.t0, it.n, it.qt, {}};
   }
@@ -942,7 +959,7 @@ __global__ __launch_bounds__(1024, 8) void k_prompt_merge(PromptParams p) {
     f32x16 o = {};
     float sum = 0.0f, top = -__builtin_inff();
     auto add = [&](f32x2 ml, const f32x4 (&x)[4]) {
-      const float by = ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - top);
+      const float by = ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f((ml[0] - top) * p.scale2);
       sum += ml[1] * by;
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i] += x[i >> 2][i & 3] * by;
@@ -971,13 +988,13 @@ __global__ __launch_bounds__(1024, 8) void k_prompt_merge(PromptParams p) {
     const int more = min(c.parts, 3);
     float all = top;
     for (int i = 0; i < more; ++i) all = fmaxf(all, tops[i][vb][lane][0]);
-    const float by0 = top == all ? 1.0f : __builtin_amdgcn_exp2f(top - all);
+    const float by0 = top == all ? 1.0f : __builtin_amdgcn_exp2f((top - all) * p.scale2);
     sum *= by0;
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] *= by0;
     for (int i = 0; i < more; ++i) {
       const f32x2 ml = tops[i][vb][lane];
-      const float by = ml[0] == all ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - all);
+      const float by = ml[0] == all ? 1.0f : __builtin_amdgcn_exp2f((ml[0] - all) * p.scale2);
       sum += ml[1] * by;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -988,7 +1005,7 @@ __global__ __launch_bounds__(1024, 8) void k_prompt_merge(PromptParams p) {
     }
     store_row(p, c.t0, c.n, c.head, row, o, vb, sum == 0.0f ? 0.0f : kValueUnit / sum, half);
     if (p.lse && vb == 0 && half == 0 && row < c.n)
-      p.lse[(int64_t)(c.t0 + row) * p.heads + c.head] = sum == 0.0f ? -__builtin_inff() : (all + __builtin_amdgcn_logf(sum)) * kLog2;
+      p.lse[(int64_t)(c.t0 + row) * p.heads + c.head] = lse_of(p, all, sum);
   }
 }
 

@@ -77,3 +77,41 @@ def test_values_of_all_sizes(waves):
     out = runner().attend(*b.args(), q_starts=b.dev_starts)
     o, _, bound, _ = b.want()
     ref.assert_within(out, o, bound, "out")
+
+
+@CUTS
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("log2,border", [(9, 300), (10, 300), (10, 330), (16, 300), (23, 300), (27, 300), (40, 300), (100, 300)])
+def test_scores_far_from_0(log2, border, sign, waves):
+    """Scores of 2^log2 and half of it that differ by a few units of their last places, all of them and their sums exact
+    in fp32: the weights are those of the differences. A numerator is rounded by up to 2^-11 (and 2^-20 for its
+    exponential), in the output's sum and in the weights', a value and the output by 2^-8 each."""
+    heads, n, length = 2, 150, 400
+    b, runner = _batch(34, heads, "bf16", [n], [length], waves)
+    pages, places = _tokens(b, 0, 0, length)
+    low = (torch.arange(length, device="cuda") < border) == (sign > 0)  # what weighs more comes later
+    size = torch.where(low, 0.5, 1.0).double() * 2.0 ** (log2 - log2 // 2)
+    step = 2.0 ** max(-1, log2 - 23)
+    units = torch.randint(0, 6, (length,), generator=b.g, device="cuda").double()
+    b.cache[pages, places, 0] = size.to(b.cache.dtype)
+    b.cache[pages, places, 512:] = 0
+    b.cache[pages, places, 512] = units.to(b.cache.dtype)
+    w = b.w.kv_b.view(heads, 2, 128, 512)
+    w[:, 0] = 0
+    w[:, 0, 0, 0] = 1.0  # a key is its latents' first value
+    w[:, 1, :, 0] = 0  # values near 1
+    b.q_nope, b.q_pe = torch.zeros_like(b.q_nope).contiguous(), torch.zeros_like(b.q_pe)
+    b.q_nope[..., 0] = sign * 2.0 ** (log2 // 2)
+    b.q_pe[..., 0] = step
+    lse = torch.empty(n, heads, device="cuda")
+    out = runner(scale=1.0).attend(*b.args(), lse=lse)
+    s = sign * size * 2.0 ** (log2 // 2) + units * step
+    see = torch.arange(length, device="cuda")[None] <= torch.arange(length - n, length, device="cuda")[:, None]
+    s = s.masked_fill(~see, -float("inf"))
+    p = torch.softmax(s, 1)
+    v = torch.stack([b.cache[pages, places, :512].double() @ w[h, 1].double().T for h in range(heads)])  # [heads, length, 128]
+    fine = 514 * ref.U32 * torch.stack([b.cache[pages, places, :512].double().abs() @ w[h, 1].double().abs().T for h in range(heads)])
+    o, size_o, fine = ((p[None] @ x).transpose(0, 1) for x in (v, v.abs(), fine))
+    ref.assert_within(out, o, (2 * ref.U16 + 2.0**-10 + 2.0**-15) * size_o + 2 * fine, "out")
+    want = torch.logsumexp(s, 1)[:, None].expand(n, heads)
+    ref.assert_within(lse.double(), want, 2.0**-11 + 2.0**-19 + 4 * ref.U32 * want.abs(), "lse")
