@@ -126,7 +126,7 @@ struct PromptParams {
   uint8_t* pe;     // rope fragments [cap / 32][4][1 KB]
   uint8_t* k;      // key fragments [heads][cap / 32][8][1 KB]
   uint8_t* v;      // value fragments [heads][cap / 32][2][4][1 KB]
-  int32_t* odd;    // [heads][cap / 64]: a tile's values are bf16, not fp16
+  int32_t* odd;    // [heads][cap / 64]: a tile's values are 0: fp16, 1: bf16, 2: bf16 and may not be finite
   PromptCut* cut;  // [shares]
   float* part_o;   // [2 shares][W][4][4][64 lanes][4]
   float* part_ml;  // [2 shares][32 W][2]
@@ -452,14 +452,16 @@ __device__ __forceinline__ void heads_blocks(const PromptParams& p, uint32_t lds
             low = min(min(low, (f2u(x) << 1) - 1), (f2u(y) << 1) - 1);
           }
       const bool half = __ballot(!(top < kValueMost) || low < (f2u(kValueLeast) << 1) - 1) == 0;
-      if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + blk] = !half;
+      const bool finite = __ballot(!(top < 0x1p127f)) == 0;  // (in bf16, too)
+      if (lane == 0) p.odd[(int64_t)head * (p.cap / kKeys) + blk] = half ? 0 : finite ? 1 : 2;
       if (half) {
         store([](float x, float y) {
           // (a fused product and sum is rounded to fp16 by the same instruction)
           return pack_f16(fmaf(x, 1.0f / kValueUnit, 0.0f), fmaf(y, 1.0f / kValueUnit, 0.0f));
         });
       } else {
-        if (lane == 0) atomicOr(&p.plan->odd, 1);
+        // (once: 16320 waves' turns that each did took a millisecond)
+        if (lane == 0 && __hip_atomic_load(&p.plan->odd, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) atomicOr(&p.plan->odd, 1);
         store([](float x, float y) { return pack_bf(x, y); });
       }
     } else {
@@ -722,13 +724,17 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
         for (int ds = 0; ds < 4; ++ds) r.q[8 + ds] = *(const bf16x8*)(qp + 16 * ds);
       }
     }
-    // whether some of the tiles have values in bf16
+    // of 64 turns from marks_from on, those whose values are bf16, and those of them with some that may not be finite
     const int32_t* odd = p.odd + (int64_t)head * (p.cap / kKeys) + it.tile;
-    bool mixed = false;
-    if (any_odd) {
-      for (int kt = from + lane; kt < upto; kt += 64) mixed |= odd[kt * TK / kKeys] != 0;
-      mixed = __ballot(mixed) != 0;
-    }
+    uint64_t marked = 0, not_finite = 0;
+    int marks_from = from;
+    auto read_marks = [&](int kt) {
+      const int mark = kt + lane < upto ? odd[(kt + lane) * TK / kKeys] : 0;
+      marked = __ballot(mark != 0);
+      not_finite = __ballot(mark == 2);
+      marks_from = kt;
+    };
+    if (any_odd) read_marks(from);
     barrier();  // every wave has read the turns of the item before
 
     r.top = -__builtin_inff();
@@ -772,125 +778,134 @@ __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {
       if (from >= whole) mask_block(r, s0, from * TK, half);
       move_max(p, r, far, top_of(s0));
     }
-    bool swapped = false;
-    while (!mixed && !far && kt + 1 < seen) {  // two blocks a time, of one turn or of two
-      turn(kt);
-      uint32_t k_at = keys_at(NB == 2 ? kt : kt + 1), v_at = vals_at(kt), next_at = keys_at(kt + 1);
-      // 20 fragments a block in turn: 12 of keys for the next block's scores, 8 of values for this one's outputs; each
-      // is read two products before its own
-      u32x4 f[3], num[2];
+    while (kt < upto) {
+      int plain = upto;  // the turns before it have values in fp16
+      if (any_odd) {
+        if (kt - marks_from >= 63) read_marks(kt);
+        const uint64_t ahead = marked >> (kt - marks_from);
+        plain = ahead != 0 ? kt + __builtin_ctzll(ahead) : marks_from + 63;
+      }
+      // two blocks a time, of one turn or of two, as long as there is a block behind them
+      const int fast = min(seen, plain + 1);
+      bool swapped = false;
+      while (!far && !swapped && kt + 1 < fast) {
+        turn(kt);
+        uint32_t k_at = keys_at(NB == 2 ? kt : kt + 1), v_at = vals_at(kt), next_at = keys_at(kt + 1);
+        // 20 fragments a block in turn: 12 of keys for the next block's scores, 8 of values for this one's outputs; each
+        // is read two products before its own
+        u32x4 f[3], num[2];
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        if (hh == 1) {
-          if (NB == 1) ++kt;
-          swapped = far || (NB == 1 && kt + 1 >= seen);
-          if (swapped) break;
-          if (NB == 1) {
-            turn(kt);
-            next_at = keys_at(kt + 1);
-            v_at = vals_at(kt);
+        for (int hh = 0; hh < 2; ++hh) {
+          if (hh == 1) {
+            if (NB == 1) ++kt;
+            swapped = far || (NB == 1 && kt + 1 >= fast);
+            if (swapped) break;
+            if (NB == 1) {
+              turn(kt);
+              next_at = keys_at(kt + 1);
+              v_at = vals_at(kt);
+            }
           }
+          f32x16 &now = hh == 0 ? s0 : s1, &then = hh == 0 ? s1 : s0;
+          auto frag = [&](int j) {
+            return lds_read<u32x4>(j >= 12  ? v_at + ((NB == 2 ? hh * 8 : 0) + j - 12) * kFrag
+                                   : hh == 0 ? k_at + key_frag<W>(NB - 1, j)
+                                             : next_at + key_frag<W>(0, j));
+          };
+          f[0] = frag(0);
+          f[1] = frag(1);
+#pragma unroll
+          for (int j = 0; j < 12; ++j) {
+            f[(j + 2) % 3] = frag(j + 2);
+            then = mfma32(__builtin_bit_cast(bf16x8, f[j % 3]), r.q[j], j == 0 ? f32x16{} : then);
+#pragma unroll
+            for (int x = j * 8 / 12; x < (j + 1) * 8 / 12; ++x) {
+              uint32_t w = pack_f16(__builtin_amdgcn_exp2f(now[2 * x] * p.scale2 - r.mu),
+                                    __builtin_amdgcn_exp2f(now[2 * x + 1] * p.scale2 - r.mu));
+              r.sum = add_f16(w, r.sum);
+              asm volatile("" : "+v"(w), "+v"(r.sum));  // (formed here, not where they are used)
+              num[x >> 2][x & 3] = w;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          // the next block's turn and first key
+          const int next_kt = NB == 2 ? kt + hh : kt + 1, key0 = NB == 2 ? kt * TK + (hh + 1) * 32 : (kt + 1) * TK;
+          float top = -__builtin_inff();
+#pragma unroll
+          for (int j = 12; j < 20; ++j) {
+            const int vb = j & 3;
+            if (j + 2 < 20) f[(j + 2) % 3] = frag(j + 2);
+            r.o[vb] = mfma32(__builtin_bit_cast(f16x8, f[j % 3]), __builtin_bit_cast(f16x8, num[(j - 12) >> 2]), r.o[vb]);
+            if (j == 14 && next_kt >= whole) mask_block(r, then, key0, half);
+            if (j >= 14) {
+#pragma unroll
+              for (int x = (j - 14) * 8 / 6; x < (j - 13) * 8 / 6; ++x) top = max3(top, then[2 * x], then[2 * x + 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          move_max(p, r, far, top);
         }
-        f32x16 &now = hh == 0 ? s0 : s1, &then = hh == 0 ? s1 : s0;
-        auto frag = [&](int j) {
-          return lds_read<u32x4>(j >= 12  ? v_at + ((NB == 2 ? hh * 8 : 0) + j - 12) * kFrag
-                                 : hh == 0 ? k_at + key_frag<W>(NB - 1, j)
-                                           : next_at + key_frag<W>(0, j));
-        };
-        f[0] = frag(0);
-        f[1] = frag(1);
+        if (!swapped) ++kt;
+      }
+      // a turn of any kind
+      int done = 0;  // blocks of it that are
+      if (swapped) {
+        s0 = s1;
+        done = NB - 1;
+      }
+      if (done == 0) turn(kt);
+      if (kt < seen) {
+        const bool in_bf = any_odd && (marked >> (kt - marks_from) & 1) != 0;
 #pragma unroll
-        for (int j = 0; j < 12; ++j) {
-          f[(j + 2) % 3] = frag(j + 2);
-          then = mfma32(__builtin_bit_cast(bf16x8, f[j % 3]), r.q[j], j == 0 ? f32x16{} : then);
+        for (int hh = 0; hh < NB; ++hh) {
+          if (hh < done) continue;
+          const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
+          const float top = r.top == -__builtin_inff() ? 0.0f : r.top, lift = in_bf ? kLift + kValueLift : kLift;
+          u32x4 num[2];
 #pragma unroll
-          for (int x = j * 8 / 12; x < (j + 1) * 8 / 12; ++x) {
-            uint32_t w = pack_f16(__builtin_amdgcn_exp2f(now[2 * x] * p.scale2 - r.mu),
-                                  __builtin_amdgcn_exp2f(now[2 * x + 1] * p.scale2 - r.mu));
-            r.sum = add_f16(w, r.sum);
-            asm volatile("" : "+v"(w), "+v"(r.sum));  // (formed here, not where they are used)
+          for (int x = 0; x < 8; ++x) {
+            const float y = __builtin_amdgcn_exp2f(fmaf(s0[2 * x] - top, p.scale2, lift));
+            const float z = __builtin_amdgcn_exp2f(fmaf(s0[2 * x + 1] - top, p.scale2, lift));
+            const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
+            r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
             num[x >> 2][x & 3] = w;
           }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        // the next block's turn and first key
-        const int next_kt = NB == 2 ? kt + hh : kt + 1, key0 = NB == 2 ? kt * TK + (hh + 1) * 32 : (kt + 1) * TK;
-        float top = -__builtin_inff();
+          if (in_bf && kt >= whole && (not_finite >> (kt - marks_from) & 1) != 0) {
+            // values that may not be finite, of tokens that some rows do not see: a key at a time, added where it is seen
 #pragma unroll
-        for (int j = 12; j < 20; ++j) {
-          const int vb = j & 3;
-          if (j + 2 < 20) f[(j + 2) % 3] = frag(j + 2);
-          r.o[vb] = mfma32(__builtin_bit_cast(f16x8, f[j % 3]), __builtin_bit_cast(f16x8, num[(j - 12) >> 2]), r.o[vb]);
-          if (j == 14 && next_kt >= whole) mask_block(r, then, key0, half);
-          if (j >= 14) {
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int x = (j - 14) * 8 / 6; x < (j - 13) * 8 / 6; ++x) top = max3(top, then[2 * x], then[2 * x + 1]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        move_max(p, r, far, top);
-      }
-      if (!swapped) ++kt;
-      if (swapped) break;
-    }
-    int done = 0;  // blocks of turn kt that are
-    if (swapped) {
-      s0 = s1;
-      done = NB - 1;
-    }
-    for (; kt < upto; ++kt, done = 0) {
-      if (done == 0) turn(kt);
-      if (kt >= seen) continue;
-      const bool in_bf = mixed && odd[kt * TK / kKeys] != 0;
-#pragma unroll
-      for (int hh = 0; hh < NB; ++hh) {
-        if (hh < done) continue;
-        const uint32_t v_at = vals_at(kt) + hh * 8 * kFrag;
-        const float top = r.top == -__builtin_inff() ? 0.0f : r.top, lift = in_bf ? kLift + kValueLift : kLift;
-        u32x4 num[2];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float y = __builtin_amdgcn_exp2f(fmaf(s0[2 * x] - top, p.scale2, lift));
-          const float z = __builtin_amdgcn_exp2f(fmaf(s0[2 * x + 1] - top, p.scale2, lift));
-          const uint32_t w = in_bf ? pack_bf(y, z) : pack_f16(y, z);
-          r.sum = in_bf ? add_bf16(w, r.sum) : add_f16(w, r.sum);
-          num[x >> 2][x & 3] = w;
-        }
-        if (in_bf && kt >= whole) {
-          // values that may not be finite, of tokens that some rows do not see: a key at a time, added where it is seen
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
+              for (int vb = 0; vb < 4; ++vb)
 #pragma unroll 1
-            for (int x = 0; x < 16; ++x) {
-              const int h = x >> 3, e = x & 7;
-              const bool sees = kt * TK + 32 * hh + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= r.sees;
-              const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
-              const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
-              const bf16x8 one = __builtin_bit_cast(bf16x8, num[t] & only);
+                for (int x = 0; x < 16; ++x) {
+                  const int h = x >> 3, e = x & 7;
+                  const bool sees = kt * TK + 32 * hh + 16 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= r.sees;
+                  const uint32_t word = half == h ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+                  const u32x4 only = {e >> 1 == 0 ? word : 0u, e >> 1 == 1 ? word : 0u, e >> 1 == 2 ? word : 0u, e >> 1 == 3 ? word : 0u};
+                  const u32x4 a = lds_read<u32x4>(v_at + (t * 4 + vb) * kFrag);
+                  const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), __builtin_bit_cast(bf16x8, num[t] & only), f32x16{});
 #pragma unroll
-              for (int vb = 0; vb < 4; ++vb) {
-                const u32x4 a = lds_read<u32x4>(v_at + (t * 4 + vb) * kFrag);
-                const f32x16 add = mfma32(__builtin_bit_cast(bf16x8, a & only), one, f32x16{});
+                  for (int i = 0; i < 16; ++i) r.o[vb][i] += sees ? add[i] : 0.0f;
+                }
+          } else if (in_bf) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) r.o[vb][i] += sees ? add[i] : 0.0f;
-              }
-            }
-        } else if (in_bf) {
+            for (int j = 0; j < 8; ++j)
+              r.o[j & 3] = mfma32(lds_read<bf16x8>(v_at + j * kFrag), __builtin_bit_cast(bf16x8, num[j >> 2]), r.o[j & 3]);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            r.o[j & 3] = mfma32(lds_read<bf16x8>(v_at + j * kFrag), __builtin_bit_cast(bf16x8, num[j >> 2]), r.o[j & 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + j * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
-        }
-        const int then = kt + (hh + 1) / NB;  // the next block's turn
-        if (then < seen) {
-          score<W>(r, s0, keys_at(then), (hh + 1) % NB);
-          if (then >= whole) mask_block(r, s0, kt * TK + (hh + 1) * 32, half);
-          move_max(p, r, far, top_of(s0));
+            for (int j = 0; j < 8; ++j)
+              r.o[j & 3] = mfma32(lds_read<f16x8>(v_at + j * kFrag), __builtin_bit_cast(f16x8, num[j >> 2]), r.o[j & 3]);
+          }
+          const int then = kt + (hh + 1) / NB;  // the next block's turn
+          if (then < seen) {
+            score<W>(r, s0, keys_at(then), (hh + 1) % NB);
+            if (then >= whole) mask_block(r, s0, kt * TK + (hh + 1) * 32, half);
+            move_max(p, r, far, top_of(s0));
+          }
         }
       }
+      s1 = f32x16{};  // (it is formed anew: without that, registers were kept for it)
+      ++kt;
     }
     const auto sw = __builtin_amdgcn_permlane32_swap(f2u(r.sum), f2u(r.sum), false, false);
     const float sum = u2f(sw[0]) + u2f(sw[1]);

@@ -115,3 +115,40 @@ def test_scores_far_from_0(log2, border, sign, waves):
     ref.assert_within(out, o, (2 * ref.U16 + 2.0**-10 + 2.0**-15) * size_o + 2 * fine, "out")
     want = torch.logsumexp(s, 1)[:, None].expand(n, heads)
     ref.assert_within(lse.double(), want, 2.0**-11 + 2.0**-19 + 4 * ref.U32 * want.abs(), "lse")
+
+
+@CUTS
+@pytest.mark.parametrize("size", [2.0**12, 2.0**-30])
+@pytest.mark.parametrize("tiles", [[0], [1, 2, 5], [3, 6, 7, 8, 14], [15], [0, 2, 4, 6, 8, 10, 12, 14], list(range(16))], ids=str)
+def test_tiles_that_fp16_does_not_hold(tiles, size, waves):
+    """Tiles of 64 tokens whose values are past fp16's range or below it, among others, in all orders."""
+    b, runner = _batch(35, 2, "bf16", [290, 40], [1000, 30], waves)
+    for t in tiles:
+        pages, places = _tokens(b, 0, 64 * t, min(1000, 64 * t + 64))
+        b.cache[pages, places, :512] = (b.cache[pages, places, :512].float() * size).to(b.cache.dtype)
+    # scores stay near 1: keys are made from the rope values alone, values from the latents
+    b.w.kv_b.view(2, 2, 128, 512)[:, 0] = 0
+    out = runner().attend(*b.args(), q_starts=b.dev_starts)
+    o, _, bound, _ = b.want()
+    ref.assert_within(out, o, bound, "out")
+    assert torch.equal(out, runner().attend(*b.args(), q_starts=b.dev_starts))
+
+
+@CUTS
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("at", [800, 830, 959, 999])
+def test_values_that_are_not_finite_among_marked_tiles(at, bad, waves):
+    """Queries that do not see such a token are as without it, those that do are not finite."""
+    b, runner = _batch(36, 2, "bf16", [290], [1000], waves)
+    pages, places = _tokens(b, 0, 640, 1000)
+    b.cache[pages, places, :512] *= 2.0**12  # finite, and past fp16's range
+    b.w.kv_b.view(2, 2, 128, 512)[:, 0] = 0
+    pages, places = _tokens(b, 0, at, at + 1)
+    good = b.cache.clone()
+    b.cache[pages, places, :512] = bad
+    out = runner().attend(*b.args())
+    b.cache = good
+    o, _, bound, _ = b.want()
+    first = at - 710
+    ref.assert_within(out[:first], o[:first], bound[:first], "before")
+    assert not torch.isfinite(out[first:].float()).any()
