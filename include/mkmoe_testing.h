@@ -51,6 +51,9 @@ void mkmoe_host_sqrt_softplus(const float* x, float* out, int64_t n);
  * to, over the batches of a step of rows rows (negative: a copy runs past its array); unit: a
  * compiled shape (MKMOE_UNIT 0 .. 8; -1 for others) */
 int mkmoe_host_pick_copy_slack(int32_t unit, int32_t rows);
+/* the cut that a call of a prompt's attention takes, whose arguments its own checks accept: 4 or 8 waves a
+ * workgroup; 0: its work is not counted in 32 bits and the call is refused */
+int mkmoe_host_prompt_waves(const mkmoe_latent_prompt_io* io);
 /* grouped top-k of one row of fp32 scores [E] with fp32 bias */
 void mkmoe_host_topk(const mkmoe_shape* shape, const float* scores, const float* bias,
                      int32_t* ids, float* weights);

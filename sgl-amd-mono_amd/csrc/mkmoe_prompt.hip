@@ -31,24 +31,16 @@
 // PFLOP/s, which make the floors.
 
 #include "mkmoe_latent.h"
+#include "mkmoe_prompt_cut.h"
 
 namespace mkmoe_latent {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// The attention's cuts, by the waves of a workgroup, W = 4 or 8: 32 W query rows a query tile, 8 W cached tokens a
-// turn, and as many equal shares of the work as two or one workgroups a CU
-constexpr int kMaxShares = 512;
-constexpr __host__ __device__ int shares_of(int waves) { return 2048 / waves; }
-constexpr __host__ __device__ int rows_of(int waves) { return 32 * waves; }
-constexpr __host__ __device__ int key_shift(int waves) { return waves == 8 ? 6 : 5; }
-constexpr int kKeys = 64;           // a sequence's packed rows are a multiple of so many
 // units of work that a share has at least (4, 6, 9: 193 tokens over 893 37.5, 36.1, 37.6 us)
 constexpr int kLeastUnits = 6;
 constexpr int kFrag = 1024;         // bytes of a fragment
 constexpr int kPromptSeqs = MKMOE_LATENT_MAX_SEQS;
-// What starting and storing a query tile takes, in turns of keys (5, 8, 12: ragged prompts' step 183, 179, 179 us)
-constexpr int kItemSetup = 8;
 constexpr float kMoveBy = 8.0f;     // a row's maximum moves where a score passes it by more than 2^kMoveBy
 constexpr float kLog2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 // Values in fp16 are held 2^kValueLift above themselves, so that fp16 is no coarser than bf16 for any from 2^-26, where its
@@ -1051,18 +1043,6 @@ inline PromptLayout prompt_layout(int heads, int64_t cap) {
   return l;
 }
 constexpr int kMaxContext = 1 << 22, kMaxPromptTokens = 1 << 20;
-inline int64_t packed_rows(int32_t context) { return ((int64_t)context + kKeys - 1) & -(int64_t)kKeys; }
-
-// 8 waves a workgroup read the keys and values half as often, 4 (two workgroups a CU) run one's start and end under the
-// other's turns. So 4 for short prompts and chunks, unless the cached tokens may be many: by the mean query tokens of a
-// sequence and what bounds its length (4 and 8 waves, us a call, 16 to 64 heads: 193 tokens over 700 38 and 44; 512 and
-// 2048 tokens alone 43 and 47, 100 and 100; 16 ragged prompts of up to 500 70 and 78, of up to 1000 209 and 224; 8 of up to 300
-// over 3000 144 and 157; 4 of up to 1024 over 4096 293 and 294; 512 over 16384 185 and 179; 300 over 65000 615 and 592; 8191 alone
-// 769 and 742)
-inline int waves_for(const mkmoe_latent_prompt_io* io) {
-  const int64_t table = (int64_t)io->max_pages * io->cache.page_size, context = io->max_context / io->seqs;
-  return io->tokens / io->seqs <= 2048 && (context < table ? context : table) <= 32768 ? 4 : 8;
-}
 inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_bytes, PromptParams& p) {
   if (!io || !ws) return MKMOE_ERR_NULL;
   if (!aligned(ws, 256)) return MKMOE_ERR_ALIGN;
@@ -1079,13 +1059,8 @@ inline int prompt_params(const mkmoe_latent_prompt_io* io, void* ws, size_t ws_b
   if (!isfinite(scale2) || io->max_pages < 1 || io->table_stride < io->max_pages) return MKMOE_ERR_ARG;
   const int64_t max_len = (int64_t)io->max_pages * io->cache.page_size;
   if (max_len > (int64_t)1 << 30) return MKMOE_ERR_ARG;
-  // the work's units are counted in 32 bits (a quarter as many with 8 waves)
-  auto countable = [&](int waves) {
-    const int64_t units = ((max_len < cap ? max_len : cap) >> key_shift(waves)) + 1 + kItemSetup;
-    return ((int64_t)io->tokens / rows_of(waves) + io->seqs) * io->heads * units <= 0x3fffffff;
-  };
-  if (!countable(8)) return MKMOE_ERR_ARG;
-  p.waves = countable(4) ? waves_for(io) : 8;
+  p.waves = prompt_waves(*io);
+  if (p.waves == 0) return MKMOE_ERR_ARG;
   const void* wide[] = {io->q_nope, io->q_pe, io->w, io->out};
   for (const void* q : wide)
     if (!aligned(q, 16)) return MKMOE_ERR_ALIGN;

@@ -8,6 +8,7 @@
 #include "mkmoe_kernels.hip"
 
 #include "../../include/mkmoe_testing.h"
+#include "mkmoe_prompt_cut.h"
 
 namespace mkmoe {
 
@@ -164,6 +165,10 @@ int mkmoe_host_pick_copy_slack(int32_t unit, int32_t rows) {
   int slack = -1;
   with_shape(unit, [&](auto c) { slack = pick_copy_slack<decltype(c)>(rows); });
   return slack;
+}
+
+int mkmoe_host_prompt_waves(const mkmoe_latent_prompt_io* io) {
+  return mkmoe_latent::prompt_waves(*io);
 }
 
 int mkmoe_device_union(int32_t unit, int32_t rows, const int32_t* ids, int32_t* picks, int32_t* experts, void* stream) {

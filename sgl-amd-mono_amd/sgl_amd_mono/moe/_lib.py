@@ -122,6 +122,7 @@ TESTING_EXPORTS = (
     "mkmoe_device_union",
     "mkmoe_host_e4m3_encode",
     "mkmoe_host_pick_copy_slack",
+    "mkmoe_host_prompt_waves",
     "mkmoe_host_sigmoid",
     "mkmoe_host_sqrt_softplus",
     "mkmoe_host_topk",
@@ -388,6 +389,7 @@ def testing_lib() -> ctypes.CDLL:
             getattr(T, name).argtypes = [vp, vp, ctypes.c_int64]
             getattr(T, name).restype = None
         T.mkmoe_host_pick_copy_slack.argtypes = [i32, i32]
+        T.mkmoe_host_prompt_waves.argtypes = [ctypes.POINTER(LatentPromptIO)]
         T.mkmoe_host_topk.argtypes = [ctypes.POINTER(Shape), vp, vp, vp, vp]
         T.mkmoe_host_topk.restype = None
         _testing_lib = T
