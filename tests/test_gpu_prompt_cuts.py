@@ -10,7 +10,7 @@ import torch.nn.functional as F
 
 import latent_ref as ref
 import prompt_ref
-from test_gpu_latent_prompt import BF, Batch, _runner, _step
+from test_gpu_latent_prompt import BF, SCALE, Batch, _runner, _step
 
 pytestmark = pytest.mark.gpu
 
@@ -232,3 +232,24 @@ def test_attention(waves):
     b.q_nope, b.q_pe = b.q[..., :128], q_pe
     assert torch.equal(out, run.attend(*b.args(), q_starts=b.dev_starts))
     b.check(out)
+
+
+@CUTS
+def test_more_items_than_a_share_lists(waves):
+    """512 short sequences of 128 heads: 65536 query tiles, 128 or 256 a share, which lists 64 at a time. The cut by 8
+    waves is taken where the other's work passes 32 bits: by a max_context of 800000 tokens."""
+    g = torch.Generator().manual_seed(5)
+    new = [1 + int(x) for x in torch.randint(0, 3, (512,), generator=g)]
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 60, (512,), generator=g))]
+    b = Batch(43, 128, "bf16", 64, new, lens)
+    run = _cut(b, waves, tokens=800000, max_context=65536 if waves == 4 else 800000)
+    lse = torch.empty(sum(new), 128, device="cuda")
+    out = run.attend(*b.args(), q_starts=b.dev_starts, lse=lse)
+    assert waves_of(run) == waves
+    run.raise_on_device_error()
+    for h in (0, 1, 63, 100, 127):
+        z = slice(h, h + 1)
+        o, l, bound, lbound = prompt_ref.attend(b.cache, b.w.kv_b.view(128, 256, 512)[z], b.q_nope[:, z], b.q_pe[:, z],
+                                                b.table, b.lens, b.starts, SCALE)  # fmt: skip
+        ref.assert_within(out[:, z], o, bound, f"head {h}")
+        ref.assert_within(lse[:, z].double(), l, lbound, f"lse of head {h}")
