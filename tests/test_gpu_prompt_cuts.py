@@ -253,3 +253,24 @@ def test_more_items_than_a_share_lists(waves):
                                                 b.table, b.lens, b.starts, SCALE)  # fmt: skip
         ref.assert_within(out[:, z], o, bound, f"head {h}")
         ref.assert_within(lse[:, z].double(), l, lbound, f"lse of head {h}")
+
+
+@CUTS
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("new,lens,heads", [([777], [777], 16), ([300, 500], [1300, 500], 8), ([200], [6000], 4)])
+def test_accuracy(new, lens, heads, fmt, waves):
+    """The error in the 2-norm. A rounding to bf16 of values whose logarithms are spread evenly is off by a root mean
+    square of r = 2^-8 sqrt((1 - 1/4) / (3 2 ln 2)) = 2^-8 0.4246 of them: an error even over a step, 2^-8 / sqrt 3 of
+    the power of two below a value, and the mean of that power's square over the value's own, (1 - 1/4) / (2 ln 2).
+    The output is rounded so; each of the 128 key values that the latents make, which moves a score of unit queries and
+    keys by r scale sqrt 128, and an output by at most so much of it; a value and a numerator to fp16, by r / 8 each. With 8 % for how
+    the values of a case lie: a numerator or value rounded to bf16 instead adds r of it, more than that."""
+    b = Batch(50 + sum(new), heads, fmt, 64, new, lens)
+    run = _cut(b, waves, **({"max_context": 8192} if waves == 4 else {}))
+    out = run.attend(*b.args(), q_starts=b.dev_starts)
+    assert waves_of(run) == waves
+    want = b.want()[0]
+    rel = ((out.double() - want).norm() / want.norm()).item()
+    r = ref.U16 * (0.75 / (6 * 0.6931472)) ** 0.5
+    print(f"\nerror {rel:.6f}", flush=True)
+    assert rel <= 1.08 * r * (1 + 128 * SCALE**2 + 2 / 64) ** 0.5
