@@ -483,10 +483,12 @@ int mkmoe_pages_workspace_bytes(int32_t pages, int32_t max_seqs, int32_t max_pag
 int mkmoe_pages_adopt(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, void* ws, size_t ws_bytes, void* stream);
 /* add[b] tokens more for each sequence: lens grows, the table gets the pages taken. The call's tokens follow
  * each other by sequence: starts [seqs + 1], positions [tokens], and slots [tokens], the cache rows (page page_size +
- * offset) they go to; -1 (position 0) for those of a sequence that does not get them, and behind the last. One launch. */
+ * offset) they go to; -1 (position 0) for those of a sequence that does not get them, and behind the last. Where the
+ * free pages do not suffice for a sequence, those behind it that need a page get none either. One launch. */
 int mkmoe_pages_grow(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, const int32_t* add, int32_t tokens,
                      int32_t* slots, int32_t* positions, int32_t* starts, void* ws, size_t ws_bytes, void* stream);
-/* Sequences cut to their first keep[b] tokens, pages behind them let go (0: freed; len or more: left as it is). Two launches. */
+/* Sequences cut to their first keep[b] tokens, pages behind them let go (0: freed; len or more: left as it is). A last
+ * page that is then partly filled and that others held before the call is copied. Two launches. */
 int mkmoe_pages_trim(const mkmoe_pages_pool* pool, const mkmoe_pages_table* table, const int32_t* keep, void* ws,
                      size_t ws_bytes, void* stream);
 /* Row b of the table goes on from row parents[b] as it was before the call (-1: empty). Full pages are shared;

@@ -146,7 +146,10 @@ class PagePool:
         [B + 1]), int32, as the runners' ``append`` and ``attend`` take them. ``lens`` grows and ``table`` gets the
         pages taken, in place. ``tokens``: rows of the outputs; those behind the sum of ``add`` have slot -1.
         ``out``: the three tensors. A sequence for which no pages are left, no entries in the table or no rows in
-        the outputs stays as it was, its tokens' slots are -1 and it is recorded (``raise_on_device_error``)."""
+        the outputs stays as it was, its tokens' slots are -1 and it is recorded (``raise_on_device_error``). Pages
+        are given in the rows' order, and none past a row that goes without for want of them: the rows behind it
+        that need a page go without too, though some may be free. What has to go on (decode steps) belongs in the
+        rows before what may wait (prompts), or in a call before."""
         seqs = self._set_table(table, lens)
         at_add = self._vec("add", add, seqs)
         if not 0 <= tokens < 1 << 31:
@@ -163,7 +166,9 @@ class PagePool:
     def trim(self, table, lens, keep: torch.Tensor) -> None:
         """Sequences cut to their first ``keep`` [B] int32 tokens, in place: their other pages are let go (0 frees
         a sequence; ``lens`` or more leaves it as it is). Where the last page kept is then partly filled and
-        others hold it too, the sequence gets a copy; it stays as it was, and is recorded, where no page is free."""
+        others held it too before the call, the sequence gets a copy; it stays as it was, and is recorded, where no
+        page was free. That holds where the call lets the others go as well: with no page to spare, free them in
+        a call before."""
         seqs = self._set_table(table, lens)
         self._call(self.lib.mkmoe_pages_trim, self._pool, self._table, self._vec("keep", keep, seqs))
 
