@@ -389,9 +389,10 @@ int mkmoe_latent_step(const mkmoe_latent_append_io* append, const mkmoe_latent_p
 /* ---- a prompt's tokens
  * The same attention with a key and a value for each head and token, made from the cached rows by
  * w: k = [W_UK c, k_pe], v = W_UV c, o = sum softmax(scale q . k) v: fewer operations than the absorbed form
- * from about 171 query tokens a sequence. Keys are rounded to bf16, values and softmax's numerators to fp16 (to
+ * from about 171 query tokens a sequence, and faster from 12 to 225 of them, the more the more is
+ * cached before them. Keys are rounded to bf16, values and softmax's numerators to fp16 (to
  * bf16 in tiles of 64 tokens with a value, not 0, outside 2^-26 .. 128), sums, scores and maxima are fp32. Values whose size
- * passes 2^100 may give infinities. Query token i of a sequence's n sees its first len - n + 1 + i tokens. */
+ * passes 2^100 may give infinities; a weight below 2^-24 of its row's largest is held to 2^-32 of that. Query token i of a sequence's n sees its first len - n + 1 + i tokens. */
 typedef struct mkmoe_latent_prompt_io {
   mkmoe_latent_cache cache;
   int32_t seqs;        /* 1 .. MKMOE_LATENT_MAX_SEQS */
@@ -399,7 +400,8 @@ typedef struct mkmoe_latent_prompt_io {
   int32_t heads;       /* 1 .. MKMOE_LATENT_MAX_HEADS */
   int32_t max_pages;   /* table entries a sequence: its length is at most max_pages page_size */
   int32_t max_context; /* cached tokens that the workspace holds: those of the sequences with query tokens, each
-                        * one's rounded up to 64; at most 2^22 */
+                        * one's rounded up to 64; at most 2^22. How the work is cut, and so the last bits and some of the
+                        * time, goes by it, the table's width, seqs and tokens */
   int32_t pad;
   int64_t table_stride;
   int64_t qn_token_stride, qn_head_stride, qp_token_stride, qp_head_stride;
@@ -411,7 +413,7 @@ typedef struct mkmoe_latent_prompt_io {
   const int32_t* lens;     /* [seqs] cached tokens, the queries' own among them; 0: none */
   const int32_t* q_starts; /* [seqs + 1] first query token of each sequence, or NULL: equal counts */
   void* out;               /* [tokens][heads][128] bf16; 0 for a query that sees nothing */
-  float* lse;              /* [tokens][heads] log of the sum of exp(s), or NULL; -inf there */
+  float* lse;              /* [tokens][heads] log of the sum of exp(s), each term rounded as above, or NULL; -inf there */
   float scale;
   int32_t pad2;
 } mkmoe_latent_prompt_io;

@@ -14,8 +14,9 @@
 //   k_latent_absorb / k_latent_expand   the two products of every head with its weights
 //   k_latent_front    a step's append and absorb in one launch
 //
-// Times below are of an MI355X, in graph replays. It copies 5.19 TB/s and multiplies bf16 matrices
-// at 1.25 PFLOP/s, which make the floors.
+// Times below are of an MI355X, in graph replays. The floors are made with 5.19 TB/s and 1.25 PFLOP/s, a large
+// copy's and bf16 product's rates when they were measured (both depend on size and operands: copies of 256 MiB to 4 GiB
+// reach 4.6 to 5.4 TB/s, products of 4096^3 to 16384^3 1.1 to 1.6 PFLOP/s).
 
 #include <type_traits>
 

@@ -24,11 +24,12 @@
 //
 // Rounded to fewer bits than fp32 are the operands of the matrix instructions: keys to bf16, whose range
 // queries need, numerators and values to fp16 (3 more bits), a tile's values to bf16 where fp16 would be coarser
-// for one of them (k_prompt_heads). Against 64 bits, in the 2-norm, where the output's own rounding is 0.0017: 0.0021 where rows see few
-// keys (bf16 numerators and values 0.0028), 0.0017 over long ones. Sums, maxima, outputs and parts are fp32.
+// for one of them (k_prompt_heads). Against 64 bits, in the 2-norm, where the output's own rounding is 0.0017: 0.0019 to
+// 0.0022 where rows see few keys (with all values in bf16 0.0028), 0.0017 over long ones. Sums, maxima, outputs and parts are fp32;
+// the sums are of the numerators as they are multiplied, so that a row's weights add up to 1.
 //
-// Times below are of an MI355X, of passes among others. It copies 4.9 TB/s and multiplies bf16 matrices at 1.39
-// PFLOP/s, which make the floors.
+// Times below are of an MI355X, of passes among others. The floors are made with 4.91 TB/s, a copy of 2 GiB, and 1.39
+// PFLOP/s, a bf16 product of 8192^3.
 
 #include "mkmoe_latent.h"
 #include "mkmoe_prompt_cut.h"
@@ -563,7 +564,7 @@ struct Rows {
   int sees;       // the last key that the row sees
 };
 // Numerators are up to 2^(kLift + kMoveBy), below fp16's largest, and what fp16 drops of them is below 2^-32 of the
-// largest one's
+// largest one's: weights from 2^-24 of the largest have bf16's precision or more, smaller ones less
 constexpr float kLift = 7.0f;
 
 // a fragment along a block of 32 keys: 8 of them, then 4 of their rope values
@@ -622,12 +623,14 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
 //   O^T += V^T P^T   A = values from LDS, B = P^T as it lies: a row's rescaling is a lane's own factor
 // Scores are formed a block of 32 keys ahead, and the code alternates their products with the numerators of the block
 // before, then the products of the outputs with the next maximum: a wave's matrix and vector instructions run under
-// each other (chunk_large below: 2.63 -> 2.03 ms). Keys and values come straight from memory to LDS two turns ahead,
-// one barrier a turn.
+// each other (8191 tokens over 16383 with 32 heads, the call: 2.63 -> 2.03 ms). Keys and values come straight from memory
+// to LDS two turns ahead, one barrier a turn. An item's last turn, those whose values are bf16 and those of scores far from 0
+// (move_max) go without that, each operand as it is needed: with all values in bf16 the same call takes 2.75 ms, 300 over 65300
+// 722 us for 680, ragged prompts' step 224 for 196.
 //
-// What bounds it: power. 8191 tokens over 16383 with 32 heads, 2.06 PFLOP, take 1.95 ms, 1.06 PFLOP/s (the floor's
-// rate is 1.39): the matrix units are busy for 61 % of the cycles and the clock falls to 1.7 GHz; counters: 3.3 vector
-// instructions to a matrix instruction, LDS busy for 31 %, without conflicts. Ahead of that, short prompts: an item's
+// What bounds it: power. 8191 tokens over 16383 with 32 heads, 2.06 PFLOP, take 2.06 ms (the median of 12; 1.98 the least), 1.0
+// PFLOP/s (the floor's rate is 1.39): the matrix units are busy for 61 % of the cycles and the clock falls to 1.7 GHz; counters: 3.3
+// vector instructions to a matrix instruction, LDS busy for 31 %, without conflicts. Ahead of that, short prompts: an item's
 // start and end (its queries, first keys, outputs) of 6 to 9 us beside turns of 1.5 to 2 us of 64 keys.
 template <int W>
 __global__ __launch_bounds__(64 * W, 2) void k_prompt_attend(PromptParams p) {

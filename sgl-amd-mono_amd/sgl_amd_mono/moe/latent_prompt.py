@@ -28,8 +28,9 @@ class LatentPromptRunner(_LatentCalls):
 
     ``max_tokens``: new tokens that ``attention`` takes at most. ``max_context``: cached tokens whose
     keys and values the workspace holds: those of a call's sequences with new tokens, each one's
-    rounded up to 64 (135 MB, and a token 1152 bytes and 512 a head). ``scale``, ``norm_eps``,
-    ``rope``: as ``LatentRunner``. One runner serves one stream at a time: calls that can overlap need
+    rounded up to 64 (135 MB, and a token 1152 bytes and 512 a head); where it is large for a call, and the call's
+    table wide, the work is cut as for long sequences, and short ones take up to a fifth longer. ``scale``,
+    ``norm_eps``, ``rope``: as ``LatentRunner``. One runner serves one stream at a time: calls that can overlap need
     runners of their own."""
 
     def __init__(self, heads: int, device=None, max_tokens: int = 8192, max_context: int = 32768,

@@ -7,7 +7,7 @@ import torch
 
 import latent_ref as ref
 import prompt_ref
-from test_gpu_latent_prompt import Batch, _runner
+from test_gpu_latent_prompt import BF, Batch, _runner
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,29 @@ def test_values_that_are_not_finite_among_marked_tiles(at, bad, waves):
     first = at - 710
     ref.assert_within(out[:first], o[:first], bound[:first], "before")
     assert not torch.isfinite(out[first:].float()).any()
+
+
+@CUTS
+def test_weights_far_below_the_largest(waves):
+    """Every key's value is an output of its own, so the outputs are the weights, from the largest down to less than
+    2^-40. A numerator is held to 2^-25, the largest is 2^7 at least: off by 2^-32 beside the rounding's own bound."""
+    heads, n, length = 2, 70, 128
+    b, runner = _batch(37, heads, "bf16", [n], [length], waves)
+    pages, places = _tokens(b, 0, 0, length)
+    at = torch.arange(length, device="cuda")
+    b.cache[pages, places] = 0
+    b.cache[pages, places, at] = 1.0
+    b.cache[pages, places, 512 + at % 32] = torch.where(at < 64, 1.0, 0.5).to(b.cache.dtype)
+    w = b.w.kv_b.view(heads, 2, 128, 512)
+    w[:] = 0
+    w[:, 1, at, at] = 1.0
+    w[:, 0, 0, :128] = (-0.25 * (at // 32)).to(w.dtype)
+    b.q_nope, b.q_pe = torch.zeros_like(b.q_nope).contiguous(), torch.zeros_like(b.q_pe)
+    b.q_nope[..., 0] = 32.0
+    b.q_pe[..., :32] = (-0.25 * torch.arange(32, device="cuda")).to(BF)
+    lse = torch.empty(n, heads, device="cuda")
+    out = runner(scale=1.0).attend(*b.args(), lse=lse)
+    o, l, bound, lbound = b.want(1.0)
+    assert o.max() > 0.1 and o[o > 0].min() < 2.0**-40
+    ref.assert_within(out, o, bound + 2.0**-32, "out")
+    ref.assert_within(lse.double(), l, lbound + 2.0**-11 + length * 2.0**-32, "lse")
